@@ -1,0 +1,440 @@
+// Rows of an embedding table, and the table's gradient.
+//
+// Forward: out[n] = scale * weight[token(n) - first], zeros for tokens of other shards.  A copy with a lookup: bound by memory.
+//
+// Gradient: dW[r] = scale * sum over the places n of token r of grad[n].  Adding place by place with atomics would give sums that
+// depend on timing, and a frequent token's row would be added to by thousands of places one after another.  Here places are
+// ordered by token first, and sums are taken over pieces of that order:
+//   index   one launch.  A workgroup owns the rows r with r % groups == its number (frequent tokens, which are neighbours in
+//           vocabularies built by merges, spread over all of them), reads ALL tokens twice, counts its own and those of
+//           workgroups before it -- so it knows where its part of the order begins without asking anyone -- and writes its places,
+//           row by row and in the order of n within a row.
+//   sum     a piece of `piece` neighbouring places of the order each: all pieces take equally long whatever the tokens are.
+//           A row that lies in one piece is written; of a row that goes over the edge of a piece a partial sum is kept, at
+//           most two of a piece.  The rest of the same launch fills the rows without places with zeros.
+//   join    adds up the partial sums of a row, in order.
+#include "ops_common.h"
+
+#include <type_traits>
+
+namespace {
+using namespace ops;
+
+constexpr int INDEX_WAVES = 16, INDEX_THREADS = 64 * INDEX_WAVES;
+constexpr int INDEX_ROWS = 512;     // rows of a workgroup: a counter for each of them and each wave is 32 KB of LDS
+constexpr int INDEX_AHEAD = 8;      // reads of tokens in flight for each lane
+constexpr int THREADS = 256;
+constexpr int FILL_ROWS = 16;       // rows that a unit of threads looks at for zeros
+
+// Row numbers and where they go.
+struct Index {
+    int64_t n, first, rows;
+    int32_t shift;       // log2 of the workgroups that share the rows
+    int32_t per_group;   // rows of a workgroup
+    int32_t *order;      // [n]  places by row
+    int32_t *row;        // [n]  ... and the row of each
+    int32_t *start;      // [groups * per_group]  of a row's places in `order`
+    int32_t *count;      // [groups * per_group]
+    int32_t *total;      // places with a row of this shard
+    __device__ __forceinline__ int64_t slot(int64_t r) const { return (r & ((1 << shift) - 1)) * per_group + (r >> shift); }
+};
+
+template <typename I> __global__ __launch_bounds__(INDEX_THREADS) void embed_index_kernel(Index x, const I *__restrict__ tokens)
+{
+    __shared__ int32_t count[INDEX_WAVES][INDEX_ROWS];
+    __shared__ int32_t sums[INDEX_WAVES], before[INDEX_WAVES];
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, group = blockIdx.x, mask = (1 << x.shift) - 1;
+    for (int i = t; i < INDEX_WAVES * INDEX_ROWS; i += INDEX_THREADS) (&count[0][0])[i] = 0;
+    __syncthreads();
+    // A wave's tokens follow each other, so that its places are in order if it takes them in order.
+    const int64_t each = (x.n + INDEX_THREADS - 1) / INDEX_THREADS * 64;
+    const int64_t from = wave * each, to = from + each < x.n ? from + each : x.n;
+    const auto row_of = [&](int64_t i) -> int64_t {   // or -1
+        if (i >= to) return -1;
+        const int64_t r = (int64_t)tokens[i] - x.first;
+        return r >= 0 && r < x.rows ? r : -1;
+    };
+    uint32_t lower = 0;
+    for (int64_t at = from; at < to; at += 64 * INDEX_AHEAD) {
+        int64_t r[INDEX_AHEAD];
+#pragma unroll
+        for (int j = 0; j < INDEX_AHEAD; ++j) r[j] = row_of(at + 64 * j + lane);
+#pragma unroll
+        for (int j = 0; j < INDEX_AHEAD; ++j)
+            if (r[j] >= 0) {
+                const int of = (int)(r[j] & mask);
+                lower += of < group;
+                if (of == group) atomicAdd(&count[wave][r[j] >> x.shift], 1);
+            }
+    }
+    lower = wave_sum(lower);
+    if (lane == 0) before[wave] = (int32_t)lower;
+    __syncthreads();
+    // counts -> where the places of each row and wave begin
+    int32_t of_row = 0;
+    if (t < x.per_group)
+        for (int w = 0; w < INDEX_WAVES; ++w) {
+            const int32_t c = count[w][t];
+            count[w][t] = of_row;
+            of_row += c;
+        }
+    int32_t upto = of_row;   // sum over the rows of a wave up to this one
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int32_t other = __shfl_up(upto, d);
+        if (lane >= d) upto += other;
+    }
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int32_t begin = upto - of_row;
+    for (int w = 0; w < INDEX_WAVES; ++w) begin += before[w] + (w < wave ? sums[w] : 0);
+    if (t < x.per_group) {
+        for (int w = 0; w < INDEX_WAVES; ++w) count[w][t] += begin;
+        x.start[(int64_t)group * x.per_group + t] = begin;
+        x.count[(int64_t)group * x.per_group + t] = of_row;
+    }
+    if (group == mask && t == INDEX_THREADS - 1) *x.total = begin + of_row;   // (rows beyond per_group have no places)
+    __syncthreads();
+    for (int64_t at = from; at < to; at += 64 * INDEX_AHEAD) {
+        int64_t r[INDEX_AHEAD];
+#pragma unroll
+        for (int j = 0; j < INDEX_AHEAD; ++j) r[j] = row_of(at + 64 * j + lane);
+#pragma unroll
+        for (int j = 0; j < INDEX_AHEAD; ++j) {
+            const bool mine = r[j] >= 0 && (int)(r[j] & mask) == group;
+            const int local = mine ? (int)(r[j] >> x.shift) : -1;
+            uint64_t left = __ballot(mine);
+            while (left) {   // one row at a time, most often the only one
+                const int leader = __builtin_ctzll(left);
+                const int row = __builtin_amdgcn_readlane(local, leader);
+                const uint64_t same = __ballot(local == row);
+                int32_t place = 0;
+                if (lane == leader) place = atomicAdd(&count[wave][row], (int)__popcll(same));
+                place = __builtin_amdgcn_readlane(place, leader);
+                if (local == row) {
+                    place += (int)__popcll(same & ((1ull << lane) - 1));
+                    x.order[place] = (int32_t)(at + 64 * j + lane);
+                    x.row[place] = (int32_t)r[j];
+                }
+                left &= ~same;
+            }
+        }
+    }
+}
+
+struct Sum {
+    Index index;
+    int64_t dim;
+    int32_t piece, pieces;
+    int32_t unit;        // threads that share a row: a power of two
+    int32_t accumulate;
+    float scale;
+    int64_t grad_stride, out_stride;
+    float *partial;      // [pieces][2][dim]: of the row that began before the piece, of the one that goes on behind it
+};
+
+template <typename O, int N> __device__ __forceinline__ void put_row(const Sum &s, typename O::raw *out, int64_t row, int64_t col, const float (&acc)[N])
+{
+    typename O::raw *p = out + row * s.out_stride + col;
+    float v[N];
+    Pack<O, N> old;
+    if (s.accumulate) old.load(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = s.accumulate ? fmaf(acc[i], s.scale, old[i]) : acc[i] * s.scale;
+    old.set(v);
+    old.store(p);
+}
+
+template <typename T, typename O, int N>
+__global__ __launch_bounds__(THREADS) void embed_sum_kernel(Sum s, const typename T::raw *__restrict__ grad, typename O::raw *__restrict__ out)
+{
+    const Index &x = s.index;
+    const int64_t unit = (int64_t)blockIdx.x * (THREADS / s.unit) + threadIdx.x / s.unit;
+    const int64_t col = ((int64_t)blockIdx.y * s.unit + threadIdx.x % s.unit) * N;
+    if (col >= s.dim) return;
+    if (unit >= s.pieces) {   // rows without places
+        if (s.accumulate) return;
+        const int64_t r0 = (unit - s.pieces) * FILL_ROWS;
+        Pack<O, N> zeros;
+        zeros.zero();
+#pragma unroll 4
+        for (int i = 0; i < FILL_ROWS; ++i)
+            if (r0 + i < x.rows && x.count[x.slot(r0 + i)] == 0) zeros.store(out + (r0 + i) * s.out_stride + col);
+        return;
+    }
+    const int64_t total = *x.total, begin = unit * s.piece;
+    if (begin >= total) return;
+    const int64_t end = begin + s.piece < total ? begin + s.piece : total;
+    const int32_t ahead = begin > 0 ? x.row[begin - 1] : -1, behind = end < total ? x.row[end] : -1;
+    float acc[N];
+    int32_t row = x.row[begin];
+    bool from_ahead = row == ahead;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+    const auto put = [&](bool goes_on) {
+        if (from_ahead || goes_on) {
+            float *p = s.partial + (unit * 2 + (from_ahead ? 0 : 1)) * s.dim + col;
+            Pack<F32, N> v;
+            v.set(acc);
+            v.store(reinterpret_cast<F32::raw *>(p));
+        } else
+            put_row<O, N>(s, out, row, col, acc);
+    };
+    constexpr int AHEAD = 8;
+    for (int64_t at = begin; at < end; at += AHEAD) {
+        Pack<T, N> v[AHEAD];
+        int32_t r[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int64_t p = at + j < end ? at + j : end - 1;
+            r[j] = x.row[p];
+            v[j].load(grad + x.order[p] * s.grad_stride + col);
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            if (at + j >= end) break;
+            if (r[j] != row) {
+                put(false);
+                row = r[j];
+                from_ahead = false;
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += v[j][i];
+        }
+    }
+    put(row == behind);
+}
+
+template <typename O, int N> __global__ __launch_bounds__(THREADS) void embed_join_kernel(Sum s, typename O::raw *__restrict__ out)
+{
+    const Index &x = s.index;
+    const int64_t unit = (int64_t)blockIdx.x * (THREADS / s.unit) + threadIdx.x / s.unit;
+    const int64_t col = ((int64_t)blockIdx.y * s.unit + threadIdx.x % s.unit) * N;
+    const int64_t total = *x.total, end = (unit + 1) * s.piece;
+    if (col >= s.dim || unit >= s.pieces || end >= total) return;
+    const int32_t row = x.row[end - 1];
+    const int64_t slot = x.slot(row), start = x.start[slot], stop = start + x.count[slot];
+    if (stop <= end || start < unit * s.piece) return;   // ends here, or began in a piece before: that one's
+    float acc[N];
+    Pack<F32, N> v;
+    v.load(reinterpret_cast<const F32::raw *>(s.partial + (unit * 2 + 1) * s.dim + col));
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = v[i];
+    const int64_t last = (stop - 1) / s.piece;
+#pragma unroll 4
+    for (int64_t u = unit + 1; u <= last; ++u) {
+        Pack<F32, N> more;
+        more.load(reinterpret_cast<const F32::raw *>(s.partial + u * 2 * s.dim + col));
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += more[i];
+    }
+    put_row<O, N>(s, out, row, col, acc);
+}
+
+struct Rows {
+    int64_t n, dim, rows, first;
+    int32_t unit, each;   // threads that share a row, rows of such a unit
+    int32_t token_type;
+    float scale;
+    int64_t weight_stride, out_stride;
+};
+
+template <typename T, typename O, int N>
+__global__ __launch_bounds__(THREADS) void embed_rows_kernel(Rows s, const void *__restrict__ tokens, const typename T::raw *__restrict__ weight,
+                                                             typename O::raw *__restrict__ out)
+{
+    const int64_t unit = (int64_t)blockIdx.x * (THREADS / s.unit) + threadIdx.x / s.unit;
+    const int64_t col = ((int64_t)blockIdx.y * s.unit + threadIdx.x % s.unit) * N;
+    if (col >= s.dim) return;
+    constexpr int AHEAD = 4;
+    const int64_t begin = unit * s.each, end = begin + s.each < s.n ? begin + s.each : s.n;
+    for (int64_t at = begin; at < end; at += AHEAD) {
+        Pack<T, N> v[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            v[j].zero();
+            if (at + j < end) {
+                const int64_t r = token_at(tokens, s.token_type, at + j) - s.first;
+                if (r >= 0 && r < s.rows) v[j].load(weight + r * s.weight_stride + col);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (at + j < end) {
+                float f[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) f[i] = v[j][i] * s.scale;
+                Pack<O, N> o;
+                o.set(f);
+                o.store(out + (at + j) * s.out_stride + col);
+            }
+    }
+}
+
+// Elements that a thread takes of a row at a time: 16 bytes of the smaller of the two types where every row starts on 16, the
+// largest power of two that all rows start on otherwise, one where that is an element.
+int elements_at_once(int64_t dim, int64_t bytes_a, int size_a, int64_t bytes_b, int size_b)
+{
+    int n = 16 / (size_a < size_b ? size_a : size_b);
+    while (n > 1 && (dim % n || (bytes_a < 16 && bytes_a % (n * size_a)) || (bytes_b < 16 && bytes_b % (n * size_b)))) n /= 2;
+    return n;
+}
+
+// The threads that share a row: enough for all of it, a power of two so that units fill a workgroup.
+int unit_of(int64_t dim, int n)
+{
+    int u = 1;
+    while (u < THREADS && (int64_t)u * n < dim) u *= 2;
+    return u;
+}
+
+template <typename F> int with_type(int t, F f)
+{
+    switch (t) {
+    case GDP_F32: return f(F32{});
+    case GDP_F16: return f(F16{});
+    default: return f(BF16{});
+    }
+}
+template <typename F> int with_count(int n, F f)
+{
+    switch (n) {
+    case 8: return f(std::integral_constant<int, 8>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    default: return f(std::integral_constant<int, 1>{});
+    }
+}
+
+// Sizes of the order and of the partial sums, by which the workspace is laid out.
+struct Layout {
+    int shift, piece;
+    int64_t per_group, pieces;
+    size_t order, row, start, count, total, partial, bytes;
+};
+
+Layout layout_of(int64_t n, int64_t rows, int64_t dim)
+{
+    Layout l;
+    l.shift = 0;
+    while (l.shift < 8 && (1ll << l.shift) < rows) ++l.shift;
+    while (ceil_div(rows, (int64_t)1 << l.shift) > INDEX_ROWS) ++l.shift;
+    l.per_group = ceil_div(rows, (int64_t)1 << l.shift);
+    // A longer piece keeps fewer partial sums (each is written and read), a shorter one fills the device.
+    l.piece = 16;
+    while (l.piece < 128 && n / (2 * l.piece) * ceil_div(dim, (int64_t)2048) >= 512) l.piece *= 2;
+    l.pieces = ceil_div(n, (int64_t)l.piece);
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += round_up(bytes, 256);
+        return here;
+    };
+    l.order = take((size_t)n * 4);
+    l.row = take((size_t)n * 4);
+    l.start = take(((size_t)l.per_group << l.shift) * 4);
+    l.count = take(((size_t)l.per_group << l.shift) * 4);
+    l.total = take(4);
+    l.partial = take((size_t)l.pieces * 2 * (size_t)dim * 4);
+    l.bytes = at;
+    return l;
+}
+
+// (grids of a few workgroups for each 4 tokens or 16 rows stay within 2^32 threads)
+constexpr int64_t MOST_TOKENS = ((int64_t)1 << 26) - 4096, MOST_ROWS = (int64_t)1 << 27;
+int check_sizes(int64_t n, int64_t rows, int64_t dim)
+{
+    if (n < 0 || rows < 0 || dim < 0) return gdp_fail(GDP_E_BADARG, "gdp_embed: a size is negative");
+    if (n > MOST_TOKENS || rows > MOST_ROWS || dim > (1 << 20))
+        return gdp_fail(GDP_E_BADARG, "gdp_embed: more than 2^26 - 4096 tokens, 2^27 rows or 2^20 columns");
+    return GDP_OK;
+}
+
+}  // namespace
+
+extern "C" int gdp_embed_forward(const gdp_embed *e, void *stream)
+{
+    gdp_clear_error();
+    if (!e) return gdp_fail(GDP_E_BADARG, "gdp_embed: null argument");
+    if (const int rc = check_sizes(e->n, e->rows, e->dim)) return rc;
+    if (!type_ok(e->weight_type) || !type_ok(e->out_type) || !token_type_ok(e->token_type))
+        return gdp_fail(GDP_E_BADARG, "gdp_embed: unknown element type");
+    if (e->n == 0 || e->dim == 0) return GDP_OK;
+    if (!e->tokens || !e->out || (e->rows && !e->weight)) return gdp_fail(GDP_E_BADARG, "gdp_embed: null pointer");
+    if (!rows_ok(e->rows, e->dim, e->weight_stride, false) || !rows_ok(e->n, e->dim, e->out_stride, true))
+        return gdp_fail(GDP_E_BADARG, "gdp_embed: a row stride is negative, too large, or below the width of rows that are written");
+    if (!aligned(e->weight, size_of(e->weight_type)) || !aligned(e->out, size_of(e->out_type)) ||
+        !aligned(e->tokens, e->token_type == GDP_I64 ? 8 : 4))
+        return gdp_fail(GDP_E_BADARG, "gdp_embed: a pointer is not aligned to its elements");
+    const int n = elements_at_once(e->dim, row_alignment(e->weight, e->weight_stride, e->weight_type), size_of(e->weight_type),
+                                   row_alignment(e->out, e->out_stride, e->out_type), size_of(e->out_type));
+    Rows s{e->n, e->dim, e->rows, e->first, unit_of(e->dim, n), 1, e->token_type, e->scale, e->weight_stride, e->out_stride};
+    const int64_t across = ceil_div(e->dim, (int64_t)s.unit * n), per = THREADS / s.unit;
+    if (ceil_div(e->n, per * 4) * across >= 2048) s.each = 4;   // rows in flight of a thread, where there are enough for all
+    const int64_t blocks = ceil_div(e->n, per * s.each);
+    return with_type(e->weight_type, [&](auto T) {
+        return with_type(e->out_type, [&](auto O) {
+            return with_count(n, [&](auto N) {
+                using TT = decltype(T);
+                using OO = decltype(O);
+                return launch("gdp_embed_forward", embed_rows_kernel<TT, OO, N.value>, dim3((unsigned)blocks, (unsigned)across), THREADS, 0, stream,
+                              s, e->tokens, static_cast<const typename TT::raw *>(e->weight), static_cast<typename OO::raw *>(e->out));
+            });
+        });
+    });
+}
+
+extern "C" int gdp_embed_grad_workspace(int64_t n, int64_t rows, int64_t dim, size_t *bytes)
+{
+    gdp_clear_error();
+    if (!bytes) return gdp_fail(GDP_E_BADARG, "gdp_embed: null argument");
+    if (const int rc = check_sizes(n, rows, dim)) return rc;
+    *bytes = layout_of(n, rows, dim).bytes;
+    return GDP_OK;
+}
+
+extern "C" int gdp_embed_backward(const gdp_embed_grad *e, void *stream)
+{
+    gdp_clear_error();
+    if (!e) return gdp_fail(GDP_E_BADARG, "gdp_embed: null argument");
+    if (const int rc = check_sizes(e->n, e->rows, e->dim)) return rc;
+    if (!type_ok(e->grad_type) || !type_ok(e->out_type) || !token_type_ok(e->token_type))
+        return gdp_fail(GDP_E_BADARG, "gdp_embed: unknown element type");
+    if (e->rows == 0 || e->dim == 0 || (e->n == 0 && e->accumulate)) return GDP_OK;
+    if ((e->n && (!e->tokens || !e->grad)) || !e->out || !e->workspace) return gdp_fail(GDP_E_BADARG, "gdp_embed: null pointer");
+    if (!rows_ok(e->n, e->dim, e->grad_stride, false) || !rows_ok(e->rows, e->dim, e->out_stride, true))
+        return gdp_fail(GDP_E_BADARG, "gdp_embed: a row stride is negative, too large, or below the width of rows that are written");
+    if (!aligned(e->grad, size_of(e->grad_type)) || !aligned(e->out, size_of(e->out_type)) ||
+        !aligned(e->tokens, e->token_type == GDP_I64 ? 8 : 4) || !aligned(e->workspace, 256))
+        return gdp_fail(GDP_E_BADARG, "gdp_embed: a pointer is not aligned to its elements, or the workspace not to 256 bytes");
+    const Layout l = layout_of(e->n, e->rows, e->dim);
+    if (e->workspace_bytes < l.bytes) return gdp_fail(GDP_E_BADARG, "gdp_embed: the workspace is smaller than gdp_embed_grad_workspace says");
+    char *const w = static_cast<char *>(e->workspace);
+    const auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(w + at); };
+    const Index x{e->n, e->first, e->rows, l.shift, (int32_t)l.per_group, ints(l.order), ints(l.row), ints(l.start), ints(l.count), ints(l.total)};
+    int rc = e->token_type == GDP_I64
+                 ? launch("gdp_embed_backward", embed_index_kernel<int64_t>, dim3(1u << l.shift), INDEX_THREADS, 0, stream, x, static_cast<const int64_t *>(e->tokens))
+                 : launch("gdp_embed_backward", embed_index_kernel<int32_t>, dim3(1u << l.shift), INDEX_THREADS, 0, stream, x, static_cast<const int32_t *>(e->tokens));
+    if (rc) return rc;
+    const int n = elements_at_once(e->dim, row_alignment(e->grad, e->grad_stride, e->grad_type), size_of(e->grad_type),
+                                   row_alignment(e->out, e->out_stride, e->out_type), size_of(e->out_type));
+    const Sum s{x, e->dim, l.piece, (int32_t)l.pieces, unit_of(e->dim, n), e->accumulate, e->scale, e->grad_stride, e->out_stride,
+                reinterpret_cast<float *>(w + l.partial)};
+    const int64_t across = ceil_div(e->dim, (int64_t)s.unit * n), per = THREADS / s.unit;
+    const int64_t units = l.pieces + (e->accumulate ? 0 : ceil_div(e->rows, (int64_t)FILL_ROWS));
+    return with_type(e->grad_type, [&](auto T) {
+        return with_type(e->out_type, [&](auto O) {
+            return with_count(n, [&](auto N) {
+                using TT = decltype(T);
+                using OO = decltype(O);
+                auto *const out = static_cast<typename OO::raw *>(e->out);
+                const int rc = launch("gdp_embed_backward", embed_sum_kernel<TT, OO, N.value>, dim3((unsigned)ceil_div(units, per), (unsigned)across), THREADS, 0,
+                                      stream, s, static_cast<const typename TT::raw *>(e->grad), out);
+                if (rc || l.pieces < 2) return rc;
+                return launch("gdp_embed_backward", embed_join_kernel<OO, N.value>, dim3((unsigned)ceil_div(l.pieces, per), (unsigned)across), THREADS, 0, stream, s, out);
+            });
+        });
+    });
+}
