@@ -23,6 +23,8 @@ using namespace ops;
 constexpr int INDEX_WAVES = 16, INDEX_THREADS = 64 * INDEX_WAVES;
 constexpr int INDEX_ROWS = 512;     // rows of a workgroup: a counter for each of them and each wave is 32 KB of LDS
 constexpr int INDEX_AHEAD = 8;      // reads of tokens in flight for each lane
+constexpr int INDEX_FOUND = 320;    // places of a wave that LDS keeps between counting and writing: 40 KB
+constexpr uint32_t NONE = ~0u;      // a token without a row
 constexpr int THREADS = 256;
 constexpr int FILL_ROWS = 16;       // rows that a unit of threads looks at for zeros
 
@@ -42,30 +44,43 @@ struct Index {
 template <typename I> __global__ __launch_bounds__(INDEX_THREADS) void embed_index_kernel(Index x, const I *__restrict__ tokens)
 {
     __shared__ int32_t count[INDEX_WAVES][INDEX_ROWS];
+    __shared__ uint2 found[INDEX_WAVES][INDEX_FOUND];   // place and row of a wave's first tokens that are the workgroup's
     __shared__ int32_t sums[INDEX_WAVES], before[INDEX_WAVES];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63, group = blockIdx.x, mask = (1 << x.shift) - 1;
     for (int i = t; i < INDEX_WAVES * INDEX_ROWS; i += INDEX_THREADS) (&count[0][0])[i] = 0;
     __syncthreads();
     // A wave's tokens follow each other, so that its places are in order if it takes them in order.
-    const int64_t each = (x.n + INDEX_THREADS - 1) / INDEX_THREADS * 64;
-    const int64_t from = wave * each, to = from + each < x.n ? from + each : x.n;
-    const auto row_of = [&](int64_t i) -> int64_t {   // or -1
-        if (i >= to) return -1;
+    const int n = (int)x.n, each = (n + INDEX_THREADS - 1) / INDEX_THREADS * 64;
+    const int from = min(wave * each, n), to = min(from + each, n);
+    const uint32_t rows = (uint32_t)x.rows;
+    const auto row_of = [&](int i) -> uint32_t {   // or NONE
         const int64_t r = (int64_t)tokens[i] - x.first;
-        return r >= 0 && r < x.rows ? r : -1;
+        return (uint64_t)r < rows ? (uint32_t)r : NONE;
     };
-    uint32_t lower = 0;
-    for (int64_t at = from; at < to; at += 64 * INDEX_AHEAD) {
-        int64_t r[INDEX_AHEAD];
+    const uint64_t below = (1ull << lane) - 1;
+    uint32_t lower = 0, n_found = 0;
+    for (int at = from; at < to; at += 64 * INDEX_AHEAD) {
+        uint32_t r[INDEX_AHEAD];
 #pragma unroll
-        for (int j = 0; j < INDEX_AHEAD; ++j) r[j] = row_of(at + 64 * j + lane);
+        for (int j = 0; j < INDEX_AHEAD; ++j) {
+            const int i = at + 64 * j + lane;
+            r[j] = row_of(min(i, n - 1));
+            if (i >= to) r[j] = NONE;
+        }
 #pragma unroll
-        for (int j = 0; j < INDEX_AHEAD; ++j)
-            if (r[j] >= 0) {
-                const int of = (int)(r[j] & mask);
-                lower += of < group;
-                if (of == group) atomicAdd(&count[wave][r[j] >> x.shift], 1);
+        for (int j = 0; j < INDEX_AHEAD; ++j) {
+            const int of = r[j] == NONE ? INT32_MAX : (int)(r[j] & mask);
+            lower += of < group;
+            const uint64_t mine = __ballot(of == group);
+            if (mine) {
+                if (of == group) {
+                    atomicAdd(&count[wave][r[j] >> x.shift], 1);
+                    const uint32_t place = n_found + (uint32_t)__popcll(mine & below);
+                    if (place < INDEX_FOUND) found[wave][place] = make_uint2((uint32_t)(at + 64 * j + lane), r[j]);
+                }
+                n_found += (uint32_t)__popcll(mine);
             }
+        }
     }
     lower = wave_sum(lower);
     if (lane == 0) before[wave] = (int32_t)lower;
@@ -95,29 +110,40 @@ template <typename I> __global__ __launch_bounds__(INDEX_THREADS) void embed_ind
     }
     if (group == mask && t == INDEX_THREADS - 1) *x.total = begin + of_row;   // (rows beyond per_group have no places)
     __syncthreads();
-    for (int64_t at = from; at < to; at += 64 * INDEX_AHEAD) {
-        int64_t r[INDEX_AHEAD];
+    const auto put = [&](uint32_t place, uint32_t row, bool mine) {
+        const int local = mine ? (int)(row >> x.shift) : -1;
+        uint64_t left = __ballot(mine);
+        while (left) {   // one row at a time, of frequent tokens most often the only one
+            const int leader = __builtin_ctzll(left);
+            const int one = __builtin_amdgcn_readlane(local, leader);
+            const uint64_t same = __ballot(local == one);
+            int32_t to_place = 0;
+            if (lane == leader) to_place = atomicAdd(&count[wave][one], (int)__popcll(same));
+            to_place = __builtin_amdgcn_readlane(to_place, leader);
+            if (local == one) {
+                to_place += (int)__popcll(same & below);
+                x.order[to_place] = (int32_t)place;
+                x.row[to_place] = (int32_t)row;
+            }
+            left &= ~same;
+        }
+    };
+    if (n_found <= INDEX_FOUND) {
+        for (uint32_t i = 0; i < n_found; i += 64) {
+            const bool mine = i + lane < n_found;
+            const uint2 f = mine ? found[wave][i + lane] : make_uint2(0, 0);
+            put(f.x, f.y, mine);
+        }
+        return;
+    }
+    for (int at = from; at < to; at += 64 * INDEX_AHEAD) {   // too many to be kept: look at all of them again
+        uint32_t r[INDEX_AHEAD];
 #pragma unroll
-        for (int j = 0; j < INDEX_AHEAD; ++j) r[j] = row_of(at + 64 * j + lane);
+        for (int j = 0; j < INDEX_AHEAD; ++j) r[j] = row_of(min(at + 64 * j + lane, n - 1));
 #pragma unroll
         for (int j = 0; j < INDEX_AHEAD; ++j) {
-            const bool mine = r[j] >= 0 && (int)(r[j] & mask) == group;
-            const int local = mine ? (int)(r[j] >> x.shift) : -1;
-            uint64_t left = __ballot(mine);
-            while (left) {   // one row at a time, most often the only one
-                const int leader = __builtin_ctzll(left);
-                const int row = __builtin_amdgcn_readlane(local, leader);
-                const uint64_t same = __ballot(local == row);
-                int32_t place = 0;
-                if (lane == leader) place = atomicAdd(&count[wave][row], (int)__popcll(same));
-                place = __builtin_amdgcn_readlane(place, leader);
-                if (local == row) {
-                    place += (int)__popcll(same & ((1ull << lane) - 1));
-                    x.order[place] = (int32_t)(at + 64 * j + lane);
-                    x.row[place] = (int32_t)r[j];
-                }
-                left &= ~same;
-            }
+            const int i = at + 64 * j + lane;
+            put((uint32_t)i, r[j], i < to && r[j] != NONE && (int)(r[j] & mask) == group);
         }
     }
 }
