@@ -93,6 +93,17 @@ template <typename T, int N> struct Pack {
                 reinterpret_cast<uint4 *>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
         }
     }
+    // ... of what is not read again soon: past the caches
+    __device__ __forceinline__ void store_past(typename T::raw *p) const
+    {
+        if constexpr (BYTES >= 16) {
+            typedef uint32_t Four __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i)
+                __builtin_nontemporal_store(Four{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]}, reinterpret_cast<Four *>(p) + i);
+        } else
+            store(p);
+    }
 };
 
 // One element of a type that is known at run time (weights, which are read once a workgroup).

@@ -26,7 +26,7 @@ constexpr int INDEX_AHEAD = 8;      // reads of tokens in flight for each lane
 constexpr int INDEX_FOUND = 320;    // places of a wave that LDS keeps between counting and writing: 40 KB
 constexpr uint32_t NONE = ~0u;      // a token without a row
 constexpr int THREADS = 256;
-constexpr int FILL_ROWS = 16;       // rows that a unit of threads looks at for zeros
+constexpr int FILL_ROWS = 64;       // rows that a unit of threads looks at for zeros
 
 // Row numbers and where they go.
 struct Index {
@@ -171,21 +171,33 @@ template <typename O, int N> __device__ __forceinline__ void put_row(const Sum &
     old.store(p);
 }
 
-template <typename T, typename O, int N>
+// WIDE: the threads that share a row are whole waves.  Then a wave's lanes read the numbers of 64 rows at once, which saves each row a
+// wait for them.
+template <typename T, typename O, int N, bool WIDE>
 __global__ __launch_bounds__(THREADS) void embed_sum_kernel(Sum s, const typename T::raw *__restrict__ grad, typename O::raw *__restrict__ out)
 {
     const Index &x = s.index;
+    const int lane = threadIdx.x & 63;
     const int64_t unit = (int64_t)blockIdx.x * (THREADS / s.unit) + threadIdx.x / s.unit;
     const int64_t col = ((int64_t)blockIdx.y * s.unit + threadIdx.x % s.unit) * N;
-    if (col >= s.dim) return;
+    const bool in = col < s.dim;
+    if (!WIDE && !in) return;
     if (unit >= s.pieces) {   // rows without places
         if (s.accumulate) return;
         const int64_t r0 = (unit - s.pieces) * FILL_ROWS;
         Pack<O, N> zeros;
         zeros.zero();
+        if constexpr (WIDE) {
+            uint64_t none = __ballot(r0 + lane < x.rows && x.count[x.slot(r0 + lane)] == 0);
+            while (none) {
+                if (in) zeros.store_past(out + (r0 + __builtin_ctzll(none)) * s.out_stride + col);
+                none &= none - 1;
+            }
+        } else {
 #pragma unroll 4
-        for (int i = 0; i < FILL_ROWS; ++i)
-            if (r0 + i < x.rows && x.count[x.slot(r0 + i)] == 0) zeros.store(out + (r0 + i) * s.out_stride + col);
+            for (int i = 0; i < FILL_ROWS; ++i)
+                if (r0 + i < x.rows && x.count[x.slot(r0 + i)] == 0) zeros.store_past(out + (r0 + i) * s.out_stride + col);
+        }
         return;
     }
     const int64_t total = *x.total, begin = unit * s.piece;
@@ -198,6 +210,7 @@ __global__ __launch_bounds__(THREADS) void embed_sum_kernel(Sum s, const typenam
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.0f;
     const auto put = [&](bool goes_on) {
+        if (!in) return;
         if (from_ahead || goes_on) {
             float *p = s.partial + (unit * 2 + (from_ahead ? 0 : 1)) * s.dim + col;
             Pack<F32, N> v;
@@ -207,14 +220,26 @@ __global__ __launch_bounds__(THREADS) void embed_sum_kernel(Sum s, const typenam
             put_row<O, N>(s, out, row, col, acc);
     };
     constexpr int AHEAD = 8;
+    int32_t rows_of = 0, places_of = 0;
     for (int64_t at = begin; at < end; at += AHEAD) {
+        if (WIDE && ((at - begin) & 63) == 0) {
+            const int64_t p = at + lane < end ? at + lane : end - 1;
+            rows_of = x.row[p], places_of = x.order[p];
+        }
         Pack<T, N> v[AHEAD];
         int32_t r[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            const int64_t p = at + j < end ? at + j : end - 1;
-            r[j] = x.row[p];
-            v[j].load(grad + x.order[p] * s.grad_stride + col);
+            int32_t place;
+            if constexpr (WIDE) {
+                const int of = (int)((at - begin) & 63) + j;
+                r[j] = __builtin_amdgcn_readlane(rows_of, of), place = __builtin_amdgcn_readlane(places_of, of);
+            } else {
+                const int64_t p = at + j < end ? at + j : end - 1;
+                r[j] = x.row[p], place = x.order[p];
+            }
+            v[j].zero();
+            if (in) v[j].load(grad + place * s.grad_stride + col);
         }
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
@@ -238,18 +263,20 @@ template <typename O, int N> __global__ __launch_bounds__(THREADS) void embed_jo
     const Index &x = s.index;
     const int64_t unit = (int64_t)blockIdx.x * (THREADS / s.unit) + threadIdx.x / s.unit;
     const int64_t col = ((int64_t)blockIdx.y * s.unit + threadIdx.x % s.unit) * N;
-    const int64_t total = *x.total, end = (unit + 1) * s.piece;
-    if (col >= s.dim || unit >= s.pieces || end >= total) return;
-    const int32_t row = x.row[end - 1];
+    const int64_t end = (unit + 1) * s.piece;
+    if (col >= s.dim || end >= x.n) return;
+    const int64_t total = *x.total;
+    const int32_t row = x.row[end - 1], next = x.row[end];   // (read together; behind `total` they are any number)
+    if (end >= total || row != next) return;
     const int64_t slot = x.slot(row), start = x.start[slot], stop = start + x.count[slot];
-    if (stop <= end || start < unit * s.piece) return;   // ends here, or began in a piece before: that one's
+    if (start < unit * s.piece) return;   // began in a piece before: that one's
     float acc[N];
     Pack<F32, N> v;
     v.load(reinterpret_cast<const F32::raw *>(s.partial + (unit * 2 + 1) * s.dim + col));
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = v[i];
     const int64_t last = (stop - 1) / s.piece;
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t u = unit + 1; u <= last; ++u) {
         Pack<F32, N> more;
         more.load(reinterpret_cast<const F32::raw *>(s.partial + u * 2 * s.dim + col));
@@ -456,8 +483,9 @@ extern "C" int gdp_embed_backward(const gdp_embed_grad *e, void *stream)
                 using TT = decltype(T);
                 using OO = decltype(O);
                 auto *const out = static_cast<typename OO::raw *>(e->out);
-                const int rc = launch("gdp_embed_backward", embed_sum_kernel<TT, OO, N.value>, dim3((unsigned)ceil_div(units, per), (unsigned)across), THREADS, 0,
-                                      stream, s, static_cast<const typename TT::raw *>(e->grad), out);
+                const int rc = launch("gdp_embed_backward", s.unit >= 64 ? embed_sum_kernel<TT, OO, N.value, true> : embed_sum_kernel<TT, OO, N.value, false>,
+                                      dim3((unsigned)ceil_div(units, per), (unsigned)across), THREADS, 0, stream, s,
+                                      static_cast<const typename TT::raw *>(e->grad), out);
                 if (rc || l.pieces < 2) return rc;
                 return launch("gdp_embed_backward", embed_join_kernel<OO, N.value>, dim3((unsigned)ceil_div(l.pieces, per), (unsigned)across), THREADS, 0, stream, s, out);
             });
