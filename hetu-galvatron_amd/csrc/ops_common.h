@@ -62,6 +62,19 @@ template <typename T, int N> struct Pack {
             }
         }
     }
+    // ... of what is not read again: past the caches
+    __device__ __forceinline__ void load_past(const typename T::raw *p)
+    {
+        if constexpr (BYTES >= 16) {
+            typedef uint32_t Four __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) {
+                const Four v = __builtin_nontemporal_load(reinterpret_cast<const Four *>(p) + i);
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+            }
+        } else
+            load(p);
+    }
     __device__ __forceinline__ void zero()
     {
 #pragma unroll
