@@ -223,7 +223,7 @@ __device__ __forceinline__ void rows_of(const Back &a, int group, int &from, int
 }
 
 template <typename T, typename S, int W, int K, int E>
-__global__ __launch_bounds__(64 * W) void norm_backward_kernel(Back a, const typename S::raw *__restrict__ stream, const typename T::raw *__restrict__ block,
+__global__ __launch_bounds__(64 * W, W <= 8 ? 4 : 1) void norm_backward_kernel(Back a, const typename S::raw *__restrict__ stream, const typename T::raw *__restrict__ block,
                                                                const typename T::raw *__restrict__ grad_normed, const typename S::raw *__restrict__ grad_stream,
                                                                typename S::raw *__restrict__ grad_residual, typename T::raw *__restrict__ grad_block)
 {
@@ -378,8 +378,7 @@ __global__ __launch_bounds__(64 * W) void norm_backward_kernel(Back a, const typ
 struct Add {
     const float *from;
     void *to;
-    int64_t rows;
-    int32_t type;
+    int32_t rows, groups, type;
 };
 struct Adds {
     Add of[COLUMNS];
@@ -392,12 +391,13 @@ __global__ __launch_bounds__(ADD_COLUMNS *ADD_ROWS) void norm_add_kernel(Adds a)
     const Add &o = a.of[blockIdx.z];
     const int c = threadIdx.x % ADD_COLUMNS, q = threadIdx.x / ADD_COLUMNS;
     const int64_t col = (int64_t)blockIdx.x * ADD_COLUMNS + c, group = blockIdx.y;
+    if (group >= o.groups) return;
     float sum = 0.0f;
     if (col < a.dim) {
         const float *p = o.from + group * o.rows * a.dim + col;
-        const int64_t each = (o.rows + ADD_ROWS - 1) / ADD_ROWS, from = q * each, to = min(from + each, o.rows);
+        const int each = (o.rows + ADD_ROWS - 1) / ADD_ROWS, from = q * each, to = min(from + each, o.rows);
 #pragma unroll 8
-        for (int64_t r = from; r < to; ++r) sum += p[r * a.dim];
+        for (int r = from; r < to; ++r) sum += p[r * a.dim];
     }
     part[q][c] = sum;
     __syncthreads();
@@ -581,25 +581,21 @@ extern "C" int gdp_norm_backward(const gdp_norm_grad *p, void *queue)
            side_of(p->post), side_of(p->pre), p->residual_scale, p->block_scale, 1.0f / (float)p->dim, p->stream_stride, p->block_stride, p->grad_normed_stride,
            p->grad_stream_stride, p->gate_stride, p->grad_residual_stride, p->grad_block_stride, p->gate, reinterpret_cast<const float4 *>(p->stats),
            static_cast<float *>(p->workspace), {}, nullptr};
-    // Sums over all rows, and those over the rows of each of several gates.
-    Adds adds{}, of_gates{};
-    adds.dim = of_gates.dim = p->dim;
+    Adds adds{};
+    adds.dim = p->dim;
     void *const outs[COLUMNS] = {p->grad_pre_weight, p->grad_pre_bias, p->grad_post_weight, p->grad_post_bias, p->grad_gate};
     const int types[COLUMNS] = {p->pre.type, p->pre.type, p->post.type, p->post.type, p->gate_type};
-    unsigned count = 0, places = 0;
-    bool several = false;
+    unsigned count = 0, most = 1;
     for (int c = 0; c < COLUMNS; ++c) {
         if (!outs[c]) continue;
-        if (c == GATE && gates > 1 && !shares.split_gates && p->n) {
+        const bool several = c == GATE && gates > 1;   // a sum for each gate, not one over all rows
+        if (several && !shares.split_gates && p->n) {
             b.grad_gate = outs[c];
             continue;
         }
-        b.of[c] = b.partial + (int64_t)places++ * shares.groups * p->dim;
-        if (c == GATE && gates > 1) {
-            of_gates.of[0] = {b.of[c], outs[c], shares.per_group, types[c]};
-            several = true;
-        } else
-            adds.of[count++] = {b.of[c], outs[c], shares.groups, types[c]};
+        b.of[c] = b.partial + (int64_t)count * shares.groups * p->dim;
+        adds.of[count++] = {b.of[c], outs[c], (int32_t)(several ? shares.per_group : shares.groups), (int32_t)(several ? gates : 1), types[c]};
+        if (several) most = (unsigned)gates;
     }
     const int rc = p->n == 0 ? GDP_OK : with_types(p->type, p->stream_type, [&](auto T, auto S) {
         using TT = decltype(T);
@@ -615,8 +611,5 @@ extern "C" int gdp_norm_backward(const gdp_norm_grad *p, void *queue)
     });
     if (rc) return rc;
     const unsigned across = (unsigned)ceil_div(p->dim, (int64_t)ADD_COLUMNS);
-    if (count)
-        if (const int rc2 = launch("gdp_norm_backward", norm_add_kernel, dim3(across, 1, count), ADD_COLUMNS * ADD_ROWS, 0, queue, adds)) return rc2;
-    if (!several) return GDP_OK;
-    return launch("gdp_norm_backward", norm_add_kernel, dim3(across, (unsigned)gates, 1), ADD_COLUMNS * ADD_ROWS, 0, queue, of_gates);
+    return count ? launch("gdp_norm_backward", norm_add_kernel, dim3(across, most, count), ADD_COLUMNS * ADD_ROWS, 0, queue, adds) : GDP_OK;
 }
