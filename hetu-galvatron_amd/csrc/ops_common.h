@@ -177,6 +177,10 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v)
 {
     return wave_fold(v, 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
+__device__ __forceinline__ uint32_t wave_min(uint32_t v)
+{
+    return wave_fold(v, ~0u, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
 __device__ __forceinline__ uint32_t wave_sum(uint32_t v)
 {
     return wave_fold(v, 0u, [](uint32_t a, uint32_t b) { return a + b; });

@@ -5,9 +5,11 @@
 // f = 2^(c (m - m')) and makes t f (t + c (m - m') s).  Then lse = scale * m + ln s and, since ln p = d ln 2 - ln s,
 // entropy = ln s - ln 2 * t / s: two terms of one sign, nothing cancels.
 //
-// The most likely tokens cost the pass one write to LDS for each quad of lanes: the largest logit of each chunk of 64 bytes.
-// The k largest logits lie in the k chunks that come first by (largest logit, then number): if one lay in another chunk, k
-// chunks would each hold a logit that comes before it.  So k chunks are read again, whatever the logits are.
+// The most likely tokens cost the pass one write to LDS for each quad of lanes: the largest logit of each chunk of 64 bytes.  Of the
+// largest logits that the 128 pairs of lanes have seen, the k-th largest is a bound: k logits reach it, so only chunks that do are
+// read again, 22 for k = 20 where logits differ.  Where they do not (a row of equal logits, or with less than k that are not ruled
+// out) the bound leaves too many; then the k chunks that come first by (largest logit, then number) are taken one by one: if one
+// of the k largest logits lay in another chunk, k chunks would each hold a logit that comes before it.
 //
 // A row is one workgroup, or, where there are few rows, several workgroups of a slice each, whose results a second kernel joins; the
 // same kernel joins the shards of a vocabulary.
@@ -18,9 +20,11 @@
 namespace {
 using namespace ops;
 
-constexpr int THREADS = 256, WAVES = THREADS / 64;
+constexpr int THREADS = 256, WAVES = THREADS / 64, PAIRS = THREADS / 2;
 constexpr int AHEAD = 4;                 // reads of 16 bytes in flight for each thread
 constexpr int MOST_CHUNKS = 8192;        // of a slice whose largest logits are asked for: 33 KB of LDS
+constexpr int MOST_CHOSEN = 128;         // chunks that are read again together (by the bound), 64 where they are taken one by one
+static_assert(MOST_CHOSEN >= GDP_MAX_TOP && PAIRS == 128 && PAIRS >= GDP_MAX_TOP, "taken one by one; two pairs for each lane");
 constexpr int MOST_SLICES = 64;          // a lane of the joining wave for each
 // Below it lse holds no digit of ln s worth having: such a row is one whose every token a mask rules out (by -inf, -1e9 or a type's
 // lowest value), and 2^(z - lse) would be 1 for each of them.
@@ -73,6 +77,7 @@ struct Scan {
     int32_t token_type, top, slices;
     int32_t width;       // vectors of a slice, a multiple of 4
     int32_t per_super;   // chunks of a super, odd
+    int32_t most_chosen; // chunks that the bound may leave
     float scale, c;
     const void *tokens;
     Out out;
@@ -94,10 +99,11 @@ __device__ __forceinline__ float top_logp(float x, float m, float s, float scale
 
 template <typename T, bool TOP> __global__ __launch_bounds__(THREADS) void logprob_scan_kernel(Scan a, const typename T::raw *__restrict__ logits)
 {
-    constexpr int VEC = T::VEC, CHUNK = 4 * VEC;
+    constexpr int VEC = T::VEC;
     extern __shared__ __align__(16) float chunk_max[];   // [64 * per_super], then their keys
     __shared__ Sums of_wave[WAVES];
-    __shared__ int32_t chosen[GDP_MAX_TOP], n_chosen, n_found;
+    __shared__ int32_t chosen[MOST_CHOSEN], n_chosen, n_found;
+    __shared__ __align__(16) uint32_t of_pair[PAIRS];
     __shared__ uint32_t least;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t row = blockIdx.x / a.slices;
@@ -139,15 +145,22 @@ template <typename T, bool TOP> __global__ __launch_bounds__(THREADS) void logpr
         }
         own = rescaled(own, most, c);
         const float from = finite_or_0(most);   // (subtracted first: a row may hold a type's lowest value alone)
+        float sum = 0.0f, sum_t = 0.0f;         // of these reads: a row's sums then are of few terms each
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float d = (p[u][i] - from) * c, e = exp2_fast(d);
-                own.s += e;
-                own.t = fmaf(e, fmaxf(d, -1e4f), own.t);   // 2^-inf * -inf would be NaN; below -1e4 the product is 0
+                sum += e;
+                sum_t = fmaf(e, fmaxf(d, -1e4f), sum_t);   // 2^-inf * -inf would be NaN; below -1e4 the product is 0
             }
         }
+        own.s += sum, own.t += sum_t;
+    }
+    if constexpr (TOP) {
+        const float b = fmaxf(own.m, dpp<QUAD_SWAP1>(own.m, own.m));
+        if ((t & 1) == 0) of_pair[t >> 1] = key_of(b);
+        if (t == 0) n_chosen = n_found = 0;
     }
     own = wave_join(own, c);
     if (lane == 0) of_wave[wave] = own;
@@ -174,57 +187,96 @@ template <typename T, bool TOP> __global__ __launch_bounds__(THREADS) void logpr
     }
     if constexpr (TOP) {
         const int chunks = v1 > v0 ? (v1 - v0 + 3) / 4 : 0, per = a.per_super;
-        uint32_t *const key = reinterpret_cast<uint32_t *>(chunk_max);
-        for (int i = t; i < 64 * per; i += THREADS) key[i] = i < chunks ? key_of(chunk_max[i]) : 0u;
-        if (t == 0) n_found = 0;
+        // The bound, in each wave: the least of the pairs' largest logits that fewer than `top` exceed.  (What follows runs once: it is
+        // kept in loops of few instructions, which are fetched sooner than unrolled ones.)
+        uint32_t bound;
+        {
+            const uint32_t one = of_pair[lane], other = of_pair[64 + lane];
+            const uint4 *const pairs = reinterpret_cast<const uint4 *>(of_pair);
+            int of_one = 0, of_other = 0;
+#pragma unroll 4
+            for (int i = 0; i < PAIRS / 4; ++i) {
+                const uint4 q = pairs[i];
+                of_one += (q.x > one) + (q.y > one) + (q.z > one) + (q.w > one);
+                of_other += (q.x > other) + (q.y > other) + (q.z > other) + (q.w > other);
+            }
+            bound = wave_min(min(of_one < a.top ? one : ~0u, of_other < a.top ? other : ~0u));
+        }
+#pragma unroll 1
+        for (int i = t; i < chunks; i += THREADS)
+            if (key_of(chunk_max[i]) >= bound) {
+                const int at_list = atomicAdd(&n_chosen, 1);
+                if (at_list < a.most_chosen) chosen[at_list] = i;
+            }
         __syncthreads();
-        if (wave == 0) {
-            // A lane has `per` neighbouring chunks, a super; their number is odd, so that lanes read from different banks.
-            uint32_t best = 0;
-            for (int i = 0; i < per; ++i) best = max(best, key[lane * per + i]);
-            int count = 0;
-            uint32_t last = 0;
-            for (; count < a.top; ++count) {
-                const uint32_t most = wave_max(best);
-                if (most == 0) break;
-                last = most;
-                const int super = __builtin_ctzll(__ballot(best == most));
-                uint32_t rest = 0;
-                bool taken = false;
-                for (int i = 0; i < per; i += 64) {
-                    const int at_key = super * per + i + lane;
-                    uint32_t k = i + lane < per ? key[at_key] : 0u;
-                    if (!taken) {
-                        const uint64_t equal = __ballot(k == most);
-                        if (equal) {
-                            taken = true;
-                            const int w = __builtin_ctzll(equal);
-                            if (lane == w) {
-                                k = 0;
-                                key[at_key] = 0;
-                                chosen[count] = super * per + i + w;
+        if (n_chosen > a.most_chosen) {
+            uint32_t *const key = reinterpret_cast<uint32_t *>(chunk_max);
+            for (int i = t; i < 64 * per; i += THREADS) key[i] = i < chunks ? key_of(chunk_max[i]) : 0u;
+            __syncthreads();
+            if (wave == 0) {
+                // A lane has `per` neighbouring chunks, a super; their number is odd, so that lanes read from different banks.
+                uint32_t best = 0;
+                for (int i = 0; i < per; ++i) best = max(best, key[lane * per + i]);
+                int count = 0;
+                uint32_t last = 0;
+                for (; count < a.top; ++count) {
+                    const uint32_t most = wave_max(best);
+                    if (most == 0) break;
+                    last = most;
+                    const int super = __builtin_ctzll(__ballot(best == most));
+                    uint32_t rest = 0;
+                    bool taken = false;
+                    for (int i = 0; i < per; i += 64) {
+                        const int at_key = super * per + i + lane;
+                        uint32_t k = i + lane < per ? key[at_key] : 0u;
+                        if (!taken) {
+                            const uint64_t equal = __ballot(k == most);
+                            if (equal) {
+                                taken = true;
+                                const int w = __builtin_ctzll(equal);
+                                if (lane == w) {
+                                    k = 0;
+                                    key[at_key] = 0;
+                                    chosen[count] = super * per + i + w;
+                                }
                             }
                         }
+                        rest = max(rest, k);
                     }
-                    rest = max(rest, k);
+                    rest = wave_max(rest);
+                    if (lane == super) best = rest;
                 }
-                rest = wave_max(rest);
-                if (lane == super) best = rest;
+                if (lane == 0) {
+                    n_chosen = count;
+                    least = count == a.top ? last : 0u;   // top chunks have a logit of this or more each
+                }
             }
-            if (lane == 0) {
-                n_chosen = count;
-                least = count == a.top ? last : 0u;   // top chunks have a logit of this or more each
-            }
+            __syncthreads();
+            bound = least;
         }
-        __syncthreads();
-        // Their logits that can be among the first, in any order; the keys of the chunks are not needed any more.
+        // Their logits that can be among the first, in any order; the largest logits of the chunks are not needed any more.
         uint64_t *const found = reinterpret_cast<uint64_t *>(chunk_max);
-        const int elements = n_chosen * CHUNK;
-        for (int i = t; i < elements; i += THREADS) {
-            const int j = (v0 + 4 * chosen[i / CHUNK]) * VEC + i % CHUNK - off;
-            if (j >= 0 && j < vocab) {
-                const uint32_t k = key_of(T::up(x[j]));
-                if (k >= least) found[atomicAdd(&n_found, 1)] = (uint64_t)k << 32 | (uint32_t)~j;
+#pragma unroll 1
+        for (int i = t; i < n_chosen * 4; i += THREADS) {
+            const int v = v0 + 4 * chosen[i >> 2] + (i & 3), j = v * VEC - off;
+            uint32_t k[VEC];
+            int count = 0;
+            if (j >= 0 && j + VEC <= vocab) {
+                Pack<T, VEC> p;
+                p.load(x + j);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) k[e] = key_of(p[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) k[e] = j + e >= 0 && j + e < vocab ? key_of(T::up(x[j + e])) : 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) count += k[e] != 0 && k[e] >= bound;   // (the bound is 0 where there are fewer than `top`)
+            if (count) {
+                int to = atomicAdd(&n_found, count);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (k[e] != 0 && k[e] >= bound) found[to++] = (uint64_t)k[e] << 32 | (uint32_t)~(j + e);
             }
         }
         __syncthreads();
@@ -232,6 +284,7 @@ template <typename T, bool TOP> __global__ __launch_bounds__(THREADS) void logpr
         for (int i = t; i < n; i += THREADS) {
             const uint64_t one = found[i];
             int place = 0;
+#pragma unroll 8
             for (int j = 0; j < n; ++j) place += found[j] > one;
             if (place < a.top) {
                 const float logit = of_key((uint32_t)(one >> 32));
@@ -255,7 +308,7 @@ template <typename T, bool TOP> __global__ __launch_bounds__(THREADS) void logpr
 
 struct Join {
     int64_t n, whole;
-    int32_t parts, top, token_type;
+    int32_t parts, top, first, token_type;   // `first` of each list for the bound
     float scale, c;
     const void *tokens;
     Part in;
@@ -263,12 +316,17 @@ struct Join {
     Part part;   // written instead of out where its stats are not null: slices of a shard
 };
 
-// A wave joins a row: a lane for each part.  The lists of the most likely tokens are merged from their heads; parts follow each other
-// as their tokens do, so that of equal logits the first lane's has the lowest number.
-__global__ __launch_bounds__(64) void logprob_join_kernel(Join a)
+// A workgroup joins a row: a lane of each wave for each part.  Of the lists of the most likely tokens, which are sorted, the first
+// few of each, twice as many as are asked for in all, give a bound that `top` of them reach: what does not reach it is left out, and
+// what does finds its place by looking at all that do.
+static_assert(GDP_MAX_TOP <= 64 && MOST_SLICES <= 64, "a lane for each");
+constexpr int JOIN_THREADS = 256;
+__global__ __launch_bounds__(JOIN_THREADS) void logprob_join_kernel(Join a)
 {
-    extern __shared__ __align__(16) uint64_t heads[];   // [parts][top]
-    const int lane = threadIdx.x;
+    extern __shared__ __align__(16) uint64_t lists[];   // [parts][top], then the first of each, and later those that reach the bound
+    __shared__ unsigned long long bound;
+    __shared__ int32_t n_found;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, waves = blockDim.x >> 6;
     const int64_t row = blockIdx.x;
     Sums own{-__builtin_inff(), 0.0f, 0.0f};
     float x = -__builtin_inff();
@@ -277,14 +335,21 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(Join a)
         own = {s.x, s.y, s.z};
         x = s.w;
     }
-    for (int i = lane; i < a.parts * a.top; i += 64) {
-        const int64_t from = ((int64_t)(i / a.top) * a.n + row) * a.top + i % a.top;
-        const int32_t token = a.in.tokens[from];
-        heads[i] = token < 0 ? 0 : (uint64_t)key_of(a.in.logits[from]) << 32 | (uint32_t)token;
-    }
+    uint64_t *const found = lists + a.parts * a.top;
+    const int first = a.first, some = first * a.parts;
+    if (lane < a.top)   // (GDP_MAX_TOP lanes: one for each place of a list)
+#pragma unroll 4
+        for (int p = wave; p < a.parts; p += waves) {
+            const int64_t from = ((int64_t)p * a.n + row) * a.top + lane;
+            const int32_t token = a.in.tokens[from];
+            const uint64_t one = token < 0 ? 0 : (uint64_t)key_of(a.in.logits[from]) << 32 | (uint32_t)~token;
+            lists[p * a.top + lane] = one;
+            if (lane < first) found[p * first + lane] = one;
+        }
+    if (t == 0) n_found = 0, bound = ~0ull;
     const Sums all = wave_join(own, a.c);
     x = wave_max(x);
-    if (lane == 0) {
+    if (t == 0) {
         if (a.part.stats)
             a.part.stats[row] = make_float4(all.m, all.s, all.t, x);
         else {
@@ -294,25 +359,40 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(Join a)
     }
     if (a.top == 0) return;
     __syncthreads();
-    int at = 0;
-    uint64_t head = lane < a.parts ? heads[lane * a.top] : 0;
-    for (int i = 0; i < a.top; ++i) {
-        const uint32_t most = wave_max((uint32_t)(head >> 32));
-        const int who = __builtin_ctzll(__ballot((uint32_t)(head >> 32) == most));   // (0 with no list left)
-        if (lane == who) {
-            const float logit = most ? of_key(most) : -__builtin_inff();
-            const int32_t token = most ? (int32_t)(uint32_t)head : -1;
-            if (a.part.stats) {
-                a.part.logits[row * a.top + i] = logit;
-                a.part.tokens[row * a.top + i] = token;
-            } else {
-                a.out.top_logp[row * a.top + i] = top_logp(logit, all.m, all.s, a.scale);
-                a.out.top_tokens[row * a.top + i] = token;
-            }
-            ++at;
-            head = at < a.top ? heads[lane * a.top + at] : 0;
-        }
+    for (int i = t; i < some; i += JOIN_THREADS) {   // the least that fewer than `top` exceed
+        const uint64_t one = found[i];
+        int larger = 0;
+#pragma unroll 8
+        for (int j = 0; j < some; ++j) larger += found[j] > one;
+        if (larger < a.top) atomicMin(&bound, (unsigned long long)one);
     }
+    __syncthreads();
+    const uint64_t least = bound;
+    if (lane < a.top)
+        for (int p = wave; p < a.parts; p += waves) {
+            const uint64_t one = lists[p * a.top + lane];
+            if (one != 0 && one >= least) found[atomicAdd(&n_found, 1)] = one;
+        }
+    __syncthreads();
+    const int n = n_found;
+    const float log_s = all.s == 0.0f ? 0.0f : logf(all.s);
+    const auto put = [&](int place, float logit, int32_t token) {
+        if (a.part.stats) {
+            a.part.logits[row * a.top + place] = logit;
+            a.part.tokens[row * a.top + place] = token;
+        } else {
+            a.out.top_logp[row * a.top + place] = all.s == 0.0f ? -__builtin_inff() : fmaf(logit - all.m, a.scale, -log_s);
+            a.out.top_tokens[row * a.top + place] = token;
+        }
+    };
+    for (int i = t; i < n; i += JOIN_THREADS) {
+        const uint64_t one = found[i];
+        int place = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) place += found[j] > one;
+        if (place < a.top) put(place, of_key((uint32_t)(one >> 32)), (int32_t)~(uint32_t)one);
+    }
+    for (int i = n + t; i < a.top; i += JOIN_THREADS) put(i, -__builtin_inff(), -1);   // parts of fewer tokens than are asked for
 }
 
 struct Grad {
@@ -408,8 +488,10 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(Grad a, const typ
 }
 
 // ---- host ----
-// How a row is shared out: enough workgroups to fill the device several times over, of 16 KB at least, and no more
-// chunks in a slice than LDS is laid out for.
+// How a row is shared out: slices of 512 vectors (8 KB) at least, 1024 workgroups, and no more chunks in a slice than LDS is laid out
+// for.  512 where alternatives are asked for: each slice then has some 5 us of work of its own.  128256 columns of bf16, top 0
+// / 20, with 512 and 1024 workgroups: 64 rows 7.8 / 16.8 and 7.6 / 20.1 us, 300 rows 22.0 / 35.1 and 19.2 / 32.1, 512 rows
+// 27.7 / 38.2 and 26.8 / 40.6.
 struct Split {
     int slices, width, per_super;
 };
@@ -418,7 +500,7 @@ Split split_of(int64_t n, int64_t vocab, int type, int top)
     const int vec = 16 / size_of(type);
     const int64_t vectors = ceil_div(vocab, (int64_t)vec) + 1;   // one more where a row begins within 16 bytes
     int64_t slices = 1;
-    while (slices < MOST_SLICES && n * slices < 2048 && vectors / (slices * 2) >= 1024) slices *= 2;
+    while (slices < MOST_SLICES && n * slices < (top ? 512 : 1024) && vectors / (slices * 2) >= 512) slices *= 2;
     if (top)
         while (slices < MOST_SLICES && ceil_div(vectors, slices) > 4 * MOST_CHUNKS) slices *= 2;
     const int64_t width = round_up((size_t)ceil_div(vectors, slices), 4);
@@ -472,7 +554,8 @@ int scan(Scan s, const void *logits, int type, const Split &split, const char *w
     s.slices = split.slices, s.width = split.width, s.per_super = split.per_super;
     s.c = s.scale * LOG2E;
     size_t lds = (size_t)64 * split.per_super * 4;
-    const size_t found = (size_t)s.top * 4 * (16 / size_of(type)) * 8;
+    s.most_chosen = s.top <= 24 ? MOST_CHOSEN / 2 : MOST_CHOSEN;   // (for 24 the bound leaves 27 chunks, for 64 it leaves 89; LDS for 64 lets 8 workgroups on a core)
+    const size_t found = (size_t)s.most_chosen * 4 * (16 / size_of(type)) * 8;
     if (lds < found) lds = found;
     return with_type(type, [&](auto T) {
         using TT = decltype(T);
@@ -482,9 +565,11 @@ int scan(Scan s, const void *logits, int type, const Split &split, const char *w
                      : launch(who, logprob_scan_kernel<TT, false>, grid, THREADS, 0, stream, s, x);
     });
 }
-int join(const Join &j, const char *who, void *stream)
+int join(Join j, const char *who, void *stream)
 {
-    return launch(who, logprob_join_kernel, dim3((unsigned)j.n), 64, (size_t)j.parts * j.top * 8, stream, j);
+    j.first = (2 * j.top + j.parts - 1) / j.parts;
+    if (j.first > j.top) j.first = j.top;
+    return launch(who, logprob_join_kernel, dim3((unsigned)j.n), j.top ? JOIN_THREADS : 64, (size_t)j.parts * j.top * 16, stream, j);
 }
 
 }  // namespace
@@ -511,13 +596,13 @@ extern "C" int gdp_logprob_forward(const gdp_logprob *l, void *stream)
     if (!l->logp || !l->lse || !l->entropy || (l->top && (!l->top_logp || !l->top_tokens))) return gdp_fail(GDP_E_BADARG, "gdp_logprob: null pointer");
     const Split split = split_of(l->n, l->vocab, l->logits_type, l->top);
     const Out out{l->logp, l->lse, l->entropy, l->top_logp, l->top_tokens};
-    Scan s{l->n, l->vocab, l->logits_stride, 0, l->vocab, l->token_type, l->top, 1, 0, 1, l->scale, 0.0f, l->tokens, out, {}};
+    Scan s{l->n, l->vocab, l->logits_stride, 0, l->vocab, l->token_type, l->top, 1, 0, 1, 0, l->scale, 0.0f, l->tokens, out, {}};
     if (split.slices == 1) return scan(s, l->logits, l->logits_type, split, "gdp_logprob_forward", stream);
     if (!aligned(l->workspace, 256) || !l->workspace || l->workspace_bytes < part_bytes(split.slices, l->n, l->top))
         return gdp_fail(GDP_E_BADARG, "gdp_logprob: the workspace is smaller than gdp_logprob_workspace says, or not aligned to 256 bytes");
     s.part = part_at(l->workspace, split.slices, l->n, l->top);
     if (const int rc = scan(s, l->logits, l->logits_type, split, "gdp_logprob_forward", stream)) return rc;
-    return join({l->n, l->vocab, split.slices, l->top, l->token_type, l->scale, l->scale * LOG2E, l->tokens, s.part, out, {}}, "gdp_logprob_forward", stream);
+    return join({l->n, l->vocab, split.slices, l->top, 0, l->token_type, l->scale, l->scale * LOG2E, l->tokens, s.part, out, {}}, "gdp_logprob_forward", stream);
 }
 
 extern "C" int gdp_logprob_parts(const gdp_logprob_part *l, void *stream)
@@ -532,13 +617,13 @@ extern "C" int gdp_logprob_parts(const gdp_logprob_part *l, void *stream)
         return gdp_fail(GDP_E_BADARG, "gdp_logprob: null pointer, or stats not aligned to 16 bytes");
     const Split split = split_of(l->n, l->vocab, l->logits_type, l->top);
     const Part own{reinterpret_cast<float4 *>(l->stats), l->top_logits, l->top_tokens};
-    Scan s{l->n, l->vocab, l->logits_stride, l->first, (int64_t)INT32_MAX, l->token_type, l->top, 1, 0, 1, l->scale, 0.0f, l->tokens, {}, own};
+    Scan s{l->n, l->vocab, l->logits_stride, l->first, (int64_t)INT32_MAX, l->token_type, l->top, 1, 0, 1, 0, l->scale, 0.0f, l->tokens, {}, own};
     if (split.slices == 1) return scan(s, l->logits, l->logits_type, split, "gdp_logprob_parts", stream);
     if (!aligned(l->workspace, 256) || !l->workspace || l->workspace_bytes < part_bytes(split.slices, l->n, l->top))
         return gdp_fail(GDP_E_BADARG, "gdp_logprob: the workspace is smaller than gdp_logprob_workspace says, or not aligned to 256 bytes");
     s.part = part_at(l->workspace, split.slices, l->n, l->top);
     if (const int rc = scan(s, l->logits, l->logits_type, split, "gdp_logprob_parts", stream)) return rc;
-    return join({l->n, (int64_t)INT32_MAX, split.slices, l->top, l->token_type, l->scale, l->scale * LOG2E, l->tokens, s.part, {}, own}, "gdp_logprob_parts", stream);
+    return join({l->n, (int64_t)INT32_MAX, split.slices, l->top, 0, l->token_type, l->scale, l->scale * LOG2E, l->tokens, s.part, {}, own}, "gdp_logprob_parts", stream);
 }
 
 extern "C" int gdp_logprob_join(const gdp_logprob_joint *l, void *stream)
@@ -556,7 +641,7 @@ extern "C" int gdp_logprob_join(const gdp_logprob_joint *l, void *stream)
     if (!aligned(l->stats, 16) || !aligned(l->tokens, l->token_type == GDP_I64 ? 8 : 4))
         return gdp_fail(GDP_E_BADARG, "gdp_logprob: stats not aligned to 16 bytes, or tokens not to their elements");
     const Part in{reinterpret_cast<float4 *>(const_cast<float *>(l->stats)), const_cast<float *>(l->top_logits), const_cast<int32_t *>(l->top_tokens)};
-    return join({l->n, l->vocab, l->parts, l->top, l->token_type, l->scale, l->scale * LOG2E, l->tokens, in, {l->logp, l->lse, l->entropy, l->top_logp, l->out_tokens}, {}},
+    return join({l->n, l->vocab, l->parts, l->top, 0, l->token_type, l->scale, l->scale * LOG2E, l->tokens, in, {l->logp, l->lse, l->entropy, l->top_logp, l->out_tokens}, {}},
                 "gdp_logprob_join", stream);
 }
 
