@@ -18,6 +18,7 @@ There is no CPU path: tensors have to be on a HIP device.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -131,10 +132,15 @@ def _ops() -> ctypes.CDLL:
     return _bound
 
 
+_stream_of = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
 def _queue(f, record, device) -> None:
     """Calls f(record, stream) on torch's current stream of the device."""
-    if device.index == torch.cuda.current_device():
-        rc = f(record, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        # (as an integer: building torch's stream object takes longer than the rest of a small call)
+        rc = f(record, _stream_of(index) if _stream_of else torch.cuda.current_stream().cuda_stream)
     else:
         with torch.cuda.device(device):
             rc = f(record, torch.cuda.current_stream().cuda_stream)
@@ -142,12 +148,19 @@ def _queue(f, record, device) -> None:
         _lib._check(rc)
 
 
-def _workspace(f, *sizes, device):
+@functools.lru_cache(maxsize=1024)
+def _bytes(name, *sizes):
+    """What a gdp_*_workspace function says, which goes by the sizes alone."""
     need = _size()
-    rc = f(*sizes, ctypes.byref(need))
+    rc = getattr(_ops(), name)(*sizes, ctypes.byref(need))
     if rc:
         _lib._check(rc)
-    return (torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None), need.value
+    return need.value
+
+
+def _workspace(name, *sizes, device):
+    need = _bytes(name, *sizes)
+    return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
 
 
 def _ptr(t):
@@ -170,10 +183,17 @@ def _same_device(device, **tensors):
             raise ValueError(f"{what} is on {t.device}, not on {device}")
 
 
+def _like(t):
+    """New memory of a tensor's shape and type, its rows in order."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _rows(t, dim, what):
     """[..., dim] as rows whose elements are neighbours, and the stride between them."""
     if t.dim() < 1 or t.shape[-1] != dim:
         raise ValueError(f"{what} must be [..., {dim}], not {list(t.shape)}")
+    if t.is_contiguous():
+        return t, dim
     if t.dim() != 2:
         t = t.reshape(-1, dim)
     if t.stride(1) != 1 and dim > 1:
@@ -270,7 +290,7 @@ def embedding_grad(tokens, grad, rows: int, *, scale: float = 1.0, first: int = 
     out_type = _type(out, "into")
     _same_device(device, tokens=tokens, into=out)
     L = _ops()
-    work, size = _workspace(L.gdp_embed_grad_workspace, n, rows, dim, device=device)
+    work, size = _workspace("gdp_embed_grad_workspace", n, rows, dim, device=device)
     _queue(L.gdp_embed_backward,
            gdp_embed_grad(n, rows, dim, first, flat.data_ptr(), token_type, grad_type, out_type, into is not None, scale,
                           grad.data_ptr(), stride, out.data_ptr(), out.stride(0) if rows else dim, _ptr(work), size), device)
@@ -308,10 +328,10 @@ def _check_top(top):
 
 def _outputs(shape, top, device):
     n = shape.numel()
-    three = torch.empty((3,) + shape, dtype=torch.float32, device=device)
+    logp, lse, entropy = torch.empty((3,) + shape, dtype=torch.float32, device=device).unbind()
     if not top:
-        return n, three[0], three[1], three[2], None, None
-    return (n, three[0], three[1], three[2], torch.empty(shape + (top,), dtype=torch.float32, device=device),
+        return n, logp, lse, entropy, None, None
+    return (n, logp, lse, entropy, torch.empty(shape + (top,), dtype=torch.float32, device=device),
             torch.empty(shape + (top,), dtype=torch.int64, device=device))
 
 
@@ -325,7 +345,7 @@ def _token_logprobs(logits, tokens, scale, top):
     n, logp, lse, entropy, top_logp, top_tokens = _outputs(shape, top, device)
     rows, stride = _rows(logits, vocab, "logits") if n and vocab else (logits, vocab)
     L = _ops()
-    work, size = _workspace(L.gdp_logprob_workspace, n, vocab, logits_type, top, device=device)
+    work, size = _workspace("gdp_logprob_workspace", n, vocab, logits_type, top, device=device)
     _queue(L.gdp_logprob_forward,
            gdp_logprob(n, vocab, rows.data_ptr(), stride, logits_type, token_type, flat.data_ptr(), scale, top,
                        logp.data_ptr(), lse.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_tokens), _ptr(work),
@@ -399,7 +419,7 @@ def token_logprobs_grad(logits, tokens, lse, grad_logp=None, *, scale: float = 1
         grad_top, top_tokens = _floats(grad_top, shape + (top,), "grad_top", device), top_tokens.contiguous()
     n = shape.numel()
     if into is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+        out = _like(logits)
     else:
         out = into
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != device:
@@ -434,7 +454,7 @@ def logprob_parts(logits, tokens, *, first: int, scale: float = 1.0, top: int = 
                          torch.empty(n, top, dtype=torch.float32, device=device),
                          torch.empty(n, top, dtype=torch.int32, device=device))
     L = _ops()
-    work, size = _workspace(L.gdp_logprob_workspace, n, columns, logits_type, top, device=device)
+    work, size = _workspace("gdp_logprob_workspace", n, columns, logits_type, top, device=device)
     _queue(L.gdp_logprob_parts,
            gdp_logprob_part(n, columns, first, rows.data_ptr(), stride, logits_type, token_type, flat.data_ptr(), scale, top,
                             parts.stats.data_ptr(), parts.top_logits.data_ptr(), parts.top_tokens.data_ptr(), _ptr(work),
@@ -476,7 +496,7 @@ class Norm(NamedTuple):
 class ResidualNorm(NamedTuple):
     stream: torch.Tensor                # residual_scale * residual + block_scale * gate * post(block)
     normed: Optional[torch.Tensor]      # pre(stream)
-    stats: torch.Tensor                 # [n, 4] float32: mean, 1 / deviation of post; of pre
+    stats: Optional[torch.Tensor]       # [n, 4] float32, where asked for: mean, 1 / deviation of post; of pre
 
 
 class ResidualNormGrads(NamedTuple):
@@ -489,24 +509,33 @@ class ResidualNormGrads(NamedTuple):
     gate: Optional[torch.Tensor]
 
 
+def _vector(t, dim, device, what):
+    """[dim] in order, and its type"""
+    code = _type(t, what)
+    if t.shape != (dim,):
+        raise ValueError(f"{what} must be {[dim]}, not {list(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, not on {device}")
+    return (t if t.is_contiguous() else t.contiguous()), code
+
+
 def _norm_params(norm, dim, device, what):
+    """The record of a norm, and what it points to."""
     if norm is None:
-        return gdp_norm_params(0, 0, 0.0, 0, None, None), None, None
-    form = _FORMS.get(norm.form)
-    if not form:
-        raise ValueError(f"{what}.form must be 'rms' or 'layer', not {norm.form!r}")
-    weight, bias, code = norm.weight, norm.bias, 0
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            code = _type(t, f"{what}.{name}")
-            if t.shape != (dim,):
-                raise ValueError(f"{what}.{name} must be {[dim]}, not {list(t.shape)}")
-            _same_device(device, **{f"{what}.{name}": t})
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError(f"{what}: weight and bias have to be of one type")
-    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    return gdp_norm_params(form, code, norm.eps, 0, _ptr(weight), _ptr(bias)), weight, bias
+        return gdp_norm_params(), None, None
+    form, weight, bias, eps = norm
+    number = _FORMS.get(form)
+    if not number:
+        raise ValueError(f"{what}.form must be 'rms' or 'layer', not {form!r}")
+    code = 0
+    if weight is not None:
+        weight, code = _vector(weight, dim, device, f"{what}.weight")
+    if bias is not None:
+        bias, of_bias = _vector(bias, dim, device, f"{what}.bias")
+        if weight is not None and of_bias != code:
+            raise ValueError(f"{what}: weight and bias have to be of one type")
+        code = of_bias
+    return gdp_norm_params(number, code, eps, 0, None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr()), weight, bias
 
 
 def _gate_rows(gate, dim, n, device):
@@ -514,14 +543,16 @@ def _gate_rows(gate, dim, n, device):
     if gate is None:
         return None, 0, 0, 0
     code = _type(gate, "gate")
-    _same_device(device, gate=gate)
+    if gate.device != device:
+        raise ValueError(f"gate is on {gate.device}, not on {device}")
     rows, stride = _rows(gate, dim, "gate")
-    if rows.shape[0] < 1 or n % rows.shape[0]:
-        raise ValueError(f"gate: {rows.shape[0]} gates do not divide {n} rows")
-    return rows, rows.shape[0], stride, code
+    count = gate.numel() // dim if dim else 0
+    if count < 1 or n % count:
+        raise ValueError(f"gate: {count} gates do not divide {n} rows")
+    return rows, count, stride, code
 
 
-def _residual_norm(residual, block, post, pre, gate, residual_scale, block_scale):
+def _residual_norm(residual, block, post, pre, gate, residual_scale, block_scale, with_stats):
     stream_type = _type(residual, "residual")
     if residual.dim() < 1:
         raise ValueError("residual must be [..., dim]")
@@ -535,22 +566,21 @@ def _residual_norm(residual, block, post, pre, gate, residual_scale, block_scale
     if block is None and pre is None:
         raise ValueError("nothing to do: neither a block nor a norm")
     code = _TYPES[kind] if block is None else _type(block, "block")
-    if block is not None and block.shape != shape:
-        raise ValueError(f"block must be {list(shape)}, not {list(block.shape)}")
-    _same_device(device, block=block)
+    if block is not None and (block.shape != shape or block.device != device):
+        raise ValueError(f"block must be {list(shape)} on {device}, not {list(block.shape)} on {block.device}")
     post_record, *keep_post = _norm_params(post, dim, device, "post")
     pre_record, *keep_pre = _norm_params(pre, dim, device, "pre")
     gates, count, gate_stride, gate_type = _gate_rows(gate, dim, n, device)
     r, r_stride = _rows(residual, dim, "residual") if n else (residual, dim)
     b, b_stride = (None, 0) if block is None else _rows(block, dim, "block") if n else (block, dim)
     same = block is None and residual_scale == 1.0
-    stream = residual if same else torch.empty(shape, dtype=residual.dtype, device=device)
-    normed = None if pre is None else torch.empty(shape, dtype=kind, device=device)
-    stats = torch.empty(n, 4, dtype=torch.float32, device=device)
+    stream = residual if same else _like(residual)
+    normed = None if pre is None else torch.empty(shape, dtype=kind, device=device) if block is None else _like(block)
+    stats = torch.empty((n, 4), dtype=torch.float32, device=device) if with_stats else None
     _queue(_ops().gdp_norm_forward,
            gdp_norm(n, dim, code, stream_type, r.data_ptr(), r_stride, _ptr(b), b_stride, post_record, pre_record,
                     _ptr(gates), count, gate_stride, gate_type, residual_scale, block_scale, 0,
-                    None if same else stream.data_ptr(), dim, _ptr(normed), dim, stats.data_ptr()), device)
+                    None if same else stream.data_ptr(), dim, _ptr(normed), dim, _ptr(stats)), device)
     return stream, normed, stats
 
 
@@ -590,13 +620,11 @@ def residual_norm_grad(stream, block, stats, grad_normed, grad_stream=None, *, p
     dh, dh_stride = rows(grad_normed, "grad_normed")
     ds, ds_stride = rows(grad_stream, "grad_stream")
 
-    def like(t):
-        return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=device)
-
-    got = ResidualNormGrads(torch.empty(shape, dtype=stream.dtype, device=device), like(block),
-                            *(like(t) for norm in (post, pre) for t in ((norm.weight, norm.bias) if norm else (None, None))), like(gate))
+    got = ResidualNormGrads(*[None if t is None else _like(t) for t in (
+        stream, block, *((post.weight, post.bias) if post else (None, None)),
+        *((pre.weight, pre.bias) if pre else (None, None)), gate)])
     L = _ops()
-    work, size = _workspace(L.gdp_norm_grad_workspace, n, dim, count, device=device)
+    work, size = _workspace("gdp_norm_grad_workspace", n, dim, count, device=device)
     _queue(L.gdp_norm_backward,
            gdp_norm_grad(n, dim, code, stream_type, s.data_ptr(), s_stride, _ptr(b), b_stride, stats.data_ptr(), _ptr(dh),
                          dh_stride, _ptr(ds), ds_stride, post_record, pre_record, _ptr(gates), count, gate_stride, gate_type,
@@ -612,7 +640,7 @@ class _ResidualNorm(torch.autograd.Function):
         # post and pre: (form, eps) or None
         post_norm = post and Norm(post[0], post_weight, post_bias, post[1])
         pre_norm = pre and Norm(pre[0], pre_weight, pre_bias, pre[1])
-        stream, normed, stats = _residual_norm(residual, block, post_norm, pre_norm, gate, residual_scale, block_scale)
+        stream, normed, stats = _residual_norm(residual, block, post_norm, pre_norm, gate, residual_scale, block_scale, True)
         ctx.save_for_backward(stream, block, stats, post_weight, post_bias, pre_weight, pre_bias, gate)
         ctx.given = (post, pre, residual_scale, block_scale)
         ctx.set_materialize_grads(False)
@@ -638,7 +666,7 @@ class _ResidualNorm(torch.autograd.Function):
 
 
 def residual_norm(residual, block=None, *, post: Optional[Norm] = None, pre: Optional[Norm] = None, gate=None,
-                  residual_scale: float = 1.0, block_scale: float = 1.0) -> ResidualNorm:
+                  residual_scale: float = 1.0, block_scale: float = 1.0, stats: bool = False) -> ResidualNorm:
     """Joins a block's output with the residual stream and norms the sum for the next block, in one pass:
 
         stream = residual_scale * residual + block_scale * gate * post(block)
@@ -647,11 +675,12 @@ def residual_norm(residual, block=None, *, post: Optional[Norm] = None, pre: Opt
     ``residual`` and ``block`` [..., dim]; ``post`` and ``pre`` are ``Norm`` or None (no norm), ``gate`` [dim], or [gates, dim]
     where a gate serves n / gates rows in turn (one for each sequence, or each row).  ``normed`` is of the block's type,
     ``stream`` of the residual's: the same, or float32.  Without a block (before the first one) ``normed`` is of the
-    stream's type, or of the norm's weight's if the stream is float32."""
+    stream's type, or of the norm's weight's if the stream is float32.  ``stats``: also what ``residual_norm_grad`` needs of
+    the two norms."""
     residual_scale, block_scale = float(residual_scale), float(block_scale)
     inputs = (residual, block, *((post.weight, post.bias) if post else (None, None)),
               *((pre.weight, pre.bias) if pre else (None, None)), gate)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in inputs]):
         return ResidualNorm(*_ResidualNorm.apply(*inputs, post and (post.form, post.eps), pre and (pre.form, pre.eps),
                                                  residual_scale, block_scale))
-    return ResidualNorm(*_residual_norm(residual, block, post, pre, gate, residual_scale, block_scale))
+    return ResidualNorm(*_residual_norm(residual, block, post, pre, gate, residual_scale, block_scale, stats))

@@ -393,7 +393,7 @@ def test_residual_norm_grad(case, with_stream):
     if pre is None and not with_stream:
         pytest.skip("no gradient at all")
     g, r, b, given = norm_inputs(case)
-    out = ops.residual_norm(r, b, **given)
+    out = ops.residual_norm(r, b, stats=True, **given)
     dh = normal(g, n, dim, dtype=dtype) if pre else None
     ds = normal(g, n, dim, dtype=stream) if with_stream else None
     got = ops.residual_norm_grad(out.stream, b, out.stats, dh, ds, **given)
@@ -407,7 +407,7 @@ def test_residual_norm_without_block_and_without_rows():
     r = normal(g, 3, 5, 96)
     pre = norm_of(g, "rms", 96, BF16)
     out = ops.residual_norm(r, pre=pre)
-    assert out.stream is r and out.normed.dtype == BF16
+    assert out.stream is r and out.normed.dtype == BF16 and out.stats is None
     ref = C.norm(r.cpu().double(), pre)[0]
     C.close(out.normed, ref, norm_bound(r.cpu().double(), pre, 0.0) + C.rounded(ref, BF16))
     halved = ops.residual_norm(r, pre=pre, residual_scale=0.5)
@@ -415,7 +415,7 @@ def test_residual_norm_without_block_and_without_rows():
     bare = ops.residual_norm(r, pre=ops.Norm("layer"))
     ref = C.norm(r.cpu().double(), ops.Norm("layer"))[0]
     C.close(bare.normed, ref, norm_bound(r.cpu().double(), ops.Norm("layer"), 0.0) + C.rounded(ref, F32))
-    empty = ops.residual_norm(r[:0], r[:0], pre=norm_of(g, "layer", 96, F32), gate=normal(g, 96))
+    empty = ops.residual_norm(r[:0], r[:0], stats=True, pre=norm_of(g, "layer", 96, F32), gate=normal(g, 96))
     assert empty.normed.shape == (0, 5, 96)
     given = dict(pre=norm_of(g, "layer", 96, F32), post=norm_of(g, "rms", 96, F32), gate=normal(g, 96))
     none = ops.residual_norm_grad(r[:0], r[:0], empty.stats, r[:0], r[:0], **given)
@@ -428,7 +428,7 @@ def test_residual_norm_strides():
     r, b = wide_r[:, 3:83], wide_b[:, 1:81]
     given = dict(post=norm_of(g, "rms", 80, BF16), pre=ops.Norm("layer", normal(g, 160)[::2], normal(g, 81)[1:]), gate=normal(g, 160)[::2],
                  residual_scale=0.9, block_scale=1.3)
-    got, same = ops.residual_norm(r, b, **given), ops.residual_norm(r.clone(), b.clone(), **given)
+    got, same = (ops.residual_norm(*x, stats=True, **given) for x in ((r, b), (r.clone(), b.clone())))
     assert all(torch.allclose(x.float(), y.float(), rtol=0.01, atol=1e-5) for x, y in zip(got, same))
     ref = C.residual_norm(r, b, given["post"], given["pre"], given["gate"], 0.9, 1.3)[1]
     assert (got.normed.cpu().double() - ref).abs().max() <= 2.0 ** -8 * ref.abs().max()
@@ -476,7 +476,7 @@ def test_together_on_another_stream_and_in_a_graph():
 
     def step():
         x = ops.embedding(t, w, scale=8.0)
-        out = ops.residual_norm(x, b, post=post, pre=pre, gate=gate)
+        out = ops.residual_norm(x, b, post=post, pre=pre, gate=gate, stats=True)
         logits = out.normed @ head
         r = ops.token_logprobs(logits, target, entropy=True, top=5)
         d = ops.token_logprobs_grad(logits, target, r.lse, torch.ones_like(r.lse) / n, entropy=r.entropy, grad_entropy=r.entropy)
