@@ -31,11 +31,27 @@ struct BF16 {
     static __device__ __forceinline__ raw down(float f) { return __builtin_bit_cast(raw, (__bf16)f); }
 };
 
-// N neighbouring elements, read and written at once: N * sizeof(raw) is 2, 4, 8, 16 or 32 bytes, and the address a multiple of
-// that, or of 16.
+// Words in memory that are aligned to an element only.
+template <int BYTES> struct Words;
+template <> struct Words<2> {
+    typedef uint32_t One __attribute__((aligned(2)));
+    typedef uint32_t Two __attribute__((ext_vector_type(2), aligned(2)));
+    typedef uint32_t Four __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <> struct Words<4> {
+    typedef uint32_t One __attribute__((aligned(4)));
+    typedef uint32_t Two __attribute__((ext_vector_type(2), aligned(4)));
+    typedef uint32_t Four __attribute__((ext_vector_type(4), aligned(4)));
+};
+
+// N neighbouring elements, read and written at once, wherever they begin: gfx950 takes addresses of any alignment, and a row that
+// begins between words costs a second cache line for some lanes, not a read for each element.
 template <typename T, int N> struct Pack {
     static constexpr int BYTES = N * (int)sizeof(typename T::raw);
     static constexpr int WORDS = BYTES >= 4 ? BYTES / 4 : 1;
+    using One = typename Words<sizeof(typename T::raw)>::One;
+    using Two = typename Words<sizeof(typename T::raw)>::Two;
+    using Four = typename Words<sizeof(typename T::raw)>::Four;
     uint32_t w[WORDS];
     __device__ __forceinline__ typename T::raw raw(int i) const
     {
@@ -50,14 +66,14 @@ template <typename T, int N> struct Pack {
         if constexpr (BYTES == 2)
             w[0] = *p;
         else if constexpr (BYTES == 4)
-            w[0] = *reinterpret_cast<const uint32_t *>(p);
+            w[0] = *reinterpret_cast<const One *>(p);
         else if constexpr (BYTES == 8) {
-            uint2 v = *reinterpret_cast<const uint2 *>(p);
+            const Two v = *reinterpret_cast<const Two *>(p);
             w[0] = v.x, w[1] = v.y;
         } else {
 #pragma unroll
             for (int i = 0; i < BYTES / 16; ++i) {
-                uint4 v = reinterpret_cast<const uint4 *>(p)[i];
+                const Four v = reinterpret_cast<const Four *>(p)[i];
                 w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
             }
         }
@@ -66,7 +82,6 @@ template <typename T, int N> struct Pack {
     __device__ __forceinline__ void load_past(const typename T::raw *p)
     {
         if constexpr (BYTES >= 16) {
-            typedef uint32_t Four __attribute__((ext_vector_type(4)));
 #pragma unroll
             for (int i = 0; i < BYTES / 16; ++i) {
                 const Four v = __builtin_nontemporal_load(reinterpret_cast<const Four *>(p) + i);
@@ -97,20 +112,28 @@ template <typename T, int N> struct Pack {
         if constexpr (BYTES == 2)
             *p = (typename T::raw)w[0];
         else if constexpr (BYTES == 4)
-            *reinterpret_cast<uint32_t *>(p) = w[0];
+            *reinterpret_cast<One *>(p) = w[0];
         else if constexpr (BYTES == 8)
-            *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<Two *>(p) = Two{w[0], w[1]};
         else {
 #pragma unroll
-            for (int i = 0; i < BYTES / 16; ++i)
-                reinterpret_cast<uint4 *>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<Four *>(p)[i] = Four{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
         }
+    }
+    // ... from element `from` on
+    __device__ __forceinline__ void store_from(typename T::raw *p, int from) const
+    {
+        if (from == 0)
+            store(p);
+        else
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i >= from) p[i] = raw(i);
     }
     // ... of what is not read again soon: past the caches
     __device__ __forceinline__ void store_past(typename T::raw *p) const
     {
         if constexpr (BYTES >= 16) {
-            typedef uint32_t Four __attribute__((ext_vector_type(4)));
 #pragma unroll
             for (int i = 0; i < BYTES / 16; ++i)
                 __builtin_nontemporal_store(Four{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]}, reinterpret_cast<Four *>(p) + i);
@@ -195,12 +218,6 @@ inline int size_of(int t) { return t == GDP_F32 ? 4 : 2; }
 inline bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 inline size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 template <typename I> inline I ceil_div(I a, I b) { return (a + b - 1) / b; }
-// Bytes that rows of `dim` elements start on, all of them: a power of two, 16 at most.
-inline int row_alignment(const void *p, int64_t stride, int type)
-{
-    const uint64_t bits = reinterpret_cast<uintptr_t>(p) | (uint64_t)(stride * size_of(type)) | 16;
-    return (int)(bits & (~bits + 1));
-}
 // Whether rows * stride + dim elements stay within what an offset in 64 bits can name, and rows do not overlap.
 inline bool rows_ok(int64_t rows, int64_t dim, int64_t stride, bool written)
 {

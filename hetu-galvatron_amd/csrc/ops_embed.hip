@@ -26,7 +26,8 @@ constexpr int INDEX_AHEAD = 8;      // reads of tokens in flight for each lane
 constexpr int INDEX_FOUND = 320;    // places of a wave that LDS keeps between counting and writing: 40 KB
 constexpr uint32_t NONE = ~0u;      // a token without a row
 constexpr int THREADS = 256;
-constexpr int FILL_ROWS = 64;       // rows that a unit of threads looks at for zeros
+// Rows that a unit of threads looks at for zeros: the lanes of a wave, or what a thread reads the counts of ahead.
+constexpr int fill_rows(bool wide) { return wide ? 64 : 8; }
 
 // Row numbers and where they go.
 struct Index {
@@ -159,16 +160,29 @@ struct Sum {
     float *partial;      // [pieces][2][dim]: of the row that began before the piece, of the one that goes on behind it
 };
 
-template <typename O, int N> __device__ __forceinline__ void put_row(const Sum &s, typename O::raw *out, int64_t row, int64_t col, const float (&acc)[N])
+// A thread's columns: N from `col` on.  Where N does not divide the width, the last thread takes the last N, some of which are
+// another's as well: both have the same sums for them.
+struct Columns {
+    int64_t col;
+    int others;   // of them, at the front
+    bool in;
+};
+template <int N> __device__ __forceinline__ Columns columns_of(int64_t dim, int unit)
 {
-    typename O::raw *p = out + row * s.out_stride + col;
+    const int64_t col = ((int64_t)blockIdx.y * unit + threadIdx.x % unit) * N;
+    return {col + N <= dim ? col : dim - N, col + N <= dim ? 0 : (int)(col + N - dim), col < dim};
+}
+
+template <typename O, int N> __device__ __forceinline__ void put_row(const Sum &s, typename O::raw *out, int64_t row, const Columns &at, const float (&acc)[N])
+{
+    typename O::raw *p = out + row * s.out_stride + at.col;
     float v[N];
     Pack<O, N> old;
     if (s.accumulate) old.load(p);
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = s.accumulate ? fmaf(acc[i], s.scale, old[i]) : acc[i] * s.scale;
     old.set(v);
-    old.store(p);
+    old.store_from(p, s.accumulate ? at.others : 0);   // (what is added to is added to once)
 }
 
 // WIDE: the threads that share a row are whole waves.  Then a wave's lanes read the numbers of 64 rows at once, which saves each row a
@@ -179,12 +193,13 @@ __global__ __launch_bounds__(THREADS) void embed_sum_kernel(Sum s, const typenam
     const Index &x = s.index;
     const int lane = threadIdx.x & 63;
     const int64_t unit = (int64_t)blockIdx.x * (THREADS / s.unit) + threadIdx.x / s.unit;
-    const int64_t col = ((int64_t)blockIdx.y * s.unit + threadIdx.x % s.unit) * N;
-    const bool in = col < s.dim;
+    const Columns at_columns = columns_of<N>(s.dim, s.unit);
+    const int64_t col = at_columns.col;
+    const bool in = at_columns.in;
     if (!WIDE && !in) return;
     if (unit >= s.pieces) {   // rows without places
         if (s.accumulate) return;
-        const int64_t r0 = (unit - s.pieces) * FILL_ROWS;
+        const int64_t r0 = (unit - s.pieces) * fill_rows(WIDE);
         Pack<O, N> zeros;
         zeros.zero();
         if constexpr (WIDE) {
@@ -194,8 +209,8 @@ __global__ __launch_bounds__(THREADS) void embed_sum_kernel(Sum s, const typenam
                 none &= none - 1;
             }
         } else {
-#pragma unroll 4
-            for (int i = 0; i < FILL_ROWS; ++i)
+#pragma unroll
+            for (int i = 0; i < fill_rows(false); ++i)
                 if (r0 + i < x.rows && x.count[x.slot(r0 + i)] == 0) zeros.store_past(out + (r0 + i) * s.out_stride + col);
         }
         return;
@@ -217,7 +232,7 @@ __global__ __launch_bounds__(THREADS) void embed_sum_kernel(Sum s, const typenam
             v.set(acc);
             v.store(reinterpret_cast<F32::raw *>(p));
         } else
-            put_row<O, N>(s, out, row, col, acc);
+            put_row<O, N>(s, out, row, at_columns, acc);
     };
     constexpr int AHEAD = 16;
     int32_t rows_of = 0, places_of = 0;
@@ -262,9 +277,10 @@ template <typename O, int N> __global__ __launch_bounds__(THREADS) void embed_jo
 {
     const Index &x = s.index;
     const int64_t unit = (int64_t)blockIdx.x * (THREADS / s.unit) + threadIdx.x / s.unit;
-    const int64_t col = ((int64_t)blockIdx.y * s.unit + threadIdx.x % s.unit) * N;
+    const Columns at_columns = columns_of<N>(s.dim, s.unit);
+    const int64_t col = at_columns.col;
     const int64_t end = (unit + 1) * s.piece;
-    if (col >= s.dim || end >= x.n) return;
+    if (!at_columns.in || end >= x.n) return;
     const int64_t total = *x.total;
     const int32_t row = x.row[end - 1], next = x.row[end];   // (read together; behind `total` they are any number)
     if (end >= total || row != next) return;
@@ -283,7 +299,7 @@ template <typename O, int N> __global__ __launch_bounds__(THREADS) void embed_jo
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] += more[i];
     }
-    put_row<O, N>(s, out, row, col, acc);
+    put_row<O, N>(s, out, row, at_columns, acc);
 }
 
 struct Rows {
@@ -299,8 +315,9 @@ __global__ __launch_bounds__(THREADS) void embed_rows_kernel(Rows s, const void 
                                                              typename O::raw *__restrict__ out)
 {
     const int64_t unit = (int64_t)blockIdx.x * (THREADS / s.unit) + threadIdx.x / s.unit;
-    const int64_t col = ((int64_t)blockIdx.y * s.unit + threadIdx.x % s.unit) * N;
-    if (col >= s.dim) return;
+    const Columns at_columns = columns_of<N>(s.dim, s.unit);
+    const int64_t col = at_columns.col;
+    if (!at_columns.in) return;
     constexpr int AHEAD = 4;
     const int64_t begin = unit * s.each, end = begin + s.each < s.n ? begin + s.each : s.n;
     for (int64_t at = begin; at < end; at += AHEAD) {
@@ -333,13 +350,11 @@ __global__ __launch_bounds__(THREADS) void embed_rows_kernel(Rows s, const void 
 // 73 us, 80 through them; what is smaller stays for the reader.
 constexpr int64_t KEPT = (int64_t)128 << 20;
 
-// Elements that a thread takes of a row at a time: 16 bytes of the smaller of the two types where every row starts on 16, the
-// largest power of two that all rows start on otherwise, one where that is an element.
-int elements_at_once(int64_t dim, int64_t bytes_a, int size_a, int64_t bytes_b, int size_b)
+// Elements that a thread takes of a row at a time: 16 bytes of the smaller of the two types, one of rows that have less.
+int elements_at_once(int64_t dim, int type_a, int type_b)
 {
-    int n = 16 / (size_a < size_b ? size_a : size_b);
-    while (n > 1 && (dim % n || (bytes_a < 16 && bytes_a % (n * size_a)) || (bytes_b < 16 && bytes_b % (n * size_b)))) n /= 2;
-    return n;
+    const int n = type_a == GDP_F32 && type_b == GDP_F32 ? 4 : 8;
+    return dim < n ? 1 : n;
 }
 
 // The threads that share a row: enough for all of it, a power of two so that units fill a workgroup.
@@ -363,7 +378,6 @@ template <typename F> int with_count(int n, F f)
     switch (n) {
     case 8: return f(std::integral_constant<int, 8>{});
     case 4: return f(std::integral_constant<int, 4>{});
-    case 2: return f(std::integral_constant<int, 2>{});
     default: return f(std::integral_constant<int, 1>{});
     }
 }
@@ -428,8 +442,7 @@ extern "C" int gdp_embed_forward(const gdp_embed *e, void *stream)
     if (!aligned(e->weight, size_of(e->weight_type)) || !aligned(e->out, size_of(e->out_type)) ||
         !aligned(e->tokens, e->token_type == GDP_I64 ? 8 : 4))
         return gdp_fail(GDP_E_BADARG, "gdp_embed: a pointer is not aligned to its elements");
-    const int n = elements_at_once(e->dim, row_alignment(e->weight, e->weight_stride, e->weight_type), size_of(e->weight_type),
-                                   row_alignment(e->out, e->out_stride, e->out_type), size_of(e->out_type));
+    const int n = elements_at_once(e->dim, e->weight_type, e->out_type);
     Rows s{e->n, e->dim, e->rows, e->first, unit_of(e->dim, n), 1, e->token_type, e->n * e->dim * size_of(e->out_type) > KEPT, e->scale, e->weight_stride, e->out_stride};
     const int64_t across = ceil_div(e->dim, (int64_t)s.unit * n), per = THREADS / s.unit;
     if (ceil_div(e->n, per * 4) * across >= 2048) s.each = 4;   // rows in flight of a thread, where there are enough for all
@@ -478,12 +491,11 @@ extern "C" int gdp_embed_backward(const gdp_embed_grad *e, void *stream)
                  ? launch("gdp_embed_backward", embed_index_kernel<int64_t>, dim3(1u << l.shift), INDEX_THREADS, 0, stream, x, static_cast<const int64_t *>(e->tokens))
                  : launch("gdp_embed_backward", embed_index_kernel<int32_t>, dim3(1u << l.shift), INDEX_THREADS, 0, stream, x, static_cast<const int32_t *>(e->tokens));
     if (rc) return rc;
-    const int n = elements_at_once(e->dim, row_alignment(e->grad, e->grad_stride, e->grad_type), size_of(e->grad_type),
-                                   row_alignment(e->out, e->out_stride, e->out_type), size_of(e->out_type));
+    const int n = elements_at_once(e->dim, e->grad_type, e->out_type);
     const Sum s{x, e->dim, l.piece, (int32_t)l.pieces, unit_of(e->dim, n), e->accumulate, e->scale, e->grad_stride, e->out_stride,
                 reinterpret_cast<float *>(w + l.partial)};
     const int64_t across = ceil_div(e->dim, (int64_t)s.unit * n), per = THREADS / s.unit;
-    const int64_t units = l.pieces + (e->accumulate ? 0 : ceil_div(e->rows, (int64_t)FILL_ROWS));
+    const int64_t units = l.pieces + (e->accumulate ? 0 : ceil_div(e->rows, (int64_t)fill_rows(s.unit >= 64)));
     return with_type(e->grad_type, [&](auto T) {
         return with_type(e->out_type, [&](auto O) {
             return with_count(n, [&](auto N) {

@@ -418,7 +418,6 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(Grad a, const typ
     const typename T::raw *const x = logits + row * a.stride;
     typename T::raw *const y = out + row * a.out_stride;
     const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(typename T::raw));
-    const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
     const int vocab = (int)a.vocab, vectors = (vocab + off + VEC - 1) / VEC;
     const int v0 = slice * a.width, v1 = v0 + a.width < vectors ? v0 + a.width : vectors;
     const float lse = a.lse[row];
@@ -472,11 +471,7 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(Grad a, const typ
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) f[i] = grad_of(p[u][i]);
                 p[u].set(f);
-                if (same)
-                    p[u].store(y + j);
-                else
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) y[j + i] = p[u].raw(i);
+                p[u].store(y + j);
             } else {
                 for (int i = 0; i < VEC; ++i)
                     if (j + i >= 0 && j + i < vocab) y[j + i] = T::down(grad_of(T::up(x[j + i])));

@@ -82,9 +82,31 @@ template <int E> __device__ __forceinline__ void row_of_weights(const void *p, i
     }
 }
 
+// A thread's columns: E from `col` on, K times.  Where E does not divide the width (TAIL), the last thread takes the last E, the first
+// `others` of which are another's: it leaves them out of sums and does not write them.  A thread behind the row's end has E others.
+template <int K, int E, bool TAIL> struct Columns {
+    int col[K], others[K];
+    bool in[K];
+    __device__ __forceinline__ Columns(int t, int threads, int dim)
+    {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            col[k] = (k * threads + t) * E;
+            in[k] = col[k] < dim;
+            others[k] = in[k] ? 0 : E;
+            if (TAIL && in[k] && col[k] + E > dim) {
+                others[k] = col[k] + E - dim;
+                col[k] = dim - E;
+            }
+        }
+    }
+    __device__ __forceinline__ bool own(int k, int i) const { return TAIL ? i >= others[k] : in[k]; }
+    __device__ __forceinline__ int from(int k) const { return TAIL ? others[k] : 0; }   // the first that is written
+};
+
 // Mean and 1 / deviation of a row of which a thread holds x[K][E].
-template <int W, int K, int E>
-__device__ __forceinline__ float2 statistics(const float (&x)[K][E], const bool (&in)[K], int form, float eps, float per_dim, RowSums<W> &shared, int &turn)
+template <int W, int K, int E, bool TAIL>
+__device__ __forceinline__ float2 statistics(const float (&x)[K][E], const Columns<K, E, TAIL> &c, int form, float eps, float per_dim, RowSums<W> &shared, int &turn)
 {
     float mean = 0.0f;
     float sum[1] = {0.0f};
@@ -92,7 +114,7 @@ __device__ __forceinline__ float2 statistics(const float (&x)[K][E], const bool 
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int i = 0; i < E; ++i) sum[0] += x[k][i];   // 0 outside
+            for (int i = 0; i < E; ++i) sum[0] += c.own(k, i) ? x[k][i] : 0.0f;
         row_sums<W, 1>(sum, shared, turn);
         mean = sum[0] * per_dim;
     }
@@ -101,7 +123,7 @@ __device__ __forceinline__ float2 statistics(const float (&x)[K][E], const bool 
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const float d = in[k] ? x[k][i] - mean : 0.0f;
+            const float d = c.own(k, i) ? x[k][i] - mean : 0.0f;
             sum[0] = fmaf(d, d, sum[0]);
         }
     row_sums<W, 1>(sum, shared, turn);
@@ -109,7 +131,7 @@ __device__ __forceinline__ float2 statistics(const float (&x)[K][E], const bool 
 }
 
 // At most W waves to a row, K times E elements to a thread; R rows to a workgroup where W is 1.
-template <typename T, typename S, int W, int K, int E, int R>
+template <typename T, typename S, int W, int K, int E, bool TAIL, int R>
 __global__ __launch_bounds__(64 * W * R) void norm_forward_kernel(Join a, const typename S::raw *__restrict__ residual, const typename T::raw *__restrict__ block,
                                                                   typename S::raw *__restrict__ stream, typename T::raw *__restrict__ normed)
 {
@@ -119,14 +141,13 @@ __global__ __launch_bounds__(64 * W * R) void norm_forward_kernel(Join a, const 
     const int row = blockIdx.x * R + (W == 1 ? threadIdx.x >> 6 : 0);
     if (W == 1 && row >= a.n) return;
     row_sums_begin(shared);
-    bool in[K];
-    int col[K];
+    const Columns<K, E, TAIL> c(t, threads, a.dim);
+    const auto &col = c.col;
+    const auto &in = c.in;
     Pack<S, E> r[K];
     Pack<T, E> b[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        col[k] = (k * threads + t) * E;
-        in[k] = col[k] < a.dim;
         r[k].zero();
         b[k].zero();
         if (in[k]) {
@@ -142,7 +163,7 @@ __global__ __launch_bounds__(64 * W * R) void norm_forward_kernel(Join a, const 
         for (int i = 0; i < E; ++i) x[k][i] = b[k][i];
     if (block) {
         if (a.post.form != GDP_NORM_NONE) {
-            const float2 s = statistics<W, K, E>(x, in, a.post.form, a.post.eps, a.per_dim, shared, turn);
+            const float2 s = statistics<W, K, E, TAIL>(x, c, a.post.form, a.post.eps, a.per_dim, shared, turn);
             stats.x = s.x, stats.y = s.y;
 #pragma unroll
             for (int k = 0; k < K; ++k)
@@ -172,11 +193,11 @@ __global__ __launch_bounds__(64 * W * R) void norm_forward_kernel(Join a, const 
         for (int i = 0; i < E; ++i) x[k][i] = block ? fmaf(r[k][i], a.residual_scale, x[k][i] * a.block_scale) : r[k][i] * a.residual_scale;
         if (stream && in[k]) {
             r[k].set(x[k]);
-            r[k].store(stream + (int64_t)row * a.stream_stride + col[k]);
+            r[k].store_from(stream + (int64_t)row * a.stream_stride + col[k], c.from(k));
         }
     }
     if (a.pre.form != GDP_NORM_NONE) {
-        const float2 s = statistics<W, K, E>(x, in, a.pre.form, a.pre.eps, a.per_dim, shared, turn);
+        const float2 s = statistics<W, K, E, TAIL>(x, c, a.pre.form, a.pre.eps, a.per_dim, shared, turn);
         stats.z = s.x, stats.w = s.y;
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -187,7 +208,7 @@ __global__ __launch_bounds__(64 * W * R) void norm_forward_kernel(Join a, const 
 #pragma unroll
                 for (int i = 0; i < E; ++i) x[k][i] = fmaf((x[k][i] - s.x) * s.y, w[i], add[i]);
                 b[k].set(x[k]);
-                b[k].store(normed + (int64_t)row * a.normed_stride + col[k]);
+                b[k].store_from(normed + (int64_t)row * a.normed_stride + col[k], c.from(k));
             }
     }
     if (a.stats && t == 0) a.stats[row] = stats;
@@ -222,8 +243,56 @@ __device__ __forceinline__ void rows_of(const Back &a, int group, int &from, int
     }
 }
 
-template <typename T, typename S, int W, int K, int E>
-__global__ __launch_bounds__(64 * W, W <= 8 ? 4 : 1) void norm_backward_kernel(Back a, const typename S::raw *__restrict__ stream, const typename T::raw *__restrict__ block,
+// A row of weights, for each row of the gradient.  HOLD: a thread keeps what it needs of them packed, in the block's 16 bits, so that four
+// rows of weights, five sums of columns and a row that is read ahead fit 168 registers, with which 12 waves are on a core.
+// Otherwise (float32, mixed types, more than 12 waves with biases) they are read again for each row, H at a time, from the caches: kept unpacked they
+// would take the registers of the sums.
+template <typename T, int K, int E, bool TAIL, bool HOLD> struct Weights {
+    static constexpr int H = E < 4 ? E : 4;
+    const void *p;
+    int type;
+    float idle;
+    Pack<T, E> w[HOLD ? K : 1];
+    __device__ __forceinline__ void read(const void *row, int type_, const Columns<K, E, TAIL> &c, float idle_)
+    {
+        p = row, type = type_, idle = idle_;
+        if constexpr (HOLD) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float f[E];
+#pragma unroll
+                for (int i = 0; i < E; ++i) f[i] = idle;
+                w[k].set(f);
+                if (p && c.in[k]) w[k].load(static_cast<const typename T::raw *>(p) + c.col[k]);
+            }
+        }
+    }
+    // Tells the compiler that they may have changed: it would unpack, or read, them once for all rows.
+    __device__ __forceinline__ void hold(int &again)
+    {
+        if constexpr (HOLD) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < Pack<T, E>::WORDS; ++i) asm volatile("" : "+v"(w[k].w[i]));
+        } else {
+            again = 0;
+            asm volatile("" : "+s"(again));
+        }
+    }
+    __device__ __forceinline__ void get(int k, int h, int again, const Columns<K, E, TAIL> &c, float (&f)[H]) const
+    {
+        if constexpr (HOLD) {
+#pragma unroll
+            for (int i = 0; i < H; ++i) f[i] = w[k][h + i];
+        } else
+            row_of_weights<H>(c.in[k] ? p : nullptr, type, c.col[k] + h + again, f, idle);
+    }
+};
+
+// BIAS: with sums for biases.
+template <typename T, typename S, bool HOLD, bool BIAS, int W, int K, int E, bool TAIL>
+__global__ __launch_bounds__(64 * W, W <= 4 ? 4 : W <= 12 ? 3 : 1) void norm_backward_kernel(Back a, const typename S::raw *__restrict__ stream, const typename T::raw *__restrict__ block,
                                                                const typename T::raw *__restrict__ grad_normed, const typename S::raw *__restrict__ grad_stream,
                                                                typename S::raw *__restrict__ grad_residual, typename T::raw *__restrict__ grad_block)
 {
@@ -231,67 +300,95 @@ __global__ __launch_bounds__(64 * W, W <= 8 ? 4 : 1) void norm_backward_kernel(B
     int turn = 0;
     const int t = threadIdx.x, threads = blockDim.x;
     row_sums_begin(shared);
-    bool in[K];
-    int col[K];
+    const Columns<K, E, TAIL> c(t, threads, a.dim);
+    const auto &col = c.col;
+    const auto &in = c.in;
     float sums[COLUMNS][K][E];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        col[k] = (k * threads + t) * E;
-        in[k] = col[k] < a.dim;
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int c = 0; c < COLUMNS; ++c)
+        for (int q = 0; q < COLUMNS; ++q)
 #pragma unroll
-            for (int i = 0; i < E; ++i) sums[c][k][i] = 0.0f;
-    }
+            for (int i = 0; i < E; ++i) sums[q][k][i] = 0.0f;
     int from, to;
     rows_of(a, blockIdx.x, from, to);
-    for (int row = from; row < to; ++row) {
+    using Row = Weights<T, K, E, TAIL, HOLD>;
+    constexpr int H = Row::H;
+    Row pre_w, post_w, post_b, gate;
+    const bool post = a.post.form != GDP_NORM_NONE;
+    pre_w.read(a.pre.weight, a.pre.type, c, 1.0f);
+    post_w.read(post ? a.post.weight : nullptr, a.post.type, c, 1.0f);
+    post_b.read(post ? a.post.bias : nullptr, a.post.type, c, 0.0f);
+    gate.read(nullptr, 0, c, 1.0f);
+    struct Read {
         Pack<S, E> r[K], ds[K];
         Pack<T, E> b[K], dh[K];
-        const float4 stats = a.stats[row];
+        float4 stats;
+    };
+    const auto read = [&](Read &o, int row) {
+        o.stats = a.stats[row];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            r[k].zero(), ds[k].zero(), b[k].zero(), dh[k].zero();
+            o.r[k].zero(), o.ds[k].zero(), o.b[k].zero(), o.dh[k].zero();
             if (in[k]) {
                 if (grad_normed) {
-                    dh[k].load(grad_normed + (int64_t)row * a.grad_normed_stride + col[k]);
-                    r[k].load(stream + (int64_t)row * a.stream_stride + col[k]);
+                    o.dh[k].load(grad_normed + (int64_t)row * a.grad_normed_stride + col[k]);
+                    o.r[k].load(stream + (int64_t)row * a.stream_stride + col[k]);
                 }
-                if (grad_stream) ds[k].load(grad_stream + (int64_t)row * a.grad_stream_stride + col[k]);
-                if (block) b[k].load(block + (int64_t)row * a.block_stride + col[k]);
+                if (grad_stream) o.ds[k].load(grad_stream + (int64_t)row * a.grad_stream_stride + col[k]);
+                if (block) o.b[k].load(block + (int64_t)row * a.block_stride + col[k]);
             }
         }
+    };
+    // Of 5 to 12 waves one workgroup is on a core, with registers to read a row ahead (16384 rows of 4096 bf16: 170 us, 181 with
+    // two workgroups that wait in turn and 128 registers); of fewer there are several (65536 of 1024: 179, 188 ahead).
+    constexpr bool AHEAD = W == 8 || W == 12;
+    Read next;
+    if (AHEAD && from < to) read(next, from);
+    for (int row = from; row < to; ++row) {
+        const int64_t g = row / a.rows_per_gate;
+        if (a.gate && (row == from || row % a.rows_per_gate == 0))
+            gate.read(static_cast<const char *>(a.gate) + g * a.gate_stride * (a.gate_type == GDP_F32 ? 4 : 2), a.gate_type, c, 1.0f);
+        int again = 0;
+        pre_w.hold(again), post_w.hold(again), post_b.hold(again), gate.hold(again);
+        if (!AHEAD) read(next, row);
+        Read now = next;
+        if (AHEAD && row + 1 < to) read(next, row + 1);
+        auto &r = now.r, &ds = now.ds;
+        auto &b = now.b, &dh = now.dh;
+        const float4 stats = now.stats;
         float d[K][E];   // of the stream
         if (grad_normed) {
-            float hat[K][E], mean[2] = {0.0f, 0.0f};   // of u * hat, of u
+            float mean[2] = {0.0f, 0.0f};   // of u * hat, of u
+            const auto hat = [&](int k, int i) { return (r[k][i] - stats.z) * stats.w; };
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                float w[E];
+            for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < E; ++i) w[i] = 0.0f;
-                if (in[k]) row_of_weights<E>(a.pre.weight, a.pre.type, col[k], w, 1.0f);
+                for (int h = 0; h < E; h += H) {
+                    float w[H];
+                    pre_w.get(k, h, again, c, w);
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    hat[k][i] = (r[k][i] - stats.z) * stats.w;
-                    sums[PRE_W][k][i] = fmaf(dh[k][i], hat[k][i], sums[PRE_W][k][i]);
-                    sums[PRE_B][k][i] += dh[k][i];
-                    d[k][i] = dh[k][i] * w[i];
-                    mean[0] = fmaf(d[k][i], hat[k][i], mean[0]);
-                    mean[1] += d[k][i];
+                    for (int i = h; i < h + H; ++i) {
+                        const float y = c.own(k, i) ? dh[k][i] : 0.0f;
+                        sums[PRE_W][k][i] = fmaf(y, hat(k, i), sums[PRE_W][k][i]);
+                        if (BIAS) sums[PRE_B][k][i] += y;
+                        d[k][i] = y * w[i - h];
+                        mean[0] = fmaf(d[k][i], hat(k, i), mean[0]);
+                        mean[1] += d[k][i];
+                    }
                 }
-            }
             row_sums<W, 2>(mean, shared, turn);
             mean[0] *= a.per_dim;
             mean[1] *= a.pre.form == GDP_NORM_LAYER ? a.per_dim : 0.0f;
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < E; ++i) d[k][i] = in[k] ? fmaf(d[k][i] - hat[k][i] * mean[0] - mean[1], stats.w, ds[k][i]) : 0.0f;
+                for (int i = 0; i < E; ++i) d[k][i] = c.own(k, i) ? fmaf(d[k][i] - hat(k, i) * mean[0] - mean[1], stats.w, ds[k][i]) : 0.0f;
         } else {
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < E; ++i) d[k][i] = ds[k][i];
+                for (int i = 0; i < E; ++i) d[k][i] = c.own(k, i) ? ds[k][i] : 0.0f;
         }
         if (grad_residual) {
 #pragma unroll
@@ -301,53 +398,45 @@ __global__ __launch_bounds__(64 * W, W <= 8 ? 4 : 1) void norm_backward_kernel(B
 #pragma unroll
                     for (int i = 0; i < E; ++i) f[i] = d[k][i] * a.residual_scale;
                     r[k].set(f);
-                    r[k].store(grad_residual + (int64_t)row * a.grad_residual_stride + col[k]);
+                    r[k].store_from(grad_residual + (int64_t)row * a.grad_residual_stride + col[k], c.from(k));
                 }
         }
         if (block) {
-            float hat[K][E], mean[2] = {0.0f, 0.0f};   // of u * hat, of u
-            const int64_t g = row / a.rows_per_gate;
+            float mean[2] = {0.0f, 0.0f};
+            const auto hat = [&](int k, int i) { return post ? (b[k][i] - stats.x) * stats.y : b[k][i]; };
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                float w[E], add[E], gate[E];
+            for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < E; ++i) w[i] = 1.0f, add[i] = 0.0f, gate[i] = 1.0f;
-                if (in[k]) {
-                    if (a.post.form != GDP_NORM_NONE) {
-                        row_of_weights<E>(a.post.weight, a.post.type, col[k], w, 1.0f);
-                        row_of_weights<E>(a.post.bias, a.post.type, col[k], add, 0.0f);
+                for (int h = 0; h < E; h += H) {
+                    float w[H], add[H], of_gate[H];
+                    post_w.get(k, h, again, c, w), post_b.get(k, h, again, c, add), gate.get(k, h, again, c, of_gate);
+#pragma unroll
+                    for (int i = h; i < h + H; ++i) {
+                        float dn = d[k][i] * a.block_scale;
+                        sums[GATE][k][i] = fmaf(dn, fmaf(hat(k, i), w[i - h], add[i - h]), sums[GATE][k][i]);
+                        dn *= of_gate[i - h];
+                        sums[POST_W][k][i] = fmaf(dn, hat(k, i), sums[POST_W][k][i]);
+                        if (BIAS) sums[POST_B][k][i] += dn;
+                        d[k][i] = dn * w[i - h];
+                        mean[0] = fmaf(d[k][i], hat(k, i), mean[0]);
+                        mean[1] += d[k][i];
                     }
-                    row_of_weights<E>(a.gate, a.gate_type, g * a.gate_stride + col[k], gate, 1.0f);
                 }
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    float dn = d[k][i] * a.block_scale;
-                    hat[k][i] = a.post.form != GDP_NORM_NONE ? (b[k][i] - stats.x) * stats.y : b[k][i];
-                    const float n = a.post.form != GDP_NORM_NONE ? fmaf(hat[k][i], w[i], add[i]) : b[k][i];
-                    sums[GATE][k][i] = fmaf(dn, n, sums[GATE][k][i]);
-                    dn *= gate[i];
-                    sums[POST_W][k][i] = fmaf(dn, hat[k][i], sums[POST_W][k][i]);
-                    sums[POST_B][k][i] += dn;
-                    d[k][i] = dn * w[i];
-                    mean[0] = fmaf(d[k][i], hat[k][i], mean[0]);
-                    mean[1] += d[k][i];
-                }
-            }
-            if (a.post.form != GDP_NORM_NONE) {
+            if (post) {
                 row_sums<W, 2>(mean, shared, turn);
                 mean[0] *= a.per_dim;
                 mean[1] *= a.post.form == GDP_NORM_LAYER ? a.per_dim : 0.0f;
 #pragma unroll
                 for (int k = 0; k < K; ++k)
 #pragma unroll
-                    for (int i = 0; i < E; ++i) d[k][i] = (d[k][i] - hat[k][i] * mean[0] - mean[1]) * stats.y;
+                    for (int i = 0; i < E; ++i) d[k][i] = (d[k][i] - hat(k, i) * mean[0] - mean[1]) * stats.y;
             }
             if (grad_block) {
 #pragma unroll
                 for (int k = 0; k < K; ++k)
                     if (in[k]) {
                         b[k].set(d[k]);
-                        b[k].store(grad_block + (int64_t)row * a.grad_block_stride + col[k]);
+                        b[k].store_from(grad_block + (int64_t)row * a.grad_block_stride + col[k], c.from(k));
                     }
             }
             if (a.grad_gate && (row + 1) % a.rows_per_gate == 0) {   // the last row of a gate, all of whose rows are this workgroup's
@@ -355,26 +444,26 @@ __global__ __launch_bounds__(64 * W, W <= 8 ? 4 : 1) void norm_backward_kernel(B
                 for (int k = 0; k < K; ++k)
 #pragma unroll
                     for (int i = 0; i < E; ++i) {
-                        if (in[k]) down_any(a.grad_gate, a.gate_type, g * a.dim + col[k] + i, sums[GATE][k][i]);
+                        if (c.own(k, i)) down_any(a.grad_gate, a.gate_type, g * a.dim + col[k] + i, sums[GATE][k][i]);
                         sums[GATE][k][i] = 0.0f;
                     }
             }
         }
     }
 #pragma unroll
-    for (int c = 0; c < COLUMNS; ++c)
-        if (a.of[c]) {
+    for (int q = 0; q < COLUMNS; ++q)
+        if (a.of[q]) {
 #pragma unroll
             for (int k = 0; k < K; ++k)
                 if (in[k]) {
                     Pack<F32, E> v;
-                    v.set(sums[c][k]);
-                    v.store(reinterpret_cast<F32::raw *>(a.of[c] + (int64_t)blockIdx.x * a.dim + col[k]));
+                    v.set(sums[q][k]);
+                    v.store_from(reinterpret_cast<F32::raw *>(a.of[q] + (int64_t)blockIdx.x * a.dim + col[k]), c.from(k));
                 }
         }
 }
 
-// out[g][col] = sum of `rows` rows of partial sums, in their order: 16 sums of a sixteenth each, joined in order.
+// out[g][col] = sum of `rows` rows of partial sums, in their order: 32 sums of a 32nd each, joined in order.
 struct Add {
     const float *from;
     void *to;
@@ -384,7 +473,7 @@ struct Adds {
     Add of[COLUMNS];
     int64_t dim;
 };
-constexpr int ADD_COLUMNS = 64, ADD_ROWS = 16;
+constexpr int ADD_COLUMNS = 32, ADD_ROWS = 32;
 __global__ __launch_bounds__(ADD_COLUMNS *ADD_ROWS) void norm_add_kernel(Adds a)
 {
     __shared__ float part[ADD_ROWS][ADD_COLUMNS];
@@ -439,19 +528,6 @@ int check_gate(const void *gate, int64_t gates, int64_t stride, int type, int64_
     return check_rows(gate, gates, dim, stride, type, false);
 }
 
-// Whether all rows can be taken in 16 bytes: of `E` elements each.
-struct Wide {
-    int64_t dim;
-    int e;
-    bool ok;
-    void rows(const void *p, int64_t stride, int type)
-    {
-        const int need = e * size_of(type) < 16 ? e * size_of(type) : 16;
-        if (p && row_alignment(p, stride, type) < need) ok = false;
-    }
-};
-Wide wide_for(int64_t dim, int type) { return {dim, 16 / size_of(type), dim % (16 / size_of(type)) == 0}; }
-
 template <typename F> int with_types(int type, int stream_type, F f)
 {
     if (type == GDP_F32) return f(F32{}, F32{});
@@ -460,20 +536,31 @@ template <typename F> int with_types(int type, int stream_type, F f)
 }
 template <int N> using Int = std::integral_constant<int, N>;
 
-// f(most waves of a row, times that a thread's elements repeat, threads): 16 bytes a thread, 16 waves at most.
-template <int E, typename F> int with_waves(int64_t dim, F f)
+// f(most waves of a row, times that a thread's elements repeat, elements, whether they do not divide the width, threads): 16 bytes of the
+// block's type a thread, 16 waves at most; rows of less than 16 bytes an element a thread.
+template <int E, bool TAIL, typename F> int with_waves(int64_t dim, F f)
 {
+    using Tail = std::integral_constant<bool, TAIL>;
     const int waves = (int)ceil_div(dim, (int64_t)64 * E);
-    if (waves <= 1) return f(Int<1>{}, Int<1>{}, 64);
-    if (waves <= 4) return f(Int<4>{}, Int<1>{}, 64 * waves);
-    if (waves <= 8) return f(Int<8>{}, Int<1>{}, 64 * waves);
-    if (waves <= 16) return f(Int<16>{}, Int<1>{}, 64 * waves);
-    if constexpr (E == 8) return f(Int<16>{}, Int<2>{}, 64 * (int)ceil_div(waves, 2));
-    if constexpr (E == 4) return f(Int<16>{}, Int<4>{}, 64 * (int)ceil_div(waves, 4));
-    if constexpr (E == 1) return f(Int<16>{}, Int<16>{}, 64 * (int)ceil_div(waves, 16));
+    if (waves <= 1) return f(Int<1>{}, Int<1>{}, Int<E>{}, Tail{}, 64);
+    if constexpr (E > 1) {
+        if (waves <= 4) return f(Int<4>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
+        if (waves <= 8) return f(Int<8>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
+        if (waves <= 12) return f(Int<12>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
+        if (waves <= 16) return f(Int<16>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
+        if constexpr (E == 8) return f(Int<16>{}, Int<2>{}, Int<E>{}, Tail{}, 64 * (int)ceil_div(waves, 2));
+    }
+    return gdp_fail(GDP_E_BADARG, "gdp_norm: too wide");   // (not reached: 4 and 1 elements a thread are for narrower rows)
 }
-static_assert(GDP_MAX_NORM_DIM <= 64 * 16 * 16, "the widest row fits");
+template <int E, typename F> int with_columns(int64_t dim, F f)
+{
+    if (dim < E) return with_waves<1, false>(dim, f);
+    // (of float32 twice that where 16 waves do not reach otherwise: fewer repetitions, whose sums are kept in registers)
+    if (E == 4 && dim > 64 * 16 * 4) return dim % 8 ? with_waves<8, true>(dim, f) : with_waves<8, false>(dim, f);
+    return dim % E ? with_waves<E, true>(dim, f) : with_waves<E, false>(dim, f);
+}
 
+static_assert(GDP_MAX_NORM_DIM <= 64 * 16 * 8 * 2, "the widest row fits");
 Side side_of(const gdp_norm_params &p) { return {p.form, p.type, p.eps, p.weight, p.bias}; }
 
 // How many workgroups take the rows of a gradient, and how: the rows of each of several gates are shared by some workgroups,
@@ -482,16 +569,18 @@ struct Shares {
     int64_t groups, per_group;
     bool split_gates;
 };
-constexpr int64_t MOST_GROUPS = 512;
-Shares shares_of(int64_t n, int64_t gates)
+Shares shares_of(int64_t n, int64_t dim, int64_t gates)
 {
     if (n == 0) return {0, 0, false};
+    // As many workgroups as are resident together, by their registers 16 waves on a core of up to 4 waves each, else 12: each writes its
+    // sums of columns, and one more than that would run alone at the end.
+    const int64_t waves = ceil_div(dim, (int64_t)512), most = 256 * (waves <= 4 ? 16 / waves : waves <= 12 ? 12 / waves : 1);
     const int64_t rows = gates > 1 ? n / gates : 1, units = n / rows;
-    if (gates > 1 && gates <= MOST_GROUPS / 2 && rows > 1) {
-        const int64_t q = MOST_GROUPS / gates < rows ? MOST_GROUPS / gates : rows;
+    if (gates > 1 && gates <= most / 2 && rows > 1) {
+        const int64_t q = most / gates < rows ? most / gates : rows;
         return {gates * q, q, true};
     }
-    const int64_t each = ceil_div(units, MOST_GROUPS);
+    const int64_t each = ceil_div(units, most);
     return {ceil_div(units, each), each * rows, false};
 }
 
@@ -513,28 +602,17 @@ extern "C" int gdp_norm_forward(const gdp_norm *p, void *queue)
     if (const int rc = check_rows(p->stream, p->n, p->dim, p->stream_stride, p->stream_type, true)) return rc;
     if (const int rc = check_rows(p->normed, p->n, p->dim, p->normed_stride, p->type, true)) return rc;
     if (!aligned(p->stats, 16)) return gdp_fail(GDP_E_BADARG, "gdp_norm: stats must be aligned to 16 bytes");
-    Wide wide = wide_for(p->dim, p->type);
-    wide.rows(p->residual, p->residual_stride, p->stream_type);
-    wide.rows(p->block, p->block_stride, p->type);
-    wide.rows(p->stream, p->stream_stride, p->stream_type);
-    wide.rows(p->normed, p->normed_stride, p->type);
-    wide.rows(p->gate, p->gate_stride, p->gate_type);
-    for (const gdp_norm_params *s : {&p->post, &p->pre})
-        if (s->form != GDP_NORM_NONE) wide.rows(s->weight, 0, s->type), wide.rows(s->bias, 0, s->type);
     const Join j{(int32_t)p->n, (int32_t)p->dim, (int32_t)(p->gate ? p->n / p->gates : p->n), side_of(p->post), side_of(p->pre), p->gate_type, p->residual_scale, p->block_scale, 1.0f / (float)p->dim,
                  p->residual_stride, p->block_stride, p->gate_stride, p->stream_stride, p->normed_stride, p->gate, reinterpret_cast<float4 *>(p->stats)};
     return with_types(p->type, p->stream_type, [&](auto T, auto S) {
         using TT = decltype(T);
         using SS = decltype(S);
-        const auto run = [&](auto E) {
-            return with_waves<E.value>(p->dim, [&](auto W, auto K, int threads) {
-                constexpr int R = W.value == 1 ? 4 : 1;
-                return launch("gdp_norm_forward", norm_forward_kernel<TT, SS, W.value, K.value, E.value, R>, dim3((unsigned)ceil_div(p->n, (int64_t)R)), threads * R, 0, queue, j,
-                              static_cast<const typename SS::raw *>(p->residual), static_cast<const typename TT::raw *>(p->block), static_cast<typename SS::raw *>(p->stream),
-                              static_cast<typename TT::raw *>(p->normed));
-            });
-        };
-        return wide.ok ? run(Int<TT::VEC>{}) : run(Int<1>{});
+        return with_columns<TT::VEC>(p->dim, [&](auto W, auto K, auto E, auto TAIL, int threads) {
+            constexpr int R = W.value == 1 ? 4 : 1;
+            return launch("gdp_norm_forward", norm_forward_kernel<TT, SS, W.value, K.value, E.value, TAIL.value, R>, dim3((unsigned)ceil_div(p->n, (int64_t)R)), threads * R, 0, queue,
+                          j, static_cast<const typename SS::raw *>(p->residual), static_cast<const typename TT::raw *>(p->block), static_cast<typename SS::raw *>(p->stream),
+                          static_cast<typename TT::raw *>(p->normed));
+        });
     });
 }
 
@@ -544,7 +622,7 @@ extern "C" int gdp_norm_grad_workspace(int64_t n, int64_t dim, int64_t gates, si
     if (!bytes) return gdp_fail(GDP_E_BADARG, "gdp_norm: null argument");
     if (const int rc = check_sizes(n, dim, GDP_F32, GDP_F32)) return rc;
     if (gates < 0 || (gates && n % gates)) return gdp_fail(GDP_E_BADARG, "gdp_norm: the number of gates must divide the number of rows");
-    *bytes = round_up((size_t)COLUMNS * shares_of(n, gates).groups * dim * 4, 256);
+    *bytes = round_up((size_t)COLUMNS * shares_of(n, dim, gates).groups * dim * 4, 256);
     return GDP_OK;
 }
 
@@ -564,17 +642,12 @@ extern "C" int gdp_norm_backward(const gdp_norm_grad *p, void *queue)
     const struct { const void *p; int64_t stride; int type; bool written; } all[] = {
         {p->stream, p->stream_stride, p->stream_type, false}, {p->block, p->block_stride, p->type, false}, {p->grad_normed, p->grad_normed_stride, p->type, false},
         {p->grad_stream, p->grad_stream_stride, p->stream_type, false}, {p->grad_residual, p->grad_residual_stride, p->stream_type, true}, {p->grad_block, p->grad_block_stride, p->type, true}};
-    Wide wide = wide_for(p->dim, p->type);
     for (const auto &a : all) {
         if (const int rc = check_rows(a.p, p->n, p->dim, a.stride, a.type, a.written)) return rc;
-        wide.rows(a.p, a.stride, a.type);
-    }
-    wide.rows(p->gate, p->gate_stride, p->gate_type);
-    for (const gdp_norm_params *s : {&p->post, &p->pre})
-        if (s->form != GDP_NORM_NONE) wide.rows(s->weight, 0, s->type), wide.rows(s->bias, 0, s->type);
+        }
     if (!aligned(p->stats, 16)) return gdp_fail(GDP_E_BADARG, "gdp_norm: stats must be aligned to 16 bytes");
     const int64_t gates = p->gate ? p->gates : 0;
-    const Shares shares = shares_of(p->n, gates);
+    const Shares shares = shares_of(p->n, p->dim, gates);
     if (!aligned(p->workspace, 256) || p->workspace_bytes < round_up((size_t)COLUMNS * shares.groups * p->dim * 4, 256))
         return gdp_fail(GDP_E_BADARG, "gdp_norm: the workspace is smaller than gdp_norm_grad_workspace says, or not aligned to 256 bytes");
     Back b{(int32_t)p->n, (int32_t)p->dim, (int32_t)(gates ? p->n / gates : p->n), (int32_t)shares.groups, (int32_t)shares.per_group, shares.split_gates, p->gate_type,
@@ -597,17 +670,26 @@ extern "C" int gdp_norm_backward(const gdp_norm_grad *p, void *queue)
         adds.of[count++] = {b.of[c], outs[c], (int32_t)(several ? shares.per_group : shares.groups), (int32_t)(several ? gates : 1), types[c]};
         if (several) most = (unsigned)gates;
     }
+    const auto of_type = [&](const void *w, int type) { return !w || type == p->type; };
+    const bool packed = of_type(p->pre.weight, p->pre.type) && of_type(p->post.weight, p->post.type) && of_type(p->post.bias, p->post.type) && of_type(p->gate, p->gate_type);
     const int rc = p->n == 0 ? GDP_OK : with_types(p->type, p->stream_type, [&](auto T, auto S) {
         using TT = decltype(T);
         using SS = decltype(S);
-        const auto run = [&](auto E) {
-            return with_waves<E.value>(p->dim, [&](auto W, auto K, int threads) {
-                return launch("gdp_norm_backward", norm_backward_kernel<TT, SS, W.value, K.value, E.value>, dim3((unsigned)shares.groups), threads, 0, queue, b,
-                              static_cast<const typename SS::raw *>(p->stream), static_cast<const typename TT::raw *>(p->block), static_cast<const typename TT::raw *>(p->grad_normed),
-                              static_cast<const typename SS::raw *>(p->grad_stream), static_cast<typename SS::raw *>(p->grad_residual), static_cast<typename TT::raw *>(p->grad_block));
-            });
-        };
-        return wide.ok ? run(Int<TT::VEC>{}) : run(Int<1>{});
+        return with_columns<TT::VEC>(p->dim, [&](auto W, auto K, auto E, auto TAIL, int threads) {
+            const auto run = [&](auto HOLD, auto BIAS) {
+                return launch("gdp_norm_backward", norm_backward_kernel<TT, SS, HOLD.value, BIAS.value, W.value, K.value, E.value, TAIL.value>, dim3((unsigned)shares.groups), threads, 0,
+                              queue, b, static_cast<const typename SS::raw *>(p->stream), static_cast<const typename TT::raw *>(p->block),
+                              static_cast<const typename TT::raw *>(p->grad_normed), static_cast<const typename SS::raw *>(p->grad_stream),
+                              static_cast<typename SS::raw *>(p->grad_residual), static_cast<typename TT::raw *>(p->grad_block));
+            };
+            const bool bias = p->grad_pre_bias || p->grad_post_bias;
+            if constexpr (sizeof(typename TT::raw) == 2 && K.value == 1 && E.value > 1) {
+                if (packed && !bias) return run(std::true_type{}, std::false_type{});
+                if constexpr (W.value <= 12)
+                    if (packed) return run(std::true_type{}, std::true_type{});
+            }
+            return bias ? run(std::false_type{}, std::true_type{}) : run(std::false_type{}, std::false_type{});
+        });
     });
     if (rc) return rc;
     const unsigned across = (unsigned)ceil_div(p->dim, (int64_t)ADD_COLUMNS);

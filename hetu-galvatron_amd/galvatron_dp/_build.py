@@ -7,6 +7,8 @@ from __future__ import annotations
 
 import os
 import subprocess
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(PKG, "csrc")
@@ -22,18 +24,34 @@ HIPCC_FLAGS = ["-O3", "-std=c++17", f"--offload-arch={ARCH}", "-fPIC", "-shared"
                "-Wno-unused-command-line-argument"]
 
 
-def build(verbose: bool = False, extra_flags=(), out: str = LIB_PATH, csrc: str = CSRC) -> str:
-    os.makedirs(os.path.dirname(out), exist_ok=True)
-    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    cmd = [hipcc] + HIPCC_FLAGS + list(extra_flags) + [os.path.join(csrc, s) for s in SOURCES] + ["-o", out]
-    if verbose:
-        print(" ".join(cmd), flush=True)
+def _run(cmd) -> str:
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     log = "\n".join(l for l in proc.stdout.splitlines() if "is not a recognized feature for this target" not in l)
     if proc.returncode != 0:
         raise RuntimeError("hipcc failed:\n" + log)
-    if verbose and log.strip():
-        print(log)
+    return log
+
+
+def build(verbose: bool = False, extra_flags=(), out: str = LIB_PATH, csrc: str = CSRC) -> str:
+    """Compiles the sources side by side and links them."""
+    os.makedirs(os.path.dirname(out), exist_ok=True)
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    flags = HIPCC_FLAGS + list(extra_flags)
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        steps = [[hipcc] + [f for f in flags if f != "-shared"] + ["-c", os.path.join(csrc, s), "-o", o]
+                 for s, o in zip(SOURCES, objects)]
+        link = [hipcc] + flags + objects + ["-o", out]
+        if verbose:
+            for cmd in steps + [link]:
+                print(" ".join(cmd), flush=True)
+        with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+            logs = list(pool.map(_run, steps))
+        logs.append(_run(link))
+    if verbose:
+        for log in logs:
+            if log.strip():
+                print(log)
     return out
 
 

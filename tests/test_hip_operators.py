@@ -335,7 +335,9 @@ NORM = [  # rows, dim, post, pre, gates, types of block and stream
     (1024, 24, "rms", "rms", 1024, BF16, F32), (12, 2048, "rms", "layer", 4, F16, F16), (3, 4104, "layer", "rms", 3, BF16, BF16),
     (4, 8200, "rms", "layer", 2, BF16, F32), (2, 16384, "layer", "layer", 1, F32, F32), (2, 16383, "layer", "rms", 2, BF16, F32),
     (3, 16384, "layer", "rms", 0, F16, F16), (5, 4097, "rms", "rms", 1, F16, F32), (7, 96, "rms", None, 1, BF16, BF16),
-    (7, 90, None, None, 7, F32, F32)]
+    (7, 90, None, None, 7, F32, F32), (6, 3000, "layer", "layer", 3, BF16, BF16), (4, 3001, "rms", "rms", 1, F16, F16),
+    (4, 5120, "layer", "layer", 4, F16, F32), (4, 7000, "rms", "rms", 2, BF16, BF16), (6, 7001, "layer", "layer", 1, BF16, F32),
+    (2000, 2500, "layer", "layer", 4, BF16, BF16), (900, 4500, "rms", "layer", 1, F16, F32), (3, 12288, "rms", "rms", 1, BF16, BF16)]
 
 
 def norm_inputs(case, seed=12):
