@@ -130,13 +130,16 @@ template <typename T, int N> struct Pack {
             for (int i = 0; i < N; ++i)
                 if (i >= from) p[i] = raw(i);
     }
-    // ... of what is not read again soon: past the caches
+    // ... of what is not read again soon: past the caches.  (Between fences for the compiler, which would make one store of this one and
+    // an ordinary one on the other side of a branch.)
     __device__ __forceinline__ void store_past(typename T::raw *p) const
     {
         if constexpr (BYTES >= 16) {
+            asm volatile("" ::: "memory");
 #pragma unroll
             for (int i = 0; i < BYTES / 16; ++i)
                 __builtin_nontemporal_store(Four{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]}, reinterpret_cast<Four *>(p) + i);
+            asm volatile("" ::: "memory");
         } else
             store(p);
     }

@@ -27,7 +27,7 @@ constexpr int INDEX_FOUND = 320;    // places of a wave that LDS keeps between c
 constexpr uint32_t NONE = ~0u;      // a token without a row
 constexpr int THREADS = 256;
 // Rows that a unit of threads looks at for zeros: the lanes of a wave, or what a thread reads the counts of ahead.
-constexpr int fill_rows(bool wide) { return wide ? 64 : 8; }
+constexpr int fill_rows(bool wide) { return wide ? 16 : 8; }
 
 // Row numbers and where they go.
 struct Index {
@@ -154,7 +154,7 @@ struct Sum {
     int64_t dim;
     int32_t piece, pieces;
     int32_t unit;        // threads that share a row: a power of two
-    int32_t accumulate;
+    int32_t accumulate, past;
     float scale;
     int64_t grad_stride, out_stride;
     float *partial;      // [pieces][2][dim]: of the row that began before the piece, of the one that goes on behind it
@@ -203,15 +203,19 @@ __global__ __launch_bounds__(THREADS) void embed_sum_kernel(Sum s, const typenam
         Pack<O, N> zeros;
         zeros.zero();
         if constexpr (WIDE) {
-            uint64_t none = __ballot(r0 + lane < x.rows && x.count[x.slot(r0 + lane)] == 0);
+            uint64_t none = __ballot(lane < fill_rows(true) && r0 + lane < x.rows && x.count[x.slot(r0 + lane)] == 0);
             while (none) {
-                if (in) zeros.store_past(out + (r0 + __builtin_ctzll(none)) * s.out_stride + col);
+                typename O::raw *const p = out + (r0 + __builtin_ctzll(none)) * s.out_stride + col;
+                if (in && s.past)
+                    zeros.store_past(p);
+                else if (in)
+                    zeros.store(p);
                 none &= none - 1;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < fill_rows(false); ++i)
-                if (r0 + i < x.rows && x.count[x.slot(r0 + i)] == 0) zeros.store_past(out + (r0 + i) * s.out_stride + col);
+                if (r0 + i < x.rows && x.count[x.slot(r0 + i)] == 0) zeros.store(out + (r0 + i) * s.out_stride + col);
         }
         return;
     }
@@ -346,9 +350,13 @@ __global__ __launch_bounds__(THREADS) void embed_rows_kernel(Rows s, const void 
     }
 }
 
-// An output of more bytes than that is not in the last cache (256 MB) any more when it is read, and is written past the caches: 268 MB in
-// 73 us, 80 through them; what is smaller stays for the reader.
-constexpr int64_t KEPT = (int64_t)128 << 20;
+// Whether an output is written past the caches.  One of more than half of the last cache's 256 MB is not in it any more when it is read:
+// a lookup of 268 MB takes 73 us, 80 through the caches; with its zeros past them a gradient of 1.05 GB takes 244 us, 282 through them.
+// Where rows do not begin with a line's 64 bytes, the caches put lines together: 131 MB of zeros 29 us, 41 past them.
+bool past_caches(const void *p, int64_t rows, int64_t dim, int64_t stride, int type)
+{
+    return rows * dim * size_of(type) > (128 << 20) && aligned(p, 64) && stride * size_of(type) % 64 == 0;
+}
 
 // Elements that a thread takes of a row at a time: 16 bytes of the smaller of the two types, one of rows that have less.
 int elements_at_once(int64_t dim, int type_a, int type_b)
@@ -396,9 +404,10 @@ Layout layout_of(int64_t n, int64_t rows, int64_t dim)
     while (l.shift < 8 && (1ll << l.shift) < rows) ++l.shift;
     while (ceil_div(rows, (int64_t)1 << l.shift) > INDEX_ROWS) ++l.shift;
     l.per_group = ceil_div(rows, (int64_t)1 << l.shift);
-    // A longer piece keeps fewer partial sums (each is written and read), a shorter one fills the device.
+    // A longer piece keeps fewer partial sums, which the join adds up one after another; a shorter one fills the device.  Up to 1024
+    // pieces do both: the gradient of 128256 x 4096 bf16 from 32768 tokens takes 244 us, 250 with 512, 263 with 2048 pieces.
     l.piece = 16;
-    while (l.piece < 128 && n / (2 * l.piece) * ceil_div(dim, (int64_t)2048) >= 2048) l.piece *= 2;
+    while (l.piece < 128 && n > 1024 * l.piece) l.piece *= 2;
     l.pieces = ceil_div(n, (int64_t)l.piece);
     size_t at = 0;
     const auto take = [&](size_t bytes) {
@@ -443,7 +452,7 @@ extern "C" int gdp_embed_forward(const gdp_embed *e, void *stream)
         !aligned(e->tokens, e->token_type == GDP_I64 ? 8 : 4))
         return gdp_fail(GDP_E_BADARG, "gdp_embed: a pointer is not aligned to its elements");
     const int n = elements_at_once(e->dim, e->weight_type, e->out_type);
-    Rows s{e->n, e->dim, e->rows, e->first, unit_of(e->dim, n), 1, e->token_type, e->n * e->dim * size_of(e->out_type) > KEPT, e->scale, e->weight_stride, e->out_stride};
+    Rows s{e->n, e->dim, e->rows, e->first, unit_of(e->dim, n), 1, e->token_type, past_caches(e->out, e->n, e->dim, e->out_stride, e->out_type), e->scale, e->weight_stride, e->out_stride};
     const int64_t across = ceil_div(e->dim, (int64_t)s.unit * n), per = THREADS / s.unit;
     if (ceil_div(e->n, per * 4) * across >= 2048) s.each = 4;   // rows in flight of a thread, where there are enough for all
     const int64_t blocks = ceil_div(e->n, per * s.each);
@@ -492,7 +501,8 @@ extern "C" int gdp_embed_backward(const gdp_embed_grad *e, void *stream)
                  : launch("gdp_embed_backward", embed_index_kernel<int32_t>, dim3(1u << l.shift), INDEX_THREADS, 0, stream, x, static_cast<const int32_t *>(e->tokens));
     if (rc) return rc;
     const int n = elements_at_once(e->dim, e->grad_type, e->out_type);
-    const Sum s{x, e->dim, l.piece, (int32_t)l.pieces, unit_of(e->dim, n), e->accumulate, e->scale, e->grad_stride, e->out_stride,
+    const Sum s{x, e->dim, l.piece, (int32_t)l.pieces, unit_of(e->dim, n), e->accumulate,
+                past_caches(e->out, e->rows, e->dim, e->out_stride, e->out_type), e->scale, e->grad_stride, e->out_stride,
                 reinterpret_cast<float *>(w + l.partial)};
     const int64_t across = ceil_div(e->dim, (int64_t)s.unit * n), per = THREADS / s.unit;
     const int64_t units = l.pieces + (e->accumulate ? 0 : ceil_div(e->rows, (int64_t)fill_rows(s.unit >= 64)));

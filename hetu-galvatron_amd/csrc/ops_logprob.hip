@@ -20,11 +20,11 @@
 namespace {
 using namespace ops;
 
-constexpr int THREADS = 256, WAVES = THREADS / 64, PAIRS = THREADS / 2;
+constexpr int THREADS = 256;
 constexpr int AHEAD = 4;                 // reads of 16 bytes in flight for each thread
 constexpr int MOST_CHUNKS = 8192;        // of a slice whose largest logits are asked for: 33 KB of LDS
 constexpr int MOST_CHOSEN = 128;         // chunks that are read again together (by the bound), 64 where they are taken one by one
-static_assert(MOST_CHOSEN >= GDP_MAX_TOP && PAIRS == 128 && PAIRS >= GDP_MAX_TOP, "taken one by one; two pairs for each lane");
+static_assert(MOST_CHOSEN >= GDP_MAX_TOP && GDP_MAX_TOP <= 64, "taken one by one; as many logits are seen apart");
 constexpr int MOST_SLICES = 64;          // a lane of the joining wave for each
 // Below it lse holds no digit of ln s worth having: such a row is one whose every token a mask rules out (by -inf, -1e9 or a type's
 // lowest value), and 2^(z - lse) would be 1 for each of them.
@@ -97,13 +97,15 @@ __device__ __forceinline__ float top_logp(float x, float m, float s, float scale
     return s == 0.0f ? -__builtin_inff() : fmaf(x - m, scale, -logf(s));
 }
 
-template <typename T, bool TOP> __global__ __launch_bounds__(THREADS) void logprob_scan_kernel(Scan a, const typename T::raw *__restrict__ logits)
+// WAVES: four to a row or slice; one where rows are short and many.
+template <typename T, bool TOP, int WAVES> __global__ __launch_bounds__(64 * WAVES) void logprob_scan_kernel(Scan a, const typename T::raw *__restrict__ logits)
 {
-    constexpr int VEC = T::VEC;
+    constexpr int VEC = T::VEC, THREADS = 64 * WAVES;
+    constexpr int SEEN = WAVES == 1 ? 64 : THREADS / 2;   // lanes, or pairs of lanes, whose largest logits give the bound
     extern __shared__ __align__(16) float chunk_max[];   // [64 * per_super], then their keys
     __shared__ Sums of_wave[WAVES];
     __shared__ int32_t chosen[MOST_CHOSEN], n_chosen, n_found;
-    __shared__ __align__(16) uint32_t of_pair[PAIRS];
+    __shared__ __align__(16) uint32_t seen[SEEN];
     __shared__ uint32_t least;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t row = blockIdx.x / a.slices;
@@ -158,8 +160,12 @@ template <typename T, bool TOP> __global__ __launch_bounds__(THREADS) void logpr
         own.s += sum, own.t += sum_t;
     }
     if constexpr (TOP) {
-        const float b = fmaxf(own.m, dpp<QUAD_SWAP1>(own.m, own.m));
-        if ((t & 1) == 0) of_pair[t >> 1] = key_of(b);
+        if constexpr (WAVES == 1) {
+            seen[t] = key_of(own.m);
+        } else {
+            const float b = fmaxf(own.m, dpp<QUAD_SWAP1>(own.m, own.m));
+            if ((t & 1) == 0) seen[t >> 1] = key_of(b);
+        }
         if (t == 0) n_chosen = n_found = 0;
     }
     own = wave_join(own, c);
@@ -187,20 +193,24 @@ template <typename T, bool TOP> __global__ __launch_bounds__(THREADS) void logpr
     }
     if constexpr (TOP) {
         const int chunks = v1 > v0 ? (v1 - v0 + 3) / 4 : 0, per = a.per_super;
-        // The bound, in each wave: the least of the pairs' largest logits that fewer than `top` exceed.  (What follows runs once: it is
+        // The bound, in each wave: the least of the largest logits seen that fewer than `top` exceed.  (What follows runs once: it is
         // kept in loops of few instructions, which are fetched sooner than unrolled ones.)
         uint32_t bound;
         {
-            const uint32_t one = of_pair[lane], other = of_pair[64 + lane];
-            const uint4 *const pairs = reinterpret_cast<const uint4 *>(of_pair);
-            int of_one = 0, of_other = 0;
+            const uint4 *const all_seen = reinterpret_cast<const uint4 *>(seen);
+            bound = ~0u;
+#pragma unroll
+            for (int mine = lane; mine < SEEN; mine += 64) {
+                const uint32_t one = seen[mine];
+                int larger = 0;
 #pragma unroll 4
-            for (int i = 0; i < PAIRS / 4; ++i) {
-                const uint4 q = pairs[i];
-                of_one += (q.x > one) + (q.y > one) + (q.z > one) + (q.w > one);
-                of_other += (q.x > other) + (q.y > other) + (q.z > other) + (q.w > other);
+                for (int i = 0; i < SEEN / 4; ++i) {
+                    const uint4 q = all_seen[i];
+                    larger += (q.x > one) + (q.y > one) + (q.z > one) + (q.w > one);
+                }
+                bound = min(bound, larger < a.top ? one : ~0u);
             }
-            bound = wave_min(min(of_one < a.top ? one : ~0u, of_other < a.top ? other : ~0u));
+            bound = wave_min(bound);
         }
 #pragma unroll 1
         for (int i = t; i < chunks; i += THREADS)
@@ -511,6 +521,9 @@ Part part_at(void *p, int64_t parts, int64_t n, int top)
     return {reinterpret_cast<float4 *>(w), reinterpret_cast<float *>(w + a), reinterpret_cast<int32_t *>(w + a + b)};
 }
 
+// Rows of up to so many vectors (32 KB), and at least so many of them: a wave for each row instead of four.  32768 rows of 1000 bf16 28 us,
+// 89 with four waves; of 8192 bf16, top 5, 181 and 214; but 8192 of 16384, top 5, 89 and 85.
+constexpr int SHORT = 2048, SHORT_ROWS = 2048;
 constexpr int64_t MOST_ROWS = (int64_t)1 << 21, MOST_GROUPS = (int64_t)1 << 23;   // a grid has less than 2^32 threads
 int check(int64_t n, int64_t vocab, int64_t first, int type, int token_type, int top)
 {
@@ -551,13 +564,18 @@ int scan(Scan s, const void *logits, int type, const Split &split, const char *w
     size_t lds = (size_t)64 * split.per_super * 4;
     s.most_chosen = s.top <= 24 ? MOST_CHOSEN / 2 : MOST_CHOSEN;   // (for 24 the bound leaves 27 chunks, for 64 it leaves 89; LDS for 64 lets 8 workgroups on a core)
     const size_t found = (size_t)s.most_chosen * 4 * (16 / size_of(type)) * 8;
-    if (lds < found) lds = found;
+    if (lds < found) lds = found;   // (a row of fewer chunks finds no more than they have)
+    const size_t whole = round_up((size_t)split.width * 16 / size_of(type) * 8, 16);
+    if (lds > whole && whole >= (size_t)64 * split.per_super * 4) lds = whole;
     return with_type(type, [&](auto T) {
         using TT = decltype(T);
         const auto *x = static_cast<const typename TT::raw *>(logits);
         const dim3 grid((unsigned)(s.n * split.slices));
-        return s.top ? launch(who, logprob_scan_kernel<TT, true>, grid, THREADS, lds, stream, s, x)
-                     : launch(who, logprob_scan_kernel<TT, false>, grid, THREADS, 0, stream, s, x);
+        if (split.slices == 1 && s.n >= SHORT_ROWS && split.width <= SHORT)
+            return s.top ? launch(who, logprob_scan_kernel<TT, true, 1>, grid, 64, lds, stream, s, x)
+                         : launch(who, logprob_scan_kernel<TT, false, 1>, grid, 64, 0, stream, s, x);
+        return s.top ? launch(who, logprob_scan_kernel<TT, true, 4>, grid, THREADS, lds, stream, s, x)
+                     : launch(who, logprob_scan_kernel<TT, false, 4>, grid, THREADS, 0, stream, s, x);
     });
 }
 int join(Join j, const char *who, void *stream)

@@ -31,9 +31,7 @@ __all__ = ["embedding", "embedding_grad", "TokenLogprobs", "token_logprobs", "to
 
 MAX_TOP = 64            # GDP_MAX_TOP
 MAX_NORM_DIM = 16384    # GDP_MAX_NORM_DIM
-EXPORTED_SYMBOLS = ("gdp_embed_forward", "gdp_embed_grad_workspace", "gdp_embed_backward", "gdp_logprob_workspace",
-                    "gdp_logprob_forward", "gdp_logprob_parts", "gdp_logprob_join", "gdp_logprob_backward",
-                    "gdp_norm_forward", "gdp_norm_grad_workspace", "gdp_norm_backward")
+EXPORTED_SYMBOLS = _lib.OPERATOR_SYMBOLS
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _TOKEN_TYPES = {torch.int32: 0, torch.int64: 1}
