@@ -97,6 +97,8 @@ __device__ __forceinline__ float top_logp(float x, float m, float s, float scale
     return s == 0.0f ? -__builtin_inff() : fmaf(x - m, scale, -logf(s));
 }
 
+// Bound by memory where rows are long: 8192 x 128256 bf16 in 365 us, 2.1 GB at 5.8 TB/s; 4096 x 50257 float32 with 5 alternatives in 158 us, 5.2
+// TB/s.  16 x 128256 bf16 with 20 alternatives: 10 us in 256 workgroups, 5 of them without alternatives: barriers and waits.
 // WAVES: four to a row or slice; one where rows are short and many.
 template <typename T, bool TOP, int WAVES> __global__ __launch_bounds__(64 * WAVES) void logprob_scan_kernel(Scan a, const typename T::raw *__restrict__ logits)
 {
@@ -329,6 +331,7 @@ struct Join {
 // A workgroup joins a row: a lane of each wave for each part.  Of the lists of the most likely tokens, which are sorted, the first
 // few of each, twice as many as are asked for in all, give a bound that `top` of them reach: what does not reach it is left out, and
 // what does finds its place by looking at all that do.
+// A launch and four waits for memory or barriers: 16 rows of 16 parts and 20 alternatives 7 us, 3 without alternatives.
 static_assert(GDP_MAX_TOP <= 64 && MOST_SLICES <= 64, "a lane for each");
 constexpr int JOIN_THREADS = 256;
 __global__ __launch_bounds__(JOIN_THREADS) void logprob_join_kernel(Join a)
@@ -415,7 +418,7 @@ struct Grad {
 };
 
 // out_j = scale * (delta_j - p_j (g + h (z_j - lse + entropy))): elementwise, bound by memory, but for the few columns with a delta, which
-// a workgroup reads first and writes again at the end (out may be the logits).
+// a workgroup reads first and writes again at the end (out may be the logits).  8192 x 128256 bf16 in 810 us, 4.2 GB at 5.2 TB/s.
 template <typename T, bool ENTROPY>
 __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(Grad a, const typename T::raw *logits, typename T::raw *out)
 {

@@ -15,8 +15,8 @@
  *
  * Results do not depend on timing: the same inputs give the same bits.  Sums and statistics are held in
  * float32; what has a smaller type is rounded once, to nearest even.  Strides are in elements, between
- * rows; the elements of a row are neighbours.  Data need only be aligned to its element; rows that start on
- * 16 bytes are read fastest.
+ * rows; the elements of a row are neighbours.  Data need only be aligned to its element; rows that all start on
+ * 16 bytes are read a little faster.
  */
 #ifndef GALVATRON_OPS_HIP_H
 #define GALVATRON_OPS_HIP_H
@@ -57,8 +57,8 @@ typedef struct gdp_embed {
 } gdp_embed;
 int gdp_embed_forward(const gdp_embed *e, void *stream);
 
-/* Its gradient:  out[r] = scale * sum over the n with tokens[n] == first + r of grad[n], in the order of n
- * for up to 128 of them, and beyond that in pieces of that order.  Every row is written, zeros where no
+/* Its gradient:  out[r] = scale * sum over the n with tokens[n] == first + r of grad[n], added up in the order of n
+ * over pieces of 16 to 128 tokens, and over the pieces in their order.  Every row is written, zeros where no
  * token asks for it; with `accumulate` the sums are added to what out holds, and other rows are not touched. */
 typedef struct gdp_embed_grad {
     int64_t n, rows, dim, first;

@@ -103,11 +103,11 @@ def norm_grad(**over):
 
 
 BAD = [("gdp_embed_forward", embed, o) for o in (
-    dict(n=-1), dict(rows=-1), dict(dim=-1), dict(n=1 << 26), dict(rows=(1 << 27) + 1), dict(dim=(1 << 20) + 1), dict(weight_type=3), dict(out_type=-1),
+    dict(n=-1), dict(rows=-1), dict(dim=-1), dict(first=-1), dict(n=1 << 26), dict(rows=(1 << 27) + 1), dict(dim=(1 << 20) + 1), dict(weight_type=3), dict(out_type=-1),
     dict(token_type=2), dict(tokens=None), dict(weight=None), dict(out=None), dict(weight_stride=-16), dict(out_stride=15), dict(weight_stride=1 << 60),
     dict(weight=P + 2), dict(out=P + 1), dict(tokens=P + 4))]
 BAD += [("gdp_embed_backward", embed_grad, o) for o in (
-    dict(n=-1), dict(rows=-1), dict(dim=-1), dict(grad_type=3), dict(out_type=5), dict(token_type=7), dict(tokens=None), dict(grad=None), dict(out=None),
+    dict(n=-1), dict(rows=-1), dict(dim=-1), dict(first=-1), dict(grad_type=3), dict(out_type=5), dict(token_type=7), dict(tokens=None), dict(grad=None), dict(out=None),
     dict(workspace=None), dict(workspace=P + 16), dict(workspace_bytes=10), dict(grad_stride=-1), dict(out_stride=8), dict(grad=P + 1), dict(tokens=P + 2))]
 BAD += [(name, make, o) for name, make in (("gdp_logprob_forward", logprob), ("gdp_logprob_parts", part)) for o in (
     dict(n=-1), dict(vocab=0), dict(vocab=(1 << 22) + 1), dict(n=(1 << 21) + 1), dict(logits_type=3), dict(token_type=2), dict(top=-1), dict(top=65),
