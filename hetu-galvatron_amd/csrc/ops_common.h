@@ -145,13 +145,7 @@ template <typename T, int N> struct Pack {
     }
 };
 
-// One element of a type that is known at run time (weights, which are read once a workgroup).
-__device__ __forceinline__ float up_any(const void *p, int type, int64_t at)
-{
-    return type == GDP_F32    ? F32::up(static_cast<const F32::raw *>(p)[at])
-           : type == GDP_BF16 ? BF16::up(static_cast<const BF16::raw *>(p)[at])
-                              : F16::up(static_cast<const F16::raw *>(p)[at]);
-}
+// One element of a type that is known at run time (sums of columns, written once).
 __device__ __forceinline__ void down_any(void *p, int type, int64_t at, float f)
 {
     if (type == GDP_F32)

@@ -585,7 +585,10 @@ int join(Join j, const char *who, void *stream)
 {
     j.first = (2 * j.top + j.parts - 1) / j.parts;
     if (j.first > j.top) j.first = j.top;
-    return launch(who, logprob_join_kernel, dim3((unsigned)j.n), j.top ? JOIN_THREADS : 64, (size_t)j.parts * j.top * 16, stream, j);
+    // At most `top` of the lists' first logits reach the bound, so at most top / first lists, half of them, reach it with all of those and
+    // can go on to the end; the others end among them.
+    const size_t reach = (size_t)j.parts * j.top / 2 + 2 * j.top + j.parts;
+    return launch(who, logprob_join_kernel, dim3((unsigned)j.n), j.top ? JOIN_THREADS : 64, ((size_t)j.parts * j.top + reach) * 8, stream, j);
 }
 
 }  // namespace

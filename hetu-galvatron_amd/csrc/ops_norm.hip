@@ -541,14 +541,17 @@ template <int N> using Int = std::integral_constant<int, N>;
 
 // f(most waves of a row, times that a thread's elements repeat, elements, whether they do not divide the width, threads): 16 bytes of the
 // block's type a thread, 16 waves at most; rows of less than 16 bytes an element a thread.
-template <int E, bool TAIL, typename F> int with_waves(int64_t dim, F f)
+template <int E, bool TAIL, bool FEW = true, typename F> int with_waves(int64_t dim, F f)   // FEW: there may be 8 waves or less
 {
     using Tail = std::integral_constant<bool, TAIL>;
     const int waves = (int)ceil_div(dim, (int64_t)64 * E);
-    if (waves <= 1) return f(Int<1>{}, Int<1>{}, Int<E>{}, Tail{}, 64);
+    if constexpr (FEW)
+        if (waves <= 1) return f(Int<1>{}, Int<1>{}, Int<E>{}, Tail{}, 64);
     if constexpr (E > 1) {
-        if (waves <= 4) return f(Int<4>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
-        if (waves <= 8) return f(Int<8>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
+        if constexpr (FEW) {
+            if (waves <= 4) return f(Int<4>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
+            if (waves <= 8) return f(Int<8>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
+        }
         if (waves <= 12) return f(Int<12>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
         if (waves <= 16) return f(Int<16>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
         if constexpr (E == 8) return f(Int<16>{}, Int<2>{}, Int<E>{}, Tail{}, 64 * (int)ceil_div(waves, 2));
@@ -559,7 +562,8 @@ template <int E, typename F> int with_columns(int64_t dim, F f)
 {
     if (dim < E) return with_waves<1, false>(dim, f);
     // (of float32 twice that where 16 waves do not reach otherwise: fewer repetitions, whose sums are kept in registers)
-    if (E == 4 && dim > 64 * 16 * 4) return dim % 8 ? with_waves<8, true>(dim, f) : with_waves<8, false>(dim, f);
+    if constexpr (E == 4)
+        if (dim > 64 * 16 * 4) return dim % 8 ? with_waves<8, true, false>(dim, f) : with_waves<8, false, false>(dim, f);
     return dim % E ? with_waves<E, true>(dim, f) : with_waves<E, false>(dim, f);
 }
 

@@ -250,6 +250,49 @@ def test_parts_of_a_vocabulary(cuts, dtype):
     C.close(torch.cat(grads, 1), ref, bound + C.rounded(ref, dtype))
 
 
+@pytest.mark.parametrize("top,best", [(64, "last"), (64, "spread"), (33, "first")])
+def test_join_of_64_parts(top, best):
+    """As many parts and alternatives as there may be; the best all in one part, or in all of them."""
+    g = gen(19)
+    x = normal(g, 3, 64 * 70, size=2.0)
+    if best != "spread":
+        at = 63 * 70 if best == "last" else 0
+        x[:, at:at + 70] += 100.0
+    t = tokens_of(g, 3, 64 * 70)
+    parts = [ops.logprob_parts(x[:, 70 * i:70 * (i + 1)], t, first=70 * i, top=top) for i in range(64)]
+    check_logprobs(x, t, ops.join_logprobs(parts, t, 64 * 70, entropy=True), 1.0, top)
+
+
+def test_offsets_above_32_bits():
+    """Tensors of more than 2^31 elements: what lies at their ends."""
+    g = gen(20)
+    big = torch.empty(17000, 128256, dtype=BF16, device="cuda")
+    big[-2:] = normal(g, 2, 128256, dtype=BF16, size=2.0)
+    big[:-2] = 0
+    t = torch.zeros(17000, dtype=torch.int64, device="cuda")
+    t[-2:] = torch.tensor([128255, 7])
+    r = ops.token_logprobs(big, t, entropy=True, top=3)
+    check_logprobs(big[-2:], t[-2:], ops.TokenLogprobs(*(f[-2:] for f in r)), 1.0, 3)
+    d = torch.ones(17000, device="cuda")
+    ref, bound = C.logprobs_grad(big[-2:], t[-2:], r.lse[-2:], d[-2:], 1.0)
+    ops.token_logprobs_grad(big, t, r.lse, d, into=big)
+    C.close(big[-2:], ref, bound + C.rounded(ref, BF16))
+    flat = big.view(-1)[:530000 * 4096].view(530000, 4096)      # a table, and a stream
+    flat[-3:] = normal(g, 3, 4096, dtype=BF16)
+    last = torch.tensor([529999, 529997, 530000, 529999], device="cuda")
+    assert torch.equal(ops.embedding(last, flat)[[0, 1]], flat[[529999, 529997]])
+    pre = norm_of(g, "rms", 4096, BF16)
+    out = ops.residual_norm(flat, flat, pre=pre, stats=True)
+    ref_stream, ref_normed = C.residual_norm(flat[-3:], flat[-3:], None, pre, None, 1.0, 1.0)
+    C.close(out.stream[-3:], ref_stream, C.rounded(ref_stream, BF16))
+    C.close(out.normed[-3:], ref_normed, norm_bound(ref_stream, pre, 8 * C.U * ref_stream.abs()) + C.rounded(ref_normed, BF16))
+    d = normal(g, 4, 4096, dtype=BF16)
+    grad = ops.embedding_grad(last, d, 530000)
+    ref, bound = C.embedding_grad(last.cpu() - 529990, d, 10, 1.0, 0)
+    C.close(grad[-10:], ref, bound + C.rounded(ref, BF16))
+    assert not grad[:-10].any()
+
+
 LOGPROB_GRAD = [(1, 1, 1.0), (3, 7, 0.5), (4, 500, 1.0), (3, 4097, 2.0), (2, 50257, 1.0), (300, 1025, 1.0), (2, 300001, 1.0), (0, 9, 1.0)]
 
 
