@@ -345,7 +345,7 @@ __global__ __launch_bounds__(64 * W, W <= 4 ? 4 : W <= 12 ? 3 : 1) void norm_bac
     };
     // Of 5 to 12 waves one workgroup is on a core, with registers to read a row ahead (16384 rows of 4096 bf16: 170 us, 181 with
     // two workgroups that wait in turn and 128 registers); of fewer there are several (65536 of 1024: 179, 188 ahead).
-    constexpr bool AHEAD = W == 8 || W == 12;
+    constexpr bool AHEAD = K == 1 && (W == 8 || W == 12);
     Read next;
     if (AHEAD && from < to) read(next, from);
     for (int row = from; row < to; ++row) {
@@ -554,7 +554,10 @@ template <int E, bool TAIL, bool FEW = true, typename F> int with_waves(int64_t 
         }
         if (waves <= 12) return f(Int<12>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
         if (waves <= 16) return f(Int<16>{}, Int<1>{}, Int<E>{}, Tail{}, 64 * waves);
-        if constexpr (E == 8) return f(Int<16>{}, Int<2>{}, Int<E>{}, Tail{}, 64 * (int)ceil_div(waves, 2));
+        if constexpr (E == 8) {
+            if (waves <= 24) return f(Int<12>{}, Int<2>{}, Int<E>{}, Tail{}, 64 * (int)ceil_div(waves, 2));
+            return f(Int<16>{}, Int<2>{}, Int<E>{}, Tail{}, 64 * (int)ceil_div(waves, 2));
+        }
     }
     return gdp_fail(GDP_E_BADARG, "gdp_norm: too wide");   // (not reached: 4 and 1 elements a thread are for narrower rows)
 }

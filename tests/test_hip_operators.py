@@ -380,7 +380,8 @@ NORM = [  # rows, dim, post, pre, gates, types of block and stream
     (3, 16384, "layer", "rms", 0, F16, F16), (5, 4097, "rms", "rms", 1, F16, F32), (7, 96, "rms", None, 1, BF16, BF16),
     (7, 90, None, None, 7, F32, F32), (6, 3000, "layer", "layer", 3, BF16, BF16), (4, 3001, "rms", "rms", 1, F16, F16),
     (4, 5120, "layer", "layer", 4, F16, F32), (4, 7000, "rms", "rms", 2, BF16, BF16), (6, 7001, "layer", "layer", 1, BF16, F32),
-    (2000, 2500, "layer", "layer", 4, BF16, BF16), (900, 4500, "rms", "layer", 1, F16, F32), (3, 12288, "rms", "rms", 1, BF16, BF16)]
+    (2000, 2500, "layer", "layer", 4, BF16, BF16), (900, 4500, "rms", "layer", 1, F16, F32), (3, 12288, "rms", "rms", 1, BF16, BF16),
+    (4, 9000, "layer", "layer", 2, F16, F32), (300, 12300, "rms", "rms", 1, BF16, BF16)]
 
 
 def norm_inputs(case, seed=12):
