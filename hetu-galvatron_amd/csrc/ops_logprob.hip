@@ -321,6 +321,7 @@ template <typename T, bool TOP, int WAVES> __global__ __launch_bounds__(64 * WAV
 struct Join {
     int64_t n, whole;
     int32_t parts, top, first, token_type;   // `first` of each list for the bound
+    int32_t reach;       // logits that LDS has room for behind the lists
     float scale, c;
     const void *tokens;
     Part in;
@@ -338,7 +339,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void logprob_join_kernel(Join a)
 {
     extern __shared__ __align__(16) uint64_t lists[];   // [parts][top], then the first of each, and later those that reach the bound
     __shared__ unsigned long long bound;
-    __shared__ int32_t n_found;
+    __shared__ int32_t n_found, used[GDP_MAX_TOP];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, waves = blockDim.x >> 6;
     const int64_t row = blockIdx.x;
     Sums own{-__builtin_inff(), 0.0f, 0.0f};
@@ -360,6 +361,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void logprob_join_kernel(Join a)
             if (lane < first) found[p * first + lane] = one;
         }
     if (t == 0) n_found = 0, bound = ~0ull;
+    if (t < GDP_MAX_TOP) used[t] = 0;
     const Sums all = wave_join(own, a.c);
     x = wave_max(x);
     if (t == 0) {
@@ -384,10 +386,17 @@ __global__ __launch_bounds__(JOIN_THREADS) void logprob_join_kernel(Join a)
     if (lane < a.top)
         for (int p = wave; p < a.parts; p += waves) {
             const uint64_t one = lists[p * a.top + lane];
-            if (one != 0 && one >= least) found[atomicAdd(&n_found, 1)] = one;
+            if (one != 0 && one >= least) {
+                const int to = atomicAdd(&n_found, 1);
+                if (to < a.reach) found[to] = one;
+            }
         }
     __syncthreads();
-    const int n = n_found;
+    // As parts leave them, their lists are in order and there is room for all that reach the bound.  Of a caller's lists that are not, more
+    // may reach it: then all of the lists are looked at.  A token that is there twice has two places, one behind the other.
+    const bool fits = n_found <= a.reach;
+    const uint64_t *const from = fits ? found : lists;
+    const int n = fits ? n_found : a.parts * a.top;
     const float log_s = all.s == 0.0f ? 0.0f : logf(all.s);
     const auto put = [&](int place, float logit, int32_t token) {
         if (a.part.stats) {
@@ -399,10 +408,11 @@ __global__ __launch_bounds__(JOIN_THREADS) void logprob_join_kernel(Join a)
         }
     };
     for (int i = t; i < n; i += JOIN_THREADS) {
-        const uint64_t one = found[i];
-        int place = 0;
+        const uint64_t one = from[i];
+        int place = one == 0 ? a.top : 0;
 #pragma unroll 8
-        for (int j = 0; j < n; ++j) place += found[j] > one;
+        for (int j = 0; j < n; ++j) place += from[j] > one;
+        if (place < a.top) place += atomicAdd(&used[place], 1);
         if (place < a.top) put(place, of_key((uint32_t)(one >> 32)), (int32_t)~(uint32_t)one);
     }
     for (int i = n + t; i < a.top; i += JOIN_THREADS) put(i, -__builtin_inff(), -1);   // parts of fewer tokens than are asked for
@@ -587,8 +597,8 @@ int join(Join j, const char *who, void *stream)
     if (j.first > j.top) j.first = j.top;
     // At most `top` of the lists' first logits reach the bound, so at most top / first lists, half of them, reach it with all of those and
     // can go on to the end; the others end among them.
-    const size_t reach = (size_t)j.parts * j.top / 2 + 2 * j.top + j.parts;
-    return launch(who, logprob_join_kernel, dim3((unsigned)j.n), j.top ? JOIN_THREADS : 64, ((size_t)j.parts * j.top + reach) * 8, stream, j);
+    j.reach = j.parts * j.top / 2 + 2 * j.top + j.parts;
+    return launch(who, logprob_join_kernel, dim3((unsigned)j.n), j.top ? JOIN_THREADS : 64, ((size_t)j.parts * j.top + j.reach) * 8, stream, j);
 }
 
 }  // namespace
@@ -621,7 +631,7 @@ extern "C" int gdp_logprob_forward(const gdp_logprob *l, void *stream)
         return gdp_fail(GDP_E_BADARG, "gdp_logprob: the workspace is smaller than gdp_logprob_workspace says, or not aligned to 256 bytes");
     s.part = part_at(l->workspace, split.slices, l->n, l->top);
     if (const int rc = scan(s, l->logits, l->logits_type, split, "gdp_logprob_forward", stream)) return rc;
-    return join({l->n, l->vocab, split.slices, l->top, 0, l->token_type, l->scale, l->scale * LOG2E, l->tokens, s.part, out, {}}, "gdp_logprob_forward", stream);
+    return join({l->n, l->vocab, split.slices, l->top, 0, l->token_type, 0, l->scale, l->scale * LOG2E, l->tokens, s.part, out, {}}, "gdp_logprob_forward", stream);
 }
 
 extern "C" int gdp_logprob_parts(const gdp_logprob_part *l, void *stream)
@@ -642,7 +652,7 @@ extern "C" int gdp_logprob_parts(const gdp_logprob_part *l, void *stream)
         return gdp_fail(GDP_E_BADARG, "gdp_logprob: the workspace is smaller than gdp_logprob_workspace says, or not aligned to 256 bytes");
     s.part = part_at(l->workspace, split.slices, l->n, l->top);
     if (const int rc = scan(s, l->logits, l->logits_type, split, "gdp_logprob_parts", stream)) return rc;
-    return join({l->n, (int64_t)INT32_MAX, split.slices, l->top, 0, l->token_type, l->scale, l->scale * LOG2E, l->tokens, s.part, {}, own}, "gdp_logprob_parts", stream);
+    return join({l->n, (int64_t)INT32_MAX, split.slices, l->top, 0, l->token_type, 0, l->scale, l->scale * LOG2E, l->tokens, s.part, {}, own}, "gdp_logprob_parts", stream);
 }
 
 extern "C" int gdp_logprob_join(const gdp_logprob_joint *l, void *stream)
@@ -660,7 +670,7 @@ extern "C" int gdp_logprob_join(const gdp_logprob_joint *l, void *stream)
     if (!aligned(l->stats, 16) || !aligned(l->tokens, l->token_type == GDP_I64 ? 8 : 4))
         return gdp_fail(GDP_E_BADARG, "gdp_logprob: stats not aligned to 16 bytes, or tokens not to their elements");
     const Part in{reinterpret_cast<float4 *>(const_cast<float *>(l->stats)), const_cast<float *>(l->top_logits), const_cast<int32_t *>(l->top_tokens)};
-    return join({l->n, l->vocab, l->parts, l->top, 0, l->token_type, l->scale, l->scale * LOG2E, l->tokens, in, {l->logp, l->lse, l->entropy, l->top_logp, l->out_tokens}, {}},
+    return join({l->n, l->vocab, l->parts, l->top, 0, l->token_type, 0, l->scale, l->scale * LOG2E, l->tokens, in, {l->logp, l->lse, l->entropy, l->top_logp, l->out_tokens}, {}},
                 "gdp_logprob_join", stream);
 }
 
