@@ -26,9 +26,9 @@ constexpr int MOST_CHUNKS = 8192;        // of a slice whose largest logits are 
 constexpr int MOST_CHOSEN = 128;         // chunks that are read again together (by the bound), 64 where they are taken one by one
 static_assert(MOST_CHOSEN >= GDP_MAX_TOP && GDP_MAX_TOP <= 64, "taken one by one; as many logits are seen apart");
 constexpr int MOST_SLICES = 64;          // a lane of the joining wave for each
-// Below it lse holds no digit of ln s worth having: such a row is one whose every token a mask rules out (by -inf, -1e9 or a type's
-// lowest value), and 2^(z - lse) would be 1 for each of them.
-constexpr float RULED_OUT = -1e5f;
+// Of a gradient from lse alone: below it lse is rounded by 1 or more, and exp(z - lse), which should be a share of 1, by a factor of e or
+// more.  Only masks lie there (-1e9, float32's or bfloat16's lowest value): their rows get zeros.
+constexpr float NO_DIGITS = -16777216.0f;
 
 // Order of logits as whole numbers: -inf and NaN lowest, equal ones equal (-0 is 0); 0 is none of them.
 __device__ __forceinline__ uint32_t key_of(float x)
@@ -65,6 +65,7 @@ __device__ __forceinline__ Sums wave_join(Sums a, float c)
 struct Out {
     float *logp, *lse, *entropy, *top_logp;
     int64_t *top_tokens;
+    float2 *row_stats;   // or null
 };
 struct Part {   // of a slice or a shard: [parts][n]
     float4 *stats;
@@ -89,6 +90,7 @@ __device__ __forceinline__ void finish_row(const Out &o, int64_t row, Sums a, fl
     const float ln_s = logf(a.s), lse = a.s == 0.0f ? -__builtin_inff() : fmaf(a.m, scale, ln_s);
     o.lse[row] = lse;
     o.entropy[row] = a.s == 0.0f ? 0.0f : ln_s - LN2 * (a.t / a.s);
+    if (o.row_stats) o.row_stats[row] = make_float2(a.m, ln_s);
     // (x - m) has no rounding where the token is likely, so a probability near 1 keeps its digits
     o.logp[row] = !has_token ? 0.0f : a.s == 0.0f ? -__builtin_inff() : fmaf(x - a.m, scale, -ln_s);
 }
@@ -425,11 +427,15 @@ struct Grad {
     const void *tokens;
     const float *lse, *grad_logp, *grad_lse, *entropy, *grad_entropy, *grad_top;
     const int64_t *top_tokens;
+    const float *row_stats;   // [n][2], or null: by lse
 };
 
-// out_j = scale * (delta_j - p_j (g + h (z_j - lse + entropy))): elementwise, bound by memory, but for the few columns with a delta, which
+// ln p_j = scale (x_j - m) - ln s, by the same steps as in the forward pass: a row's level cancels.  From lse alone scale x_j - lse, whose two
+// terms are off by what lse is rounded by.
+// out_j = scale * (delta_j - p_j (g + h (ln p_j + entropy))): elementwise, bound by memory, but for the few columns with a delta, which
 // a workgroup reads first and writes again at the end (out may be the logits).  8192 x 128256 bf16 in 810 us, 4.2 GB at 5.2 TB/s.
-template <typename T, bool ENTROPY>
+// STATS: from row_stats; a subtraction more for each logit, 517 x 32003 f16 with entropies 16.4 us and 15.8 from lse.
+template <typename T, bool ENTROPY, bool STATS>
 __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(Grad a, const typename T::raw *logits, typename T::raw *out)
 {
     constexpr int VEC = T::VEC;
@@ -443,8 +449,9 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(Grad a, const typ
     const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(typename T::raw));
     const int vocab = (int)a.vocab, vectors = (vocab + off + VEC - 1) / VEC;
     const int v0 = slice * a.width, v1 = v0 + a.width < vectors ? v0 + a.width : vectors;
-    const float lse = a.lse[row];
-    const bool dead = lse < RULED_OUT;
+    const float largest = STATS ? a.row_stats[2 * row] : 0.0f, log_sum = STATS ? a.row_stats[2 * row + 1] : a.lse[row];
+    const bool dead = log_sum < (STATS ? -__FLT_MAX__ : NO_DIGITS);
+    const float minus = dead ? 0.0f : -a.scale;
     const int64_t token = token_at(a.tokens, a.token_type, row);
     const float of_token = a.grad_logp && token >= 0 && token < a.whole ? a.grad_logp[row] : 0.0f;
     const int entries = 1 + a.top;
@@ -459,11 +466,13 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(Grad a, const typ
         h = a.grad_entropy[row];
         rest = a.entropy[row];
     }
+    if (dead) g = h = rest = 0.0f;   // (all p are 0, and nothing is multiplied by them)
+    const float from = dead ? 0.0f : largest, away = dead ? __builtin_inff() : log_sum;
     const auto grad_of = [&](float f) {
-        const float q = fmaf(f, a.scale, -lse);
+        const float q = fmaf(STATS ? f - from : f, a.scale, -away);
         const float p = exp2_fast(q * LOG2E);
         const float w = ENTROPY ? fmaf(h, fmaxf(q, -1e4f) + rest, g) : g;   // (p is 0 below)
-        return dead ? 0.0f : -a.scale * (p * w);
+        return minus * (p * w);
     };
     // the columns with a delta: theirs without it, from the logit, before anything is written
     float again = 0.0f;
@@ -613,10 +622,9 @@ extern "C" int gdp_logprob_workspace(int64_t n, int64_t vocab, int32_t logits_ty
     return GDP_OK;
 }
 
-extern "C" int gdp_logprob_forward(const gdp_logprob *l, void *stream)
+static int forward_rows(const gdp_logprob *l, float *row_stats, void *stream)
 {
-    gdp_clear_error();
-    if (!l) return gdp_fail(GDP_E_BADARG, "gdp_logprob: null argument");
+    if (!aligned(row_stats, 8)) return gdp_fail(GDP_E_BADARG, "gdp_logprob: row_stats must be aligned to 8 bytes");
     if (const int rc = check(l->n, l->vocab, 0, l->logits_type, l->token_type, l->top)) return rc;
     if (l->top > l->vocab) return gdp_fail(GDP_E_BADARG, "gdp_logprob: top is above the number of columns");
     if (const int rc = check_scale(l->scale)) return rc;
@@ -624,7 +632,7 @@ extern "C" int gdp_logprob_forward(const gdp_logprob *l, void *stream)
     if (const int rc = check_logits(l->logits, l->n, l->vocab, l->logits_stride, l->logits_type, l->tokens, l->token_type, false)) return rc;
     if (!l->logp || !l->lse || !l->entropy || (l->top && (!l->top_logp || !l->top_tokens))) return gdp_fail(GDP_E_BADARG, "gdp_logprob: null pointer");
     const Split split = split_of(l->n, l->vocab, l->logits_type, l->top);
-    const Out out{l->logp, l->lse, l->entropy, l->top_logp, l->top_tokens};
+    const Out out{l->logp, l->lse, l->entropy, l->top_logp, l->top_tokens, reinterpret_cast<float2 *>(row_stats)};
     Scan s{l->n, l->vocab, l->logits_stride, 0, l->vocab, l->token_type, l->top, 1, 0, 1, 0, l->scale, 0.0f, l->tokens, out, {}};
     if (split.slices == 1) return scan(s, l->logits, l->logits_type, split, "gdp_logprob_forward", stream);
     if (!aligned(l->workspace, 256) || !l->workspace || l->workspace_bytes < part_bytes(split.slices, l->n, l->top))
@@ -632,6 +640,19 @@ extern "C" int gdp_logprob_forward(const gdp_logprob *l, void *stream)
     s.part = part_at(l->workspace, split.slices, l->n, l->top);
     if (const int rc = scan(s, l->logits, l->logits_type, split, "gdp_logprob_forward", stream)) return rc;
     return join({l->n, l->vocab, split.slices, l->top, 0, l->token_type, 0, l->scale, l->scale * LOG2E, l->tokens, s.part, out, {}}, "gdp_logprob_forward", stream);
+}
+
+extern "C" int gdp_logprob_forward(const gdp_logprob *l, void *stream)
+{
+    gdp_clear_error();
+    return l ? forward_rows(l, nullptr, stream) : gdp_fail(GDP_E_BADARG, "gdp_logprob: null argument");
+}
+
+extern "C" int gdp_logprob_forward_stats(const gdp_logprob_stats *l, void *stream)
+{
+    gdp_clear_error();
+    if (!l || (!l->row_stats && l->given.n != 0)) return gdp_fail(GDP_E_BADARG, "gdp_logprob: null argument");
+    return forward_rows(&l->given, l->row_stats, stream);
 }
 
 extern "C" int gdp_logprob_parts(const gdp_logprob_part *l, void *stream)
@@ -655,10 +676,9 @@ extern "C" int gdp_logprob_parts(const gdp_logprob_part *l, void *stream)
     return join({l->n, (int64_t)INT32_MAX, split.slices, l->top, 0, l->token_type, 0, l->scale, l->scale * LOG2E, l->tokens, s.part, {}, own}, "gdp_logprob_parts", stream);
 }
 
-extern "C" int gdp_logprob_join(const gdp_logprob_joint *l, void *stream)
+static int join_rows(const gdp_logprob_joint *l, float *row_stats, void *stream)
 {
-    gdp_clear_error();
-    if (!l) return gdp_fail(GDP_E_BADARG, "gdp_logprob: null argument");
+    if (!aligned(row_stats, 8)) return gdp_fail(GDP_E_BADARG, "gdp_logprob: row_stats must be aligned to 8 bytes");
     if (l->n < 0 || l->n > MOST_ROWS || l->vocab < 1 || l->vocab > INT32_MAX) return gdp_fail(GDP_E_BADARG, "gdp_logprob: a size is out of range");
     if (l->parts < 1 || l->parts > GDP_MAX_LOGPROB_PARTS) return gdp_fail(GDP_E_BADARG, "gdp_logprob: parts must be 1 to GDP_MAX_LOGPROB_PARTS");
     if (l->top < 0 || l->top > GDP_MAX_TOP || l->top > l->vocab) return gdp_fail(GDP_E_BADARG, "gdp_logprob: top must be 0 to GDP_MAX_TOP and at most the vocabulary");
@@ -670,21 +690,33 @@ extern "C" int gdp_logprob_join(const gdp_logprob_joint *l, void *stream)
     if (!aligned(l->stats, 16) || !aligned(l->tokens, l->token_type == GDP_I64 ? 8 : 4))
         return gdp_fail(GDP_E_BADARG, "gdp_logprob: stats not aligned to 16 bytes, or tokens not to their elements");
     const Part in{reinterpret_cast<float4 *>(const_cast<float *>(l->stats)), const_cast<float *>(l->top_logits), const_cast<int32_t *>(l->top_tokens)};
-    return join({l->n, l->vocab, l->parts, l->top, 0, l->token_type, 0, l->scale, l->scale * LOG2E, l->tokens, in, {l->logp, l->lse, l->entropy, l->top_logp, l->out_tokens}, {}},
+    return join({l->n, l->vocab, l->parts, l->top, 0, l->token_type, 0, l->scale, l->scale * LOG2E, l->tokens, in, {l->logp, l->lse, l->entropy, l->top_logp, l->out_tokens, reinterpret_cast<float2 *>(row_stats)}, {}},
                 "gdp_logprob_join", stream);
 }
 
-extern "C" int gdp_logprob_backward(const gdp_logprob_grad *l, void *stream)
+extern "C" int gdp_logprob_join(const gdp_logprob_joint *l, void *stream)
 {
     gdp_clear_error();
-    if (!l) return gdp_fail(GDP_E_BADARG, "gdp_logprob: null argument");
+    return l ? join_rows(l, nullptr, stream) : gdp_fail(GDP_E_BADARG, "gdp_logprob: null argument");
+}
+
+extern "C" int gdp_logprob_join_stats(const gdp_logprob_joint_stats *l, void *stream)
+{
+    gdp_clear_error();
+    if (!l || (!l->row_stats && l->given.n != 0)) return gdp_fail(GDP_E_BADARG, "gdp_logprob: null argument");
+    return join_rows(&l->given, l->row_stats, stream);
+}
+
+static int backward_rows(const gdp_logprob_grad *l, const float *row_stats, void *stream)
+{
+    if (!aligned(row_stats, 8)) return gdp_fail(GDP_E_BADARG, "gdp_logprob: row_stats must be aligned to 8 bytes");
     if (const int rc = check(l->n, l->vocab, l->first, l->logits_type, l->token_type, l->top)) return rc;
     if (l->whole_vocab < 1) return gdp_fail(GDP_E_BADARG, "gdp_logprob: a size is out of range");
     if (const int rc = check_scale(l->scale)) return rc;
     if (l->n == 0) return GDP_OK;
     if (const int rc = check_logits(l->logits, l->n, l->vocab, l->logits_stride, l->logits_type, l->tokens, l->token_type, false)) return rc;
     if (const int rc = check_logits(l->out, l->n, l->vocab, l->out_stride, l->logits_type, l->tokens, l->token_type, true)) return rc;
-    if (!l->lse || !l->entropy != !l->grad_entropy || (l->top && (!l->top_tokens || !l->grad_top))) return gdp_fail(GDP_E_BADARG, "gdp_logprob: null pointer");
+    if ((!l->lse && !row_stats) || !l->entropy != !l->grad_entropy || (l->top && (!l->top_tokens || !l->grad_top))) return gdp_fail(GDP_E_BADARG, "gdp_logprob: null pointer");
     if (l->out == l->logits && l->out_stride != l->logits_stride) return gdp_fail(GDP_E_BADARG, "gdp_logprob: a gradient in the place of the logits needs their stride");
     const int vec = 16 / size_of(l->logits_type);
     const int64_t vectors = ceil_div(l->vocab, (int64_t)vec) + 1;
@@ -693,13 +725,29 @@ extern "C" int gdp_logprob_backward(const gdp_logprob_grad *l, void *stream)
     const int64_t width = ceil_div(vectors, slices);
     slices = ceil_div(vectors, width);
     const Grad g{l->vocab, l->logits_stride, l->out_stride, l->first, l->whole_vocab, l->token_type, l->top, (int32_t)slices, (int32_t)width, l->scale,
-                 l->tokens, l->lse, l->grad_logp, l->grad_lse, l->entropy, l->grad_entropy, l->grad_top, l->top_tokens};
+                 l->tokens, l->lse, l->grad_logp, l->grad_lse, l->entropy, l->grad_entropy, l->grad_top, l->top_tokens, row_stats};
     return with_type(l->logits_type, [&](auto T) {
         using TT = decltype(T);
         const auto *x = static_cast<const typename TT::raw *>(l->logits);
         auto *y = static_cast<typename TT::raw *>(l->out);
         const dim3 grid((unsigned)(l->n * slices));
-        return l->entropy ? launch("gdp_logprob_backward", logprob_grad_kernel<TT, true>, grid, THREADS, 0, stream, g, x, y)
-                          : launch("gdp_logprob_backward", logprob_grad_kernel<TT, false>, grid, THREADS, 0, stream, g, x, y);
+        const auto run = [&](auto ENTROPY, auto STATS) {
+            return launch("gdp_logprob_backward", logprob_grad_kernel<TT, ENTROPY.value, STATS.value>, grid, THREADS, 0, stream, g, x, y);
+        };
+        const auto with = [&](auto ENTROPY) { return row_stats ? run(ENTROPY, std::true_type{}) : run(ENTROPY, std::false_type{}); };
+        return l->entropy ? with(std::true_type{}) : with(std::false_type{});
     });
+}
+
+extern "C" int gdp_logprob_backward(const gdp_logprob_grad *l, void *stream)
+{
+    gdp_clear_error();
+    return l ? backward_rows(l, nullptr, stream) : gdp_fail(GDP_E_BADARG, "gdp_logprob: null argument");
+}
+
+extern "C" int gdp_logprob_backward_stats(const gdp_logprob_grad_stats *l, void *stream)
+{
+    gdp_clear_error();
+    if (!l || (!l->row_stats && l->given.n != 0)) return gdp_fail(GDP_E_BADARG, "gdp_logprob: null argument");
+    return backward_rows(&l->given, l->row_stats, stream);
 }

@@ -46,6 +46,7 @@ EXPORTED_SYMBOLS = ("gdp_solve", "gdp_solve_batch", "gdp_solve_static", "gdp_pla
 # of include/galvatron_ops_hip.h (galvatron_dp.operators has their signatures)
 OPERATOR_SYMBOLS = ("gdp_embed_forward", "gdp_embed_grad_workspace", "gdp_embed_backward", "gdp_logprob_workspace",
                     "gdp_logprob_forward", "gdp_logprob_parts", "gdp_logprob_join", "gdp_logprob_backward",
+                    "gdp_logprob_forward_stats", "gdp_logprob_join_stats", "gdp_logprob_backward_stats",
                     "gdp_norm_forward", "gdp_norm_grad_workspace", "gdp_norm_backward")
 
 _i32p = ctypes.POINTER(ctypes.c_int32)

@@ -75,10 +75,11 @@ class ModelEnds:
         if self.shards > 1:
             raise ValueError("a shard's loss needs the parts of the others: forward, join_logprobs, token_logprobs_grad")
         joined, logits = self.logits(self.embed(tokens), block, stats=True)
-        r = ops.token_logprobs(logits, targets, entropy=True)
+        row_stats = torch.empty(*targets.shape, 2, device=logits.device)
+        r = ops.token_logprobs(logits, targets, entropy=True, row_stats=row_stats)
         held = (targets >= 0) & (targets < self.vocab)
         each = held / held.sum().clamp(min=1)
-        d_logits = ops.token_logprobs_grad(logits, targets, r.lse, -each.float(), into=logits)
+        d_logits = ops.token_logprobs_grad(logits, targets, None, -each.float(), row_stats=row_stats, into=logits)
         rows, normed = (t.reshape(-1, t.shape[-1]) for t in (d_logits, joined.normed))
         d_normed, d_head = rows @ self.head, rows.t() @ normed
         g = ops.residual_norm_grad(joined.stream, block, joined.stats, d_normed.view_as(joined.normed), pre=self.norm)

@@ -77,6 +77,18 @@ class gdp_logprob_grad(ctypes.Structure):
                 ("top_tokens", _p), ("grad_top", _p), ("out", _p), ("out_stride", _i64)]
 
 
+class gdp_logprob_stats(ctypes.Structure):
+    _fields_ = [("given", gdp_logprob), ("row_stats", _p)]
+
+
+class gdp_logprob_joint_stats(ctypes.Structure):
+    _fields_ = [("given", gdp_logprob_joint), ("row_stats", _p)]
+
+
+class gdp_logprob_grad_stats(ctypes.Structure):
+    _fields_ = [("given", gdp_logprob_grad), ("row_stats", _p)]
+
+
 class gdp_norm_params(ctypes.Structure):
     _fields_ = [("form", _i32), ("type", _i32), ("eps", _f32), ("reserved", _i32), ("weight", _p), ("bias", _p)]
 
@@ -117,6 +129,9 @@ def _ops() -> ctypes.CDLL:
         for name, record in (("gdp_embed_forward", gdp_embed), ("gdp_embed_backward", gdp_embed_grad),
                              ("gdp_logprob_forward", gdp_logprob), ("gdp_logprob_parts", gdp_logprob_part),
                              ("gdp_logprob_join", gdp_logprob_joint), ("gdp_logprob_backward", gdp_logprob_grad),
+                             ("gdp_logprob_forward_stats", gdp_logprob_stats),
+                             ("gdp_logprob_join_stats", gdp_logprob_joint_stats),
+                             ("gdp_logprob_backward_stats", gdp_logprob_grad_stats),
                              ("gdp_norm_forward", gdp_norm), ("gdp_norm_backward", gdp_norm_grad)):
             f = getattr(L, name)
             f.argtypes, f.restype = [ctypes.POINTER(record), ctypes.c_void_p], ctypes.c_int
@@ -333,29 +348,43 @@ def _outputs(shape, top, device):
             torch.empty(shape + (top,), dtype=torch.int64, device=device))
 
 
-def _token_logprobs(logits, tokens, scale, top):
+def _row_stats(t, shape, device):
+    """Whether there are any, after checking them."""
+    if t is None:
+        return False
+    if t.shape != shape + (2,) or t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
+        raise ValueError(f"row_stats must be {list(shape + (2,))} float32 on {device}, in order")
+    return True
+
+
+def _token_logprobs(logits, tokens, scale, top, row_stats):
     logits_type = _type(logits, "logits")
     if logits.dim() < 1:
         raise ValueError("logits must be [..., vocab]")
     _check_top(top)
     device, vocab, shape = logits.device, logits.shape[-1], logits.shape[:-1]
     flat, token_type = _tokens_for(tokens, shape, device)
+    with_stats = _row_stats(row_stats, shape, device)
     n, logp, lse, entropy, top_logp, top_tokens = _outputs(shape, top, device)
     rows, stride = _rows(logits, vocab, "logits") if n and vocab else (logits, vocab)
     L = _ops()
     work, size = _workspace("gdp_logprob_workspace", n, vocab, logits_type, top, device=device)
-    _queue(L.gdp_logprob_forward,
-           gdp_logprob(n, vocab, rows.data_ptr(), stride, logits_type, token_type, flat.data_ptr(), scale, top,
-                       logp.data_ptr(), lse.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_tokens), _ptr(work),
-                       size), device)
+    given = gdp_logprob(n, vocab, rows.data_ptr(), stride, logits_type, token_type, flat.data_ptr(), scale, top,
+                        logp.data_ptr(), lse.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_tokens), _ptr(work), size)
+    if with_stats and n:
+        _queue(L.gdp_logprob_forward_stats, gdp_logprob_stats(given, row_stats.data_ptr()), device)
+    else:
+        _queue(L.gdp_logprob_forward, given, device)
     return logp, lse, entropy, top_logp, top_tokens
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, scale, top):
-        logp, lse, entropy, top_logp, top_tokens = _token_logprobs(logits, tokens, scale, top)
-        ctx.save_for_backward(logits, tokens, lse, entropy, top_tokens)
+    def forward(ctx, logits, tokens, scale, top, row_stats):
+        if row_stats is None:
+            row_stats = torch.empty(logits.shape[:-1] + (2,), dtype=torch.float32, device=logits.device)
+        logp, lse, entropy, top_logp, top_tokens = _token_logprobs(logits, tokens, scale, top, row_stats)
+        ctx.save_for_backward(logits, tokens, row_stats, entropy, top_tokens)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         if top_tokens is not None:
@@ -365,33 +394,42 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_logp, d_lse, d_entropy, d_top, _):
-        logits, tokens, lse, entropy, top_tokens = ctx.saved_tensors
-        return token_logprobs_grad(logits, tokens, lse, d_logp, scale=ctx.scale, grad_lse=d_lse,
+        logits, tokens, row_stats, entropy, top_tokens = ctx.saved_tensors
+        return token_logprobs_grad(logits, tokens, None, d_logp, scale=ctx.scale, grad_lse=d_lse,
                                    entropy=None if d_entropy is None else entropy, grad_entropy=d_entropy,
-                                   top_tokens=None if d_top is None else top_tokens, grad_top=d_top), None, None, None
+                                   top_tokens=None if d_top is None else top_tokens, grad_top=d_top,
+                                   row_stats=row_stats), None, None, None, None
 
 
-def token_logprobs(logits, tokens, *, scale: float = 1.0, entropy: bool = False, top: int = 0) -> TokenLogprobs:
+def token_logprobs(logits, tokens, *, scale: float = 1.0, entropy: bool = False, top: int = 0,
+                   row_stats: Optional[torch.Tensor] = None) -> TokenLogprobs:
     """Log probabilities of ``tokens`` [...] under softmax(scale * logits) over the last dimension of ``logits`` [..., vocab],
     the log of the sum of exponentials, with ``entropy`` each row's entropy, and the ``top`` (at most 64) most likely
     tokens: equal logits by number, the lowest first.  All in float32, from one pass over the logits.
 
     A token outside [0, vocab), such as -100, is none: its log probability is 0, and it gives no gradient.  Logits of
     -inf are tokens that are ruled out; a row of nothing else has lse and log probabilities of -inf, entropy 0, and a
-    gradient of zeros.  NaN or +inf make their row's results NaN."""
+    gradient of zeros.  NaN or +inf make their row's results NaN.  Any other row, one of a mask's -1e9 alone among them, has
+    the log probabilities, entropy and gradient of its logits less the largest.
+
+    ``row_stats`` [..., 2] float32: written, the largest logit and the log of the sum relative to it, for
+    ``token_logprobs_grad``."""
     if torch.is_grad_enabled() and logits.requires_grad:
-        r = _TokenLogprobs.apply(logits, tokens, float(scale), int(top))
+        r = _TokenLogprobs.apply(logits, tokens, float(scale), int(top), row_stats)
     else:
-        r = _token_logprobs(logits, tokens, float(scale), int(top))
+        r = _token_logprobs(logits, tokens, float(scale), int(top), row_stats)
     return TokenLogprobs(r[0], r[1], r[2] if entropy else None, r[3], r[4])
 
 
 def token_logprobs_grad(logits, tokens, lse, grad_logp=None, *, scale: float = 1.0, grad_lse=None, entropy=None,
                         grad_entropy=None, top_tokens=None, grad_top=None, first: int = 0,
-                        vocab: Optional[int] = None, into: Optional[torch.Tensor] = None):
+                        vocab: Optional[int] = None, into: Optional[torch.Tensor] = None,
+                        row_stats: Optional[torch.Tensor] = None):
     """Gradient with respect to ``logits`` [..., columns], in their type, from those of ``token_logprobs``' results.
 
-    ``lse`` (and ``entropy``, ``top_tokens`` where they have gradients) are what the forward pass gave.  Of a vocabulary in
+    ``row_stats``: what the forward pass wrote there; ``lse`` is not read then and may be None.  From ``lse`` alone, which float32
+    rounds by one part in 2^24, probabilities are off by |lse| / 2^24 of themselves, and rows whose lse is below -2^24 (nothing but
+    a mask's -1e9) have zeros.  ``lse`` (and ``entropy``, ``top_tokens`` where they have gradients) are what the forward pass gave.  Of a vocabulary in
     shards, ``logits`` are those of the shard that begins with token ``first``, of ``vocab`` tokens in all, and ``lse``,
     ``entropy`` and ``top_tokens`` those of ``join_logprobs``.  ``into``: written there; it may be ``logits`` itself."""
     logits_type = _type(logits, "logits")
@@ -403,9 +441,10 @@ def token_logprobs_grad(logits, tokens, lse, grad_logp=None, *, scale: float = 1
     flat, token_type = _tokens_for(tokens, shape, device)
     if (entropy is None) != (grad_entropy is None) or (top_tokens is None) != (grad_top is None):
         raise ValueError("entropy and grad_entropy, top_tokens and grad_top come together")
-    lse = _floats(lse, shape, "lse", device)
-    if lse is None:
-        raise ValueError("lse is needed")
+    with_stats = _row_stats(row_stats, shape, device)
+    lse = None if with_stats else _floats(lse, shape, "lse", device)
+    if lse is None and not with_stats:
+        raise ValueError("row_stats or lse is needed")
     grad_logp, grad_lse = _floats(grad_logp, shape, "grad_logp", device), _floats(grad_lse, shape, "grad_lse", device)
     entropy, grad_entropy = _floats(entropy, shape, "entropy", device), _floats(grad_entropy, shape, "grad_entropy", device)
     top = 0
@@ -431,10 +470,13 @@ def token_logprobs_grad(logits, tokens, lse, grad_logp=None, *, scale: float = 1
             raise RuntimeError
     except RuntimeError:
         raise ValueError("into must have rows that are neighbouring elements at one stride") from None
-    _queue(_ops().gdp_logprob_backward,
-           gdp_logprob_grad(n, columns, first, vocab, rows.data_ptr(), stride, logits_type, token_type, flat.data_ptr(), scale,
-                            top, lse.data_ptr(), _ptr(grad_logp), _ptr(grad_lse), _ptr(entropy), _ptr(grad_entropy),
-                            _ptr(top_tokens), _ptr(grad_top), to.data_ptr(), to.stride(0)), device)
+    given = gdp_logprob_grad(n, columns, first, vocab, rows.data_ptr(), stride, logits_type, token_type, flat.data_ptr(), scale,
+                             top, _ptr(lse), _ptr(grad_logp), _ptr(grad_lse), _ptr(entropy), _ptr(grad_entropy),
+                             _ptr(top_tokens), _ptr(grad_top), to.data_ptr(), to.stride(0))
+    if with_stats:
+        _queue(_ops().gdp_logprob_backward_stats, gdp_logprob_grad_stats(given, row_stats.data_ptr()), device)
+    else:
+        _queue(_ops().gdp_logprob_backward, given, device)
     return out
 
 
@@ -460,9 +502,11 @@ def logprob_parts(logits, tokens, *, first: int, scale: float = 1.0, top: int = 
     return parts
 
 
-def join_logprobs(parts, tokens, vocab: int, *, scale: float = 1.0, entropy: bool = False) -> TokenLogprobs:
+def join_logprobs(parts, tokens, vocab: int, *, scale: float = 1.0, entropy: bool = False,
+                  row_stats: Optional[torch.Tensor] = None) -> TokenLogprobs:
     """``token_logprobs`` of a vocabulary of ``vocab`` tokens from the parts of its shards: ``LogprobParts`` in the order of
-    their tokens, or one whose tensors have a leading dimension for the shards, as gathering them leaves it."""
+    their tokens, or one whose tensors have a leading dimension for the shards, as gathering them leaves it.  ``row_stats``: as
+    there, of the whole rows."""
     if not isinstance(parts, LogprobParts):
         parts = LogprobParts(*(torch.stack(t) for t in zip(*parts)))
     stats, top_logits, top_tokens = (t.contiguous() for t in parts)
@@ -474,11 +518,15 @@ def join_logprobs(parts, tokens, vocab: int, *, scale: float = 1.0, entropy: boo
     device, count, shape, top = stats.device, stats.shape[0], stats.shape[1:2], top_logits.shape[2]
     _same_device(device, top_logits=top_logits, top_tokens=top_tokens)
     flat, token_type = _tokens_for(tokens, shape, device)
+    with_stats = _row_stats(row_stats, shape, device)
     n, logp, lse, ent, top_logp, out_tokens = _outputs(shape, top, device)
-    _queue(_ops().gdp_logprob_join,
-           gdp_logprob_joint(n, vocab, count, top, scale, token_type, flat.data_ptr(), stats.data_ptr(),
-                             top_logits.data_ptr(), top_tokens.data_ptr(), logp.data_ptr(), lse.data_ptr(), ent.data_ptr(),
-                             _ptr(top_logp), _ptr(out_tokens)), device)
+    given = gdp_logprob_joint(n, vocab, count, top, scale, token_type, flat.data_ptr(), stats.data_ptr(), top_logits.data_ptr(),
+                              top_tokens.data_ptr(), logp.data_ptr(), lse.data_ptr(), ent.data_ptr(), _ptr(top_logp),
+                              _ptr(out_tokens))
+    if with_stats and n:
+        _queue(_ops().gdp_logprob_join_stats, gdp_logprob_joint_stats(given, row_stats.data_ptr()), device)
+    else:
+        _queue(_ops().gdp_logprob_join, given, device)
     return TokenLogprobs(logp, lse, ent if entropy else None, top_logp, out_tokens)
 
 

@@ -84,7 +84,8 @@ int gdp_embed_backward(const gdp_embed_grad *e, void *stream);
  *   top_*   = the `top` largest logits, largest first, equal ones by number: log probability and token.
  *             NaN counts as -inf there.
  * A logit of -inf is a token that is ruled out.  Where all are, lse and logp are -inf and the entropy is 0.  A row
- * with NaN or +inf has NaN for its lse, logp and entropy. */
+ * with NaN or +inf has NaN for its lse, logp and entropy.  lse is rounded to float32: -inf or inf where it is outside
+ * of its range, though logp and entropy, which the row's level has no part in, are not. */
 typedef struct gdp_logprob {
     int64_t n, vocab;       /* rows, columns                              */
     const void *logits;     /* [n][vocab]                                 */
@@ -102,6 +103,14 @@ typedef struct gdp_logprob {
 } gdp_logprob;
 int gdp_logprob_workspace(int64_t n, int64_t vocab, int32_t logits_type, int32_t top, size_t *bytes);
 int gdp_logprob_forward(const gdp_logprob *l, void *stream);
+/* ... and row_stats [n][2]: the row's largest logit m, and log(sum(exp(scale * (logits[row] - m)))).  Their sum, scale * m
+ * added, is lse; apart they keep the digits that lse is rounded by, which the gradient of rows far from zero needs.
+ * 8-byte aligned. */
+typedef struct gdp_logprob_stats {
+    gdp_logprob given;
+    float *row_stats;
+} gdp_logprob_stats;
+int gdp_logprob_forward_stats(const gdp_logprob_stats *l, void *stream);
 
 /* The same for a vocabulary in shards: `parts` of each shard, whose first column is token `first`, are joined
  * after the ranks have exchanged them (20 + 8 * top bytes a row instead of the row).  Of a part:
@@ -139,12 +148,19 @@ typedef struct gdp_logprob_joint {
     int64_t *out_tokens;    /* [n][top]                                   */
 } gdp_logprob_joint;
 int gdp_logprob_join(const gdp_logprob_joint *l, void *stream);
+typedef struct gdp_logprob_joint_stats {
+    gdp_logprob_joint given;
+    float *row_stats;       /* as of gdp_logprob_stats, of the whole row  */
+} gdp_logprob_joint_stats;
+int gdp_logprob_join_stats(const gdp_logprob_joint_stats *l, void *stream);
 
 /* Gradient with respect to the logits (of a shard whose first column is token `first`), from the gradients of
  * logp, lse, entropy and top_logp:
  *   out_j = scale * (g (1[j = token] - p_j) + l p_j - h p_j (z_j - lse + entropy) + sum_i t_i (1[j = top_tokens_i] - p_j))
- * Zeros for a row whose lse is below -1e5: a mask (-inf, -1e9, a type's lowest value) rules out all of its tokens.
- * A token outside the vocabulary has no g.  out may be logits itself, and does not overlap them otherwise. */
+ * with p_j = exp(z_j - lse), of the lse that is given.  float32 rounds lse by one part in 2^24, so p_j is off by |lse| / 2^24
+ * of itself; a row whose lse is below -2^24 has zeros (all of its tokens are masked, by -inf, -1e9 or the lowest value of
+ * float32 or bfloat16).  gdp_logprob_backward_stats takes row_stats instead, with which rows at any level have the gradient
+ * of their logp, and only one whose logits are all -inf has zeros.  A token outside the vocabulary has no g.  out may be logits itself, and does not overlap them otherwise. */
 typedef struct gdp_logprob_grad {
     int64_t n, vocab, first;
     int64_t whole_vocab;       /* tokens outside [0, whole_vocab) are none */
@@ -164,6 +180,11 @@ typedef struct gdp_logprob_grad {
     int64_t out_stride;
 } gdp_logprob_grad;
 int gdp_logprob_backward(const gdp_logprob_grad *l, void *stream);
+typedef struct gdp_logprob_grad_stats {
+    gdp_logprob_grad given;    /* its lse is not read and may be NULL     */
+    const float *row_stats;    /* [n][2], of the whole row                */
+} gdp_logprob_grad_stats;
+int gdp_logprob_backward_stats(const gdp_logprob_grad_stats *l, void *stream);
 
 /* A block's output joined with the residual stream, with norms on both sides of the join:
  *   b      = post-norm of block (where post is not GDP_NORM_NONE), times gate

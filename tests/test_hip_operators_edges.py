@@ -47,3 +47,139 @@ def test_join_of_lists_that_parts_do_not_leave(parts, top, order):
         ref = torch.tensor([-v for v, _ in best], dtype=torch.float64) - got.lse[row].double().cpu()
         # lse is rounded, and so are the logit's distance and the logarithm that top_logp is made of
         C.close(got.top_logp[row], ref, 8 * C.U * (2 * logits[row].double().abs().max() + 10))
+
+# ---- gradients of rows far from zero ------------------------------------------------------------------------
+def far_rows(g, dtype, vocab):
+    """Rows of finite logits at any level, of masks alone, and one of which nothing is left."""
+    low = torch.finfo(dtype).min
+    step = {F32: 1.0, F16: 32.0, BF16: 512.0}[dtype]        # what the type can tell apart there
+    at = {F32: -1.2e5, F16: -6.0e4, BF16: -1.2e5}[dtype]
+    x = torch.randn(7, vocab, generator=g)
+    x[1] = at + step * torch.randint(0, 4, (vocab,), generator=g)
+    x[2] = low
+    x[3] = at if dtype == F16 else -1e9
+    x[4] = -at + step * torch.randint(0, 4, (vocab,), generator=g)
+    x[5] = low
+    x[5, vocab // 2:] = torch.randn(vocab - vocab // 2, generator=g)
+    x[6] = -math.inf
+    return x.to(dtype).cuda()
+
+
+def softmax_grads(x, t, scale, a, b, c, d, top, columns=slice(None)):
+    """(gradient of a logp + b entropy + c top_logp + d lse, a bound on its float32 error), from the definition: the shift by the largest
+    logit cancels exactly.  A probability's exponent has three roundings of its own size, the logarithm of the sum those of its terms."""
+    x = x.detach().cpu().double()
+    n, vocab = x.shape
+    z = (x - x.amax(1, keepdim=True).clamp(min=-1e300)) * scale
+    q = z - torch.logsumexp(z, 1, keepdim=True).clamp(min=-1e300)
+    p = q.exp()
+    alive = torch.isfinite(x).any(1)
+    a, b, c, d = (v.cpu().double() for v in (a, b, c, d))
+    rows = torch.arange(n)
+    entropy = -torch.where(p > 0, p * q, 0.0).sum(1)
+    hit, of_hit = torch.zeros(n, vocab, dtype=torch.float64), torch.zeros(n, vocab, dtype=torch.float64)
+    held = (t.cpu() >= 0) & (t.cpu() < vocab)
+    a = a * held
+    hit[rows[held], t.cpu()[held]] += a[held]
+    of_hit[rows[held], t.cpu()[held]] += a[held].abs()
+    for i in range(c.shape[1]):
+        hit[rows, top[:, i].cpu()] += c[:, i]
+        of_hit[rows, top[:, i].cpu()] += c[:, i].abs()
+    weight, of_weight = (a + c.sum(1) - d)[:, None], (a.abs() + c.abs().sum(1) + d.abs())[:, None]
+    away = torch.where(p > 0, q + entropy[:, None], 0.0)
+    grad = hit - p * (weight + b[:, None] * away)
+    size = of_hit + p * (of_weight + b.abs()[:, None] * (torch.where(p > 0, q.abs(), 0.0) + entropy[:, None]))
+    ln_v = math.log(max(vocab, 2))
+    relative = C.U * (80 + 8 * ln_v + vocab / 256 + c.shape[1] + 8 * torch.where(p > 0, q.abs(), 0.0))
+    off = size * relative + p * b.abs()[:, None] * C.logprob_bound(torch.zeros(1, vocab), 1.0)[2]
+    grad, off = (torch.where(alive[:, None], v, 0.0)[:, columns] * scale for v in (grad, off))
+    return grad, off
+
+
+@pytest.mark.parametrize("scale", [1.0, 1.25, 0.5], ids=str)
+@pytest.mark.parametrize("vocab", [9, 2500, 70001])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_gradients_do_not_go_by_the_level_of_a_row(dtype, vocab, scale):
+    """A row's logits may lie anywhere: its gradient is the softmax's, as its log probabilities are, and zeros where nothing is left."""
+    g = gen(32)
+    x = far_rows(g, dtype, vocab).requires_grad_()
+    n, k = x.shape[0], 3
+    t = torch.randint(0, vocab, (n,), generator=g).cuda()
+    t[0] = -100
+    a, b, c, d = normal(g, n), normal(g, n), normal(g, n, k), normal(g, n)
+    r = ops.token_logprobs(x, t, scale=scale, entropy=True, top=k)
+    used = torch.isfinite(r.lse)                      # (float32's lowest value times 1.25 has no float32)
+    loss = (r.logp[used] * a[used]).sum() + (r.entropy * b).sum() + (r.top_logp[used] * c[used]).sum() + (r.lse[used] * d[used]).sum()
+    got, = torch.autograd.grad(loss, x)
+    u = used.float()
+    ref, off = softmax_grads(x, t, scale, a * u, b, c * u[:, None], d * u, r.top_tokens)
+    C.close(got, ref, off + C.rounded(ref, dtype))
+    # by hand, in the logits' place, and of a vocabulary in shards
+    stats = torch.empty(n, 2, device="cuda")
+    with torch.no_grad():
+        r = ops.token_logprobs(x, t, scale=scale, entropy=True, top=k, row_stats=stats)
+        given = dict(scale=scale, entropy=r.entropy, grad_entropy=b, top_tokens=r.top_tokens, grad_top=c, grad_lse=d)
+        ref, off = softmax_grads(x, t, scale, a, b, c, d, r.top_tokens)
+        place = x.detach().clone()
+        C.close(ops.token_logprobs_grad(place, t, None, a, row_stats=stats, into=place, **given), ref, off + C.rounded(ref, dtype))
+        cut = vocab // 3
+        shards = [x.detach()[:, :cut], x.detach()[:, cut:]]
+        of_join = torch.empty(n, 2, device="cuda")
+        parts = [ops.logprob_parts(s, t, first=f, scale=scale, top=k) for s, f in zip(shards, (0, cut))]
+        j = ops.join_logprobs(parts, t, vocab, scale=scale, entropy=True, row_stats=of_join)
+        assert torch.equal(j.top_tokens, r.top_tokens)
+        given.update(entropy=j.entropy, vocab=vocab)
+        for s, f in zip(shards, (0, cut)):
+            part, of_part = softmax_grads(x, t, scale, a, b, c, d, r.top_tokens, slice(f, f + s.shape[1]))
+            C.close(ops.token_logprobs_grad(s, t, None, a, row_stats=of_join, first=f, **given), part, of_part + C.rounded(part, dtype))
+
+
+def test_gradient_at_a_low_temperature():
+    g = gen(33)
+    x = (normal(g, 4, 300) * 1e-4 - 20.0).requires_grad_()
+    t = torch.randint(0, 300, (4,), generator=g).cuda()
+    one, none = torch.ones(4, device="cuda"), torch.zeros(4, device="cuda")
+    got, = torch.autograd.grad(ops.token_logprobs(x, t, scale=1e4).logp.sum(), x)
+    ref, off = softmax_grads(x, t, 1e4, one, none, torch.zeros(4, 0), none, None)
+    C.close(got, ref, off + C.rounded(ref, F32))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_gradient_from_lse_alone(dtype):
+    """float32 holds lse to one part in 2^24: by hand from lse alone a row's probabilities are those of the lse that is given, and a row below
+    -2^24, where it says nothing of the sum any more, has zeros."""
+    g = gen(34)
+    x = far_rows(g, dtype, 600)
+    t = torch.randint(0, 600, (7,), generator=g).cuda()
+    r = ops.token_logprobs(x, t)
+    got = ops.token_logprobs_grad(x, t, r.lse, torch.ones(7, device="cuda")).cpu().double()
+    f = x.cpu().double()
+    p = (f - r.lse.cpu().double()[:, None]).exp()
+    dead = r.lse.cpu() < -2.0 ** 24
+    assert dead.tolist() == [False, False, dtype != F16, dtype != F16, False, False, True]
+    ref = torch.where(dead[:, None], 0.0, -p)
+    ref[torch.arange(7)[~dead], t.cpu()[~dead]] += 1.0
+    off = C.U * (24 + 6 * (f - r.lse.cpu().double()[:, None]).abs().clamp(max=200.0)) * (p.clamp(max=2.0) + 1.0)
+    C.close(got, ref, off + C.rounded(ref, dtype))
+
+
+def test_row_stats_are_the_largest_logit_and_the_logarithm_of_the_sum():
+    g = gen(35)
+    x = normal(g, 5, 40000, size=2.0)
+    x[4] = -math.inf
+    t = torch.zeros(5, dtype=torch.int64, device="cuda")
+    for rows, cut in ((slice(0, 5), 40000), (slice(0, 5), 100)):      # a row in slices, and whole
+        stats = torch.empty(5, 2, device="cuda")
+        ops.token_logprobs(x[rows, :cut], t, scale=0.7, row_stats=stats)
+        f = x[rows, :cut].cpu().double()
+        assert torch.equal(stats[:, 0].cpu().double(), f.amax(1))
+        ref = torch.logsumexp((f - f.amax(1, keepdim=True).clamp(min=-1e300)) * 0.7, 1)
+        C.close(stats[:, 1], ref, C.logprob_bound(torch.zeros(1, cut), 1.0)[0][0].item())
+    x = x[:3]
+    for bad in (torch.empty(3, 2), torch.empty(2, 2, device="cuda"), torch.empty(3, 2, device="cuda", dtype=F16), torch.empty(2, 3, device="cuda").t()):
+        with pytest.raises(ValueError, match="row_stats"):
+            ops.token_logprobs(x, t[:3], row_stats=bad)
+        with pytest.raises(ValueError, match="row_stats"):
+            ops.token_logprobs_grad(x, t[:3], None, t[:3].float(), row_stats=bad)
+    with pytest.raises(ValueError, match="row_stats"):
+        ops.token_logprobs_grad(x, t[:3], None, t[:3].float())
