@@ -176,6 +176,12 @@ def _workspace(name, *sizes, device):
     return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
 
 
+def _written(t):
+    """Tells autograd that a tensor of the caller has been written, as torch's own functions do: a graph that holds it says so, rather than
+    going on with other values."""
+    torch.autograd.graph.increment_version(t)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -307,6 +313,8 @@ def embedding_grad(tokens, grad, rows: int, *, scale: float = 1.0, first: int = 
     _queue(L.gdp_embed_backward,
            gdp_embed_grad(n, rows, dim, first, flat.data_ptr(), token_type, grad_type, out_type, into is not None, scale,
                           grad.data_ptr(), stride, out.data_ptr(), out.stride(0) if rows else dim, _ptr(work), size), device)
+    if into is not None and n:
+        _written(into)
     return out
 
 
@@ -364,14 +372,13 @@ def _token_logprobs(logits, tokens, scale, top, row_stats):
     _check_top(top)
     device, vocab, shape = logits.device, logits.shape[-1], logits.shape[:-1]
     flat, token_type = _tokens_for(tokens, shape, device)
-    with_stats = _row_stats(row_stats, shape, device)
     n, logp, lse, entropy, top_logp, top_tokens = _outputs(shape, top, device)
     rows, stride = _rows(logits, vocab, "logits") if n and vocab else (logits, vocab)
     L = _ops()
     work, size = _workspace("gdp_logprob_workspace", n, vocab, logits_type, top, device=device)
     given = gdp_logprob(n, vocab, rows.data_ptr(), stride, logits_type, token_type, flat.data_ptr(), scale, top,
                         logp.data_ptr(), lse.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_tokens), _ptr(work), size)
-    if with_stats and n:
+    if row_stats is not None and n:
         _queue(L.gdp_logprob_forward_stats, gdp_logprob_stats(given, row_stats.data_ptr()), device)
     else:
         _queue(L.gdp_logprob_forward, given, device)
@@ -414,6 +421,8 @@ def token_logprobs(logits, tokens, *, scale: float = 1.0, entropy: bool = False,
 
     ``row_stats`` [..., 2] float32: written, the largest logit and the log of the sum relative to it, for
     ``token_logprobs_grad``."""
+    if _row_stats(row_stats, logits.shape[:-1], logits.device):
+        _written(row_stats)
     if torch.is_grad_enabled() and logits.requires_grad:
         r = _TokenLogprobs.apply(logits, tokens, float(scale), int(top), row_stats)
     else:
@@ -477,6 +486,8 @@ def token_logprobs_grad(logits, tokens, lse, grad_logp=None, *, scale: float = 1
         _queue(_ops().gdp_logprob_backward_stats, gdp_logprob_grad_stats(given, row_stats.data_ptr()), device)
     else:
         _queue(_ops().gdp_logprob_backward, given, device)
+    if into is not None:
+        _written(into)
     return out
 
 
@@ -525,6 +536,7 @@ def join_logprobs(parts, tokens, vocab: int, *, scale: float = 1.0, entropy: boo
                               _ptr(out_tokens))
     if with_stats and n:
         _queue(_ops().gdp_logprob_join_stats, gdp_logprob_joint_stats(given, row_stats.data_ptr()), device)
+        _written(row_stats)
     else:
         _queue(_ops().gdp_logprob_join, given, device)
     return TokenLogprobs(logp, lse, ent if entropy else None, top_logp, out_tokens)

@@ -183,3 +183,39 @@ def test_row_stats_are_the_largest_logit_and_the_logarithm_of_the_sum():
             ops.token_logprobs_grad(x, t[:3], None, t[:3].float(), row_stats=bad)
     with pytest.raises(ValueError, match="row_stats"):
         ops.token_logprobs_grad(x, t[:3], None, t[:3].float())
+
+
+# ---- what is written in place ---------------------------------------------------------------------------------
+def test_autograd_sees_what_is_written_in_place():
+    """Of logits that a graph holds, and of buffers: overwritten behind autograd's back they would give a wrong gradient without an error."""
+    g = gen(36)
+    w, t = normal(g, 3, 9).requires_grad_(), torch.tensor([1, 2, 3], device="cuda")
+    one = torch.ones(3, device="cuda")
+    logits = w * 2.0
+    r = ops.token_logprobs(logits, t)
+    ops.token_logprobs_grad(logits.detach(), t, r.lse.detach(), one, into=logits.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.logp.sum().backward()
+    stats = torch.empty(3, 2, device="cuda")
+    r = ops.token_logprobs(w, t, row_stats=stats)
+    ops.token_logprobs(w.detach() + 1.0, t, row_stats=stats)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.logp.sum().backward()
+    main = torch.zeros(9, 4, device="cuda")
+    squares = (main * w.new_ones(1).requires_grad_()).square().sum() + (main * main.new_ones(9, 4).requires_grad_()).sum()
+    ops.embedding_grad(t, torch.ones(3, 4, device="cuda"), 9, into=main)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        squares.backward()
+    parts = [ops.logprob_parts(w.detach()[:, a:a + 3], t, first=a) for a in (0, 3, 6)]
+    before = stats._version
+    ops.join_logprobs(parts, t, 9, row_stats=stats)
+    assert stats._version > before
+    # nothing to write: nothing has changed.  And in inference mode there are no versions
+    before = main._version
+    ops.embedding_grad(t[:0], torch.ones(0, 4, device="cuda"), 9, into=main)
+    assert main._version == before
+    with torch.inference_mode():
+        x = torch.randn(3, 9, device="cuda")
+        assert ops.token_logprobs_grad(x, t, ops.token_logprobs(x, t).lse, one, into=x) is x
+        ops.embedding_grad(t, torch.ones(3, 4, device="cuda"), 9, into=torch.zeros(9, 4, device="cuda"))
+    assert ops.token_logprobs_grad(x, t, ops.token_logprobs(x, t).lse, one, into=x) is x
