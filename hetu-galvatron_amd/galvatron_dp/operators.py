@@ -349,7 +349,11 @@ def _check_top(top):
 
 def _outputs(shape, top, device):
     n = shape.numel()
-    logp, lse, entropy = torch.empty((3,) + shape, dtype=torch.float32, device=device).unbind()
+    if n and shape:
+        # One allocation, but no views of it: parts of one tensor could not be changed in place, and would share their version.
+        logp, lse, entropy = torch.empty((3 * shape[0],) + shape[1:], dtype=torch.float32, device=device).unsafe_chunk(3)
+    else:
+        logp, lse, entropy = [torch.empty(shape, dtype=torch.float32, device=device) for _ in range(3)]
     if not top:
         return n, logp, lse, entropy, None, None
     return (n, logp, lse, entropy, torch.empty(shape + (top,), dtype=torch.float32, device=device),

@@ -219,3 +219,35 @@ def test_autograd_sees_what_is_written_in_place():
         assert ops.token_logprobs_grad(x, t, ops.token_logprobs(x, t).lse, one, into=x) is x
         ops.embedding_grad(t, torch.ones(3, 4, device="cuda"), 9, into=torch.zeros(9, 4, device="cuda"))
     assert ops.token_logprobs_grad(x, t, ops.token_logprobs(x, t).lse, one, into=x) is x
+
+
+# ---- outputs are a program's own ------------------------------------------------------------------------------
+def test_outputs_can_be_changed_in_place():
+    """Each is a tensor of its own: changing one is allowed, does not touch the others and is no change of them for autograd."""
+    g = gen(37)
+    x, t = normal(g, 4, 50), torch.tensor([1, -100, 3, 4], device="cuda")
+    weights = torch.tensor([1.0, 2.0, 3.0, 4.0], device="cuda").requires_grad_()
+    leaf = x.clone().requires_grad_()
+    parts = [ops.logprob_parts(x, t, first=0)]
+    for r in (ops.token_logprobs(x, t, entropy=True), ops.token_logprobs(leaf, t, entropy=True), ops.join_logprobs(parts, t, 50, entropy=True)):
+        lse, entropy = r.lse.detach().clone(), r.entropy.detach().clone()
+        squares = r.lse.square().sum() + (r.entropy * weights).sum()
+        r.logp.masked_fill_(t < 0, 7.0)
+        r.logp.mul_(weights)
+        assert r.logp[1] == 14.0 and torch.equal(r.lse, lse) and torch.equal(r.entropy, entropy)
+        (squares + r.logp.sum()).backward()
+    # the gradient knows of the change: the place that was filled has none
+    ref = x.cpu().double()
+    p = torch.softmax(ref, 1)
+    q, entropy = torch.log_softmax(ref, 1), -(p * torch.log_softmax(ref, 1)).sum(1, keepdim=True)
+    w = weights.detach().cpu().double()[:, None]
+    hit = torch.zeros(4, 50, dtype=torch.float64)
+    hit[[0, 2, 3], [1, 3, 4]] = 1.0
+    held = hit.sum(1, keepdim=True)
+    want = w * (hit - held * p) - w * p * (q + entropy) + 2 * torch.logsumexp(ref, 1, keepdim=True) * p
+    size = w * (hit + p) + w * p * (q.abs() + entropy) + 2 * torch.logsumexp(ref, 1, keepdim=True) * p
+    C.close(leaf.grad, want, C.U * 200 * size)
+    with torch.no_grad():
+        r = ops.token_logprobs(leaf, t, entropy=True)
+        r.entropy.zero_()
+    (r.logp * weights).sum().backward()
