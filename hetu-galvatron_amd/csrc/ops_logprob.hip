@@ -717,7 +717,7 @@ static int backward_rows(const gdp_logprob_grad *l, const float *row_stats, void
     if (const int rc = check_logits(l->logits, l->n, l->vocab, l->logits_stride, l->logits_type, l->tokens, l->token_type, false)) return rc;
     if (const int rc = check_logits(l->out, l->n, l->vocab, l->out_stride, l->logits_type, l->tokens, l->token_type, true)) return rc;
     if ((!l->lse && !row_stats) || !l->entropy != !l->grad_entropy || (l->top && (!l->top_tokens || !l->grad_top))) return gdp_fail(GDP_E_BADARG, "gdp_logprob: null pointer");
-    if (l->out == l->logits && l->out_stride != l->logits_stride) return gdp_fail(GDP_E_BADARG, "gdp_logprob: a gradient in the place of the logits needs their stride");
+    if (l->out == l->logits && l->n > 1 && l->out_stride != l->logits_stride) return gdp_fail(GDP_E_BADARG, "gdp_logprob: a gradient in the place of the logits needs their stride");
     const int vec = 16 / size_of(l->logits_type);
     const int64_t vectors = ceil_div(l->vocab, (int64_t)vec) + 1;
     int64_t slices = 1;   // two rounds of reads for each workgroup, more where the grid would be too large

@@ -251,3 +251,21 @@ def test_outputs_can_be_changed_in_place():
         r = ops.token_logprobs(leaf, t, entropy=True)
         r.entropy.zero_()
     (r.logp * weights).sum().backward()
+
+
+# ---- single rows, and none --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_gradient_in_the_place_of_one_padded_row(dtype):
+    g = gen(38)
+    for shape, cut in (((4, 1008), 1), ((2, 3, 1008), 1), ((5, 40), 1)):
+        padded = normal(g, *shape, dtype=dtype, size=2.0)
+        rest = padded.clone()
+        x = padded[:cut, ..., :37] if len(shape) == 2 else padded[:cut, :1, :37]
+        t = torch.full(x.shape[:-1], 5, device="cuda")
+        r = ops.token_logprobs(x, t)
+        one = torch.ones(x.shape[:-1], device="cuda")
+        want = ops.token_logprobs_grad(x, t, r.lse, one)
+        assert ops.token_logprobs_grad(x, t, r.lse, one, into=x) is x
+        assert torch.equal(x, want)
+        rest[(slice(0, 1),) * (len(shape) - 1) + (slice(0, 37),)] = want
+        assert torch.equal(padded, rest), "what lies beside the row stays"
