@@ -8,7 +8,8 @@ reference's profiler fills it in from whole training runs, model_profiler.py:302
     python -m galvatron_dp.model_ends --hidden 4096 --vocab 128256 --seq 4096 --bsz 1 2 3 4 5 6 7 8 \\
         --profile configs/computation_profiling_bf16_llama.json
 
-measures those entries and writes them into the file, next to the entries of the layers that are there.
+measures those entries and writes them into the file, next to the entries of the layers that are there.  An entry is of the whole
+vocabulary on one GPU: the search divides it by the tensor-parallel degree itself, so a shard's time is printed only.
 """
 from __future__ import annotations
 
@@ -123,16 +124,19 @@ def main(argv=None) -> dict:
     p.add_argument("--bsz", type=int, nargs="+", default=[1])
     p.add_argument("--precision", choices=sorted(DTYPES), default="bf16")
     p.add_argument("--norm", choices=("rms", "layer"), default="rms")
-    p.add_argument("--shards", type=int, default=1, help="vocabulary-parallel degree: measures one shard")
+    p.add_argument("--shards", type=int, default=1, help="vocabulary-parallel degree: measures one shard, which is no entry of a profile")
     p.add_argument("--backward", action="store_true", help="prints forward and backward passes as well")
     p.add_argument("--profile", help="computation profile to write the entries into")
     a = p.parse_args(argv)
+    if a.profile and a.shards > 1:
+        p.error("--profile takes the time of the whole vocabulary, which the search divides by the parallel degree: not with --shards")
     ends = ModelEnds(a.hidden, a.vocab, dtype=DTYPES[a.precision], norm=a.norm, shards=a.shards)
     times = {}
     for seq in a.seq:
         for bsz in a.bsz:
             times[bsz, seq] = measure(ends, bsz, seq)
-            line = "layertype_other_bsz%d_seq%d: %.4f ms a sample" % (bsz, seq, times[bsz, seq])
+            name = "layertype_other_bsz%d_seq%d" if a.shards == 1 else "a shard of %d, bsz %%d, seq %%d" % a.shards
+            line = (name + ": %.4f ms a sample") % (bsz, seq, times[bsz, seq])
             if a.backward and a.shards == 1:
                 line += ", forward and backward %.4f" % measure(ends, bsz, seq, backward=True)
             print(line, flush=True)

@@ -37,3 +37,22 @@ def test_row_stats_refused_on_the_host(name):
         assert getattr(lib, name)(ctypes.byref(bad), None) == _lib.GDP_E_BADARG
         assert lib.gdp_last_error().startswith(b"gdp_")
     assert getattr(lib, name)(ctypes.byref(record(given(n=0), None)), None) == _lib.GDP_OK
+
+
+# ---- the command that measures a model's ends -------------------------------------------------------------------
+def test_a_shards_time_is_not_written_as_the_whole_parts(tmp_path, capsys, monkeypatch):
+    """The search divides the profile's entry by the tensor-parallel degree itself: a shard's time would be divided twice."""
+    from galvatron_dp import model_ends
+    path = tmp_path / "computation_profiling_bf16_small.json"
+    path.write_text('{"layertype_other_bsz1_seq64": 3.5}')
+    monkeypatch.setattr(model_ends, "ModelEnds", lambda *a, **k: None)
+    monkeypatch.setattr(model_ends, "measure", lambda *a, **k: 1.0)
+    given = ["--hidden", "128", "--vocab", "2000", "--seq", "64", "--shards", "4"]
+    with pytest.raises(SystemExit):
+        model_ends.main(given + ["--profile", str(path)])
+    assert "--profile" in capsys.readouterr().err
+    assert path.read_text() == '{"layertype_other_bsz1_seq64": 3.5}'
+    assert model_ends.main(given) == {(1, 64): 1.0}          # measured and printed, not under the entry's name
+    assert "layertype_other" not in capsys.readouterr().out
+    model_ends.main(given[:-2] + ["--profile", str(path)])
+    assert '"layertype_other_bsz1_seq64": 1.0' in path.read_text()
