@@ -14,6 +14,8 @@ vocabulary on one GPU: the search divides it by the tensor-parallel degree itsel
 from __future__ import annotations
 
 import argparse
+import functools
+import math
 import os
 from typing import NamedTuple, Optional
 
@@ -71,16 +73,27 @@ class ModelEnds:
             return ops.logprob_parts(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1), first=self.first, top=top)
         return ops.token_logprobs(logits, targets, entropy=entropy, top=top)
 
-    def loss_and_grads(self, tokens, targets, block, into: Optional[torch.Tensor] = None) -> EndGrads:
-        """The mean loss over the targets and its gradients (a whole vocabulary).  ``into`` [rows, hidden]: the table's is added to it."""
+    def loss_and_grads(self, tokens, targets, block, into: Optional[torch.Tensor] = None, *,
+                       loss_scale: Optional[float] = None) -> EndGrads:
+        """The mean loss over the targets and its gradients (a whole vocabulary).  ``into`` [rows, hidden]: the table's is added to it.
+
+        The gradients, not the loss, are multiplied by ``loss_scale`` (1 by default).  float16 needs one: the logits' gradients are
+        shares of 1 over the number of targets, and what is below float16's least step, 6e-8, is lost.  The number of targets
+        times some sixteen brings them into its range."""
         if self.shards > 1:
             raise ValueError("a shard's loss needs the parts of the others: forward, join_logprobs, token_logprobs_grad")
+        if loss_scale is None:
+            if self.table.dtype == torch.float16:
+                raise ValueError("float16 needs a loss_scale: the gradient of a mean over many targets is below its least step")
+            loss_scale = 1.0
+        if not 0.0 < loss_scale < math.inf:
+            raise ValueError(f"loss_scale must be positive and finite, not {loss_scale}")
         joined, logits = self.logits(self.embed(tokens), block, stats=True)
         row_stats = torch.empty(*targets.shape, 2, device=logits.device)
         r = ops.token_logprobs(logits, targets, entropy=True, row_stats=row_stats)
         held = (targets >= 0) & (targets < self.vocab)
         each = held / held.sum().clamp(min=1)
-        d_logits = ops.token_logprobs_grad(logits, targets, None, -each.float(), row_stats=row_stats, into=logits)
+        d_logits = ops.token_logprobs_grad(logits, targets, None, each * -loss_scale, row_stats=row_stats, into=logits)
         rows, normed = (t.reshape(-1, t.shape[-1]) for t in (d_logits, joined.normed))
         d_normed, d_head = rows @ self.head, rows.t() @ normed
         g = ops.residual_norm_grad(joined.stream, block, joined.stats, d_normed.view_as(joined.normed), pre=self.norm)
@@ -94,7 +107,10 @@ def measure(ends: ModelEnds, bsz: int, seq: int, *, repeats: int = 20, backward:
     g = torch.Generator(device=device).manual_seed(1)
     tokens = torch.randint(0, ends.vocab, (bsz, seq + 1), generator=g, device=device)
     block = torch.randn(bsz, seq, hidden, generator=g, device=device).to(ends.table.dtype)
-    step = ends.loss_and_grads if backward else ends.forward
+    if backward:    # (float16: its range needs a scale, its time does not depend on which)
+        step = functools.partial(ends.loss_and_grads, loss_scale=bsz * seq * 16.0 if ends.table.dtype == torch.float16 else None)
+    else:
+        step = ends.forward
     times = []
     for i in range(3 + repeats):
         begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
