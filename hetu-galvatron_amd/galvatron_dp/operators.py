@@ -9,11 +9,11 @@ torch tensors:
     logprob_parts, join_logprobs                        ... of a vocabulary in shards
     residual_norm, residual_norm_grad                   norms after a block and before the next, gate, scales
 
-``embedding``, ``token_logprobs`` and ``residual_norm`` are differentiable (once); the ``*_grad`` functions are what
-their backward passes call, for programs that run their own.  Work is queued on torch's current stream of the tensors'
-device; nothing waits.  Types: float32, float16, bfloat16; token numbers int32 or int64.  Per-token tensors may
-have any strides (one whose rows' elements are not neighbours is copied first); a table's rows have to lie as they are.
-There is no CPU path: tensors have to be on a HIP device.
+``embedding``, ``token_logprobs`` and ``residual_norm`` are differentiable (once, backwards: tensors with forward-mode
+tangents are refused); the ``*_grad`` functions are what their backward passes call, for programs that run their own.
+Work is queued on torch's current stream of the tensors' device; nothing waits.  Types: float32, float16, bfloat16; token
+numbers int32 or int64.  Per-token tensors may have any strides (one whose rows' elements are not neighbours is copied
+first); a table's rows have to lie as they are.  There is no CPU path: tensors have to be on a HIP device.
 """
 from __future__ import annotations
 
@@ -22,6 +22,7 @@ import functools
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -176,6 +177,19 @@ def _workspace(name, *sizes, device):
     return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
 
 
+def _no_tangents(*tensors):
+    """Refuses what the kernels would drop: a result without a tangent, from an input with one.  (Asked where a level is open; else there
+    are none.)"""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("the operators have no forward-mode derivatives")
+
+
+def _of_norms(*norms):
+    """The weights and biases of norms that may be None."""
+    return [t for norm in norms for t in ((norm.weight, norm.bias) if norm else (None, None))]
+
+
 def _written(t):
     """Tells autograd that a tensor of the caller has been written, as torch's own functions do: a graph that holds it says so, rather than
     going on with other values."""
@@ -275,6 +289,8 @@ def embedding(tokens, weight, *, scale: float = 1.0, first: int = 0, dtype: Opti
 
     ``weight`` [rows, dim] is the shard of a table whose row 0 belongs to token ``first``; a token that it does not hold
     gives zeros, so that the sum over the shards is the lookup in the whole table."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(weight)
     if weight.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(tokens, weight, float(scale), int(first), dtype)
     return _embedding(tokens, weight, float(scale), int(first), dtype)
@@ -286,6 +302,8 @@ def embedding_grad(tokens, grad, rows: int, *, scale: float = 1.0, first: int = 
     places that hold the same token, in ``dtype`` (the gradient's by default), zeros for rows without any.
 
     ``into`` [rows, dim]: the sums are added to it instead, rows without places are left alone, and it is returned."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(grad, into)
     token_type, grad_type = _type(tokens, "tokens", _TOKEN_TYPES), _type(grad, "grad")
     device = grad.device
     if grad.shape[:-1] != tokens.shape or grad.dim() != tokens.dim() + 1:
@@ -360,13 +378,9 @@ def _outputs(shape, top, device):
             torch.empty(shape + (top,), dtype=torch.int64, device=device))
 
 
-def _row_stats(t, shape, device):
-    """Whether there are any, after checking them."""
-    if t is None:
-        return False
+def _check_row_stats(t, shape, device):
     if t.shape != shape + (2,) or t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
         raise ValueError(f"row_stats must be {list(shape + (2,))} float32 on {device}, in order")
-    return True
 
 
 def _token_logprobs(logits, tokens, scale, top, row_stats):
@@ -425,7 +439,10 @@ def token_logprobs(logits, tokens, *, scale: float = 1.0, entropy: bool = False,
 
     ``row_stats`` [..., 2] float32: written, the largest logit and the log of the sum relative to it, for
     ``token_logprobs_grad``."""
-    if _row_stats(row_stats, logits.shape[:-1], logits.device):
+    if forward_ad._current_level >= 0:
+        _no_tangents(logits)
+    if row_stats is not None:
+        _check_row_stats(row_stats, logits.shape[:-1], logits.device)
         _written(row_stats)
     if torch.is_grad_enabled() and logits.requires_grad:
         r = _TokenLogprobs.apply(logits, tokens, float(scale), int(top), row_stats)
@@ -442,9 +459,12 @@ def token_logprobs_grad(logits, tokens, lse, grad_logp=None, *, scale: float = 1
 
     ``row_stats``: what the forward pass wrote there; ``lse`` is not read then and may be None.  From ``lse`` alone, which float32
     rounds by one part in 2^24, probabilities are off by |lse| / 2^24 of themselves, and rows whose lse is below -2^24 (nothing but
-    a mask's -1e9) have zeros.  ``lse`` (and ``entropy``, ``top_tokens`` where they have gradients) are what the forward pass gave.  Of a vocabulary in
-    shards, ``logits`` are those of the shard that begins with token ``first``, of ``vocab`` tokens in all, and ``lse``,
-    ``entropy`` and ``top_tokens`` those of ``join_logprobs``.  ``into``: written there; it may be ``logits`` itself."""
+    a mask's -1e9) have zeros.  ``lse`` (and ``entropy``, ``top_tokens`` where they have gradients) are what the forward pass
+    gave.  Of a vocabulary in shards, ``logits`` are those of the shard that begins with token ``first``, of ``vocab`` tokens in
+    all, and ``row_stats``, ``lse``, ``entropy`` and ``top_tokens`` those of ``join_logprobs``.  ``into``: written there; it may be
+    ``logits`` itself."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(logits, lse, grad_logp, grad_lse, entropy, grad_entropy, grad_top, into, row_stats)
     logits_type = _type(logits, "logits")
     if logits.dim() < 1:
         raise ValueError("logits must be [..., vocab]")
@@ -454,10 +474,12 @@ def token_logprobs_grad(logits, tokens, lse, grad_logp=None, *, scale: float = 1
     flat, token_type = _tokens_for(tokens, shape, device)
     if (entropy is None) != (grad_entropy is None) or (top_tokens is None) != (grad_top is None):
         raise ValueError("entropy and grad_entropy, top_tokens and grad_top come together")
-    with_stats = _row_stats(row_stats, shape, device)
-    lse = None if with_stats else _floats(lse, shape, "lse", device)
-    if lse is None and not with_stats:
+    if row_stats is not None:
+        _check_row_stats(row_stats, shape, device)
+        lse = None
+    elif lse is None:
         raise ValueError("row_stats or lse is needed")
+    lse = _floats(lse, shape, "lse", device)
     grad_logp, grad_lse = _floats(grad_logp, shape, "grad_logp", device), _floats(grad_lse, shape, "grad_lse", device)
     entropy, grad_entropy = _floats(entropy, shape, "entropy", device), _floats(grad_entropy, shape, "grad_entropy", device)
     top = 0
@@ -486,7 +508,7 @@ def token_logprobs_grad(logits, tokens, lse, grad_logp=None, *, scale: float = 1
     given = gdp_logprob_grad(n, columns, first, vocab, rows.data_ptr(), stride, logits_type, token_type, flat.data_ptr(), scale,
                              top, _ptr(lse), _ptr(grad_logp), _ptr(grad_lse), _ptr(entropy), _ptr(grad_entropy),
                              _ptr(top_tokens), _ptr(grad_top), to.data_ptr(), to.stride(0))
-    if with_stats:
+    if row_stats is not None:
         _queue(_ops().gdp_logprob_backward_stats, gdp_logprob_grad_stats(given, row_stats.data_ptr()), device)
     else:
         _queue(_ops().gdp_logprob_backward, given, device)
@@ -498,6 +520,8 @@ def token_logprobs_grad(logits, tokens, lse, grad_logp=None, *, scale: float = 1
 def logprob_parts(logits, tokens, *, first: int, scale: float = 1.0, top: int = 0) -> LogprobParts:
     """``token_logprobs`` of a shard of the vocabulary, ``logits`` [n, columns] of the tokens from ``first`` on, up to what
     the other shards have to say: 16 + 8 * top bytes for each row, to be gathered from all shards and joined."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(logits)
     logits_type = _type(logits, "logits")
     if logits.dim() != 2:
         raise ValueError(f"logits must be [n, columns], not {list(logits.shape)}")
@@ -524,6 +548,8 @@ def join_logprobs(parts, tokens, vocab: int, *, scale: float = 1.0, entropy: boo
     there, of the whole rows."""
     if not isinstance(parts, LogprobParts):
         parts = LogprobParts(*(torch.stack(t) for t in zip(*parts)))
+    if forward_ad._current_level >= 0:
+        _no_tangents(*parts[:2])
     stats, top_logits, top_tokens = (t.contiguous() for t in parts)
     if stats.dim() != 3 or stats.shape[2] != 4 or top_logits.shape[:2] != stats.shape[:2] or top_tokens.shape != top_logits.shape:
         raise ValueError("parts must be stats [parts, n, 4], top_logits and top_tokens [parts, n, top]")
@@ -533,12 +559,13 @@ def join_logprobs(parts, tokens, vocab: int, *, scale: float = 1.0, entropy: boo
     device, count, shape, top = stats.device, stats.shape[0], stats.shape[1:2], top_logits.shape[2]
     _same_device(device, top_logits=top_logits, top_tokens=top_tokens)
     flat, token_type = _tokens_for(tokens, shape, device)
-    with_stats = _row_stats(row_stats, shape, device)
+    if row_stats is not None:
+        _check_row_stats(row_stats, shape, device)
     n, logp, lse, ent, top_logp, out_tokens = _outputs(shape, top, device)
     given = gdp_logprob_joint(n, vocab, count, top, scale, token_type, flat.data_ptr(), stats.data_ptr(), top_logits.data_ptr(),
                               top_tokens.data_ptr(), logp.data_ptr(), lse.data_ptr(), ent.data_ptr(), _ptr(top_logp),
                               _ptr(out_tokens))
-    if with_stats and n:
+    if row_stats is not None and n:
         _queue(_ops().gdp_logprob_join_stats, gdp_logprob_joint_stats(given, row_stats.data_ptr()), device)
         _written(row_stats)
     else:
@@ -652,6 +679,8 @@ def residual_norm_grad(stream, block, stats, grad_normed, grad_stream=None, *, p
     """Gradients of ``residual_norm``'s inputs from ``grad_normed`` and, where the stream is used further on,
     ``grad_stream``.  ``stream``, ``stats`` and ``block`` are those of the forward pass.  Gradients of weights, biases and gate
     have their types and shapes and are None for what is not there."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(stream, block, stats, grad_normed, grad_stream, *_of_norms(post, pre), gate)
     stream_type = _type(stream, "stream")
     device, dim, shape = stream.device, stream.shape[-1], stream.shape
     n = shape[:-1].numel()
@@ -683,8 +712,7 @@ def residual_norm_grad(stream, block, stats, grad_normed, grad_stream=None, *, p
     ds, ds_stride = rows(grad_stream, "grad_stream")
 
     got = ResidualNormGrads(*[None if t is None else _like(t) for t in (
-        stream, block, *((post.weight, post.bias) if post else (None, None)),
-        *((pre.weight, pre.bias) if pre else (None, None)), gate)])
+        stream, block, *_of_norms(post, pre), gate)])
     L = _ops()
     work, size = _workspace("gdp_norm_grad_workspace", n, dim, count, device=device)
     _queue(L.gdp_norm_backward,
@@ -740,8 +768,9 @@ def residual_norm(residual, block=None, *, post: Optional[Norm] = None, pre: Opt
     stream's type, or of the norm's weight's if the stream is float32.  ``stats``: also what ``residual_norm_grad`` needs of
     the two norms."""
     residual_scale, block_scale = float(residual_scale), float(block_scale)
-    inputs = (residual, block, *((post.weight, post.bias) if post else (None, None)),
-              *((pre.weight, pre.bias) if pre else (None, None)), gate)
+    inputs = (residual, block, *_of_norms(post, pre), gate)
+    if forward_ad._current_level >= 0:
+        _no_tangents(*inputs)
     if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in inputs]):
         return ResidualNorm(*_ResidualNorm.apply(*inputs, post and (post.form, post.eps), pre and (pre.form, pre.eps),
                                                  residual_scale, block_scale))

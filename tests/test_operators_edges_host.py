@@ -56,3 +56,30 @@ def test_a_shards_time_is_not_written_as_the_whole_parts(tmp_path, capsys, monke
     assert "layertype_other" not in capsys.readouterr().out
     model_ends.main(given[:-2] + ["--profile", str(path)])
     assert '"layertype_other_bsz1_seq64": 1.0' in path.read_text()
+
+
+# ---- derivatives that there are none of ----------------------------------------------------------------------------
+def test_tangents_are_refused():
+    """Forward-mode derivatives would be dropped without a word: the operators say that they have none, whichever tensor carries one."""
+    import torch.autograd.forward_ad as fw
+    t, w, x, v = torch.zeros(3, dtype=torch.int64), torch.ones(5, 8), torch.zeros(3, 9), torch.zeros(3)
+    parts = ops.LogprobParts(torch.zeros(1, 3, 4), torch.zeros(1, 3, 0), torch.zeros(1, 3, 0, dtype=torch.int32))
+    norm = ops.Norm("layer", torch.ones(9), torch.zeros(9))
+    calls = [lambda d: ops.embedding(t, d(w)), lambda d: ops.embedding_grad(t, d(w[:3]), 5), lambda d: ops.embedding_grad(t, w[:3], 5, into=d(w)),
+             lambda d: ops.token_logprobs(d(x), t), lambda d: ops.token_logprobs_grad(d(x), t, v, v), lambda d: ops.token_logprobs_grad(x, t, d(v), v),
+             lambda d: ops.token_logprobs_grad(x, t, v, d(v)), lambda d: ops.token_logprobs_grad(x, t, v, grad_lse=d(v)),
+             lambda d: ops.token_logprobs_grad(x, t, v, entropy=v, grad_entropy=d(v)), lambda d: ops.logprob_parts(d(x), t, first=0),
+             lambda d: ops.join_logprobs(parts._replace(stats=d(parts.stats)), t, 9), lambda d: ops.residual_norm(d(x), x, pre=norm),
+             lambda d: ops.residual_norm(x, d(x), pre=norm), lambda d: ops.residual_norm(x, x, pre=norm._replace(weight=d(norm.weight))),
+             lambda d: ops.residual_norm(x, x, post=norm._replace(bias=d(norm.bias)), pre=norm), lambda d: ops.residual_norm(x, x, pre=norm, gate=d(norm.weight)),
+             lambda d: ops.residual_norm_grad(x, x, torch.zeros(3, 4), d(x), pre=norm), lambda d: ops.residual_norm_grad(d(x), x, torch.zeros(3, 4), x, pre=norm),
+             lambda d: ops.residual_norm_grad(x, x, torch.zeros(3, 4), x, x, pre=norm._replace(weight=d(norm.weight)))]
+    for leaf in (False, True):
+        for call in calls:
+            with fw.dual_level():
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(lambda p: fw.make_dual(p.clone().requires_grad_(leaf), torch.ones_like(p)))
+                with pytest.raises(ValueError, match="HIP device"):      # no tangent: goes on to the other checks
+                    call(lambda p: p)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda p: ops.token_logprobs(p, t).logp, (x,), (x,))
