@@ -696,7 +696,7 @@ def residual_norm_grad(stream, block, stats, grad_normed, grad_stream=None, *, p
         if t is not None and (t.shape != shape or t.dtype != dtype):
             raise ValueError(f"{what} must be {list(shape)} of {dtype}, not {list(t.shape)} of {t.dtype}")
     _same_device(device, block=block, grad_normed=grad_normed, grad_stream=grad_stream, stats=stats)
-    if stats.shape != (n, 4) or stats.dtype != torch.float32:
+    if stats is None or stats.shape != (n, 4) or stats.dtype != torch.float32:
         raise ValueError(f"stats must be {[n, 4]}, float32")
     stats = stats.contiguous()
     post_record, *keep_post = _norm_params(post, dim, device, "post")

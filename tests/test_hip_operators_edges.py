@@ -269,3 +269,10 @@ def test_gradient_in_the_place_of_one_padded_row(dtype):
         assert torch.equal(x, want)
         rest[(slice(0, 1),) * (len(shape) - 1) + (slice(0, 37),)] = want
         assert torch.equal(padded, rest), "what lies beside the row stays"
+
+
+# ---- what a program leaves out or mixes up is a ValueError that names it ----------------------------------------
+def test_norm_gradient_without_stats_is_refused():
+    x = torch.zeros(3, 8, device="cuda")
+    with pytest.raises(ValueError, match="stats"):
+        ops.residual_norm_grad(x, x, None, x, pre=ops.Norm("rms"))
