@@ -654,7 +654,7 @@ def _residual_norm(residual, block, post, pre, gate, residual_scale, block_scale
         raise ValueError("post and gate need a block")
     if block is None and pre is None:
         raise ValueError("nothing to do: neither a block nor a norm")
-    code = _TYPES[kind] if block is None else _type(block, "block")
+    code = _type(residual if kind == residual.dtype else pre.weight, "pre.weight") if block is None else _type(block, "block")
     if block is not None and (block.shape != shape or block.device != device):
         raise ValueError(f"block must be {list(shape)} on {device}, not {list(block.shape)} on {block.device}")
     post_record, *keep_post = _norm_params(post, dim, device, "post")

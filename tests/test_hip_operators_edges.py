@@ -276,3 +276,11 @@ def test_norm_gradient_without_stats_is_refused():
     x = torch.zeros(3, 8, device="cuda")
     with pytest.raises(ValueError, match="stats"):
         ops.residual_norm_grad(x, x, None, x, pre=ops.Norm("rms"))
+
+
+def test_norm_weights_of_other_types_are_refused():
+    x, w = torch.zeros(3, 8, device="cuda"), torch.ones(8, device="cuda", dtype=torch.float64)
+    for t in (x, x.half()):
+        for block in (None, t):
+            with pytest.raises(ValueError, match="weight"):
+                ops.residual_norm(t, block, pre=ops.Norm("rms", w))
