@@ -547,6 +547,9 @@ def join_logprobs(parts, tokens, vocab: int, *, scale: float = 1.0, entropy: boo
     their tokens, or one whose tensors have a leading dimension for the shards, as gathering them leaves it.  ``row_stats``: as
     there, of the whole rows."""
     if not isinstance(parts, LogprobParts):
+        parts = list(parts)
+        if not parts or any(a.shape != b.shape for p in parts for a, b in zip(p, parts[0])):
+            raise ValueError("parts must be one of each shard, of the same rows and alternatives")
         parts = LogprobParts(*(torch.stack(t) for t in zip(*parts)))
     if forward_ad._current_level >= 0:
         _no_tangents(*parts[:2])

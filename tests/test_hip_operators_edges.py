@@ -284,3 +284,11 @@ def test_norm_weights_of_other_types_are_refused():
         for block in (None, t):
             with pytest.raises(ValueError, match="weight"):
                 ops.residual_norm(t, block, pre=ops.Norm("rms", w))
+
+
+def test_parts_that_do_not_belong_together_are_refused():
+    x, t = torch.zeros(3, 8, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    one, more, fewer = ops.logprob_parts(x, t, first=0, top=1), ops.logprob_parts(x, t, first=8, top=2), ops.logprob_parts(x[:2], t[:2], first=8, top=1)
+    for bad in ([], [one, more], [one, fewer]):
+        with pytest.raises(ValueError, match="parts"):
+            ops.join_logprobs(bad, t, 16)
