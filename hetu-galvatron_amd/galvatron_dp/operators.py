@@ -637,6 +637,8 @@ def _gate_rows(gate, dim, n, device):
     code = _type(gate, "gate")
     if gate.device != device:
         raise ValueError(f"gate is on {gate.device}, not on {device}")
+    if n == 0 and dim and gate.numel() == 0 and gate.shape[-1] == dim:
+        return None, 0, 0, 0        # no rows, and a gate for each
     rows, stride = _rows(gate, dim, "gate")
     count = gate.numel() // dim if dim else 0
     if count < 1 or n % count:

@@ -292,3 +292,20 @@ def test_parts_that_do_not_belong_together_are_refused():
     for bad in ([], [one, more], [one, fewer]):
         with pytest.raises(ValueError, match="parts"):
             ops.join_logprobs(bad, t, 16)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_no_rows_with_a_gate_for_each(dtype):
+    """An empty batch has no gates either: nothing to do, and gradients of zeros for what is there."""
+    g = gen(39)
+    x, w, gate = normal(g, 0, 5, 24, dtype=dtype), normal(g, 24, dtype=dtype), normal(g, 0, 24, dtype=dtype)
+    post, pre = ops.Norm("layer", w, w), ops.Norm("rms", w)
+    out = ops.residual_norm(x, x, post=post, pre=pre, gate=gate, stats=True)
+    assert out.stream.shape == out.normed.shape == (0, 5, 24)
+    got = ops.residual_norm_grad(out.stream, x, out.stats, x, x, post=post, pre=pre, gate=gate)
+    assert got.gate.shape == (0, 24) and got.block.shape == (0, 5, 24) and not got.pre_weight.any() and not got.post_bias.any()
+    leaf = gate.clone().requires_grad_()
+    ops.residual_norm(x, x, pre=pre, gate=leaf).normed.sum().backward()
+    assert leaf.grad.shape == (0, 24)
+    with pytest.raises(ValueError, match="gate"):
+        ops.residual_norm(normal(g, 2, 24, dtype=dtype), normal(g, 2, 24, dtype=dtype), pre=pre, gate=gate)
