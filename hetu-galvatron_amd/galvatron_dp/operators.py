@@ -777,6 +777,7 @@ def residual_norm(residual, block=None, *, post: Optional[Norm] = None, pre: Opt
     if forward_ad._current_level >= 0:
         _no_tangents(*inputs)
     if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in inputs]):
-        return ResidualNorm(*_ResidualNorm.apply(*inputs, post and (post.form, post.eps), pre and (pre.form, pre.eps),
-                                                 residual_scale, block_scale))
+        stream, normed, given = _ResidualNorm.apply(*inputs, post and (post.form, post.eps), pre and (pre.form, pre.eps),
+                                                    residual_scale, block_scale)
+        return ResidualNorm(stream, normed, given if stats else None)
     return ResidualNorm(*_residual_norm(residual, block, post, pre, gate, residual_scale, block_scale, stats))

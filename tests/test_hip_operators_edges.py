@@ -309,3 +309,11 @@ def test_no_rows_with_a_gate_for_each(dtype):
     assert leaf.grad.shape == (0, 24)
     with pytest.raises(ValueError, match="gate"):
         ops.residual_norm(normal(g, 2, 24, dtype=dtype), normal(g, 2, 24, dtype=dtype), pre=pre, gate=gate)
+
+
+def test_norm_statistics_are_there_where_they_are_asked_for():
+    """With gradients as without."""
+    x = normal(gen(40), 3, 8)
+    for t in (x, x.clone().requires_grad_()):
+        assert ops.residual_norm(t, pre=ops.Norm("rms")).stats is None
+        assert ops.residual_norm(t, t, pre=ops.Norm("rms"), stats=True).stats.shape == (3, 4)
