@@ -372,9 +372,10 @@ bool past_caches(const void *p, int64_t rows, int64_t dim, int64_t stride, int t
 }
 
 // Elements that a thread takes of a row at a time: 16 bytes of the smaller of the two types, one of rows that have less.
+template <typename T, typename O> constexpr int AT_ONCE = T::VEC > O::VEC ? T::VEC : O::VEC;
 int elements_at_once(int64_t dim, int type_a, int type_b)
 {
-    const int n = type_a == GDP_F32 && type_b == GDP_F32 ? 4 : 8;
+    const int n = type_a == GDP_F32 && type_b == GDP_F32 ? AT_ONCE<F32, F32> : AT_ONCE<F16, F16>;
     return dim < n ? 1 : n;
 }
 
@@ -394,13 +395,9 @@ template <typename F> int with_type(int t, F f)
     default: return f(BF16{});
     }
 }
-template <typename F> int with_count(int n, F f)
+template <typename T, typename O, typename F> int with_count(int n, F f)
 {
-    switch (n) {
-    case 8: return f(std::integral_constant<int, 8>{});
-    case 4: return f(std::integral_constant<int, 4>{});
-    default: return f(std::integral_constant<int, 1>{});
-    }
+    return n == 1 ? f(std::integral_constant<int, 1>{}) : f(std::integral_constant<int, AT_ONCE<T, O>>{});
 }
 
 // Sizes of the order and of the partial sums, by which the workspace is laid out.
@@ -471,9 +468,9 @@ extern "C" int gdp_embed_forward(const gdp_embed *e, void *stream)
     const int64_t blocks = ceil_div(e->n, per * s.each);
     return with_type(e->weight_type, [&](auto T) {
         return with_type(e->out_type, [&](auto O) {
-            return with_count(n, [&](auto N) {
-                using TT = decltype(T);
-                using OO = decltype(O);
+            using TT = decltype(T);
+            using OO = decltype(O);
+            return with_count<TT, OO>(n, [&](auto N) {
                 return launch("gdp_embed_forward", embed_rows_kernel<TT, OO, N.value>, dim3((unsigned)blocks, (unsigned)across), THREADS, 0, stream,
                               s, e->tokens, static_cast<const typename TT::raw *>(e->weight), static_cast<typename OO::raw *>(e->out));
             });
@@ -521,12 +518,14 @@ extern "C" int gdp_embed_backward(const gdp_embed_grad *e, void *stream)
     const int64_t units = l.pieces + (e->accumulate ? 0 : ceil_div(e->rows, (int64_t)fill_rows(s.unit >= 64)));
     return with_type(e->grad_type, [&](auto T) {
         return with_type(e->out_type, [&](auto O) {
-            return with_count(n, [&](auto N) {
-                using TT = decltype(T);
-                using OO = decltype(O);
+            using TT = decltype(T);
+            using OO = decltype(O);
+            return with_count<TT, OO>(n, [&](auto N) {
                 auto *const out = static_cast<typename OO::raw *>(e->out);
-                const int rc = launch("gdp_embed_backward", s.unit >= 64 ? embed_sum_kernel<TT, OO, N.value, true> : embed_sum_kernel<TT, OO, N.value, false>,
-                                      dim3((unsigned)ceil_div(units, per), (unsigned)across), THREADS, 0, stream, s,
+                auto kernel = embed_sum_kernel<TT, OO, N.value, false>;
+                if constexpr (N.value > 1)   // (rows of single elements are shared by less than a wave)
+                    if (s.unit >= 64) kernel = embed_sum_kernel<TT, OO, N.value, true>;
+                const int rc = launch("gdp_embed_backward", kernel, dim3((unsigned)ceil_div(units, per), (unsigned)across), THREADS, 0, stream, s,
                                       static_cast<const typename TT::raw *>(e->grad), out);
                 if (rc || l.pieces < 2) return rc;
                 constexpr int J = N.value < 4 ? N.value : 4;

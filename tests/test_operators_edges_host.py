@@ -83,3 +83,20 @@ def test_tangents_are_refused():
                     call(lambda p: p)
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda p: ops.token_logprobs(p, t).logp, (x,), (x,))
+
+
+# ---- what is compiled ------------------------------------------------------------------------------------------------
+@pytest.mark.skipif(shutil.which("nm") is None, reason="no nm")
+def test_every_embedding_kernel_has_calls_that_reach_it():
+    """Rows of less than 16 bytes are taken an element at a time, by less than a wave; others 16 bytes of the smaller type at a time: 4 elements
+    where both types are float32, 8 otherwise."""
+    names = subprocess.run(["nm", "-C", _lib.LIB_PATH], capture_output=True, text=True, check=True).stdout
+    got = {(k, *a.replace("ops::", "").split(", ")) for k, a in re.findall(r" (embed_\w+_kernel)<([^>]*)>", names.replace("(anonymous namespace)::", " "))}
+    types = ("F32", "F16", "BF16")
+    want = {("embed_index_kernel", t) for t in ("int", "long")} | {("embed_join_kernel", o, n) for o in types for n in "14"}
+    for t in types:
+        for o in types:
+            wide = "4" if t == o == "F32" else "8"
+            want |= {("embed_rows_kernel", t, o, n) for n in ("1", wide)}
+            want |= {("embed_sum_kernel", t, o, "1", "false"), ("embed_sum_kernel", t, o, wide, "false"), ("embed_sum_kernel", t, o, wide, "true")}
+    assert got == want
