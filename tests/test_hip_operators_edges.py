@@ -317,3 +317,38 @@ def test_norm_statistics_are_there_where_they_are_asked_for():
     for t in (x, x.clone().requires_grad_()):
         assert ops.residual_norm(t, pre=ops.Norm("rms")).stats is None
         assert ops.residual_norm(t, t, pre=ops.Norm("rms"), stats=True).stats.shape == (3, 4)
+
+
+# ---- from several threads ------------------------------------------------------------------------------------------
+def test_calls_of_two_threads():
+    """Each thread has its own stream, workspaces and errors."""
+    import threading
+    g = gen(41)
+    x, t, d = normal(g, 20, 70001, dtype=BF16, size=2.0), torch.randint(0, 70001, (20,), generator=g).cuda(), normal(g, 20, 64)
+    torch.cuda.synchronize()
+
+    def step():
+        r = ops.token_logprobs(x, t, entropy=True, top=20)
+        return [*r, ops.token_logprobs_grad(x, t, r.lse, r.logp), ops.embedding_grad(t, d, 70001)]
+
+    want, got, refused = step(), {}, {}
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            try:
+                for _ in range(20):
+                    got[i] = step()
+                    try:
+                        ops.token_logprobs(x, t, top=65) if i else ops.token_logprobs(x, t, scale=0.0)
+                    except ValueError as e:
+                        refused[i] = str(e)
+            finally:
+                torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for one in threads:
+        one.start()
+    for one in threads:
+        one.join()
+    assert all(torch.equal(a, b) for i in range(2) for a, b in zip(got[i], want))
+    assert "scale" in refused[0] and "top" in refused[1]
