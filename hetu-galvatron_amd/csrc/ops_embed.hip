@@ -42,7 +42,8 @@ struct Index {
     __device__ __forceinline__ int64_t slot(int64_t r) const { return (r & ((1 << shift) - 1)) * per_group + (r >> shift); }
 };
 
-// Bound by instructions: each workgroup looks at every token, some twelve of them a token and lane.  32768 tokens 12 us, 65536 20.
+// Bound by instructions: each workgroup looks at every token, some twelve of them a token and lane.  32768 tokens 12 us, 65536 20:
+// of narrow tables with many tokens that is what counts, 65536 x 1024 bf16 into 32000 rows takes 74 us, 1.8 times its bytes' time.
 template <typename I> __global__ __launch_bounds__(INDEX_THREADS) void embed_index_kernel(Index x, const I *__restrict__ tokens)
 {
     __shared__ int32_t count[INDEX_WAVES][INDEX_ROWS];
@@ -186,7 +187,7 @@ template <typename O, int N> __device__ __forceinline__ void put_row(const Sum &
     old.store_from(p, s.accumulate ? at.others : 0);   // (what is added to is added to once)
 }
 
-// Bound by memory: 32768 places of 4096 bf16 added up and 128256 rows written in 219 us, 1.32 GB at 6.0 TB/s; 16384 places into 19008 rows of
+// Bound by memory: 32768 places of 4096 bf16 added up and 128256 rows written in 217 us, 1.32 GB at 6.1 TB/s; 16384 places into 19008 rows of
 // 5120 float32 in 66 us, 328 MB at 5.0 TB/s.  Sixteen rows are on their way to each thread, past the caches, since each is read once.
 // WIDE: the threads that share a row are whole waves.  Then a wave's lanes read the numbers of 64 rows at once, which saves each row a
 // wait for them.
@@ -325,7 +326,8 @@ struct Rows {
     int64_t weight_stride, out_stride;
 };
 
-// Bound by memory: 32768 tokens of 4096 bf16, half the table: 72 us, 350 MB at 4.9 TB/s.  64 tokens of 1024: 2.8 us, a launch.
+// Bound by memory: 32768 tokens of 4096 bf16, half the table: 71 us, 350 MB at 4.9 TB/s, where calls follow each other; traced, each
+// behind a wait, 77.  64 tokens of 1024: 3.0 us, a launch.
 template <typename T, typename O, int N>
 __global__ __launch_bounds__(THREADS) void embed_rows_kernel(Rows s, const void *__restrict__ tokens, const typename T::raw *__restrict__ weight,
                                                              typename O::raw *__restrict__ out)
@@ -415,7 +417,7 @@ Layout layout_of(int64_t n, int64_t rows, int64_t dim)
     while (ceil_div(rows, (int64_t)1 << l.shift) > INDEX_ROWS) ++l.shift;
     l.per_group = ceil_div(rows, (int64_t)1 << l.shift);
     // A longer piece keeps fewer partial sums, which the join adds up one after another; a shorter one fills the device.  Up to 1024
-    // pieces do both: the gradient of 128256 x 4096 bf16 from 32768 tokens takes 244 us, 250 with 512, 263 with 2048 pieces.
+    // pieces do both: the gradient of 128256 x 4096 bf16 from 32768 tokens takes 240 us, 247 with 512, 251 with 2048 pieces.
     l.piece = 16;
     while (l.piece < 128 && n > 1024 * l.piece) l.piece *= 2;
     l.pieces = ceil_div(n, (int64_t)l.piece);

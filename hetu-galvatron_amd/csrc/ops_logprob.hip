@@ -99,8 +99,9 @@ __device__ __forceinline__ float top_logp(float x, float m, float s, float scale
     return s == 0.0f ? -__builtin_inff() : fmaf(x - m, scale, -logf(s));
 }
 
-// Bound by memory where rows are long: 8192 x 128256 bf16 in 365 us, 2.1 GB at 5.8 TB/s; 4096 x 50257 float32 with 5 alternatives in 158 us, 5.2
-// TB/s.  16 x 128256 bf16 with 20 alternatives: 10 us in 256 workgroups, 5 of them without alternatives: barriers and waits.
+// Bound by memory where rows are long: 8192 x 128256 bf16 in 364 us, 2.1 GB at 5.8 TB/s; 4096 x 50257 float32 with 5 alternatives in 158 us, 5.2
+// TB/s; a shard's 8192 x 16032 bf16 53 us, 4.9 TB/s.  16 x 128256 bf16 with 20 alternatives: 10 us in 256 workgroups, 5 of them without alternatives: barriers and waits.
+// Of short rows the choice takes longer than the reading: 15744 x 2304 bf16 23 us, 70 with 20 alternatives.
 // WAVES: four to a row or slice; one where rows are short and many.
 template <typename T, bool TOP, int WAVES> __global__ __launch_bounds__(64 * WAVES) void logprob_scan_kernel(Scan a, const typename T::raw *__restrict__ logits)
 {
@@ -543,7 +544,7 @@ Part part_at(void *p, int64_t parts, int64_t n, int top)
     return {reinterpret_cast<float4 *>(w), reinterpret_cast<float *>(w + a), reinterpret_cast<int32_t *>(w + a + b)};
 }
 
-// Rows of up to so many vectors (32 KB), and at least so many of them: a wave for each row instead of four.  32768 rows of 1000 bf16 28 us,
+// Rows of up to so many vectors (32 KB), and at least so many of them: a wave for each row instead of four.  32768 rows of 1000 bf16 25 us,
 // 89 with four waves; of 8192 bf16, top 5, 181 and 214; but 8192 of 16384, top 5, 89 and 85.
 constexpr int SHORT = 2048, SHORT_ROWS = 2048;
 constexpr int64_t MOST_ROWS = (int64_t)1 << 21, MOST_GROUPS = (int64_t)1 << 23;   // a grid has less than 2^32 threads

@@ -131,7 +131,8 @@ __device__ __forceinline__ float2 statistics(const float (&x)[K][E], const Colum
 }
 
 // At most W waves to a row, K times E elements to a thread; R rows to a workgroup where W is 1.  16384 x 4096 bf16 with both norms and a
-// gate: 109 us, 537 MB at 4.9 TB/s; 65536 x 1024 104 us; 8 x 4096 4.3 us, a launch and two barriers.
+// gate: 108 us, 537 MB at 5.0 TB/s; 65536 x 1024 102 us; 8 x 4096 4.4 us, a launch and two barriers.  Rows below 512 elements of 16 bits leave
+// lanes of their wave idle: 65536 x 128 36 us, 2.6 times its bytes' time.
 template <typename T, typename S, int W, int K, int E, bool TAIL, int R>
 __global__ __launch_bounds__(64 * W * R) void norm_forward_kernel(Join a, const typename S::raw *__restrict__ residual, const typename T::raw *__restrict__ block,
                                                                   typename S::raw *__restrict__ stream, typename T::raw *__restrict__ normed)
@@ -291,8 +292,10 @@ template <typename T, int K, int E, bool TAIL, bool HOLD> struct Weights {
     }
 };
 
-// 16384 x 4096 bf16 (mean of squares, gate) in 170 us, 805 MB at 4.7 TB/s; 16384 x 3584 with mean, biases, a gate for each of 4 sequences and a
-// float32 stream in 217 us and 6 for the sums, 1.06 GB at 4.9 TB/s.
+// 16384 x 4096 bf16 (mean of squares, gate) in 168 us, 805 MB at 4.8 TB/s; 16384 x 3584 with mean, biases, a gate for each of 4 sequences and a
+// float32 stream in 215 us and 6 for the sums, 1.06 GB at 4.9 TB/s.
+// Above 8192 elements (K = 2) sums and a row do not fit the registers and some are spilled: 8192 x 12288 bf16 601 us, 2.4 times its
+// bytes' time, x 16384 1070 us, 3.2 times.
 // BIAS: with sums for biases.
 template <typename T, typename S, bool HOLD, bool BIAS, int W, int K, int E, bool TAIL>
 __global__ __launch_bounds__(64 * W, W <= 4 ? 4 : W <= 12 ? 3 : 1) void norm_backward_kernel(Back a, const typename S::raw *__restrict__ stream, const typename T::raw *__restrict__ block,
@@ -582,8 +585,11 @@ struct Shares {
 Shares shares_of(int64_t n, int64_t dim, int64_t gates)
 {
     if (n == 0) return {0, 0, false};
-    // As many workgroups as are resident together, by their registers 16 waves on a core of up to 4 waves each, else 12: each writes its
-    // sums of columns, and one more than that would run alone at the end.
+    // Of 16-bit types as many workgroups as are resident together, by their registers 16 waves on a core of up to 4 waves each, else 12: each
+    // writes its sums of columns, and one more than that would run alone at the end.  Waves are counted as of 512 columns; float32 up to 4096
+    // columns has 256 a wave, so there are up to four times the workgroups that are resident: 16384 x 1024 91 us, 8192 x 2048 91, 8192 x 4096 170,
+    // 1.1, 1.1 and 1.0 times their bytes' time.  Where rows are few each workgroup has one, and the sums weigh as much as the rows: 2048
+    // x 1024 bf16 21 us, 4 times its bytes' time.
     const int64_t waves = ceil_div(dim, (int64_t)512), most = 256 * (waves <= 4 ? 16 / waves : waves <= 12 ? 12 / waves : 1);
     const int64_t rows = gates > 1 ? n / gates : 1, units = n / rows;
     if (gates > 1 && gates <= most / 2 && rows > 1) {

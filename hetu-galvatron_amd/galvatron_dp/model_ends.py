@@ -9,7 +9,8 @@ reference's profiler fills it in from whole training runs, model_profiler.py:302
         --profile configs/computation_profiling_bf16_llama.json
 
 measures those entries and writes them into the file, next to the entries of the layers that are there.  An entry is of the whole
-vocabulary on one GPU: the search divides it by the tensor-parallel degree itself, so a shard's time is printed only.
+vocabulary on one GPU: the search divides it by the tensor-parallel degree itself, so a shard's time is printed only.  What is timed
+are this package's operators: an entry is right for a program that runs its ends with them, and an estimate for one that does not.
 """
 from __future__ import annotations
 

@@ -16,7 +16,7 @@
  * Results do not depend on timing: the same inputs give the same bits.  Sums and statistics are held in
  * float32; what has a smaller type is rounded once, to nearest even.  Strides are in elements, between
  * rows; the elements of a row are neighbours.  Data need only be aligned to its element; rows that all start on
- * 16 bytes are read a little faster.
+ * 16 bytes are read a little faster.  Outputs overlap neither inputs nor each other, but where it is said that they may.
  */
 #ifndef GALVATRON_OPS_HIP_H
 #define GALVATRON_OPS_HIP_H
@@ -113,9 +113,9 @@ typedef struct gdp_logprob_stats {
 int gdp_logprob_forward_stats(const gdp_logprob_stats *l, void *stream);
 
 /* The same for a vocabulary in shards: `parts` of each shard, whose first column is token `first`, are joined
- * after the ranks have exchanged them (20 + 8 * top bytes a row instead of the row).  Of a part:
+ * after the ranks have exchanged them (16 + 8 * top bytes a row instead of the row).  Of a part:
  * stats [n][4] float32 (largest logit; sum of exp2; sum of exp2 times its exponent; the token's logit or
- * -inf), top_logits [n][top] float32 and top_tokens [n][top] int32, -1 behind the last of a shard with
+ * -inf), top_logits [n][top] float32, largest first, and top_tokens [n][top] int32, -1 behind the last of a shard with
  * fewer than `top` columns. */
 typedef struct gdp_logprob_part {
     int64_t n, vocab, first;
