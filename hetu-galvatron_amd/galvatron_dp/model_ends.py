@@ -90,7 +90,7 @@ class ModelEnds:
         if not 0.0 < loss_scale < math.inf:
             raise ValueError(f"loss_scale must be positive and finite, not {loss_scale}")
         joined, logits = self.logits(self.embed(tokens), block, stats=True)
-        row_stats = torch.empty(*targets.shape, 2, device=logits.device)
+        row_stats = torch.empty(*targets.shape, 2, dtype=torch.float32, device=logits.device)
         r = ops.token_logprobs(logits, targets, entropy=True, row_stats=row_stats)
         held = (targets >= 0) & (targets < self.vocab)
         each = held / held.sum().clamp(min=1)

@@ -58,3 +58,18 @@ def test_scaled_loss_of_the_other_types_and_the_command():
     for x, y in zip(one[2:], many[2:]):
         assert torch.equal(x * 64.0, y)          # (a power of two: the same digits)
     model_ends.main(["--hidden", "64", "--vocab", "500", "--seq", "32", "--precision", "fp16", "--backward"])
+
+
+@pytest.mark.gpu
+def test_another_default_type_of_the_program():
+    ends = model_ends.ModelEnds(32, 300, dtype=torch.bfloat16)
+    t, block = torch.arange(40, device="cuda").reshape(2, 20), torch.ones(2, 20, 32, device="cuda", dtype=torch.bfloat16)
+    want = ends.loss_and_grads(t, t, block)
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        got = ends.loss_and_grads(t, t, block)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    # (the shares of the mean are divided in the default type: one rounding of it more in each gradient)
+    for x, y in zip(got, want):
+        assert (x.double() - y.double()).abs().max() <= 4 * C.HALF_UNIT[torch.bfloat16] * y.double().abs().max()
