@@ -23,7 +23,7 @@ own = False     # False: plain forms.  True: the calls that a user makes of the 
 TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 SIZE = {"bf16": 2, "f16": 2, "f32": 4}
 BIASES = 48     # tokens with a bias of their own in each row
-LEAST_REST = 2.0 ** -24     # what float32 log probabilities tell from a list that holds everything
+LEAST_REST = 2.0 ** -22     # what float32 log probabilities tell from a list that holds everything: a smaller rest is none, or this for beta 1
 
 
 def _distill(name, N, V, K, type, beta=0.0, rest=True, targets=True, scale=1.0, masked=0.0, index="i64"):
@@ -109,10 +109,10 @@ def work(c):
     n, e = c["N"] * c["V"], SIZE[c["type"]]
     index = 8 if c["index"] == "i64" else 4
     if c["kind"] == "distill":
-        rows = c["K"] * (index + 8) + 20 + (index + 4 if c["targets"] else 0)
+        rows = c["K"] * (index + 8) + 28 + (index + 4 if c["targets"] else 0)
         return dict(bytes=n * e + c["N"] * rows, flops=4 * n)
     if c["kind"] == "distill_grad":
-        rows = c["K"] * (index + 4) + 16 + (index + 4 if c["targets"] else 0)
+        rows = c["K"] * (index + 4) + 24 + (index + 4 if c["targets"] else 0)
         return dict(bytes=2 * n * e + c["N"] * rows, flops=4 * n)
     held = 0.625 * c["N"] * c["H"]      # places that count, on average
     bits = n / 8 if c["allowed"] is not None else 0
@@ -237,37 +237,45 @@ def _in_pieces(f, c):
     return torch.cat([f(slice(at, at + step)) for at in range(0, c["N"], step)])
 
 
+def _level(x):
+    """A largest logit to subtract: 0 where there is none above -inf."""
+    return torch.where(torch.isneginf(x), 0.0, x)
+
+
 def _left(c, rows=slice(None)):
     x, t = c["logits"][rows].float(), c["tokens"][rows].long()
     N, V, scale, beta = x.shape[0], x.shape[1], c["scale"], c["beta"]
     lq = c["teacher"][rows].double()
     used = (t >= 0) & (t < V) & (lq > -math.inf)
     at = torch.where(used, t, 0)
-    largest = x.amax(1, keepdim=True)
-    d = (x - largest) * scale
-    e = torch.exp(d)
     is_listed = torch.zeros(N, V + 1, dtype=torch.bool, device=x.device).scatter_(1, torch.where(used, t, V), True)[:, :V]
-    s_out = torch.where(is_listed, 0.0, e).sum(1).double()
-    d_k = d.gather(1, at).double()
-    s = s_out + torch.where(used, torch.exp(d_k), 0.0).sum(1)
-    log_s = torch.log(s)
+    rest = x.masked_fill(is_listed, -math.inf)
+    others = rest.amax(1, keepdim=True)
+    of_rest = torch.exp((rest - _level(others)) * scale).sum(1)
+    x_k = torch.where(used, x.gather(1, at), -math.inf)
+    largest = torch.maximum(others, x_k.amax(1, keepdim=True))
+    d_k, d_out = (x_k - largest).double() * scale, (others - largest)[:, 0].double() * scale
+    s_out = of_rest.double() * torch.exp(d_out)
+    s = s_out + torch.exp(d_k).sum(1)
+    log_s, log_s_out = torch.log(s), torch.log(of_rest)
     lp = torch.where(used, d_k - log_s[:, None], -math.inf)
     p, p_out = torch.exp(lp), s_out / s
     q = torch.exp(torch.where(used, lq, -math.inf))
     mass = q.sum(1, keepdim=True)
     if c["rest"]:
-        r = torch.where(s_out > 0, (1.0 - mass[:, 0]).clamp(min=LEAST_REST), 0.0)
+        r = 1.0 - mass[:, 0]
+        r = torch.where((s_out > 0) & ((r >= LEAST_REST) | (beta == 1.0)), r.clamp(min=LEAST_REST), 0.0)
     else:
         q, r = q / mass.clamp(min=1e-300), torch.zeros_like(s)
-    lq, lr, l_out = torch.log(q), torch.log(r), torch.log(p_out)
+    lq, lr, l_out = torch.log(q), torch.log(r), d_out + log_s_out.double() - log_s
     total = q.sum(1) + r
     if beta == 0.0:
         loss = torch.where(used, q * (lq - lp), 0.0).sum(1) + torch.where(r > 0, r * (lr - l_out), 0.0)
-        pull, c_out = p * total[:, None] - q, total - torch.where(r > 0, r / p_out, 0.0)
+        pull, c_out = p * total[:, None] - q, total * p_out - r
     elif beta == 1.0:
         a, a_out = torch.where(used, lp - lq, 0.0), torch.where(s_out > 0, l_out - lr, 0.0)
         loss = (p * a).sum(1) + p_out * a_out
-        pull, c_out = p * (a - loss[:, None]), a_out - loss
+        pull, c_out = p * (a - loss[:, None]), p_out * (a_out - loss)
     else:
         m, m_out = beta * q + (1 - beta) * p, beta * r + (1 - beta) * p_out
         a = torch.where(p > 0, lp - torch.log(m), 0.0)
@@ -275,30 +283,30 @@ def _left(c, rows=slice(None)):
         to = torch.where(q > 0, q * (lq - torch.log(m)), 0.0).sum(1) + torch.where(r > 0, r * (lr - torch.log(m_out)), 0.0)
         mean = (p * a).sum(1) + p_out * a_out
         loss = beta * to + (1 - beta) * mean
-        pull, c_out = (1 - beta) * p * (a - mean[:, None]), (1 - beta) * (a_out - mean)
-    pull, c_out = torch.where(used, pull, 0.0), torch.where(s_out > 0, c_out, 0.0)
+        pull, c_out = (1 - beta) * p * (a - mean[:, None]), (1 - beta) * p_out * (a_out - mean)
+    pull = torch.where(used, pull, 0.0)
     got = {"loss": loss.float(), "lse": (largest[:, 0].double() * scale + log_s).float(),
-           "stats": torch.cat([largest, log_s[:, None].float(), c_out[:, None].float(), pull.float()], 1)}
+           "stats": torch.cat([largest, log_s[:, None].float(), others, log_s_out[:, None], c_out[:, None].float(), pull.float()], 1)}
     if c["target"] is not None:
         w = c["target"][rows].long()
         here = (w >= 0) & (w < V)
-        got["logp"] = torch.where(here, d.gather(1, torch.where(here, w, 0)[:, None])[:, 0] - log_s, 0.0).float()
+        got["logp"] = torch.where(here, (x.gather(1, torch.where(here, w, 0)[:, None]) - largest)[:, 0] * scale - log_s, 0.0).float()
     return got
 
 
 def _distill_grad_plain(c):
     x, scale, stats = c["logits"].float(), c["scale"], c["stats"]
     V = x.shape[1]
-    p = torch.exp((x - stats[:, 0:1]) * scale - stats[:, 1:2])
+    share = torch.exp((x - _level(stats[:, 2:3])) * scale - _level(stats[:, 3:4]))      # of what is not listed
     t = c["tokens"].long() - c["first"]
     here = (t >= 0) & (t < V) & (c["tokens"] >= 0)
-    g = torch.cat([c["d_loss"][:, None] * stats[:, 2:3] * p, torch.zeros_like(p[:, :1])], 1)
-    g.scatter_(1, torch.where(here, t, V), c["d_loss"][:, None] * stats[:, 3:])     # (the last column takes what is elsewhere)
+    g = torch.cat([c["d_loss"][:, None] * stats[:, 4:5] * share, torch.zeros_like(x[:, :1])], 1)
+    g.scatter_(1, torch.where(here, t, V), c["d_loss"][:, None] * stats[:, 5:])     # (the last column takes what is elsewhere)
     if c["target"] is not None:
         held = (c["target"] >= 0) & (c["target"] < c["vocab"])
         d = torch.where(held, c["d_logp"], 0.0)
         w = c["target"].long() - c["first"]
-        g[:, :V] -= d[:, None] * p
+        g[:, :V] -= torch.exp((x - stats[:, 0:1]) * scale - stats[:, 1:2]).mul_(d[:, None])
         g.scatter_add_(1, torch.where(held & (w >= 0) & (w < V), w, V)[:, None], d[:, None])
     return (g[:, :V] * scale).to(c["logits"].dtype)
 
@@ -419,13 +427,17 @@ def _exact_distill(c, rows):
     others = ell.clone()
     others[row[~gone], t[~gone]] = -math.inf
     u = torch.cat([ell.gather(1, t.clamp(0, V - 1)).masked_fill(gone, -1e300), torch.logsumexp(others, 1)[:, None]], 1)
+    of_others = others.amax(1, keepdim=True)
+    of_others = torch.cat([c["logits"][rows].double().masked_fill(torch.isneginf(others), -math.inf).amax(1, keepdim=True), u[:, -1:] - of_others], 1)
     del others
     no_rest = torch.isneginf(u[:, -1:])
     u = u.masked_fill(torch.cat([torch.zeros_like(gone), no_rest], 1), -1e300).requires_grad_(True)
     lp = torch.log_softmax(u, 1)
     lq = lq.masked_fill(gone, -math.inf)
     if c["rest"]:
-        left = (1.0 - lq.exp().sum(1, keepdim=True)).clamp(min=LEAST_REST).log().masked_fill(no_rest, -math.inf)
+        left = 1.0 - lq.exp().sum(1, keepdim=True)
+        none = no_rest if c["beta"] == 1.0 else no_rest | (left < LEAST_REST)
+        left = left.clamp(min=LEAST_REST).log().masked_fill(none, -math.inf)
         lq = torch.cat([lq, left], 1)
     else:
         lq = torch.cat([lq - torch.logsumexp(lq, 1, keepdim=True), torch.full_like(lq[:, :1], -math.inf)], 1)
@@ -443,10 +455,9 @@ def _exact_distill(c, rows):
         loss = beta * (q * (lq - lm)).sum(1) + (1 - beta) * (p * (torch.where(there, lp, 0.0) - lm)).sum(1)
     d, = torch.autograd.grad(loss.sum(), u)
     with torch.no_grad():
-        share = torch.where(no_rest, 1.0, lp[:, -1:].exp())
         lse = torch.logsumexp(c["logits"][rows].double() * c["scale"], 1)
-        at_rest = torch.where(no_rest, 0.0, d[:, -1:] / share)
-        stats = torch.cat([largest[:, None], (lse - largest * c["scale"])[:, None], at_rest, torch.where(gone, 0.0, d[:, :-1])], 1)
+        stats = torch.cat([largest[:, None], (lse - largest * c["scale"])[:, None], of_others, torch.where(no_rest, 0.0, d[:, -1:]),
+                           torch.where(gone, 0.0, d[:, :-1])], 1)
         out = {"loss": loss.detach(), "lse": lse, "stats": stats}
         if c["target"] is not None:
             w = c["target"][rows].long()
@@ -457,18 +468,18 @@ def _exact_distill(c, rows):
 def _exact_distill_grad(c, rows):
     x, s = c["logits"][rows].double(), c["stats"][rows].double()
     n, V = x.shape
-    share = torch.exp(c["scale"] * (x - s[:, :1]) - s[:, 1:2])
     d = c["d_loss"][rows].double()[:, None]
-    out = share * (s[:, 2:3] * d)
+    out = torch.exp(c["scale"] * (x - s[:, 2:3].clamp(min=-1e300)) - s[:, 3:4].clamp(min=-1e300)) * (s[:, 4:5] * d)
+    out.masked_fill_(torch.isneginf(x), 0.0)
     row = torch.arange(n, device=x.device)
     t = c["tokens"][rows].long()
     local = t - c["first"]
     inside = (t >= 0) & (local >= 0) & (local < V)
-    out[row[:, None].expand_as(t)[inside], local[inside]] = (s[:, 3:] * d)[inside]
+    out[row[:, None].expand_as(t)[inside], local[inside]] = (s[:, 5:] * d)[inside]
     if c["target"] is not None:
         w = c["target"][rows].long()
         g = c["d_logp"][rows].double() * ((w >= 0) & (w < c["vocab"]))
-        out -= g[:, None] * share
+        out -= g[:, None] * torch.exp(c["scale"] * (x - s[:, :1]) - s[:, 1:2])
         w = w - c["first"]
         inside = (w >= 0) & (w < V)
         out[row[inside], w[inside]] += g[inside]
