@@ -208,7 +208,17 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t v)
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // 1 ulp; below 2^-126: 0
 
+__device__ __forceinline__ float finite_or_0(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+
 // ---- host ----
+template <typename F> int with_type(int t, F f)
+{
+    switch (t) {
+    case GDP_F32: return f(F32{});
+    case GDP_F16: return f(F16{});
+    default: return f(BF16{});
+    }
+}
 inline bool type_ok(int t) { return t == GDP_F32 || t == GDP_F16 || t == GDP_BF16; }
 inline bool token_type_ok(int t) { return t == GDP_I32 || t == GDP_I64; }
 inline int size_of(int t) { return t == GDP_F32 ? 4 : 2; }

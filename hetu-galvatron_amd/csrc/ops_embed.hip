@@ -389,14 +389,6 @@ int unit_of(int64_t dim, int n)
     return u;
 }
 
-template <typename F> int with_type(int t, F f)
-{
-    switch (t) {
-    case GDP_F32: return f(F32{});
-    case GDP_F16: return f(F16{});
-    default: return f(BF16{});
-    }
-}
 template <typename T, typename O, typename F> int with_count(int n, F f)
 {
     return n == 1 ? f(std::integral_constant<int, 1>{}) : f(std::integral_constant<int, AT_ONCE<T, O>>{});

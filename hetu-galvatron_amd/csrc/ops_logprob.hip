@@ -46,7 +46,6 @@ __device__ __forceinline__ float of_key(uint32_t k)
 struct Sums {
     float m, s, t;
 };
-__device__ __forceinline__ float finite_or_0(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 // (a part without any probability has s = t = 0 and m = -inf)
 __device__ __forceinline__ Sums rescaled(Sums a, float m, float c)
 {
@@ -569,15 +568,6 @@ int check_logits(const void *p, int64_t n, int64_t vocab, int64_t stride, int ty
     if (!aligned(p, size_of(type)) || !aligned(tokens, token_type == GDP_I64 ? 8 : 4))
         return gdp_fail(GDP_E_BADARG, "gdp_logprob: a pointer is not aligned to its elements");
     return GDP_OK;
-}
-
-template <typename F> int with_type(int t, F f)
-{
-    switch (t) {
-    case GDP_F32: return f(F32{});
-    case GDP_F16: return f(F16{});
-    default: return f(BF16{});
-    }
 }
 
 int scan(Scan s, const void *logits, int type, const Split &split, const char *who, void *stream)

@@ -9,7 +9,13 @@ torch tensors:
     logprob_parts, join_logprobs                        ... of a vocabulary in shards
     residual_norm, residual_norm_grad                   norms after a block and before the next, gate, scales
 
-``embedding``, ``token_logprobs`` and ``residual_norm`` are differentiable (once, backwards: tensors with forward-mode
+and what is done with the logits there:
+
+    distillation, distillation_grad                     divergence from a teacher's most likely tokens
+    distillation_parts, join_distillation               ... of a vocabulary in shards
+    adjust_logits, adjust_logits_grad                   penalties for repeated tokens, biases, a grammar's mask, temperature
+
+``embedding``, ``token_logprobs``, ``residual_norm``, ``distillation`` and ``adjust_logits`` are differentiable (once, backwards: tensors with forward-mode
 tangents are refused); the ``*_grad`` functions are what their backward passes call, for programs that run their own.
 Work is queued on torch's current stream of the tensors' device; nothing waits.  Types: float32, float16, bfloat16; token
 numbers int32 or int64.  Per-token tensors may have any strides (one whose rows' elements are not neighbours is copied
@@ -28,10 +34,13 @@ from . import _lib
 
 __all__ = ["embedding", "embedding_grad", "TokenLogprobs", "token_logprobs", "token_logprobs_grad", "LogprobParts",
            "logprob_parts", "join_logprobs", "Norm", "ResidualNorm", "ResidualNormGrads", "residual_norm",
-           "residual_norm_grad", "MAX_TOP", "MAX_NORM_DIM"]
+           "residual_norm_grad", "Distillation", "distillation", "distillation_grad", "DistillationParts", "distillation_parts",
+           "join_distillation", "adjust_logits", "adjust_logits_grad", "MAX_TOP", "MAX_NORM_DIM", "MAX_LISTED", "MAX_BIASES"]
 
 MAX_TOP = 64            # GDP_MAX_TOP
 MAX_NORM_DIM = 16384    # GDP_MAX_NORM_DIM
+MAX_LISTED = 256        # GDP_MAX_LISTED
+MAX_BIASES = 1024       # GDP_MAX_BIASES
 EXPORTED_SYMBOLS = _lib.OPERATOR_SYMBOLS
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -113,6 +122,50 @@ class gdp_norm_grad(ctypes.Structure):
                 ("grad_post_bias", _p), ("grad_gate", _p), ("workspace", _p), ("workspace_bytes", _size)]
 
 
+class gdp_distill(ctypes.Structure):
+    _fields_ = [("n", _i64), ("vocab", _i64), ("logits", _p), ("logits_stride", _i64), ("logits_type", _i32),
+                ("list_type", _i32), ("target_type", _i32), ("listed", _i32), ("tokens", _p), ("teacher", _p), ("targets", _p),
+                ("scale", _f32), ("beta", _f32), ("rest", _i32), ("reserved", _i32), ("loss", _p), ("lse", _p), ("logp", _p),
+                ("stats", _p), ("workspace", _p), ("workspace_bytes", _size)]
+
+
+class gdp_distill_part(ctypes.Structure):
+    _fields_ = [("n", _i64), ("vocab", _i64), ("first", _i64), ("logits", _p), ("logits_stride", _i64), ("logits_type", _i32),
+                ("list_type", _i32), ("target_type", _i32), ("listed", _i32), ("tokens", _p), ("teacher", _p), ("targets", _p),
+                ("scale", _f32), ("reserved", _i32), ("sums", _p), ("listed_logits", _p), ("workspace", _p),
+                ("workspace_bytes", _size)]
+
+
+class gdp_distill_joint(ctypes.Structure):
+    _fields_ = [("n", _i64), ("vocab", _i64), ("parts", _i32), ("list_type", _i32), ("target_type", _i32), ("listed", _i32),
+                ("tokens", _p), ("teacher", _p), ("targets", _p), ("scale", _f32), ("beta", _f32), ("rest", _i32),
+                ("reserved", _i32), ("sums", _p), ("listed_logits", _p), ("loss", _p), ("lse", _p), ("logp", _p), ("stats", _p)]
+
+
+class gdp_distill_grad(ctypes.Structure):
+    _fields_ = [("n", _i64), ("vocab", _i64), ("first", _i64), ("whole_vocab", _i64), ("logits", _p), ("logits_stride", _i64),
+                ("logits_type", _i32), ("list_type", _i32), ("target_type", _i32), ("listed", _i32), ("tokens", _p),
+                ("targets", _p), ("stats", _p), ("grad_loss", _p), ("grad_lse", _p), ("grad_logp", _p), ("scale", _f32),
+                ("reserved", _i32), ("out", _p), ("out_stride", _i64)]
+
+
+class gdp_adjust_history(ctypes.Structure):
+    _fields_ = [("tokens", _p), ("places", _i64), ("stride", _i64), ("token_type", _i32), ("length_type", _i32),
+                ("prompt_type", _i32), ("repetition", _f32), ("frequency", _f32), ("presence", _f32), ("lengths", _p),
+                ("prompts", _p), ("repetitions", _p), ("frequencies", _p), ("presences", _p)]
+
+
+class gdp_adjust(ctypes.Structure):
+    _fields_ = [("n", _i64), ("vocab", _i64), ("first", _i64), ("logits", _p), ("logits_stride", _i64), ("logits_type", _i32),
+                ("out_type", _i32), ("history", gdp_adjust_history), ("bias_tokens", _p), ("bias", _p), ("bias_stride", _i64),
+                ("biases", _i32), ("bias_token_type", _i32), ("allowed", _p), ("allowed_stride", _i64), ("words", _i64),
+                ("scales", _p), ("scale", _f32), ("reserved", _i32), ("out", _p), ("out_stride", _i64)]
+
+
+class gdp_adjust_grad(ctypes.Structure):
+    _fields_ = [("given", gdp_adjust), ("grad", _p), ("grad_stride", _i64)]
+
+
 _bound = None
 
 
@@ -133,14 +186,18 @@ def _ops() -> ctypes.CDLL:
                              ("gdp_logprob_forward_stats", gdp_logprob_stats),
                              ("gdp_logprob_join_stats", gdp_logprob_joint_stats),
                              ("gdp_logprob_backward_stats", gdp_logprob_grad_stats),
-                             ("gdp_norm_forward", gdp_norm), ("gdp_norm_backward", gdp_norm_grad)):
+                             ("gdp_norm_forward", gdp_norm), ("gdp_norm_backward", gdp_norm_grad),
+                             ("gdp_distill_forward", gdp_distill), ("gdp_distill_parts", gdp_distill_part),
+                             ("gdp_distill_join", gdp_distill_joint), ("gdp_distill_backward", gdp_distill_grad),
+                             ("gdp_adjust_forward", gdp_adjust), ("gdp_adjust_backward", gdp_adjust_grad)):
             f = getattr(L, name)
             f.argtypes, f.restype = [ctypes.POINTER(record), ctypes.c_void_p], ctypes.c_int
         size = ctypes.POINTER(_size)
         L.gdp_embed_grad_workspace.argtypes = [_i64, _i64, _i64, size]
         L.gdp_logprob_workspace.argtypes = [_i64, _i64, _i32, _i32, size]
         L.gdp_norm_grad_workspace.argtypes = [_i64, _i64, _i64, size]
-        for name in ("gdp_embed_grad_workspace", "gdp_logprob_workspace", "gdp_norm_grad_workspace"):
+        L.gdp_distill_workspace.argtypes = [_i64, _i64, _i32, _i32, size]
+        for name in ("gdp_embed_grad_workspace", "gdp_logprob_workspace", "gdp_norm_grad_workspace", "gdp_distill_workspace"):
             getattr(L, name).restype = ctypes.c_int
         _bound = L
     return _bound
@@ -194,6 +251,14 @@ def _written(t):
     """Tells autograd that a tensor of the caller has been written, as torch's own functions do: a graph that holds it says so, rather than
     going on with other values."""
     torch.autograd.graph.increment_version(t)
+
+
+def _constants(**tensors):
+    """Refuses inputs that want a gradient which there is none of."""
+    if torch.is_grad_enabled():
+        for what, t in tensors.items():
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                raise ValueError(f"{what} gets no gradient: detach it")
 
 
 def _ptr(t):
@@ -781,3 +846,450 @@ def residual_norm(residual, block=None, *, post: Optional[Norm] = None, pre: Opt
                                                     residual_scale, block_scale)
         return ResidualNorm(stream, normed, given if stats else None)
     return ResidualNorm(*_residual_norm(residual, block, post, pre, gate, residual_scale, block_scale, stats))
+
+
+# ---- distillation ------------------------------------------------------------------------------------------
+class Distillation(NamedTuple):
+    loss: torch.Tensor                          # [...]       divergence of each row
+    lse: torch.Tensor                           # [...]       log of the sum of exponentials of scale * logits
+    logp: Optional[torch.Tensor] = None         # [...]       of the targets, 0 where there is none
+    stats: Optional[torch.Tensor] = None        # [..., 5 + listed] where asked for: what the gradient takes
+
+
+class DistillationParts(NamedTuple):
+    """What a shard of the vocabulary knows of its rows, to be exchanged and joined."""
+    sums: torch.Tensor                          # [n, 4]      float32
+    listed_logits: torch.Tensor                 # [n, listed] float32
+
+
+_STATS = 5      # numbers of a row's stats in front of those of its places
+
+
+def _list_of(tokens, teacher, targets, shape, device):
+    """Checked lists and targets: tokens, their type, log probabilities, targets, their type."""
+    list_type = _type(tokens, "tokens", _TOKEN_TYPES)
+    listed = tokens.shape[-1] if tokens.dim() else 0
+    if tokens.dim() != len(shape) + 1 or tokens.shape[:-1] != shape or not 1 <= listed <= MAX_LISTED:
+        raise ValueError(f"tokens must be {list(shape) + ['listed']} with 1 to {MAX_LISTED} listed, not {list(tokens.shape)}")
+    _same_device(device, tokens=tokens)
+    teacher = _floats(teacher, tokens.shape, "teacher", device)
+    target_type = 0
+    if targets is not None:
+        target_type = _type(targets, "targets", _TOKEN_TYPES)
+        if targets.shape != shape:
+            raise ValueError(f"targets must be {list(shape)}, not {list(targets.shape)}")
+        _same_device(device, targets=targets)
+        targets = targets.contiguous()
+    return tokens.contiguous(), list_type, teacher, targets, target_type, listed
+
+
+def _distillation_outputs(shape, with_logp, stats, listed, device):
+    n, count = shape.numel(), 3 if with_logp else 2
+    if n and shape:
+        # One allocation, but no views of it: parts of one tensor could not be changed in place, and would share their version.
+        rows = torch.empty((count * shape[0],) + shape[1:], dtype=torch.float32, device=device).unsafe_chunk(count)
+    else:
+        rows = [torch.empty(shape, dtype=torch.float32, device=device) for _ in range(count)]
+    left = torch.empty(shape + (_STATS + listed,), dtype=torch.float32, device=device) if stats else None
+    return n, rows[0], rows[1], rows[2] if with_logp else None, left
+
+
+def _distillation(logits, tokens, teacher, targets, scale, beta, rest, stats):
+    logits_type = _type(logits, "logits")
+    if logits.dim() < 1:
+        raise ValueError("logits must be [..., vocab]")
+    device, vocab, shape = logits.device, logits.shape[-1], logits.shape[:-1]
+    flat, list_type, teacher, targets, target_type, listed = _list_of(tokens, teacher, targets, shape, device)
+    n, loss, lse, logp, left = _distillation_outputs(shape, targets is not None, stats, listed, device)
+    rows, stride = _rows(logits, vocab, "logits") if n and vocab else (logits, vocab)
+    work, size = _workspace("gdp_distill_workspace", n, vocab, logits_type, listed, device=device)
+    _queue(_ops().gdp_distill_forward,
+           gdp_distill(n, vocab, rows.data_ptr(), stride, logits_type, list_type, target_type, listed, flat.data_ptr(),
+                       teacher.data_ptr(), _ptr(targets), scale, beta, rest, 0, loss.data_ptr(), lse.data_ptr(), _ptr(logp),
+                       _ptr(left), _ptr(work), size), device)
+    return loss, lse, logp, left
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, teacher, targets, scale, beta, rest):
+        loss, lse, logp, left = _distillation(logits, tokens, teacher, targets, scale, beta, rest, True)
+        ctx.save_for_backward(logits, tokens, targets, left)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(left)
+        return loss, lse, logp, left
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_loss, d_lse, d_logp, _):
+        logits, tokens, targets, left = ctx.saved_tensors
+        return distillation_grad(logits, tokens, left, d_loss, scale=ctx.scale, targets=targets, grad_lse=d_lse,
+                                 grad_logp=d_logp), None, None, None, None, None, None
+
+
+def distillation(logits, tokens, teacher, *, scale: float = 1.0, beta: float = 0.0, rest: bool = True, targets=None,
+                 stats: bool = False) -> Distillation:
+    """How far softmax(scale * logits) over the last dimension of ``logits`` [..., vocab] is from a teacher, of which the log
+    probabilities ``teacher`` [..., listed] of the ``tokens`` [..., listed] (at most 256) are known: the ``top_logp`` and
+    ``top_tokens`` of its ``token_logprobs``, at the temperature that ``scale`` stands for.  All in float32.
+
+    With q of the teacher and p of the logits, over the listed tokens and the rest of the vocabulary as one more: ``beta`` 0 the sum of
+    q log(q / p), 1 that of p log(p / q), and between them beta * (q against a) + (1 - beta) * (p against a) for
+    a = beta * q + (1 - beta) * p.  Without ``rest`` the teacher's scores, whatever they are relative to, are normed over its list and q of
+    the rest is 0, which ``beta`` 1 does not permit.  (What float32 cannot tell from a list that holds everything, a rest below 2^-22, is
+    0, and 2^-22 for ``beta`` 1.)
+
+    A place whose token is outside [0, vocab), such as -1, or whose log probability is -inf is not used; a token in several places counts once,
+    with the sum of its probabilities.  Rows of logits without an unlisted token above -inf have no rest.  A listed token that a row
+    rules out makes its loss inf at ``beta`` 0.  Rows of nothing but -inf, and without ``rest`` those of an empty list, have a loss of 0
+    and no gradient from it; NaN or +inf make their row's results NaN.
+
+    ``targets`` [...]: their log probabilities ride along, as ``token_logprobs`` gives them, for a loss that has both.  ``stats``: returned,
+    for ``distillation_grad``.  The teacher gets no gradient."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(logits, teacher)
+    _constants(teacher=teacher)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        r = _Distillation.apply(logits, tokens, teacher, targets, float(scale), float(beta), bool(rest))
+    else:
+        r = _distillation(logits, tokens, teacher, targets, float(scale), float(beta), bool(rest), stats)
+    return Distillation(r[0], r[1], r[2], r[3] if stats else None)
+
+
+def distillation_grad(logits, tokens, stats, grad_loss=None, *, scale: float = 1.0, targets=None, grad_lse=None, grad_logp=None,
+                      first: int = 0, vocab: Optional[int] = None, into: Optional[torch.Tensor] = None):
+    """Gradient with respect to ``logits`` [..., columns], in their type, from those of ``distillation``'s results.
+
+    ``tokens`` and ``targets`` as they were given to the forward pass, ``stats`` as it left them.  Of a vocabulary in shards, ``logits`` are
+    those of the shard that begins with token ``first``, of ``vocab`` tokens in all, and ``stats`` those of ``join_distillation``.
+    ``into``: written there; it may be ``logits`` itself."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(logits, stats, grad_loss, grad_lse, grad_logp, into)
+    logits_type = _type(logits, "logits")
+    if logits.dim() < 1:
+        raise ValueError("logits must be [..., vocab]")
+    device, columns, shape = logits.device, logits.shape[-1], logits.shape[:-1]
+    if vocab is None:
+        vocab = first + columns
+    flat, list_type, _, targets, target_type, listed = _list_of(tokens, None, targets, shape, device)
+    if stats.dtype != torch.float32:
+        raise ValueError(f"stats must be as distillation gives them: float32, not {stats.dtype}")
+    stats = _floats(stats, shape + (_STATS + listed,), "stats", device)
+    if grad_logp is not None and targets is None:
+        raise ValueError("grad_logp needs the targets")
+    grad_loss, grad_lse = _floats(grad_loss, shape, "grad_loss", device), _floats(grad_lse, shape, "grad_lse", device)
+    grad_logp = _floats(grad_logp, shape, "grad_logp", device)
+    n = shape.numel()
+    out, to = _gradient_place(logits, into, n and columns)
+    if not n or not columns:
+        return out
+    rows, stride = _rows(logits, columns, "logits")
+    _queue(_ops().gdp_distill_backward,
+           gdp_distill_grad(n, columns, first, vocab, rows.data_ptr(), stride, logits_type, list_type, target_type, listed,
+                            flat.data_ptr(), _ptr(targets), stats.data_ptr(), _ptr(grad_loss), _ptr(grad_lse), _ptr(grad_logp),
+                            scale, 0, to.data_ptr(), to.stride(0)), device)
+    if into is not None:
+        _written(into)
+    return out
+
+
+def _gradient_place(logits, into, some):
+    """What is returned, and the same as rows where there are some."""
+    if into is None:
+        out = _like(logits)
+    else:
+        out = into
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+            raise ValueError("into must have the shape, type and device of logits")
+    return out, _rows_in_place(out, "into") if some else None
+
+
+def _rows_in_place(t, what):
+    """[..., columns] as rows at one stride, which are the tensor's own memory."""
+    columns = t.shape[-1]
+    try:
+        rows = t if t.dim() == 2 else t.view(-1, columns)
+        if columns > 1 and rows.stride(1) != 1:
+            raise RuntimeError
+    except RuntimeError:
+        raise ValueError(f"{what} must have rows that are neighbouring elements at one stride") from None
+    return rows
+
+
+def distillation_parts(logits, tokens, teacher, *, first: int, scale: float = 1.0, targets=None) -> DistillationParts:
+    """``distillation`` of a shard of the vocabulary, ``logits`` [n, columns] of the tokens from ``first`` on, up to what the other
+    shards have to say: 16 + 4 * listed bytes for each row, to be gathered from all shards and joined."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(logits, teacher)
+    _constants(teacher=teacher)
+    logits_type = _type(logits, "logits")
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [n, columns], not {list(logits.shape)}")
+    device, (n, columns) = logits.device, logits.shape
+    flat, list_type, teacher, targets, target_type, listed = _list_of(tokens, teacher, targets, logits.shape[:1], device)
+    rows, stride = _rows(logits, columns, "logits") if n and columns else (logits, columns)
+    parts = DistillationParts(torch.empty(n, 4, dtype=torch.float32, device=device),
+                              torch.empty(n, listed, dtype=torch.float32, device=device))
+    work, size = _workspace("gdp_distill_workspace", n, columns, logits_type, listed, device=device)
+    _queue(_ops().gdp_distill_parts,
+           gdp_distill_part(n, columns, first, rows.data_ptr(), stride, logits_type, list_type, target_type, listed,
+                            flat.data_ptr(), teacher.data_ptr(), _ptr(targets), scale, 0, parts.sums.data_ptr(),
+                            parts.listed_logits.data_ptr(), _ptr(work), size), device)
+    return parts
+
+
+def join_distillation(parts, tokens, teacher, vocab: int, *, scale: float = 1.0, beta: float = 0.0, rest: bool = True, targets=None,
+                      stats: bool = False) -> Distillation:
+    """``distillation`` of a vocabulary of ``vocab`` tokens from the parts of its shards: ``DistillationParts``, or one whose tensors
+    have a leading dimension for the shards, as gathering them leaves it."""
+    if not isinstance(parts, DistillationParts):
+        parts = list(parts)
+        if not parts or any(a.shape != b.shape for p in parts for a, b in zip(p, parts[0])):
+            raise ValueError("parts must be one of each shard, of the same rows and listed tokens")
+        parts = DistillationParts(*(torch.stack(t) for t in zip(*parts)))
+    if forward_ad._current_level >= 0:
+        _no_tangents(*parts, teacher)
+    _constants(teacher=teacher)
+    sums, listed_logits = (t.contiguous() for t in parts)
+    if sums.dim() != 3 or sums.shape[2] != 4 or listed_logits.dim() != 3 or listed_logits.shape[:2] != sums.shape[:2]:
+        raise ValueError("parts must be sums [parts, n, 4] and listed_logits [parts, n, listed]")
+    if sums.dtype != torch.float32 or listed_logits.dtype != torch.float32:
+        raise ValueError("parts must be as distillation_parts gives them: float32")
+    _type(sums, "parts")
+    device, count, shape = sums.device, sums.shape[0], sums.shape[1:2]
+    _same_device(device, listed_logits=listed_logits)
+    flat, list_type, teacher, targets, target_type, listed = _list_of(tokens, teacher, targets, shape, device)
+    if listed != listed_logits.shape[2]:
+        raise ValueError(f"parts are of {listed_logits.shape[2]} listed tokens, not of {listed}")
+    n, loss, lse, logp, left = _distillation_outputs(shape, targets is not None, stats, listed, device)
+    _queue(_ops().gdp_distill_join,
+           gdp_distill_joint(n, vocab, count, list_type, target_type, listed, flat.data_ptr(), teacher.data_ptr(), _ptr(targets),
+                             scale, beta, rest, 0, sums.data_ptr(), listed_logits.data_ptr(), loss.data_ptr(), lse.data_ptr(),
+                             _ptr(logp), _ptr(left)), device)
+    return Distillation(loss, lse, logp, left)
+
+
+# ---- logits as they are chosen from ------------------------------------------------------------------------
+def _per_row(value, otherwise, shape, what, device):
+    """(number for all rows, or float32 of each)"""
+    if value is None:
+        return otherwise, None
+    if not isinstance(value, torch.Tensor):
+        return float(value), None
+    return otherwise, _floats(value.expand(shape) if value.dim() == 0 else value, shape, what, device)
+
+
+def _numbers(t, shape, what, device):
+    """Whole numbers for each row, in order, and their type."""
+    if t is None:
+        return None, 0
+    if not isinstance(t, torch.Tensor) or t.shape != shape:
+        raise ValueError(f"{what} must be a tensor {list(shape)}")
+    code = _type(t, what, _TOKEN_TYPES)
+    _same_device(device, **{what: t})
+    return t.contiguous(), code
+
+
+def _rows_or_one(t, shape, what):
+    """[..., n] of each row, or [n] of all: the rows and the stride between them, 0 of the latter."""
+    if t.dim() == 1 and shape:
+        return t.contiguous(), 0
+    if t.dim() != len(shape) + 1 or t.shape[:-1] != shape:
+        raise ValueError(f"{what} must be {list(shape) + ['...']} or ['...'], not {list(t.shape)}")
+    return _rows(t, t.shape[-1], what) if t.numel() else (t, 0)
+
+
+class _Adjust(NamedTuple):
+    """What is done to logits: checked tensors, in the record's order."""
+    history: gdp_adjust_history
+    biases: tuple       # tokens, values, stride, number, type
+    mask: tuple         # words, stride, number
+    scale: tuple        # of each row, of all
+    keep: tuple         # tensors that the record points to
+
+
+def _adjust_of(shape, device, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale):
+    keep = []
+    of_history = gdp_adjust_history(None, 0, 0, 0, 0, 0, 1.0, 0.0, 0.0, None, None, None, None, None)
+    if history is not None:
+        token_type = _type(history, "history", _TOKEN_TYPES)
+        _same_device(device, history=history)
+        if history.dim() < 1:
+            raise ValueError("history must be [..., places] or [places]")
+        tokens, stride = _rows_or_one(history, shape, "history")
+        lengths, length_type = _numbers(lengths, shape, "lengths", device)
+        prompts, prompt_type = _numbers(prompts, shape, "prompts", device)
+        r, f, p = (_per_row(v, o, shape, what, device) for v, o, what in (
+            (repetition, 1.0, "repetition"), (frequency, 0.0, "frequency"), (presence, 0.0, "presence")))
+        keep += [tokens, lengths, prompts, r[1], f[1], p[1]]
+        if history.shape[-1]:
+            of_history = gdp_adjust_history(tokens.data_ptr(), history.shape[-1], stride, token_type, length_type, prompt_type, r[0],
+                                            f[0], p[0], _ptr(lengths), _ptr(prompts), _ptr(r[1]), _ptr(f[1]), _ptr(p[1]))
+    else:
+        for what, given in (("lengths", lengths), ("prompts", prompts), ("repetition", repetition), ("frequency", frequency),
+                            ("presence", presence)):
+            if given is not None:
+                raise ValueError(f"{what} needs a history")
+    of_biases = (None, None, 0, 0, 0)
+    if (bias_tokens is None) != (bias is None):
+        raise ValueError("bias_tokens and bias come together")
+    if bias is not None:
+        code = _type(bias_tokens, "bias_tokens", _TOKEN_TYPES)
+        _same_device(device, bias_tokens=bias_tokens)
+        count = bias_tokens.shape[-1] if bias_tokens.dim() else 0
+        if bias_tokens.dim() < 1 or count > MAX_BIASES:
+            raise ValueError(f"bias_tokens must be [..., biases] or [biases] of at most {MAX_BIASES}, not {list(bias_tokens.shape)}")
+        values = _floats(bias, bias_tokens.shape, "bias", device)
+        tokens, stride = _rows_or_one(bias_tokens.contiguous(), shape, "bias_tokens")
+        keep += [tokens, values]
+        if bias_tokens.numel():
+            of_biases = (tokens.data_ptr(), values.data_ptr(), stride, count, code)
+    of_mask = (None, 0, 0)
+    if allowed is not None:
+        if allowed.dtype not in (torch.int32, torch.uint32):
+            raise ValueError(f"allowed must be words of 32 bits, int32 or uint32, not {allowed.dtype}")
+        if not allowed.is_cuda or allowed.dim() < 1:
+            raise ValueError("allowed must be [..., words] or [words] on a HIP device")
+        _same_device(device, allowed=allowed)
+        words, stride = _rows_or_one(allowed, shape, "allowed")
+        keep += [words]
+        of_mask = (words.data_ptr() if words.numel() else None, stride, allowed.shape[-1])
+    one, each = _per_row(scale, 1.0, shape, "scale", device)
+    return _Adjust(of_history, of_biases, of_mask, (_ptr(each), one), tuple(keep) + (each,))
+
+
+def _out_dtype(dtype, logits_dtype, into):
+    if into is not None and dtype is not None and dtype != into.dtype:
+        raise ValueError("dtype is that of into")
+    dtype = into.dtype if into is not None else dtype or logits_dtype
+    if dtype not in (logits_dtype, torch.float32):
+        raise ValueError(f"dtype must be that of the logits or float32, not {dtype}")
+    return dtype
+
+
+def _check_mask(allowed, first, columns):
+    if allowed is not None and allowed.shape[-1] * 32 < first + columns:
+        raise ValueError(f"allowed: {allowed.shape[-1]} words are not enough for tokens up to {first + columns}")
+
+
+def _adjust_logits(logits, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale, first, dtype, into):
+    logits_type = _type(logits, "logits")
+    if logits.dim() < 1:
+        raise ValueError("logits must be [..., vocab]")
+    device, columns, shape = logits.device, logits.shape[-1], logits.shape[:-1]
+    dtype = _out_dtype(dtype, logits.dtype, into)
+    given = _adjust_of(shape, device, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale)
+    _check_mask(allowed, first, columns)
+    n = shape.numel()
+    if into is None:
+        out = torch.empty(logits.shape, dtype=dtype, device=device)
+    else:
+        out = into
+        if out.shape != logits.shape or out.device != device:
+            raise ValueError("into must have the shape and device of logits")
+    if not n or not columns:
+        return out
+    rows, stride = _rows(logits, columns, "logits")
+    to = _rows_in_place(out, "into")
+    _queue(_ops().gdp_adjust_forward,
+           gdp_adjust(n, columns, first, rows.data_ptr(), stride, logits_type, _TYPES[dtype], given.history, *given.biases, *given.mask,
+                      *given.scale, 0, to.data_ptr(), to.stride(0)), device)
+    return out
+
+
+def _adjust_logits_grad(logits, dtype, grad, history, lengths, repetition, allowed, scale, first, into):
+    grad_type = _type(grad, "grad")
+    device, columns, shape = grad.device, grad.shape[-1], grad.shape[:-1]
+    if grad.dtype not in (dtype, torch.float32):
+        raise ValueError(f"grad must have the type of the logits or float32, not {grad.dtype}")
+    given = _adjust_of(shape, device, history, lengths, None, repetition, None, None, None, None, allowed, scale)
+    _check_mask(allowed, first, columns)
+    n = shape.numel()
+    if into is None:
+        out = torch.empty(grad.shape, dtype=dtype, device=device)
+    else:
+        out = into
+        if out.shape != grad.shape or out.dtype != dtype or out.device != device:
+            raise ValueError("into must have the shape, type and device of logits")
+    if not n or not columns:
+        return out
+    rows, stride = _rows(grad, columns, "grad")
+    x, x_stride = _rows(logits, columns, "logits") if logits is not None else (None, columns)
+    to = _rows_in_place(out, "into")
+    record = gdp_adjust(n, columns, first, _ptr(x), x_stride, _TYPES[dtype], grad_type, given.history, *given.biases, *given.mask,
+                        *given.scale, 0, to.data_ptr(), to.stride(0))
+    _queue(_ops().gdp_adjust_backward, gdp_adjust_grad(record, rows.data_ptr(), stride), device)
+    return out
+
+
+class _AdjustLogits(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale, first, dtype):
+        out = _adjust_logits(logits, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale, first,
+                             dtype, None)
+        # Only a repetition's factor goes by the logits, and by the history.
+        by_history = history is not None and (isinstance(repetition, torch.Tensor) or repetition not in (None, 1.0))
+        tensor = lambda v: v if isinstance(v, torch.Tensor) else None   # noqa: E731
+        ctx.save_for_backward(*((logits, history, lengths, tensor(repetition)) if by_history else (None,) * 4), allowed, tensor(scale))
+        ctx.given = (logits.dtype, repetition if by_history and tensor(repetition) is None else None, scale if tensor(scale) is None else None, first)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        logits, history, lengths, repetitions, allowed, scales = ctx.saved_tensors
+        dtype, repetition, scale, first = ctx.given
+        return (_adjust_logits_grad(logits, dtype, grad, history, lengths, repetition if repetitions is None else repetitions, allowed,
+                                    scale if scales is None else scales, first, None),) + (None,) * 12
+
+
+def adjust_logits(logits, history=None, *, lengths=None, prompts=None, repetition=None, frequency=None, presence=None,
+                  bias_tokens=None, bias=None, allowed=None, scale=None, first: int = 0, dtype: Optional[torch.dtype] = None,
+                  into: Optional[torch.Tensor] = None):
+    """``logits`` [..., vocab] as a program chooses from them, in ``dtype`` (theirs by default, or float32):
+
+        scale * (pen(logits) - frequency * count - presence * (count > 0) + bias),  and -inf for what is not allowed
+
+    ``history`` [..., places], or [places] for all rows: tokens that a row has had, of which the first ``lengths`` [...] count (all by
+    default); those outside the vocabulary, such as -1, do not.  pen(x) is x / ``repetition`` above 0 and x * ``repetition`` below for the
+    tokens in it; ``count`` is how often a token is in it behind its first ``prompts`` [...] places (none by default).
+    ``bias`` of ``bias_tokens``, both [..., biases] or [biases] for all rows, at most 1024; a token that is there twice has the sum.  ``allowed``
+    [..., words] or [words], int32 or uint32: token t in bit t % 32 of word t // 32; what it rules out is -inf, NaN too.
+    ``repetition``, ``frequency``, ``presence`` and ``scale`` (1 / temperature): numbers, or tensors [...] of each row's; repetitions and
+    scales have to be above 0, which is looked at for numbers only.
+
+    ``logits`` of a shard of the vocabulary begin with token ``first``; everything else is of all of it.  ``into``: written there; it may be
+    ``logits`` itself, of which 16 bytes without a change are neither read nor written where there is no scale.  Differentiable with respect to
+    ``logits`` (not ``into`` a tensor); nothing else gets a gradient."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(*(t for t in (logits, repetition, frequency, presence, bias, scale, into) if isinstance(t, torch.Tensor)))
+    _constants(repetition=repetition, frequency=frequency, presence=presence, bias=bias, scale=scale)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        if into is not None:
+            raise ValueError("into: logits that want a gradient are not written over, nor adjusted into a tensor")
+        return _AdjustLogits.apply(logits, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale,
+                                   int(first), dtype)
+    out = _adjust_logits(logits, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale, int(first),
+                         dtype, into)
+    if into is not None:
+        _written(into)
+    return out
+
+
+def adjust_logits_grad(logits, grad, history=None, *, lengths=None, repetition=None, allowed=None, scale=None, first: int = 0,
+                       into: Optional[torch.Tensor] = None):
+    """Gradient with respect to ``logits`` [..., vocab], in their type, from that of ``adjust_logits``' result, in its type.  The rest as
+    it was given to the forward pass, of which frequencies, presences, prompts and biases have no part in the gradient.  Where the
+    mask rules a token out it is 0, whatever ``grad`` is there.  ``into``: written there; it may be ``grad`` itself."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(*(t for t in (logits, grad, repetition, scale, into) if isinstance(t, torch.Tensor)))
+    _type(logits, "logits")
+    _type(grad, "grad")
+    if logits.dim() < 1 or grad.shape != logits.shape:
+        raise ValueError(f"grad must be {list(logits.shape)} as logits, not {list(grad.shape)}")
+    _same_device(logits.device, grad=grad)
+    out = _adjust_logits_grad(logits, logits.dtype, grad, history, lengths, repetition, allowed, scale, int(first), into)
+    if into is not None:
+        _written(into)
+    return out

@@ -4,7 +4,8 @@
  * The parts of a model that no layer covers, and that the search engine prices for every
  * vocabulary-parallel degree (the keys of other_time_cost / other_mem_cost of a DP call): the embedding
  * lookup before the first layer, the residual join and norm behind a block, the log probabilities behind the
- * head, and their gradients.  Every operator takes a shard of the vocabulary as well as all of it.
+ * head, and their gradients; and what is done to the logits behind the head, distillation from a teacher and
+ * penalties, biases and masks.  Every operator takes a shard of the vocabulary as well as all of it.
  *
  * Unlike the entry points of galvatron_dp_hip.h these take DEVICE pointers, queue their work on the stream
  * they are given (a hipStream_t; NULL is the null stream) on the calling thread's current device, and return
@@ -185,6 +186,160 @@ typedef struct gdp_logprob_grad_stats {
     const float *row_stats;    /* [n][2], of the whole row                */
 } gdp_logprob_grad_stats;
 int gdp_logprob_backward_stats(const gdp_logprob_grad_stats *l, void *stream);
+
+/* Distillation: how far a row is from a teacher's distribution, of which a list of tokens and their log probabilities is known (what
+ * gdp_logprob's top_* give).  z = scale * logits[row], p = softmax(z).  A place of the list whose token is outside [0, vocab),
+ * or whose log probability is -inf, is not used; a token in several places counts once, with the sum of its probabilities q.
+ * The tokens that are not listed are one alternative more, the rest:
+ *   p_rest = the sum of their p                 of these alone, so it keeps its digits where it is next to nothing
+ *   q_rest = 1 - sum(q)                         with `rest`; below 2^-22, which is what float32 log probabilities of a list
+ *                                               that holds everything leave, it is 0, and 2^-22 for beta 1
+ *          = 0, and the q are divided by their sum (any scores will do for `teacher` then)   without it
+ * A row without an unlisted logit above -inf has no rest.  Over the listed tokens and the rest
+ *   loss = sum(q * log(q / p))                                                        beta 0
+ *        = sum(p * log(p / q))                                                        beta 1 (needs `rest`)
+ *        = beta * sum(q * log(q / a)) + (1 - beta) * sum(p * log(p / a)), a = beta * q + (1 - beta) * p    between
+ * where 0 * log 0 is 0; a listed token that the row rules out (-inf) has a loss of inf at beta 0.  lse and logp (of a
+ * target) are those of gdp_logprob.  A row of nothing but -inf, and without `rest` one whose list is empty, has a loss of 0; a row
+ * with NaN or +inf, in the logits or at a place that counts, NaN.
+ * What the gradient takes, stats [n][5 + listed]: the row's largest logit m and log(sum(exp(scale * (logits[row] - m)))); the same of
+ * the unlisted tokens alone (-inf where there are none); the derivative of the loss with respect to a shift of all unlisted z; and
+ * with respect to z of the token at each place (0 for a token outside [0, vocab)).
+ * The sums over the list are taken in float64, those over the vocabulary in float32. */
+#define GDP_MAX_LISTED 256
+typedef struct gdp_distill {
+    int64_t n, vocab;       /* rows, columns                              */
+    const void *logits;     /* [n][vocab]                                 */
+    int64_t logits_stride;
+    int32_t logits_type;
+    int32_t list_type;      /* of tokens                                  */
+    int32_t target_type;
+    int32_t listed;         /* 1 .. GDP_MAX_LISTED                        */
+    const void *tokens;     /* [n][listed]                                */
+    const float *teacher;   /* [n][listed]                                */
+    const void *targets;    /* [n] or NULL                                */
+    float scale, beta;
+    int32_t rest;
+    int32_t reserved;
+    float *loss, *lse;      /* [n] each                                   */
+    float *logp;            /* [n]; NULL without targets                  */
+    float *stats;           /* [n][5 + listed] or NULL                    */
+    void *workspace;
+    size_t workspace_bytes;
+} gdp_distill;
+int gdp_distill_workspace(int64_t n, int64_t vocab, int32_t logits_type, int32_t listed, size_t *bytes);
+int gdp_distill_forward(const gdp_distill *d, void *stream);
+
+/* The same for a vocabulary in shards: `parts` of each, joined after the ranks have exchanged them (16 + 4 * listed
+ * bytes a row).  Of a part: sums [n][4] float32 (largest unlisted logit; sum of exp2 over the unlisted; the target's logit or -inf;
+ * 0), and the listed tokens' logits, -inf for those of other shards. */
+typedef struct gdp_distill_part {
+    int64_t n, vocab, first;
+    const void *logits;
+    int64_t logits_stride;
+    int32_t logits_type;
+    int32_t list_type;
+    int32_t target_type;
+    int32_t listed;
+    const void *tokens;
+    const float *teacher;
+    const void *targets;
+    float scale;
+    int32_t reserved;
+    float *sums, *listed_logits; /* [n][4], [n][listed]                   */
+    void *workspace;
+    size_t workspace_bytes; /* gdp_distill_workspace of the shard's sizes */
+} gdp_distill_part;
+int gdp_distill_parts(const gdp_distill_part *d, void *stream);
+
+typedef struct gdp_distill_joint {
+    int64_t n, vocab;       /* of the whole vocabulary                    */
+    int32_t parts;          /* 1 .. GDP_MAX_LOGPROB_PARTS, in any order   */
+    int32_t list_type;
+    int32_t target_type;
+    int32_t listed;
+    const void *tokens;
+    const float *teacher;
+    const void *targets;
+    float scale, beta;
+    int32_t rest;
+    int32_t reserved;
+    const float *sums;          /* [parts][n][4]                          */
+    const float *listed_logits; /* [parts][n][listed]                     */
+    float *loss, *lse, *logp, *stats;
+} gdp_distill_joint;
+int gdp_distill_join(const gdp_distill_joint *d, void *stream);
+
+/* Gradient with respect to the logits (of a shard whose first column is token `first`), from those of loss, lse and logp:
+ *   out_j = scale * (g_loss * dloss/dz_j + g_lse * p_j + g_logp * (1[j = target] - p_j))
+ * with dloss/dz_j of a listed token as stats has it, and of others their share of the unlisted times the derivative that stats has for
+ * all of these.  out may be logits itself, and does not overlap them otherwise. */
+typedef struct gdp_distill_grad {
+    int64_t n, vocab, first;
+    int64_t whole_vocab;    /* tokens outside [0, whole_vocab) are none   */
+    const void *logits;
+    int64_t logits_stride;
+    int32_t logits_type;    /* also out's                                 */
+    int32_t list_type;
+    int32_t target_type;
+    int32_t listed;
+    const void *tokens;     /* [n][listed]                                */
+    const void *targets;    /* [n] or NULL                                */
+    const float *stats;     /* [n][5 + listed]                            */
+    const float *grad_loss, *grad_lse, *grad_logp; /* [n] each, or NULL   */
+    float scale;
+    int32_t reserved;
+    void *out;
+    int64_t out_stride;
+} gdp_distill_grad;
+int gdp_distill_backward(const gdp_distill_grad *d, void *stream);
+
+/* Logits as they are chosen from:  out_j = scale * (pen(x_j) - frequency * count_j - presence * 1[count_j > 0] + bias_j), and -inf where
+ * the mask does not allow token j, whatever x_j is.  pen(x) is x / repetition above 0 and x * repetition else for the tokens of the row's history,
+ * and x for others; count_j is how often token j is in it from place `prompt` on; bias_j the sum of the biases that the row has for it.
+ * Any of the four may be missing.  The places of a history from `length` on do not count (a length above `places` is taken as `places`), nor do
+ * tokens of other shards or outside the vocabulary.  Each term is rounded to float32, the result once more to its type.
+ * Repetitions and scales have to be above 0; what the device holds of them is not looked at. */
+#define GDP_MAX_BIASES 1024
+typedef struct gdp_adjust_history {
+    const void *tokens;     /* [n][places] or NULL                        */
+    int64_t places, stride; /* a stride of 0: one history for all rows    */
+    int32_t token_type;
+    int32_t length_type, prompt_type;
+    float repetition, frequency, presence;    /* of all rows, where the next are NULL */
+    const void *lengths, *prompts;            /* [n] or NULL: all places; no prompt */
+    const float *repetitions, *frequencies, *presences; /* [n] or NULL    */
+} gdp_adjust_history;
+typedef struct gdp_adjust {
+    int64_t n, vocab, first;    /* rows, columns (of a shard), the token of column 0 */
+    const void *logits;     /* [n][vocab]                                 */
+    int64_t logits_stride;
+    int32_t logits_type;
+    int32_t out_type;       /* that of the logits, or GDP_F32             */
+    gdp_adjust_history history;
+    const void *bias_tokens; /* [n][biases] or NULL                       */
+    const float *bias;      /* [n][biases]                                */
+    int64_t bias_stride;    /* of both; 0: one list for all rows          */
+    int32_t biases;         /* 0 .. GDP_MAX_BIASES                        */
+    int32_t bias_token_type;
+    const uint32_t *allowed; /* [n][words] or NULL: bit t % 32 of word t / 32 is set for each token t that is allowed, of the whole vocabulary */
+    int64_t allowed_stride, words; /* a stride of 0: one mask for all rows; at least (first + vocab + 31) / 32 words */
+    const float *scales;    /* [n] or NULL: `scale`                       */
+    float scale;
+    int32_t reserved;
+    void *out;              /* [n][vocab]; may be logits itself with their type: 16 bytes in which nothing changes are not written then */
+    int64_t out_stride;
+} gdp_adjust;
+int gdp_adjust_forward(const gdp_adjust *a, void *stream);
+
+/* Its gradient with respect to the logits:  grad_j * scale, divided by or times the repetition as pen(x_j) is, and 0 where the mask
+ * does not allow token j, whatever grad_j is.  Frequencies, presences, prompts and biases have no part in it. */
+typedef struct gdp_adjust_grad {
+    gdp_adjust given;       /* its out is the gradient of the logits, of their type; out_type is that of grad; out may be grad itself with that type */
+    const void *grad;       /* [n][vocab]                                 */
+    int64_t grad_stride;
+} gdp_adjust_grad;
+int gdp_adjust_backward(const gdp_adjust_grad *a, void *stream);
 
 /* A block's output joined with the residual stream, with norms on both sides of the join:
  *   b      = post-norm of block (where post is not GDP_NORM_NONE), times gate
