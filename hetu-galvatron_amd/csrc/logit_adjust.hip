@@ -15,12 +15,11 @@
 namespace {
 using namespace ops;
 
-constexpr int THREADS = 256;
-constexpr int AHEAD = 4;                    // vectors that a thread has in flight
-constexpr int HISTORY_AHEAD = 8;            // tokens
+constexpr int COLUMNS = 8192;               // of a slice; with a table 32 KB of LDS, four workgroups on a core
+constexpr int threads_of(bool table) { return table ? 512 : 256; }
+constexpr int HISTORY_AHEAD = 4;            // tokens of the history that a thread has in flight
 constexpr uint32_t OF_PROMPT = 1u << 31, HAS_BIAS = 1u << 30, COUNT = HAS_BIAS - 1;
 constexpr int64_t MOST_PLACES = COUNT;      // of a history
-constexpr int TABLE_COLUMNS = 8192;         // of a slice with a table: 32 KB of LDS, five workgroups on a core
 
 struct Bias {
     int32_t column;      // of the slice
@@ -28,7 +27,7 @@ struct Bias {
 };
 struct Adjust {
     int64_t vocab, stride, out_stride, grad_stride, first;
-    int32_t slices, width;   // vectors of a slice
+    int32_t slices;
     gdp_adjust_history history;
     const void *bias_tokens;
     const float *bias;
@@ -47,15 +46,31 @@ __device__ __forceinline__ int64_t at_most(const void *p, int type, int64_t row,
     return n < 0 ? 0 : n > most ? most : n;
 }
 
+// Tokens from `begin` on, every THREADS-th, less `base`; above every column behind `end`.
+template <int THREADS, int N> __device__ __forceinline__ void load_tokens(uint64_t (&to)[N], const void *tokens, int type, int64_t begin, int64_t i, int64_t end)
+{
+    if (type == GDP_I64) {
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if (i + u * THREADS < end) to[u] = (uint64_t) static_cast<const int64_t *>(tokens)[begin + i + u * THREADS];
+    } else {
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if (i + u * THREADS < end) to[u] = (uint64_t)(int64_t) static_cast<const int32_t *>(tokens)[begin + i + u * THREADS];
+    }
+}
+
 // T: of the logits; O: of what is written, or of the gradient that is read (BACK).  TABLE: there is a history or are biases.
+// A thread has all of its columns, VECTORS times 16 bytes of the smaller type, in registers from the start, while tokens are counted.
 template <typename T, typename O, bool TABLE, bool BACK>
-__global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typename T::raw *logits, const typename O::raw *grad,
-                                                         typename std::conditional<BACK, T, O>::type::raw *out)
+__global__ __launch_bounds__(threads_of(TABLE)) void adjust_kernel(Adjust a, const typename T::raw *logits, const typename O::raw *grad,
+                                                                   typename std::conditional<BACK, T, O>::type::raw *out)
 {
     using W = typename std::conditional<BACK, T, O>::type;      // written
     using R = typename std::conditional<BACK, O, T>::type;      // read, column by column
-    constexpr int VEC = T::VEC;
-    extern __shared__ __align__(16) uint32_t table[];   // [width * VEC], then the slice's biases
+    constexpr int VEC = T::VEC, THREADS = threads_of(TABLE), VECTORS = COLUMNS / VEC / THREADS;
+    constexpr uint32_t ALL = (1u << VEC) - 1;
+    extern __shared__ __align__(16) uint32_t table[];   // [COLUMNS], then the slice's biases
     __shared__ int32_t n_biases;
     const int t = threadIdx.x;
     const int64_t row = blockIdx.x / a.slices;
@@ -67,61 +82,27 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
     else
         from_row = x;
     typename W::raw *const y = out + row * a.out_stride;
+    // Vectors are counted from the 16 bytes that the row begins in: the first and the last may be cut.
     const int off = (int)((reinterpret_cast<uintptr_t>(from_row) & 15) / sizeof(typename R::raw)) % VEC;
-    const int vocab = (int)a.vocab, vectors = (vocab + off + VEC - 1) / VEC;
-    const int v0 = slice * a.width, v1 = v0 + a.width < vectors ? v0 + a.width : vectors;
-    const int from = v0 * VEC - off, span = (v1 - v0) * VEC;     // the slice's first column (cut by the row), its columns
+    const int vocab = (int)a.vocab, from = slice * COLUMNS - off;   // the slice's first column
     const gdp_adjust_history &h = a.history;
-    Bias *const biases = reinterpret_cast<Bias *>(table + a.width * VEC);
+    Bias *const biases = reinterpret_cast<Bias *>(table + COLUMNS);
+    constexpr int BIAS_WAVE = THREADS - 64;
+    uint64_t token[HISTORY_AHEAD], bias_token = 0;
+    int64_t length = 0, prompt = 0;
+    float bias_value = 0.0f;
+    const int64_t first = a.first + from;     // token of the slice's first column
     if constexpr (TABLE) {
-        for (int i = t; i < a.width * VEC / 4; i += THREADS) reinterpret_cast<uint4 *>(table)[i] = make_uint4(0, 0, 0, 0);
-        if (t == 0) n_biases = 0;
-        __syncthreads();
         if (h.tokens) {
-            const int64_t length = at_most(h.lengths, h.length_type, row, h.places, h.places);
-            const int64_t prompt = at_most(h.prompts, h.prompt_type, row, 0, length);
-            const int64_t base_token = a.first + from;
-            const uint64_t columns = span > 0 ? span : 0;
-            const int64_t begin = row * h.stride;
-            for (int64_t base = 0; base < length; base += THREADS * HISTORY_AHEAD) {
-                uint64_t local[HISTORY_AHEAD];   // (of other slices, or none: above every column)
-#pragma unroll
-                for (int u = 0; u < HISTORY_AHEAD; ++u) {
-                    const int64_t i = base + u * THREADS + t;
-                    local[u] = i < length ? (uint64_t)token_at(h.tokens, h.token_type, begin + i) - (uint64_t)base_token : ~0ull;
-                }
-#pragma unroll
-                for (int u = 0; u < HISTORY_AHEAD; ++u) {
-                    if (local[u] >= columns) continue;
-                    if (base + u * THREADS + t < prompt)
-                        atomicOr(&table[local[u]], OF_PROMPT);
-                    else
-                        atomicAdd(&table[local[u]], 1u);
-                }
-            }
+            length = at_most(h.lengths, h.length_type, row, h.places, h.places);
+            prompt = at_most(h.prompts, h.prompt_type, row, 0, length);
+            load_tokens<THREADS>(token, h.tokens, h.token_type, row * h.stride, t, length);
         }
         if constexpr (!BACK)
-            if (a.biases && t < 64) {   // one wave, in order
-                int count = 0;
-                for (int base = 0; base < a.biases; base += 64) {
-                    const int i = base + t;
-                    uint64_t local = ~0ull;
-                    float value = 0.0f;
-                    if (i < a.biases) {
-                        local = (uint64_t)token_at(a.bias_tokens, a.bias_token_type, row * a.bias_stride + i) - (uint64_t)(a.first + from);
-                        value = a.bias[row * a.bias_stride + i];
-                    }
-                    const bool here = span > 0 && local < (uint64_t)span;
-                    const uint64_t all = __ballot(here);
-                    if (here) {
-                        biases[count + __popcll(all & ((1ull << t) - 1))] = {(int32_t)local, value};
-                        atomicOr(&table[local], HAS_BIAS);
-                    }
-                    count += __popcll(all);
-                }
-                if (t == 0) n_biases = count;
+            if (t - BIAS_WAVE >= 0 && t - BIAS_WAVE < a.biases) {
+                bias_token = (uint64_t)token_at(a.bias_tokens, a.bias_token_type, row * a.bias_stride + t - BIAS_WAVE);
+                bias_value = a.bias[row * a.bias_stride + t - BIAS_WAVE];
             }
-        __syncthreads();
     }
     const float scale = a.scales ? a.scales[row] : a.scale;
     float repetition = 1.0f, frequency = 0.0f, presence = 0.0f;
@@ -130,32 +111,97 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
         frequency = h.frequencies ? h.frequencies[row] : h.frequency;
         presence = h.presences ? h.presences[row] : h.presence;
     }
+    // VEC bits of the mask for each vector, 0 outside of the row
     const uint32_t *const words = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-    const float ruled_out = BACK ? 0.0f : -__builtin_inff();
-    // VEC bits of the mask, from column j on: the row's own columns only
-    const auto allowed_of = [&](int j) -> uint32_t {
-        constexpr uint32_t ALL = (1u << VEC) - 1;
-        uint32_t inside = ALL;
-        int skip = 0;
-        if (j < 0) skip = -j, inside = ALL << skip & ALL;
-        if (j + VEC > vocab) inside &= ALL >> (j + VEC - vocab);
-        if (!words || !inside) return inside;
-        const int64_t bit = a.first + j + skip;
-        const int at = (int)(bit & 31);
-        const int64_t last = a.first + (j + VEC < vocab ? j + VEC : vocab) - 1;
-        uint64_t w = words[bit >> 5];
-        if (last >> 5 != bit >> 5) w |= (uint64_t)words[last >> 5] << 32;
-        return (uint32_t)(w >> at) << skip & inside;
-    };
-    const auto of_column = [&](float f, int local) -> float {   // local: of the slice
+    uint32_t mask[VECTORS];
+#pragma unroll
+    for (int u = 0; u < VECTORS; ++u) {
+        const int j = from + (u * THREADS + t) * VEC;
+        const int skip = j < 0 ? -j : 0;
+        uint32_t inside = j >= vocab ? 0 : ALL << skip & ALL;
+        if (j + VEC > vocab && j < vocab) inside &= ALL >> (j + VEC - vocab);
+        mask[u] = inside;
+        if (words && inside) {
+            const int64_t bit = a.first + j + skip, last = a.first + (j + VEC < vocab ? j + VEC : vocab) - 1;
+            uint64_t w = words[bit >> 5];
+            if (last >> 5 != bit >> 5) w |= (uint64_t)words[last >> 5] << 32;
+            mask[u] = (uint32_t)(w >> (bit & 31)) << skip & inside;
+        }
+    }
+    if constexpr (TABLE) {
+#pragma unroll
+        for (int i = 0; i < COLUMNS / 4 / THREADS; ++i) reinterpret_cast<uint4 *>(table)[i * THREADS + t] = make_uint4(0, 0, 0, 0);
+        if (t == 0) n_biases = 0;
+    }
+    Pack<R, VEC> p[VECTORS];
+#pragma unroll
+    for (int u = 0; u < VECTORS; ++u) {
+        const int j = from + (u * THREADS + t) * VEC;
+        if (j >= 0 && j + VEC <= vocab && mask[u] && !(a.in_place && mask[u] == ALL)) p[u].load(from_row + j);
+    }
+    if constexpr (TABLE) {
+        __syncthreads();
+        for (int64_t i = t; i < length;) {
+#pragma unroll
+            for (int u = 0; u < HISTORY_AHEAD; ++u) {
+                const uint64_t local = token[u] - (uint64_t)first;
+                if (i + u * THREADS >= length || local >= COLUMNS) continue;
+                if (i + u * THREADS < prompt)
+                    atomicOr(&table[local], OF_PROMPT);
+                else
+                    atomicAdd(&table[local], 1u);
+            }
+            i += THREADS * HISTORY_AHEAD;
+            load_tokens<THREADS>(token, h.tokens, h.token_type, row * h.stride, i, length);
+        }
+        if constexpr (!BACK)
+            if (a.biases && t >= BIAS_WAVE) {   // one wave, in order
+                const int lane = t - BIAS_WAVE;
+                int count = 0;
+                for (int i = lane; i - lane < a.biases; i += 64) {
+                    if (i >= 64 && i < a.biases) {
+                        bias_token = (uint64_t)token_at(a.bias_tokens, a.bias_token_type, row * a.bias_stride + i);
+                        bias_value = a.bias[row * a.bias_stride + i];
+                    }
+                    const uint64_t local = bias_token - (uint64_t)first;
+                    const bool here = i < a.biases && local < COLUMNS;
+                    const uint64_t all = __ballot(here);
+                    if (here) {
+                        biases[count + __popcll(all & ((1ull << lane) - 1))] = {(int32_t)local, bias_value};
+                        atomicOr(&table[local], HAS_BIAS);
+                    }
+                    count += __popcll(all);
+                }
+                if (lane == 0) n_biases = count;
+            }
+        __syncthreads();
+    }
+    // Of a vector with tokens of the history or biases, and of what is not changed otherwise
+    bool touched[VECTORS];
+    Pack<T, VEC> sign[VECTORS];
+#pragma unroll
+    for (int u = 0; u < VECTORS; ++u) {
+        touched[u] = false;
+        if constexpr (TABLE) {
+            const uint4 *const c = reinterpret_cast<const uint4 *>(table + (u * THREADS + t) * VEC);
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < VEC / 4; ++i) any |= c[i].x | c[i].y | c[i].z | c[i].w;
+            touched[u] = any != 0;
+            const int j = from + (u * THREADS + t) * VEC;
+            if (touched[u] && j >= 0 && j + VEC <= vocab) {
+                if (a.in_place && mask[u] == ALL) p[u].load(from_row + j);
+                if constexpr (BACK) sign[u].load(x + j);
+            }
+        }
+    }
+    // `of` is the logit by whose sign a repetition goes
+    const auto of_column = [&](float f, float of, int local) -> float {
         if constexpr (TABLE) {
             const uint32_t c = table[local];
-            if constexpr (BACK) {
-                f *= scale;
-                if (c & (OF_PROMPT | COUNT)) f = T::up(x[from + local]) > 0.0f ? f / repetition : f * repetition;
-                return f;
-            }
-            if (c & (OF_PROMPT | COUNT)) f = f > 0.0f ? f / repetition : f * repetition;
+            if constexpr (BACK) f *= scale;
+            if (c & (OF_PROMPT | COUNT)) f = of > 0.0f ? f / repetition : f * repetition;
+            if constexpr (BACK) return f;
             if (c & COUNT) f = f - frequency * (float)(c & COUNT) - presence;
             if (c & HAS_BIAS) {
                 float sum = 0.0f;
@@ -165,58 +211,43 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
         }
         return f * scale;
     };
-    for (int base = v0; base < v1; base += THREADS * AHEAD) {
-        Pack<R, VEC> p[AHEAD];
-        uint32_t mask[AHEAD];
-        bool touched[AHEAD];
+    const float ruled_out = BACK ? 0.0f : -__builtin_inff();
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int v = base + u * THREADS + t;
-            mask[u] = v < v1 ? allowed_of(v * VEC - off) : 0;
-        }
+    for (int u = 0; u < VECTORS; ++u) {
+        const int v = u * THREADS + t, j = from + v * VEC;
+        if (j >= vocab) continue;
+        if (j >= 0 && j + VEC <= vocab) {
+            if (a.in_place && mask[u] == ALL && !touched[u]) continue;
+            float f[VEC];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int v = base + u * THREADS + t, j = v * VEC - off;
-            touched[u] = false;
-            if constexpr (TABLE)
-                if (v < v1) {
-                    const uint4 *const c = reinterpret_cast<const uint4 *>(table + (v - v0) * VEC);
-                    uint32_t any = 0;
+            for (int i = 0; i < VEC; ++i) f[i] = p[u][i] * scale;
+            if (touched[u])
 #pragma unroll
-                    for (int i = 0; i < VEC / 4; ++i) any |= c[i].x | c[i].y | c[i].z | c[i].w;
-                    touched[u] = any != 0;
+                for (int i = 0; i < VEC; ++i) {
+                    if constexpr (BACK)
+                        f[i] = of_column(p[u][i], sign[u][i], v * VEC + i);
+                    else
+                        f[i] = of_column(p[u][i], p[u][i], v * VEC + i);
                 }
-            if (v < v1 && j >= 0 && j + VEC <= vocab && mask[u] && !(a.in_place && mask[u] == (1u << VEC) - 1 && !touched[u])) p[u].load(from_row + j);
-        }
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int v = base + u * THREADS + t, j = v * VEC - off;
-            if (v >= v1) continue;
-            const bool whole = j >= 0 && j + VEC <= vocab;
-            if (whole) {
-                if (a.in_place && mask[u] == (1u << VEC) - 1 && !touched[u]) continue;
-                float f[VEC];
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) f[i] = p[u][i] * scale;
-                if (touched[u])
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) f[i] = of_column(p[u][i], (v - v0) * VEC + i);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) f[i] = mask[u] >> i & 1 ? f[i] : ruled_out;
-                Pack<W, VEC> q;
-                q.set(f);
-                q.store(y + j);
-            } else {
-                for (int i = 0; i < VEC; ++i)
-                    if (j + i >= 0 && j + i < vocab && !(a.in_place && mask[u] >> i & 1 && (!TABLE || table[(v - v0) * VEC + i] == 0)))
-                        y[j + i] = W::down(mask[u] >> i & 1 ? of_column(R::up(from_row[j + i]), (v - v0) * VEC + i) : ruled_out);
+            for (int i = 0; i < VEC; ++i) f[i] = mask[u] >> i & 1 ? f[i] : ruled_out;
+            Pack<W, VEC> q;
+            q.set(f);
+            q.store(y + j);
+        } else {
+            for (int i = 0; i < VEC; ++i) {
+                if (j + i < 0 || j + i >= vocab) continue;
+                const bool allowed = mask[u] >> i & 1;
+                if (a.in_place && allowed && (!TABLE || table[v * VEC + i] == 0)) continue;
+                const float f = R::up(from_row[j + i]);
+                y[j + i] = W::down(!allowed ? ruled_out : of_column(f, BACK && touched[u] ? T::up(x[j + i]) : f, v * VEC + i));
             }
         }
     }
 }
 
 // ---- host ----
-constexpr int64_t MOST_ROWS = (int64_t)1 << 21, MOST_GROUPS = (int64_t)1 << 23;   // a grid has less than 2^32 threads
+constexpr int64_t MOST_ROWS = (int64_t)1 << 21, MOST_GROUPS = ((int64_t)1 << 23) - 1;   // a grid has less than 2^32 threads
 bool token_aligned(const void *p, int type) { return aligned(p, type == GDP_I64 ? 8 : 4); }
 
 int check(const gdp_adjust &a)
@@ -266,18 +297,14 @@ template <bool BACK> int run(const gdp_adjust &a, const void *grad, int64_t grad
 {
     // Of the gradient only the repetition is of interest
     const bool history = a.history.tokens && a.history.places > 0, table = history || (!BACK && a.biases > 0);
-    const int vec = 16 / size_of(a.logits_type);
-    const int64_t vectors = ceil_div(a.vocab, (int64_t)vec) + 1;   // one more where a row begins within 16 bytes
-    // Slices of 8192 columns with a table, of two rounds of reads without, more where the grid would be too large.
-    const int64_t columns = table ? TABLE_COLUMNS : 2 * THREADS * AHEAD * vec;
-    const int64_t slices = ceil_div(vectors * vec, columns);
-    const int64_t width = ceil_div(vectors, slices);
+    // one more vector where a row begins within 16 bytes
+    const int64_t vec = 16 / size_of(a.logits_type), slices = ceil_div((ceil_div(a.vocab, vec) + 1) * vec, (int64_t)COLUMNS);
     if (a.n * slices > MOST_GROUPS) return gdp_fail(GDP_E_BADARG, "gdp_adjust: too many rows of so many columns");
-    Adjust k{a.vocab, a.logits_stride, a.out_stride, grad_stride, a.first, (int32_t)ceil_div(vectors, width), (int32_t)width, a.history, a.bias_tokens, a.bias,
+    Adjust k{a.vocab, a.logits_stride, a.out_stride, grad_stride, a.first, (int32_t)slices, a.history, a.bias_tokens, a.bias,
              a.bias_stride, BACK ? 0 : a.biases, a.bias_token_type, a.allowed, a.allowed_stride, a.scales, a.scale, 0};
     if (!history) k.history.tokens = nullptr;
     k.in_place = a.out == (BACK ? grad : a.logits) && !a.scales && a.scale == 1.0f;
-    const size_t lds = table ? (size_t)width * vec * 4 + (size_t)k.biases * sizeof(Bias) : 0;
+    const size_t lds = table ? COLUMNS * 4 + (size_t)k.biases * sizeof(Bias) : 0;
     return with_type(a.logits_type, [&](auto T) {
         using TT = decltype(T);
         const auto with = [&](auto O) {
@@ -286,8 +313,8 @@ template <bool BACK> int run(const gdp_adjust &a, const void *grad, int64_t grad
             const auto *g = static_cast<const typename OO::raw *>(grad);
             auto *y = static_cast<typename std::conditional<BACK, TT, OO>::type::raw *>(a.out);
             const dim3 grid((unsigned)(a.n * k.slices));
-            return table ? launch(who, adjust_kernel<TT, OO, true, BACK>, grid, THREADS, lds, stream, k, x, g, y)
-                         : launch(who, adjust_kernel<TT, OO, false, BACK>, grid, THREADS, 0, stream, k, x, g, y);
+            return table ? launch(who, adjust_kernel<TT, OO, true, BACK>, grid, threads_of(true), lds, stream, k, x, g, y)
+                         : launch(who, adjust_kernel<TT, OO, false, BACK>, grid, threads_of(false), 0, stream, k, x, g, y);
         };
         return a.out_type == GDP_F32 ? with(F32{}) : with(TT{});
     });
