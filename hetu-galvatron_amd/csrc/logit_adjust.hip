@@ -1,13 +1,12 @@
 // Penalties for repeated tokens, biases of single tokens, a grammar's mask and a temperature on rows of logits, and the gradient.
 //
-// A workgroup has a slice of a row's columns.  It reads the row's history and counts the slice's tokens in a table in LDS, 4 bytes for each
-// column: bit 31 for a token of the prompt, bit 30 for a token with a bias, and below them how often the token is in what was drawn.
-// Then it passes over its columns once, 16 bytes at a time, with their bits of the mask and their places of the table.  Counts are whole
-// numbers, so the order in which atomics add them up does not show.  Biases are kept as a list in the order they are given: a column whose bit 30
-// is set adds up its own.
+// A workgroup has a slice of a row's columns, in registers from the start.  Meanwhile it reads the row's history and counts the slice's
+// tokens in a table in LDS: for each column a bit for a token of the prompt, one for a token with a bias, and below them how often the
+// token is in what was drawn.  Counts are whole numbers, so the order in which atomics add them up does not show.  Biases are kept as
+// a list in the order they are given; a column with one adds up its own.  The gradient needs two bits: whether a token is in the history
+// and whether its logit is above 0, which is read where the token is met.
 //
-// Columns that the mask rules out are not read; where the result takes the logits' place and nothing else changes, neither read nor written.
-// Bound by memory; with long histories by reading them once for each slice.
+// Few steps wait for each other: history, mask and columns are read side by side, the table is waited for once.
 #include "ops_common.h"
 
 #include <type_traits>
@@ -15,19 +14,21 @@
 namespace {
 using namespace ops;
 
-constexpr int COLUMNS = 8192;               // of a slice; with a table 32 KB of LDS, four workgroups on a core
-constexpr int threads_of(bool table) { return table ? 512 : 256; }
-constexpr int HISTORY_AHEAD = 4;            // tokens of the history that a thread has in flight
-constexpr uint32_t OF_PROMPT = 1u << 31, HAS_BIAS = 1u << 30, COUNT = HAS_BIAS - 1;
-constexpr int64_t MOST_PLACES = COUNT;      // of a history
+constexpr int THREADS = 512;
+constexpr int HISTORY_AHEAD = 1;            // reads of 16 bytes of the history that a thread has in flight
+constexpr int64_t MOST_PLACES = 1 << 29, FEW_PLACES = (1 << 14) - 1;   // of a history; of one whose counts fit an entry of 16 bits
 
+// What a workgroup knows of its columns' tokens.
+enum Table { NONE, HALVES, WORDS, BITS };   // nothing; entries of 16 or 32 bits; two bits (the gradient)
+
+typedef uint16_t TwoBytes __attribute__((aligned(1)));
 struct Bias {
     int32_t column;      // of the slice
     float value;
 };
 struct Adjust {
     int64_t vocab, stride, out_stride, grad_stride, first;
-    int32_t slices;
+    int32_t slices;          // of a row
     gdp_adjust_history history;
     const void *bias_tokens;
     const float *bias;
@@ -38,6 +39,7 @@ struct Adjust {
     const float *scales;
     float scale;
     int32_t in_place;        // what does not change need not be written
+    int32_t past;            // written past the caches
 };
 
 __device__ __forceinline__ int64_t at_most(const void *p, int type, int64_t row, int64_t otherwise, int64_t most)
@@ -46,31 +48,31 @@ __device__ __forceinline__ int64_t at_most(const void *p, int type, int64_t row,
     return n < 0 ? 0 : n > most ? most : n;
 }
 
-// Tokens from `begin` on, every THREADS-th, less `base`; above every column behind `end`.
-template <int THREADS, int N> __device__ __forceinline__ void load_tokens(uint64_t (&to)[N], const void *tokens, int type, int64_t begin, int64_t i, int64_t end)
-{
-    if (type == GDP_I64) {
-#pragma unroll
-        for (int u = 0; u < N; ++u)
-            if (i + u * THREADS < end) to[u] = (uint64_t) static_cast<const int64_t *>(tokens)[begin + i + u * THREADS];
-    } else {
-#pragma unroll
-        for (int u = 0; u < N; ++u)
-            if (i + u * THREADS < end) to[u] = (uint64_t)(int64_t) static_cast<const int32_t *>(tokens)[begin + i + u * THREADS];
-    }
-}
+// Neighbouring tokens of a history, as they lie there: 16 bytes at once, at any address that a token may have.
+struct Tokens {
+    static constexpr int WORDS = 4;
+    Words<4>::Four w;
+    __device__ __forceinline__ void load(const uint32_t *p) { w = *reinterpret_cast<const Words<4>::Four *>(p); }
+    // The column of the one in word i, of a slice whose first column has token `first`; above every column for one of none.
+    __device__ __forceinline__ uint32_t column(int i, bool wide, uint32_t first) const { return wide && w[i + 1] != 0 ? ~0u : w[i] - first; }
+};
 
-// T: of the logits; O: of what is written, or of the gradient that is read (BACK).  TABLE: there is a history or are biases.
-// A thread has all of its columns, VECTORS times 16 bytes of the smaller type, in registers from the start, while tokens are counted.
-template <typename T, typename O, bool TABLE, bool BACK>
-__global__ __launch_bounds__(threads_of(TABLE)) void adjust_kernel(Adjust a, const typename T::raw *logits, const typename O::raw *grad,
-                                                                   typename std::conditional<BACK, T, O>::type::raw *out)
+constexpr int columns_of(int vec, int vectors) { return THREADS * vec * vectors; }
+constexpr int bytes_of(Table table, int columns) { return table == HALVES ? 2 * columns : table == WORDS ? 4 * columns : table == BITS ? columns / 4 : 0; }
+
+// T: of the logits; O: of what is written, or of the gradient that is read (BACK).  VECTORS: times 16 bytes of the logits' type that a
+// thread has, one after another by workgroups.
+template <typename T, typename O, Table TABLE, bool BACK, int VECTORS>
+__global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typename T::raw *logits, const typename O::raw *grad,
+                                                         typename std::conditional<BACK, T, O>::type::raw *out)
 {
     using W = typename std::conditional<BACK, T, O>::type;      // written
     using R = typename std::conditional<BACK, O, T>::type;      // read, column by column
-    constexpr int VEC = T::VEC, THREADS = threads_of(TABLE), VECTORS = COLUMNS / VEC / THREADS;
+    constexpr int VEC = T::VEC, COLUMNS = columns_of(VEC, VECTORS), TABLE_WORDS = bytes_of(TABLE, COLUMNS) / 4;
     constexpr uint32_t ALL = (1u << VEC) - 1;
-    extern __shared__ __align__(16) uint32_t table[];   // [COLUMNS], then the slice's biases
+    constexpr int ENTRY = TABLE == HALVES ? 16 : 32;            // bits of a table's entry
+    constexpr uint32_t OF_PROMPT = 1u << (ENTRY - 1), HAS_BIAS = 1u << (ENTRY - 2), COUNT = HAS_BIAS - 1;
+    extern __shared__ __align__(16) uint32_t table[];           // then the slice's biases; BITS: in the history, then above 0
     __shared__ int32_t n_biases;
     const int t = threadIdx.x;
     const int64_t row = blockIdx.x / a.slices;
@@ -86,168 +88,222 @@ __global__ __launch_bounds__(threads_of(TABLE)) void adjust_kernel(Adjust a, con
     const int off = (int)((reinterpret_cast<uintptr_t>(from_row) & 15) / sizeof(typename R::raw)) % VEC;
     const int vocab = (int)a.vocab, from = slice * COLUMNS - off;   // the slice's first column
     const gdp_adjust_history &h = a.history;
-    Bias *const biases = reinterpret_cast<Bias *>(table + COLUMNS);
+    Bias *const biases = reinterpret_cast<Bias *>(table + TABLE_WORDS);
     constexpr int BIAS_WAVE = THREADS - 64;
-    uint64_t token[HISTORY_AHEAD], bias_token = 0;
-    int64_t length = 0, prompt = 0;
-    float bias_value = 0.0f;
     const int64_t first = a.first + from;     // token of the slice's first column
-    if constexpr (TABLE) {
+    uint64_t bias_token = 0;
+    float bias_value = 0.0f;
+    int length = 0, prompt = 0;               // in words of 32 bits
+    const bool wide = h.token_type == GDP_I64;
+    const uint32_t *history = nullptr;
+    Tokens token[HISTORY_AHEAD];
+    if constexpr (TABLE != NONE) {
         if (h.tokens) {
-            length = at_most(h.lengths, h.length_type, row, h.places, h.places);
-            prompt = at_most(h.prompts, h.prompt_type, row, 0, length);
-            load_tokens<THREADS>(token, h.tokens, h.token_type, row * h.stride, t, length);
-        }
-        if constexpr (!BACK)
-            if (t - BIAS_WAVE >= 0 && t - BIAS_WAVE < a.biases) {
-                bias_token = (uint64_t)token_at(a.bias_tokens, a.bias_token_type, row * a.bias_stride + t - BIAS_WAVE);
-                bias_value = a.bias[row * a.bias_stride + t - BIAS_WAVE];
+            length = (int)at_most(h.lengths, h.length_type, row, h.places, h.places);
+            prompt = (int)at_most(h.prompts, h.prompt_type, row, 0, length) << wide;
+            length <<= wide;
+            history = static_cast<const uint32_t *>(h.tokens) + ((row * h.stride) << wide);
+#pragma unroll
+            for (int u = 0; u < HISTORY_AHEAD; ++u) {
+                const int i = (u * THREADS + t) * Tokens::WORDS;
+                if (i + Tokens::WORDS <= length) token[u].load(history + i);
             }
+        }
+        if (!BACK && t - BIAS_WAVE >= 0 && t - BIAS_WAVE < a.biases) {
+            bias_token = (uint64_t)token_at(a.bias_tokens, a.bias_token_type, row * a.bias_stride + t - BIAS_WAVE);
+            bias_value = a.bias[row * a.bias_stride + t - BIAS_WAVE];
+        }
     }
-    const float scale = a.scales ? a.scales[row] : a.scale;
-    float repetition = 1.0f, frequency = 0.0f, presence = 0.0f;
-    if (TABLE && h.tokens) {
-        repetition = h.repetitions ? h.repetitions[row] : h.repetition;
-        frequency = h.frequencies ? h.frequencies[row] : h.frequency;
-        presence = h.presences ? h.presences[row] : h.presence;
-    }
-    // VEC bits of the mask for each vector, 0 outside of the row
-    const uint32_t *const words = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+    // VEC bits of the mask for each whole vector, from the byte or the two that hold them
+    const uint8_t *const allowed = a.allowed ? reinterpret_cast<const uint8_t *>(a.allowed + row * a.allowed_stride) : nullptr;
+    const auto bit_of = [&](int j) { return (uint32_t)a.first + (uint32_t)j; };
     uint32_t mask[VECTORS];
 #pragma unroll
     for (int u = 0; u < VECTORS; ++u) {
         const int j = from + (u * THREADS + t) * VEC;
-        const int skip = j < 0 ? -j : 0;
-        uint32_t inside = j >= vocab ? 0 : ALL << skip & ALL;
-        if (j + VEC > vocab && j < vocab) inside &= ALL >> (j + VEC - vocab);
-        mask[u] = inside;
-        if (words && inside) {
-            const int64_t bit = a.first + j + skip, last = a.first + (j + VEC < vocab ? j + VEC : vocab) - 1;
-            uint64_t w = words[bit >> 5];
-            if (last >> 5 != bit >> 5) w |= (uint64_t)words[last >> 5] << 32;
-            mask[u] = (uint32_t)(w >> (bit & 31)) << skip & inside;
+        mask[u] = ALL;
+        if (allowed && j >= 0 && j + VEC <= vocab) {
+            const uint32_t bit = bit_of(j), shift = bit & 7;
+            mask[u] = (shift + VEC > 8 ? (uint32_t)*reinterpret_cast<const TwoBytes *>(allowed + (bit >> 3)) : allowed[bit >> 3]) >> shift & ALL;
         }
     }
-    if constexpr (TABLE) {
+    if constexpr (TABLE != NONE) {
 #pragma unroll
-        for (int i = 0; i < COLUMNS / 4 / THREADS; ++i) reinterpret_cast<uint4 *>(table)[i * THREADS + t] = make_uint4(0, 0, 0, 0);
+        for (int i = t; i < TABLE_WORDS / 4; i += THREADS) reinterpret_cast<uint4 *>(table)[i] = make_uint4(0, 0, 0, 0);
         if (t == 0) n_biases = 0;
     }
     Pack<R, VEC> p[VECTORS];
 #pragma unroll
     for (int u = 0; u < VECTORS; ++u) {
         const int j = from + (u * THREADS + t) * VEC;
-        if (j >= 0 && j + VEC <= vocab && mask[u] && !(a.in_place && mask[u] == ALL)) p[u].load(from_row + j);
+        // With a table without waiting for the mask
+        if (j >= 0 && j + VEC <= vocab && (TABLE != NONE ? !a.in_place : mask[u] && !(a.in_place && mask[u] == ALL))) p[u].load(from_row + j);
     }
-    if constexpr (TABLE) {
+    const float scale = a.scales ? a.scales[row] : a.scale;
+    float repetition = 1.0f, inverse = 1.0f, frequency = 0.0f, presence = 0.0f;
+    if constexpr (TABLE != NONE) {
+        if (h.tokens) {
+            repetition = h.repetitions ? h.repetitions[row] : h.repetition;
+            inverse = 1.0f / repetition;
+            frequency = h.frequencies ? h.frequencies[row] : h.frequency;
+            presence = h.presences ? h.presences[row] : h.presence;
+        }
         __syncthreads();
-        for (int64_t i = t; i < length;) {
+        // N tokens' columns; those of other slices, or of none, are above all.  The first `of_prompt` are of the prompt.
+        const auto count = [&](auto N, const uint32_t *column, int of_prompt) {
+            if constexpr (TABLE == BITS) {
+                bool positive[N.value];
+#pragma unroll
+                for (int k = 0; k < N.value; ++k) {
+                    const int j = from + (int)column[k];
+                    positive[k] = column[k] < COLUMNS && j >= 0 && j < vocab && T::up(x[j]) > 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < N.value; ++k)
+                    if (column[k] < COLUMNS) {
+                        atomicOr(&table[column[k] >> 5], 1u << (column[k] & 31));
+                        if (positive[k]) atomicOr(&table[TABLE_WORDS / 2 + (column[k] >> 5)], 1u << (column[k] & 31));
+                    }
+            } else {
+#pragma unroll
+                for (int k = 0; k < N.value; ++k)
+                    if (column[k] < COLUMNS) {
+                        uint32_t *const at = &table[TABLE == HALVES ? column[k] >> 1 : column[k]];
+                        const int shift = TABLE == HALVES ? (column[k] & 1) * 16 : 0;
+                        if (k < of_prompt)
+                            atomicOr(at, OF_PROMPT << shift);
+                        else
+                            atomicAdd(at, 1u << shift);
+                    }
+            }
+        };
+        const int of_wave = __builtin_amdgcn_readfirstlane(t) * Tokens::WORDS;
+        for (int base = 0; base < length; base += THREADS * HISTORY_AHEAD * Tokens::WORDS) {
 #pragma unroll
             for (int u = 0; u < HISTORY_AHEAD; ++u) {
-                const uint64_t local = token[u] - (uint64_t)first;
-                if (i + u * THREADS >= length || local >= COLUMNS) continue;
-                if (i + u * THREADS < prompt)
-                    atomicOr(&table[local], OF_PROMPT);
-                else
-                    atomicAdd(&table[local], 1u);
-            }
-            i += THREADS * HISTORY_AHEAD;
-            load_tokens<THREADS>(token, h.tokens, h.token_type, row * h.stride, i, length);
-        }
-        if constexpr (!BACK)
-            if (a.biases && t >= BIAS_WAVE) {   // one wave, in order
-                const int lane = t - BIAS_WAVE;
-                int count = 0;
-                for (int i = lane; i - lane < a.biases; i += 64) {
-                    if (i >= 64 && i < a.biases) {
-                        bias_token = (uint64_t)token_at(a.bias_tokens, a.bias_token_type, row * a.bias_stride + i);
-                        bias_value = a.bias[row * a.bias_stride + i];
+                const int i = base + (u * THREADS + t) * Tokens::WORDS;
+                if (i + Tokens::WORDS <= length) {
+                    uint32_t column[Tokens::WORDS];
+#pragma unroll
+                    for (int k = 0; k < Tokens::WORDS; ++k) column[k] = wide && k % 2 != 0 ? ~0u : token[u].column(k, wide, (uint32_t)first);
+                    // (most waves' tokens are all of the prompt or all drawn)
+                    constexpr std::integral_constant<int, Tokens::WORDS> N;
+                    const int at = base + u * THREADS * Tokens::WORDS + of_wave;
+                    if (at >= prompt)
+                        count(N, column, 0);
+                    else if (at + 64 * Tokens::WORDS <= prompt)
+                        count(N, column, Tokens::WORDS);
+                    else
+                        count(N, column, prompt - i);
+                } else {   // the last, one by one
+                    for (int k = i; k < length; k += 1 + wide) {
+                        const uint32_t column = wide && history[k + 1] != 0 ? ~0u : history[k] - (uint32_t)first;
+                        count(std::integral_constant<int, 1>{}, &column, prompt - k);
                     }
-                    const uint64_t local = bias_token - (uint64_t)first;
-                    const bool here = i < a.biases && local < COLUMNS;
-                    const uint64_t all = __ballot(here);
-                    if (here) {
-                        biases[count + __popcll(all & ((1ull << lane) - 1))] = {(int32_t)local, bias_value};
-                        atomicOr(&table[local], HAS_BIAS);
-                    }
-                    count += __popcll(all);
                 }
-                if (lane == 0) n_biases = count;
+                const int next = i + THREADS * HISTORY_AHEAD * Tokens::WORDS;
+                if (next + Tokens::WORDS <= length) token[u].load(history + next);
             }
+        }
+        if (!BACK && a.biases && t >= BIAS_WAVE) {   // one wave, in order
+            const int lane = t - BIAS_WAVE;
+            int found = 0;
+            for (int i = lane; i - lane < a.biases; i += 64) {
+                if (i >= 64 && i < a.biases) {
+                    bias_token = (uint64_t)token_at(a.bias_tokens, a.bias_token_type, row * a.bias_stride + i);
+                    bias_value = a.bias[row * a.bias_stride + i];
+                }
+                const uint64_t local = bias_token - (uint64_t)first;
+                const bool here = i < a.biases && local < COLUMNS;
+                const uint64_t all = __ballot(here);
+                if (here) {
+                    biases[found + __popcll(all & ((1ull << lane) - 1))] = {(int32_t)local, bias_value};
+                    atomicOr(&table[TABLE == HALVES ? local >> 1 : local], TABLE == HALVES ? HAS_BIAS << (local & 1) * 16 : HAS_BIAS);
+                }
+                found += __popcll(all);
+            }
+            if (lane == 0) n_biases = found;
+        }
         __syncthreads();
     }
-    // Of a vector with tokens of the history or biases, and of what is not changed otherwise
-    bool touched[VECTORS];
-    Pack<T, VEC> sign[VECTORS];
-#pragma unroll
-    for (int u = 0; u < VECTORS; ++u) {
-        touched[u] = false;
-        if constexpr (TABLE) {
-            const uint4 *const c = reinterpret_cast<const uint4 *>(table + (u * THREADS + t) * VEC);
-            uint32_t any = 0;
-#pragma unroll
-            for (int i = 0; i < VEC / 4; ++i) any |= c[i].x | c[i].y | c[i].z | c[i].w;
-            touched[u] = any != 0;
-            const int j = from + (u * THREADS + t) * VEC;
-            if (touched[u] && j >= 0 && j + VEC <= vocab) {
-                if (a.in_place && mask[u] == ALL) p[u].load(from_row + j);
-                if constexpr (BACK) sign[u].load(x + j);
-            }
-        }
-    }
-    // `of` is the logit by whose sign a repetition goes
-    const auto of_column = [&](float f, float of, int local) -> float {
-        if constexpr (TABLE) {
-            const uint32_t c = table[local];
-            if constexpr (BACK) f *= scale;
-            if (c & (OF_PROMPT | COUNT)) f = of > 0.0f ? f / repetition : f * repetition;
-            if constexpr (BACK) return f;
-            if (c & COUNT) f = f - frequency * (float)(c & COUNT) - presence;
-            if (c & HAS_BIAS) {
-                float sum = 0.0f;
-                for (int i = 0; i < n_biases; ++i) sum += biases[i].column == local ? biases[i].value : 0.0f;
-                f += sum;
-            }
-        }
-        return f * scale;
-    };
-    const float ruled_out = BACK ? 0.0f : -__builtin_inff();
+    constexpr uint32_t RULED_OUT = BACK ? 0u : 0xff800000u;   // 0, -inf
 #pragma unroll
     for (int u = 0; u < VECTORS; ++u) {
         const int v = u * THREADS + t, j = from + v * VEC;
         if (j >= vocab) continue;
-        if (j >= 0 && j + VEC <= vocab) {
-            if (a.in_place && mask[u] == ALL && !touched[u]) continue;
-            float f[VEC];
+        // the vector's entries
+        uint32_t c[TABLE == BITS ? 2 : VEC * ENTRY / 32], any = 0;
+        bool biased = false;
+        if constexpr (TABLE == BITS) {
+            const uint8_t *const bytes = reinterpret_cast<const uint8_t *>(table);
+            const int at = VEC == 8 ? v : v >> 1, shift = VEC == 8 ? 0 : 4 * (v & 1);
+            any = c[0] = bytes[at] >> shift & ALL;
+            c[1] = bytes[TABLE_WORDS * 2 + at] >> shift;
+        } else if constexpr (TABLE != NONE) {
+            Pack<F32, VEC * ENTRY / 32> entries;
+            entries.load(table + v * (VEC * ENTRY / 32));
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) f[i] = p[u][i] * scale;
-            if (touched[u])
+            for (int i = 0; i < VEC * ENTRY / 32; ++i) any |= c[i] = entries.w[i];
+            biased = any & (TABLE == HALVES ? HAS_BIAS << 16 | HAS_BIAS : HAS_BIAS);
+        }
+        const auto of_column = [&](float f, int i) -> float {
+            if constexpr (TABLE == BITS) {
+                f *= scale;
+                return c[0] >> i & 1 ? f * (c[1] >> i & 1 ? inverse : repetition) : f;
+            }
+            if constexpr (TABLE == HALVES || TABLE == WORDS) {
+                const uint32_t e = TABLE == HALVES ? c[i / 2] >> (i % 2) * 16 & 0xffff : c[i], n = e & COUNT;
+                f *= e & (OF_PROMPT | COUNT) ? f > 0.0f ? inverse : repetition : 1.0f;
+                f = fmaf(-frequency, (float)n, f) - (n ? presence : 0.0f);
+                if (biased && e & HAS_BIAS) {
+                    float sum = 0.0f;
+                    for (int b = 0; b < n_biases; ++b) sum += biases[b].column == v * VEC + i ? biases[b].value : 0.0f;
+                    f += sum;
+                }
+            }
+            return f * scale;
+        };
+        if (j >= 0 && j + VEC <= vocab) {
+            if (a.in_place) {
+                if (mask[u] == ALL && !any) continue;
+                if (TABLE != NONE) p[u].load(from_row + j);
+            }
+            float f[VEC];
+            if (any) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[i] = of_column(p[u][i], i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[i] = p[u][i] * scale;
+            }
+            if (allowed)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    if constexpr (BACK)
-                        f[i] = of_column(p[u][i], sign[u][i], v * VEC + i);
-                    else
-                        f[i] = of_column(p[u][i], p[u][i], v * VEC + i);
+                    const uint32_t keep = (uint32_t)((int32_t)(mask[u] << (31 - i)) >> 31);
+                    f[i] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, f[i]) & keep) | (RULED_OUT & ~keep));
                 }
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) f[i] = mask[u] >> i & 1 ? f[i] : ruled_out;
             Pack<W, VEC> q;
             q.set(f);
-            q.store(y + j);
+            if (a.past)
+                q.store_past(y + j);
+            else
+                q.store(y + j);
         } else {
+#pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 if (j + i < 0 || j + i >= vocab) continue;
-                const bool allowed = mask[u] >> i & 1;
-                if (a.in_place && allowed && (!TABLE || table[v * VEC + i] == 0)) continue;
-                const float f = R::up(from_row[j + i]);
-                y[j + i] = W::down(!allowed ? ruled_out : of_column(f, BACK && touched[u] ? T::up(x[j + i]) : f, v * VEC + i));
+                const bool keep = !allowed || allowed[bit_of(j + i) >> 3] >> (bit_of(j + i) & 7) & 1;
+                if (a.in_place && keep && !any) continue;
+                y[j + i] = W::down(keep ? of_column(R::up(from_row[j + i]), i) : __builtin_bit_cast(float, RULED_OUT));
             }
         }
     }
 }
 
 // ---- host ----
-constexpr int64_t MOST_ROWS = (int64_t)1 << 21, MOST_GROUPS = ((int64_t)1 << 23) - 1;   // a grid has less than 2^32 threads
+constexpr int64_t PAST_BYTES = 128 << 20;
+constexpr int64_t FEW_COLUMNS = 256 * 16384;
+constexpr int64_t MOST_ROWS = (int64_t)1 << 21, MOST_GROUPS = UINT32_MAX / THREADS;   // a grid has less than 2^32 threads
 bool token_aligned(const void *p, int type) { return aligned(p, type == GDP_I64 ? 8 : 4); }
 
 int check(const gdp_adjust &a)
@@ -259,7 +315,7 @@ int check(const gdp_adjust &a)
     if (a.out_type != a.logits_type && a.out_type != GDP_F32) return gdp_fail(GDP_E_BADARG, "gdp_adjust: out_type must be that of the logits, or GDP_F32");
     const gdp_adjust_history &h = a.history;
     if (h.tokens) {
-        if (h.places < 0 || h.places > MOST_PLACES) return gdp_fail(GDP_E_BADARG, "gdp_adjust: a history must have 0 to 2^30 - 1 places");
+        if (h.places < 0 || h.places > MOST_PLACES) return gdp_fail(GDP_E_BADARG, "gdp_adjust: a history must have 0 to 2^29 places");
         if (!token_type_ok(h.token_type) || (h.lengths && !token_type_ok(h.length_type)) || (h.prompts && !token_type_ok(h.prompt_type)))
             return gdp_fail(GDP_E_BADARG, "gdp_adjust: unknown type of a history's numbers");
         if (!rows_ok(a.n, h.places, h.stride, false)) return gdp_fail(GDP_E_BADARG, "gdp_adjust: a history's stride is negative or too large");
@@ -295,26 +351,37 @@ int check_rows(const void *p, int64_t n, int64_t vocab, int64_t stride, int type
 
 template <bool BACK> int run(const gdp_adjust &a, const void *grad, int64_t grad_stride, const char *who, void *stream)
 {
-    // Of the gradient only the repetition is of interest
-    const bool history = a.history.tokens && a.history.places > 0, table = history || (!BACK && a.biases > 0);
-    // one more vector where a row begins within 16 bytes
-    const int64_t vec = 16 / size_of(a.logits_type), slices = ceil_div((ceil_div(a.vocab, vec) + 1) * vec, (int64_t)COLUMNS);
-    if (a.n * slices > MOST_GROUPS) return gdp_fail(GDP_E_BADARG, "gdp_adjust: too many rows of so many columns");
-    Adjust k{a.vocab, a.logits_stride, a.out_stride, grad_stride, a.first, (int32_t)slices, a.history, a.bias_tokens, a.bias,
-             a.bias_stride, BACK ? 0 : a.biases, a.bias_token_type, a.allowed, a.allowed_stride, a.scales, a.scale, 0};
+    const bool history = a.history.tokens && a.history.places > 0;
+    Adjust k{a.vocab, a.logits_stride, a.out_stride, grad_stride, a.first, 0, a.history, a.bias_tokens, a.bias, a.bias_stride, BACK ? 0 : a.biases,
+             a.bias_token_type, a.allowed, a.allowed_stride, a.scales, a.scale, 0, 0};
     if (!history) k.history.tokens = nullptr;
+    k.past = a.n * a.vocab * size_of(BACK ? a.logits_type : a.out_type) >= PAST_BYTES;
     k.in_place = a.out == (BACK ? grad : a.logits) && !a.scales && a.scale == 1.0f;
-    const size_t lds = table ? COLUMNS * 4 + (size_t)k.biases * sizeof(Bias) : 0;
     return with_type(a.logits_type, [&](auto T) {
         using TT = decltype(T);
         const auto with = [&](auto O) {
             using OO = decltype(O);
-            const auto *x = static_cast<const typename TT::raw *>(a.logits);
-            const auto *g = static_cast<const typename OO::raw *>(grad);
-            auto *y = static_cast<typename std::conditional<BACK, TT, OO>::type::raw *>(a.out);
-            const dim3 grid((unsigned)(a.n * k.slices));
-            return table ? launch(who, adjust_kernel<TT, OO, true, BACK>, grid, threads_of(true), lds, stream, k, x, g, y)
-                         : launch(who, adjust_kernel<TT, OO, false, BACK>, grid, threads_of(false), 0, stream, k, x, g, y);
+            const auto go = [&](auto TABLE, auto VECTORS) {
+                constexpr int columns = columns_of(TT::VEC, VECTORS.value);
+                // one more vector where a row begins within 16 bytes
+                const int64_t slices = ceil_div((ceil_div(a.vocab, (int64_t)TT::VEC) + 1) * TT::VEC, (int64_t)columns);
+                if (a.n * slices > MOST_GROUPS) return gdp_fail(GDP_E_BADARG, "gdp_adjust: too many rows of so many columns");
+                k.slices = (int32_t)slices;
+                return launch(who, adjust_kernel<TT, OO, TABLE.value, BACK, VECTORS.value>, dim3((unsigned)(a.n * slices)), THREADS,
+                              (size_t)bytes_of(TABLE.value, columns) + (size_t)k.biases * sizeof(Bias), stream, k,
+                              static_cast<const typename TT::raw *>(a.logits), static_cast<const typename OO::raw *>(grad),
+                              static_cast<typename std::conditional<BACK, TT, OO>::type::raw *>(a.out));
+            };
+            const auto of_size = [&](auto TABLE) {
+                return a.n * a.vocab < FEW_COLUMNS ? go(TABLE, std::integral_constant<int, 1>{}) : go(TABLE, std::integral_constant<int, 4>{});
+            };
+            if constexpr (BACK)
+                return history ? of_size(std::integral_constant<Table, BITS>{}) : of_size(std::integral_constant<Table, NONE>{});
+            else {
+                if (!history && !a.biases) return of_size(std::integral_constant<Table, NONE>{});
+                return a.history.places <= FEW_PLACES || !history ? of_size(std::integral_constant<Table, HALVES>{})
+                                                                  : go(std::integral_constant<Table, WORDS>{}, std::integral_constant<int, 4>{});
+            }
         };
         return a.out_type == GDP_F32 ? with(F32{}) : with(TT{});
     });

@@ -303,7 +303,7 @@ int gdp_distill_backward(const gdp_distill_grad *d, void *stream);
 #define GDP_MAX_BIASES 1024
 typedef struct gdp_adjust_history {
     const void *tokens;     /* [n][places] or NULL                        */
-    int64_t places, stride; /* a stride of 0: one history for all rows    */
+    int64_t places, stride; /* 0 .. 2^29; a stride of 0: one history for all rows */
     int32_t token_type;
     int32_t length_type, prompt_type;
     float repetition, frequency, presence;    /* of all rows, where the next are NULL */
