@@ -15,8 +15,8 @@ and what is done with the logits there:
     distillation_parts, join_distillation               ... of a vocabulary in shards
     adjust_logits, adjust_logits_grad                   penalties for repeated tokens, biases, a grammar's mask, temperature
 
-``embedding``, ``token_logprobs``, ``residual_norm``, ``distillation`` and ``adjust_logits`` are differentiable (once, backwards: tensors with forward-mode
-tangents are refused); the ``*_grad`` functions are what their backward passes call, for programs that run their own.
+``embedding``, ``token_logprobs``, ``residual_norm``, ``distillation`` and ``adjust_logits`` are differentiable (once, backwards:
+tensors with forward-mode tangents are refused); the ``*_grad`` functions are what their backward passes call, for programs that run their own.
 Work is queued on torch's current stream of the tensors' device; nothing waits.  Types: float32, float16, bfloat16; token
 numbers int32 or int64.  Per-token tensors may have any strides (one whose rows' elements are not neighbours is copied
 first); a table's rows have to lie as they are.  There is no CPU path: tensors have to be on a HIP device.
@@ -253,12 +253,10 @@ def _written(t):
     torch.autograd.graph.increment_version(t)
 
 
-def _constants(**tensors):
-    """Refuses inputs that want a gradient which there is none of."""
-    if torch.is_grad_enabled():
-        for what, t in tensors.items():
-            if isinstance(t, torch.Tensor) and t.requires_grad:
-                raise ValueError(f"{what} gets no gradient: detach it")
+def _constant(t, what):
+    """Refuses an input that wants a gradient which there is none of.  (Asked where gradients are taken.)"""
+    if isinstance(t, torch.Tensor) and t.requires_grad:
+        raise ValueError(f"{what} gets no gradient: detach it")
 
 
 def _ptr(t):
@@ -307,7 +305,7 @@ def _floats(t, shape, what, device):
         raise ValueError(f"{what} must be {list(shape)}, not {list(t.shape)}")
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, not on {device}")
-    return t.to(torch.float32).contiguous()
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
 def _table(t, what):
@@ -949,8 +947,11 @@ def distillation(logits, tokens, teacher, *, scale: float = 1.0, beta: float = 0
     for ``distillation_grad``.  The teacher gets no gradient."""
     if forward_ad._current_level >= 0:
         _no_tangents(logits, teacher)
-    _constants(teacher=teacher)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    by_autograd = False
+    if torch.is_grad_enabled():
+        _constant(teacher, "teacher")
+        by_autograd = logits.requires_grad
+    if by_autograd:
         r = _Distillation.apply(logits, tokens, teacher, targets, float(scale), float(beta), bool(rest))
     else:
         r = _distillation(logits, tokens, teacher, targets, float(scale), float(beta), bool(rest), stats)
@@ -981,40 +982,32 @@ def distillation_grad(logits, tokens, stats, grad_loss=None, *, scale: float = 1
     grad_loss, grad_lse = _floats(grad_loss, shape, "grad_loss", device), _floats(grad_lse, shape, "grad_lse", device)
     grad_logp = _floats(grad_logp, shape, "grad_logp", device)
     n = shape.numel()
-    out, to = _gradient_place(logits, into, n and columns)
+    out = _like(logits) if into is None else into
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != device:
+        raise ValueError("into must have the shape, type and device of logits")
     if not n or not columns:
         return out
     rows, stride = _rows(logits, columns, "logits")
     _queue(_ops().gdp_distill_backward,
            gdp_distill_grad(n, columns, first, vocab, rows.data_ptr(), stride, logits_type, list_type, target_type, listed,
                             flat.data_ptr(), _ptr(targets), stats.data_ptr(), _ptr(grad_loss), _ptr(grad_lse), _ptr(grad_logp),
-                            scale, 0, to.data_ptr(), to.stride(0)), device)
+                            scale, 0, *_place(out, columns)), device)
     if into is not None:
         _written(into)
     return out
 
 
-def _gradient_place(logits, into, some):
-    """What is returned, and the same as rows where there are some."""
-    if into is None:
-        out = _like(logits)
-    else:
-        out = into
-        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
-            raise ValueError("into must have the shape, type and device of logits")
-    return out, _rows_in_place(out, "into") if some else None
-
-
-def _rows_in_place(t, what):
-    """[..., columns] as rows at one stride, which are the tensor's own memory."""
-    columns = t.shape[-1]
+def _place(t, columns):
+    """The address of what is written and the stride of its rows, which are the tensor's own memory."""
+    if t.is_contiguous():
+        return t.data_ptr(), columns
     try:
         rows = t if t.dim() == 2 else t.view(-1, columns)
         if columns > 1 and rows.stride(1) != 1:
             raise RuntimeError
     except RuntimeError:
-        raise ValueError(f"{what} must have rows that are neighbouring elements at one stride") from None
-    return rows
+        raise ValueError("into must have rows that are neighbouring elements at one stride") from None
+    return rows.data_ptr(), rows.stride(0)
 
 
 def distillation_parts(logits, tokens, teacher, *, first: int, scale: float = 1.0, targets=None) -> DistillationParts:
@@ -1022,7 +1015,8 @@ def distillation_parts(logits, tokens, teacher, *, first: int, scale: float = 1.
     shards have to say: 16 + 4 * listed bytes for each row, to be gathered from all shards and joined."""
     if forward_ad._current_level >= 0:
         _no_tangents(logits, teacher)
-    _constants(teacher=teacher)
+    if torch.is_grad_enabled():
+        _constant(teacher, "teacher")
     logits_type = _type(logits, "logits")
     if logits.dim() != 2:
         raise ValueError(f"logits must be [n, columns], not {list(logits.shape)}")
@@ -1050,7 +1044,8 @@ def join_distillation(parts, tokens, teacher, vocab: int, *, scale: float = 1.0,
         parts = DistillationParts(*(torch.stack(t) for t in zip(*parts)))
     if forward_ad._current_level >= 0:
         _no_tangents(*parts, teacher)
-    _constants(teacher=teacher)
+    if torch.is_grad_enabled():
+        _constant(teacher, "teacher")
     sums, listed_logits = (t.contiguous() for t in parts)
     if sums.dim() != 3 or sums.shape[2] != 4 or listed_logits.dim() != 3 or listed_logits.shape[:2] != sums.shape[:2]:
         raise ValueError("parts must be sums [parts, n, 4] and listed_logits [parts, n, listed]")
@@ -1071,92 +1066,95 @@ def join_distillation(parts, tokens, teacher, vocab: int, *, scale: float = 1.0,
 
 
 # ---- logits as they are chosen from ------------------------------------------------------------------------
-def _per_row(value, otherwise, shape, what, device):
-    """(number for all rows, or float32 of each)"""
+def _per_row(value, otherwise, shape, what, device, keep):
+    """(number for all rows, address of float32 of each or None)"""
     if value is None:
         return otherwise, None
     if not isinstance(value, torch.Tensor):
         return float(value), None
-    return otherwise, _floats(value.expand(shape) if value.dim() == 0 else value, shape, what, device)
+    t = _floats(value if value.shape == shape else value.expand(shape) if value.dim() == 0 else value, shape, what, device)
+    if t is not value:
+        keep.append(t)
+    return otherwise, t.data_ptr()
 
 
-def _numbers(t, shape, what, device):
-    """Whole numbers for each row, in order, and their type."""
+def _numbers(t, shape, what, device, keep):
+    """The address of whole numbers for each row, and their type."""
     if t is None:
         return None, 0
     if not isinstance(t, torch.Tensor) or t.shape != shape:
         raise ValueError(f"{what} must be a tensor {list(shape)}")
     code = _type(t, what, _TOKEN_TYPES)
-    _same_device(device, **{what: t})
-    return t.contiguous(), code
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, not on {device}")
+    if not t.is_contiguous():
+        t = t.contiguous()
+        keep.append(t)
+    return t.data_ptr(), code
 
 
-def _rows_or_one(t, shape, what):
-    """[..., n] of each row, or [n] of all: the rows and the stride between them, 0 of the latter."""
+def _rows_or_one(t, shape, what, device, keep):
+    """[..., n] of each row, or [n] of all: the address and the stride between rows, 0 of the latter."""
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, not on {device}")
     if t.dim() == 1 and shape:
-        return t.contiguous(), 0
-    if t.dim() != len(shape) + 1 or t.shape[:-1] != shape:
+        rows, stride = (t if t.is_contiguous() else t.contiguous()), 0
+    elif t.dim() != len(shape) + 1 or t.shape[:-1] != shape:
         raise ValueError(f"{what} must be {list(shape) + ['...']} or ['...'], not {list(t.shape)}")
-    return _rows(t, t.shape[-1], what) if t.numel() else (t, 0)
+    elif t.is_contiguous():
+        return t.data_ptr(), t.shape[-1]
+    else:
+        rows, stride = _rows(t, t.shape[-1], what) if t.numel() else (t, 0)
+    if rows is not t:
+        keep.append(rows)
+    return rows.data_ptr(), stride
 
 
-class _Adjust(NamedTuple):
-    """What is done to logits: checked tensors, in the record's order."""
-    history: gdp_adjust_history
-    biases: tuple       # tokens, values, stride, number, type
-    mask: tuple         # words, stride, number
-    scale: tuple        # of each row, of all
-    keep: tuple         # tensors that the record points to
+_NO_HISTORY = gdp_adjust_history(None, 0, 0, 0, 0, 0, 1.0, 0.0, 0.0, None, None, None, None, None)
+_NO_BIASES, _NO_MASK = (None, None, 0, 0, 0), (None, 0, 0)
 
 
-def _adjust_of(shape, device, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale):
-    keep = []
-    of_history = gdp_adjust_history(None, 0, 0, 0, 0, 0, 1.0, 0.0, 0.0, None, None, None, None, None)
+def _adjust_of(shape, device, keep, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale):
+    """What is done to logits, after checking it: the record's members from the history to the scale.  ``keep`` gets the copies that
+    these point to."""
+    of_history, of_biases, of_mask = _NO_HISTORY, _NO_BIASES, _NO_MASK
     if history is not None:
         token_type = _type(history, "history", _TOKEN_TYPES)
-        _same_device(device, history=history)
         if history.dim() < 1:
             raise ValueError("history must be [..., places] or [places]")
-        tokens, stride = _rows_or_one(history, shape, "history")
-        lengths, length_type = _numbers(lengths, shape, "lengths", device)
-        prompts, prompt_type = _numbers(prompts, shape, "prompts", device)
-        r, f, p = (_per_row(v, o, shape, what, device) for v, o, what in (
-            (repetition, 1.0, "repetition"), (frequency, 0.0, "frequency"), (presence, 0.0, "presence")))
-        keep += [tokens, lengths, prompts, r[1], f[1], p[1]]
+        tokens, stride = _rows_or_one(history, shape, "history", device, keep)
+        lengths, length_type = _numbers(lengths, shape, "lengths", device, keep)
+        prompts, prompt_type = _numbers(prompts, shape, "prompts", device, keep)
+        r, rs = _per_row(repetition, 1.0, shape, "repetition", device, keep)
+        f, fs = _per_row(frequency, 0.0, shape, "frequency", device, keep)
+        p, ps = _per_row(presence, 0.0, shape, "presence", device, keep)
         if history.shape[-1]:
-            of_history = gdp_adjust_history(tokens.data_ptr(), history.shape[-1], stride, token_type, length_type, prompt_type, r[0],
-                                            f[0], p[0], _ptr(lengths), _ptr(prompts), _ptr(r[1]), _ptr(f[1]), _ptr(p[1]))
-    else:
-        for what, given in (("lengths", lengths), ("prompts", prompts), ("repetition", repetition), ("frequency", frequency),
-                            ("presence", presence)):
-            if given is not None:
-                raise ValueError(f"{what} needs a history")
-    of_biases = (None, None, 0, 0, 0)
+            of_history = gdp_adjust_history(tokens, history.shape[-1], stride, token_type, length_type, prompt_type, r, f, p, lengths,
+                                            prompts, rs, fs, ps)
+    elif not (lengths is prompts is repetition is frequency is presence is None):
+        raise ValueError("lengths, prompts, repetition, frequency and presence need a history")
     if (bias_tokens is None) != (bias is None):
         raise ValueError("bias_tokens and bias come together")
     if bias is not None:
         code = _type(bias_tokens, "bias_tokens", _TOKEN_TYPES)
-        _same_device(device, bias_tokens=bias_tokens)
         count = bias_tokens.shape[-1] if bias_tokens.dim() else 0
         if bias_tokens.dim() < 1 or count > MAX_BIASES:
             raise ValueError(f"bias_tokens must be [..., biases] or [biases] of at most {MAX_BIASES}, not {list(bias_tokens.shape)}")
         values = _floats(bias, bias_tokens.shape, "bias", device)
-        tokens, stride = _rows_or_one(bias_tokens.contiguous(), shape, "bias_tokens")
-        keep += [tokens, values]
-        if bias_tokens.numel():
-            of_biases = (tokens.data_ptr(), values.data_ptr(), stride, count, code)
-    of_mask = (None, 0, 0)
+        whole = bias_tokens if bias_tokens.is_contiguous() else bias_tokens.contiguous()
+        tokens, stride = _rows_or_one(whole, shape, "bias_tokens", device, keep)
+        keep += [values, whole]
+        if count:
+            of_biases = (tokens, values.data_ptr(), stride, count, code)
     if allowed is not None:
-        if allowed.dtype not in (torch.int32, torch.uint32):
+        if allowed.dtype is not torch.int32 and allowed.dtype is not torch.uint32:
             raise ValueError(f"allowed must be words of 32 bits, int32 or uint32, not {allowed.dtype}")
         if not allowed.is_cuda or allowed.dim() < 1:
             raise ValueError("allowed must be [..., words] or [words] on a HIP device")
-        _same_device(device, allowed=allowed)
-        words, stride = _rows_or_one(allowed, shape, "allowed")
-        keep += [words]
-        of_mask = (words.data_ptr() if words.numel() else None, stride, allowed.shape[-1])
-    one, each = _per_row(scale, 1.0, shape, "scale", device)
-    return _Adjust(of_history, of_biases, of_mask, (_ptr(each), one), tuple(keep) + (each,))
+        words, stride = _rows_or_one(allowed, shape, "allowed", device, keep)
+        of_mask = (words, stride, allowed.shape[-1])
+    one, each = _per_row(scale, 1.0, shape, "scale", device, keep)
+    return (of_history, *of_biases, *of_mask, each, one)
 
 
 def _out_dtype(dtype, logits_dtype, into):
@@ -1169,7 +1167,7 @@ def _out_dtype(dtype, logits_dtype, into):
 
 
 def _check_mask(allowed, first, columns):
-    if allowed is not None and allowed.shape[-1] * 32 < first + columns:
+    if allowed.shape[-1] * 32 < first + columns:
         raise ValueError(f"allowed: {allowed.shape[-1]} words are not enough for tokens up to {first + columns}")
 
 
@@ -1179,8 +1177,10 @@ def _adjust_logits(logits, history, lengths, prompts, repetition, frequency, pre
         raise ValueError("logits must be [..., vocab]")
     device, columns, shape = logits.device, logits.shape[-1], logits.shape[:-1]
     dtype = _out_dtype(dtype, logits.dtype, into)
-    given = _adjust_of(shape, device, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale)
-    _check_mask(allowed, first, columns)
+    keep = []
+    given = _adjust_of(shape, device, keep, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale)
+    if allowed is not None:
+        _check_mask(allowed, first, columns)
     n = shape.numel()
     if into is None:
         out = torch.empty(logits.shape, dtype=dtype, device=device)
@@ -1191,10 +1191,8 @@ def _adjust_logits(logits, history, lengths, prompts, repetition, frequency, pre
     if not n or not columns:
         return out
     rows, stride = _rows(logits, columns, "logits")
-    to = _rows_in_place(out, "into")
     _queue(_ops().gdp_adjust_forward,
-           gdp_adjust(n, columns, first, rows.data_ptr(), stride, logits_type, _TYPES[dtype], given.history, *given.biases, *given.mask,
-                      *given.scale, 0, to.data_ptr(), to.stride(0)), device)
+           gdp_adjust(n, columns, first, rows.data_ptr(), stride, logits_type, _TYPES[dtype], *given, 0, *_place(out, columns)), device)
     return out
 
 
@@ -1203,8 +1201,10 @@ def _adjust_logits_grad(logits, dtype, grad, history, lengths, repetition, allow
     device, columns, shape = grad.device, grad.shape[-1], grad.shape[:-1]
     if grad.dtype not in (dtype, torch.float32):
         raise ValueError(f"grad must have the type of the logits or float32, not {grad.dtype}")
-    given = _adjust_of(shape, device, history, lengths, None, repetition, None, None, None, None, allowed, scale)
-    _check_mask(allowed, first, columns)
+    keep = []
+    given = _adjust_of(shape, device, keep, history, lengths, None, repetition, None, None, None, None, allowed, scale)
+    if allowed is not None:
+        _check_mask(allowed, first, columns)
     n = shape.numel()
     if into is None:
         out = torch.empty(grad.shape, dtype=dtype, device=device)
@@ -1216,9 +1216,7 @@ def _adjust_logits_grad(logits, dtype, grad, history, lengths, repetition, allow
         return out
     rows, stride = _rows(grad, columns, "grad")
     x, x_stride = _rows(logits, columns, "logits") if logits is not None else (None, columns)
-    to = _rows_in_place(out, "into")
-    record = gdp_adjust(n, columns, first, _ptr(x), x_stride, _TYPES[dtype], grad_type, given.history, *given.biases, *given.mask,
-                        *given.scale, 0, to.data_ptr(), to.stride(0))
+    record = gdp_adjust(n, columns, first, _ptr(x), x_stride, _TYPES[dtype], grad_type, *given, 0, *_place(out, columns))
     _queue(_ops().gdp_adjust_backward, gdp_adjust_grad(record, rows.data_ptr(), stride), device)
     return out
 
@@ -1264,8 +1262,13 @@ def adjust_logits(logits, history=None, *, lengths=None, prompts=None, repetitio
     ``logits`` (not ``into`` a tensor); nothing else gets a gradient."""
     if forward_ad._current_level >= 0:
         _no_tangents(*(t for t in (logits, repetition, frequency, presence, bias, scale, into) if isinstance(t, torch.Tensor)))
-    _constants(repetition=repetition, frequency=frequency, presence=presence, bias=bias, scale=scale)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    by_autograd = False
+    if torch.is_grad_enabled():
+        for t, what in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence"), (bias, "bias"), (scale, "scale")):
+            if t is not None:
+                _constant(t, what)
+        by_autograd = logits.requires_grad
+    if by_autograd:
         if into is not None:
             raise ValueError("into: logits that want a gradient are not written over, nor adjusted into a tensor")
         return _AdjustLogits.apply(logits, history, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, allowed, scale,
