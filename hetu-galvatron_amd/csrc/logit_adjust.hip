@@ -62,7 +62,8 @@ constexpr int bytes_of(Table table, int columns) { return table == HALVES ? 2 * 
 
 // T: of the logits; O: of what is written, or of the gradient that is read (BACK).  VECTORS: times 16 bytes of the logits' type that a
 // thread has, one after another by workgroups.
-template <typename T, typename O, Table TABLE, bool BACK, int VECTORS>
+// PAST: read past the caches.
+template <typename T, typename O, Table TABLE, bool BACK, int VECTORS, bool PAST>
 __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typename T::raw *logits, const typename O::raw *grad,
                                                          typename std::conditional<BACK, T, O>::type::raw *out)
 {
@@ -137,7 +138,12 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
     for (int u = 0; u < VECTORS; ++u) {
         const int j = from + (u * THREADS + t) * VEC;
         // With a table without waiting for the mask
-        if (j >= 0 && j + VEC <= vocab && (TABLE != NONE ? !a.in_place : mask[u] && !(a.in_place && mask[u] == ALL))) p[u].load(from_row + j);
+        if (j >= 0 && j + VEC <= vocab && (TABLE != NONE ? !a.in_place : mask[u] && !(a.in_place && mask[u] == ALL))) {
+            if constexpr (PAST)
+                p[u].load_past(from_row + j);
+            else
+                p[u].load(from_row + j);
+        }
     }
     const float scale = a.scales ? a.scales[row] : a.scale;
     float repetition = 1.0f, inverse = 1.0f, frequency = 0.0f, presence = 0.0f;
@@ -301,8 +307,15 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
 }
 
 // ---- host ----
-constexpr int64_t PAST_BYTES = 128 << 20;
-constexpr int64_t FEW_COLUMNS = 256 * 16384;
+// The last of the caches has 256 MB.  Logits that do not fit it are read past the caches, results of half as much written past them: 1024 x 128256
+// bf16 with histories, biases and masks 132 us with neither, 126 with results and 121 with both past the caches, the gradient of 2048 rows 258, 249 and
+// 241.  What fits is left to who reads it next.
+constexpr int64_t READ_PAST = 256 << 20, WRITE_PAST = 128 << 20;
+// Four vectors a thread where that leaves no core without a workgroup, else one: 16 x 128256 bf16 with histories of 2048 12.2 us with four and 8.0
+// with one, 77 x 32003 float32 (gradient) 10.6 and 11.8.
+constexpr int64_t CORES = 256;
+// Slices of a row; one more vector where it begins within 16 bytes.
+constexpr int64_t slices_of(int64_t vocab, int vec, int columns) { return ((vocab + vec - 1) / vec * vec + vec + columns - 1) / columns; }
 constexpr int64_t MOST_ROWS = (int64_t)1 << 21, MOST_GROUPS = UINT32_MAX / THREADS;   // a grid has less than 2^32 threads
 bool token_aligned(const void *p, int type) { return aligned(p, type == GDP_I64 ? 8 : 4); }
 
@@ -355,32 +368,37 @@ template <bool BACK> int run(const gdp_adjust &a, const void *grad, int64_t grad
     Adjust k{a.vocab, a.logits_stride, a.out_stride, grad_stride, a.first, 0, a.history, a.bias_tokens, a.bias, a.bias_stride, BACK ? 0 : a.biases,
              a.bias_token_type, a.allowed, a.allowed_stride, a.scales, a.scale, 0, 0};
     if (!history) k.history.tokens = nullptr;
-    k.past = a.n * a.vocab * size_of(BACK ? a.logits_type : a.out_type) >= PAST_BYTES;
+    k.past = a.n * a.vocab * size_of(BACK ? a.logits_type : a.out_type) >= WRITE_PAST;
     k.in_place = a.out == (BACK ? grad : a.logits) && !a.scales && a.scale == 1.0f;
     return with_type(a.logits_type, [&](auto T) {
         using TT = decltype(T);
         const auto with = [&](auto O) {
             using OO = decltype(O);
-            const auto go = [&](auto TABLE, auto VECTORS) {
+            const auto go = [&](auto TABLE, auto VECTORS, auto PAST) {
                 constexpr int columns = columns_of(TT::VEC, VECTORS.value);
-                // one more vector where a row begins within 16 bytes
-                const int64_t slices = ceil_div((ceil_div(a.vocab, (int64_t)TT::VEC) + 1) * TT::VEC, (int64_t)columns);
+                const int64_t slices = slices_of(a.vocab, TT::VEC, columns);
                 if (a.n * slices > MOST_GROUPS) return gdp_fail(GDP_E_BADARG, "gdp_adjust: too many rows of so many columns");
                 k.slices = (int32_t)slices;
-                return launch(who, adjust_kernel<TT, OO, TABLE.value, BACK, VECTORS.value>, dim3((unsigned)(a.n * slices)), THREADS,
+                return launch(who, adjust_kernel<TT, OO, TABLE.value, BACK, VECTORS.value, PAST.value>, dim3((unsigned)(a.n * slices)), THREADS,
                               (size_t)bytes_of(TABLE.value, columns) + (size_t)k.biases * sizeof(Bias), stream, k,
                               static_cast<const typename TT::raw *>(a.logits), static_cast<const typename OO::raw *>(grad),
                               static_cast<typename std::conditional<BACK, TT, OO>::type::raw *>(a.out));
             };
+            const auto of_four = [&](auto TABLE) {
+                const std::integral_constant<int, 4> four;
+                return a.n * a.vocab * (int)sizeof(typename std::conditional<BACK, OO, TT>::type::raw) >= READ_PAST ? go(TABLE, four, std::true_type{})
+                                                                                                                    : go(TABLE, four, std::false_type{});
+            };
             const auto of_size = [&](auto TABLE) {
-                return a.n * a.vocab < FEW_COLUMNS ? go(TABLE, std::integral_constant<int, 1>{}) : go(TABLE, std::integral_constant<int, 4>{});
+                return a.n * slices_of(a.vocab, TT::VEC, columns_of(TT::VEC, 4)) < CORES ? go(TABLE, std::integral_constant<int, 1>{}, std::false_type{})
+                                                                                         : of_four(TABLE);
             };
             if constexpr (BACK)
                 return history ? of_size(std::integral_constant<Table, BITS>{}) : of_size(std::integral_constant<Table, NONE>{});
             else {
                 if (!history && !a.biases) return of_size(std::integral_constant<Table, NONE>{});
                 return a.history.places <= FEW_PLACES || !history ? of_size(std::integral_constant<Table, HALVES>{})
-                                                                  : go(std::integral_constant<Table, WORDS>{}, std::integral_constant<int, 4>{});
+                                                                  : of_four(std::integral_constant<Table, WORDS>{});
             }
         };
         return a.out_type == GDP_F32 ? with(F32{}) : with(TT{});

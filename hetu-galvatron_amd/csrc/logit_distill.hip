@@ -21,7 +21,7 @@ namespace {
 using namespace ops;
 
 constexpr int THREADS = 256;
-constexpr int AHEAD = 4;                 // reads of 16 bytes in flight for each thread
+constexpr int AHEAD = 2;                 // reads of 16 bytes in flight for each thread
 constexpr int MOST_SLICES = 64;
 constexpr int MOST_BITS = 1 << 18;       // columns of a slice: 32 KB of LDS
 static_assert((int64_t)MOST_BITS * MOST_SLICES / 2 > GDP_MAX_VOCAB + 64, "slices go up to MOST_SLICES by factors of two");
@@ -42,10 +42,27 @@ __device__ __forceinline__ Sums wave_join(Sums a, float c)
     const float m = wave_max(a.m);
     return {m, wave_sum(rescaled(a, m, c).s)};
 }
-__device__ __forceinline__ double wave_sum(double v)   // in the same order for all lanes
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ double plus_moved(double v)   // + 0 where there is no source
 {
-    for (int step = 32; step; step >>= 1) v += __shfl_xor(v, step);
-    return v;
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint64_t moved = (uint64_t)dpp<CTRL, ROWS>((uint32_t)(b >> 32), 0u) << 32 | dpp<CTRL, ROWS>((uint32_t)b, 0u);
+    return v + __builtin_bit_cast(double, moved);
+}
+__device__ __forceinline__ double of_lane(double v, int lane)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint64_t there = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)b, lane);
+    return __builtin_bit_cast(double, there);
+}
+__device__ __forceinline__ double wave_sum(double v)
+{
+    v = plus_moved<ROW_SHR1>(v);
+    v = plus_moved<ROW_SHR2>(v);
+    v = plus_moved<ROW_SHR4>(v);
+    v = plus_moved<ROW_SHR8>(v);
+    v = plus_moved<BCAST15, 0xa>(v);
+    v = plus_moved<BCAST31, 0xc>(v);
+    return of_lane(v, 63);
 }
 
 struct List {   // of each row, and its target
@@ -65,15 +82,17 @@ struct Part {   // of slices or shards: [parts][n][4], [parts][n][listed]
 };
 
 // The finish of a row, by one wave: PLACES places for each lane.  `all` of the unlisted; token (-1: none here), teacher and logit x of the
-// places; x_target of the row's target.  LDS: `seen` and `probability` of GDP_MAX_LISTED each.
+// places; x_target of the row's target; whether tokens may be there at several places.  LDS: `seen` and `probability` of 64 PLACES each.
+// Some 8 exponentials and logarithms of float64, each of which takes a wave a tenth of a microsecond or two.
 template <int PLACES>
 __device__ void finish_row(const Out &o, const List &l, int64_t row, int lane, Sums all, const int32_t (&token)[PLACES], const float (&teacher)[PLACES],
-                           const float (&x)[PLACES], float x_target, int32_t *seen, double *probability)
+                           const float (&x)[PLACES], float x_target, bool repeats, int32_t *seen, double *probability)
 {
     constexpr double INF = __builtin_inf();
     const double scale = o.scale;
     double q[PLACES], lq[PLACES];   // of the token at a place, over all of its places
-    bool counts[PLACES];            // the first place of a listed token
+    bool is_listed[PLACES];         // ... is at a place that is used
+    bool counts[PLACES];            // the first of these
     float m = all.m;
     // without `rest` any scores will do: their largest is taken off first
     double level = 0.0;
@@ -86,96 +105,98 @@ __device__ void finish_row(const Out &o, const List &l, int64_t row, int lane, S
     }
 #pragma unroll
     for (int j = 0; j < PLACES; ++j) {
-        const int i = lane + 64 * j;
-        const bool used = token[j] >= 0 && teacher[j] != -__builtin_inff();
-        lq[j] = used ? (double)teacher[j] - level : -INF;
-        q[j] = used ? exp(lq[j]) : 0.0;
-        if (i < l.listed) {
-            seen[i] = used ? token[j] : -1;
-            probability[i] = q[j];
-        }
-        if (used) m = fmaxf(m, x[j]);
+        counts[j] = is_listed[j] = token[j] >= 0 && teacher[j] != -__builtin_inff();
+        lq[j] = counts[j] ? (double)teacher[j] - level : -INF;
+        q[j] = exp(lq[j]);
+        if (counts[j]) m = fmaxf(m, x[j]);
     }
     m = wave_max(m);
-    __builtin_amdgcn_wave_barrier();
-    __threadfence_block();
-    bool is_listed[PLACES];
+    if (repeats) {
 #pragma unroll
-    for (int j = 0; j < PLACES; ++j) {
-        const int i = lane + 64 * j;
-        int first = GDP_MAX_LISTED, times = 0;
-        double sum = 0.0;
-        if (i < l.listed && token[j] >= 0)
-            for (int k = 0; k < l.listed; ++k)
-                if (seen[k] == token[j]) {
-                    sum += probability[k];
-                    first = first < k ? first : k;
-                    ++times;
-                }
-        is_listed[j] = times > 0;
-        counts[j] = first == i;
-        // (the same bits at all places of a token, an unused one among them)
-        if (times > 1)
-            q[j] = sum, lq[j] = log(sum);
-        else if (times == 1 && first != i)
-            q[j] = sum, lq[j] = (double)l.teacher[row * l.listed + first] - level;
+        for (int j = 0; j < PLACES; ++j) {
+            seen[lane + 64 * j] = counts[j] ? token[j] : -1;
+            probability[lane + 64 * j] = q[j];
+        }
+        __builtin_amdgcn_wave_barrier();
+        __threadfence_block();
+#pragma unroll
+        for (int j = 0; j < PLACES; ++j) {
+            const int i = lane + 64 * j;
+            int first = i, times = 0;
+            double sum = 0.0;
+            if (token[j] >= 0)
+                for (int k = 0; k < l.listed; ++k)
+                    if (seen[k] == token[j]) {
+                        sum += probability[k];
+                        first = times++ ? first : k;
+                    }
+            is_listed[j] = times > 0;
+            counts[j] = times > 0 && first == i;
+            // (the same bits at all places of a token, an unused one among them)
+            if (times > 1)
+                q[j] = sum, lq[j] = log(sum);
+            else if (times == 1 && first != i)
+                q[j] = sum, lq[j] = (double)l.teacher[row * l.listed + first] - level;
+        }
     }
-    // probabilities of the student: of places, of the rest
+    // probabilities of the student, relative to its largest logit: of places, of the rest
     const float from = finite_or_0(m);
-    const double d_out = ((double)finite_or_0(all.m) - from) * scale;
-    double s = 0.0, d[PLACES];
+    const double d_out = ((double)finite_or_0(all.m) - from) * scale, s_out = all.s == 0.0f ? 0.0 : all.s * exp(d_out);
+    double s = 0.0, mass = 0.0, lp[PLACES], p[PLACES];
 #pragma unroll
     for (int j = 0; j < PLACES; ++j) {
-        d[j] = token[j] >= 0 ? ((double)x[j] - from) * scale : -INF;
-        if (counts[j]) s += exp(d[j]);
+        lp[j] = token[j] >= 0 ? ((double)x[j] - from) * scale : -INF;
+        p[j] = exp(lp[j]);
+        s += counts[j] ? p[j] : 0.0;
+        mass += counts[j] ? q[j] : 0.0;
     }
-    const double s_out = all.s == 0.0f ? 0.0 : all.s * exp(d_out);
     s = wave_sum(s) + s_out;
-    const bool nothing = s == 0.0;
-    const double log_s = log(s), l_out = all.s == 0.0f ? -INF : d_out + log((double)all.s) - log_s, p_out = s_out / s;
-    // of the teacher: over its list, of the rest
-    double mass = 0.0;
-#pragma unroll
-    for (int j = 0; j < PLACES; ++j) mass += counts[j] ? q[j] : 0.0;
     mass = wave_sum(mass);
-    double r = 0.0;
+    // of the teacher: its rest, or its list normed
+    double r = 0.0, norm = 1.0;
     if (o.rest) {
-        r = 1.0 - mass;
-        if (all.s == 0.0f) r = 0.0;
-        else if (r < LEAST_REST) r = o.beta == 1.0f ? LEAST_REST : 0.0;
-    } else {
-        const double by = mass > 0.0 ? 1.0 / mass : mass == 0.0 ? 0.0 : mass, log_mass = mass == 0.0 ? 0.0 : log(mass);
+        r = all.s == 0.0f ? 0.0 : 1.0 - mass;
+        if (all.s != 0.0f && r < LEAST_REST) r = o.beta == 1.0f ? LEAST_REST : 0.0;
+    } else if (mass != 0.0)
+        norm = mass;
+    // the logarithms of four numbers, a lane for each
+    const double logs = log(lane == 0 ? s : lane == 1 ? (double)all.s : lane == 2 ? norm : r);
+    const double log_s = of_lane(logs, 0), log_out = of_lane(logs, 1), log_norm = of_lane(logs, 2), lr = of_lane(logs, 3);
+    const bool nothing = s == 0.0;
+    const double l_out = all.s == 0.0f ? -INF : d_out + log_out - log_s, of_s = 1.0 / s, p_out = s_out * of_s, of_norm = 1.0 / norm;
+    mass *= of_norm;
 #pragma unroll
-        for (int j = 0; j < PLACES; ++j) q[j] *= by, lq[j] -= log_mass;
-        mass = mass == 0.0 ? 0.0 : mass * by;
-    }
-    const double lr = log(r), beta = o.beta;
-    double lp[PLACES], p[PLACES], a[PLACES];
-    double loss = 0.0, mean = 0.0, a_out = 0.0, of_rest = 0.0;
-#pragma unroll
-    for (int j = 0; j < PLACES; ++j) lp[j] = d[j] - log_s, p[j] = exp(lp[j]);
+    for (int j = 0; j < PLACES; ++j) q[j] *= of_norm, lq[j] -= log_norm, lp[j] -= log_s, p[j] *= of_s;
+    const double beta = o.beta;
+    double loss = 0.0, mean = 0.0, of_rest, pull[PLACES];
     if (beta == 0.0) {
 #pragma unroll
-        for (int j = 0; j < PLACES; ++j)
+        for (int j = 0; j < PLACES; ++j) {
             if (counts[j] && q[j] != 0.0) loss += q[j] * (lq[j] - lp[j]);
+            pull[j] = p[j] * (mass + r) - q[j];
+        }
         loss = wave_sum(loss) + (r > 0.0 ? r * (lr - l_out) : 0.0);
         of_rest = (mass + r) * p_out - r;
     } else {
+        const bool between = beta != 1.0;
+        const double of_p = between ? 1.0 - beta : 1.0;
+        double a[PLACES];   // ln p less that of what it is held against
 #pragma unroll
         for (int j = 0; j < PLACES; ++j) {
-            const double lm = beta == 1.0 ? lq[j] : log(beta * q[j] + (1.0 - beta) * p[j]);
+            const double lm = between ? log(beta * q[j] + of_p * p[j]) : lq[j];
             a[j] = p[j] == 0.0 ? 0.0 : lp[j] - lm;
             if (counts[j]) {
                 mean += p[j] * a[j];
-                if (beta != 1.0 && q[j] != 0.0) loss += q[j] * (lq[j] - lm);
+                if (between && q[j] != 0.0) loss += q[j] * (lq[j] - lm);
             }
         }
-        const double lm = beta == 1.0 ? lr : log(beta * r + (1.0 - beta) * p_out);
-        a_out = p_out == 0.0 ? 0.0 : l_out - lm;
+        const double lm = between ? log(beta * r + of_p * p_out) : lr, a_out = p_out == 0.0 ? 0.0 : l_out - lm;
         mean = wave_sum(mean) + p_out * a_out;
-        loss = wave_sum(loss) + (beta != 1.0 && r > 0.0 ? r * (lr - lm) : 0.0);
-        loss = beta == 1.0 ? mean : beta * loss + (1.0 - beta) * mean;
-        of_rest = (beta == 1.0 ? 1.0 : 1.0 - beta) * p_out * (a_out - mean);
+        if (between) loss = wave_sum(loss) + (r > 0.0 ? r * (lr - lm) : 0.0);
+        loss = between ? beta * loss + of_p * mean : mean;
+        of_rest = of_p * p_out * (a_out - mean);
+#pragma unroll
+        for (int j = 0; j < PLACES; ++j) pull[j] = of_p * p[j] * (a[j] - mean);
     }
     const bool empty = nothing || (!o.rest && mass == 0.0 && s == s);   // no row, or no list
     if (s != s) loss = s;
@@ -192,20 +213,16 @@ __device__ void finish_row(const Out &o, const List &l, int64_t row, int lane, S
     float *const to = o.stats + row * (HEAD + l.listed);
     if (lane == 0) {
         to[0] = m, to[1] = (float)log_s;
-        to[2] = all.m, to[3] = all.s == 0.0f ? -__builtin_inff() : logf(all.s);
+        to[2] = all.m, to[3] = (float)log_out;
         to[4] = empty || all.s == 0.0f ? 0.0f : (float)of_rest;
     }
 #pragma unroll
     for (int j = 0; j < PLACES; ++j) {
         const int i = lane + 64 * j;
-        double pull;
-        if (!is_listed[j])
-            pull = of_rest * exp((double)x[j] * scale - (double)finite_or_0(all.m) * scale - log((double)all.s));   // its share of the rest
-        else if (beta == 0.0)
-            pull = p[j] * (mass + r) - q[j];
-        else
-            pull = (beta == 1.0 ? 1.0 : 1.0 - beta) * p[j] * (a[j] - mean);
-        if (i < l.listed) to[HEAD + i] = token[j] < 0 || empty || (!is_listed[j] && x[j] == -__builtin_inff()) ? 0.0f : (float)pull;
+        if (i >= l.listed) continue;
+        const bool of_others = token[j] >= 0 && !is_listed[j];   // a token at places that are not used: its share of the rest
+        if (of_others) pull[j] = x[j] == -__builtin_inff() ? 0.0 : of_rest * exp(((double)x[j] - all.m) * scale - log_out);
+        to[HEAD + i] = token[j] < 0 || empty ? 0.0f : (float)pull[j];
     }
 }
 
@@ -218,13 +235,14 @@ struct Scan {
     Part part;
 };
 
-template <typename T, int PLACES>
+// PAST: read past the caches.
+template <typename T, int PLACES, bool PAST>
 __global__ __launch_bounds__(THREADS) void distill_scan_kernel(Scan a, const typename T::raw *__restrict__ logits)
 {
     constexpr int VEC = T::VEC, WAVES = THREADS / 64;
     extern __shared__ __align__(16) uint32_t bits[];   // a bit for each column of the slice's vectors
     __shared__ Sums of_wave[WAVES];
-    __shared__ int32_t seen[64 * PLACES];
+    __shared__ int32_t seen[64 * PLACES], repeats;
     __shared__ double probability[64 * PLACES];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t row = blockIdx.x / a.slices;
@@ -235,45 +253,16 @@ __global__ __launch_bounds__(THREADS) void distill_scan_kernel(Scan a, const typ
     const int vocab = (int)a.vocab, vectors = (vocab + off + VEC - 1) / VEC;
     const int v0 = slice * a.width, v1 = v0 + a.width < vectors ? v0 + a.width : vectors;
     const int from = v0 * VEC - off, to = v1 * VEC - off;   // columns of the slice, cut by the row's
-    for (int i = t; i < (a.width * VEC + 31) / 32; i += THREADS) bits[i] = 0;
-    int32_t token[PLACES];
-    float teacher[PLACES], at_place[PLACES], of_target = -__builtin_inff();
-    if (wave == 0) {
-#pragma unroll
-        for (int j = 0; j < PLACES; ++j) {
-            const int i = lane + 64 * j;
-            token[j] = -1, teacher[j] = at_place[j] = -__builtin_inff();
-            if (i < a.list.listed) {
-                const int64_t one = token_at(a.list.tokens, a.list.list_type, row * a.list.listed + i), local = one < 0 ? -1 : one - a.first;
-                teacher[j] = a.list.teacher[row * a.list.listed + i];
-                if (local >= 0 && local < vocab && local >= from && local < to) {
-                    token[j] = (int32_t)local;
-                    at_place[j] = T::up(x[local]);
-                }
-            }
-        }
-        if (lane == 0 && a.list.targets) {
-            const int64_t target = token_at(a.list.targets, a.list.target_type, row), local = target < 0 ? -1 : target - a.first;
-            if (local >= 0 && local < vocab && local >= from && local < to) of_target = T::up(x[local]);
-        }
-    }
-    __syncthreads();
-    if (wave == 0) {
-#pragma unroll
-        for (int j = 0; j < PLACES; ++j)
-            if (token[j] >= 0 && teacher[j] != -__builtin_inff()) atomicOr(&bits[(token[j] - from) >> 5], 1u << ((token[j] - from) & 31));
-    }
-    __syncthreads();
-    const float c = a.c;
-    const uint8_t *const bytes = reinterpret_cast<const uint8_t *>(bits);
-    Sums own{-__builtin_inff(), 0.0f};
-    for (int base = v0; base < v1; base += THREADS * AHEAD) {
-        Pack<T, VEC> p[AHEAD];
+    Pack<T, VEC> p[AHEAD];
+    const auto load = [&](int base) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int v = base + u * THREADS + t, j = v * VEC - off;
             if (v < v1 && j >= 0 && j + VEC <= vocab) {
-                p[u].load(x + j);
+                if constexpr (PAST)
+                    p[u].load_past(x + j);
+                else
+                    p[u].load(x + j);
             } else {
                 float f[VEC];
 #pragma unroll
@@ -281,6 +270,51 @@ __global__ __launch_bounds__(THREADS) void distill_scan_kernel(Scan a, const typ
                 p[u].set(f);
             }
         }
+    };
+    int32_t token[PLACES];
+    float teacher[PLACES];
+    if (wave == 0) {
+#pragma unroll
+        for (int j = 0; j < PLACES; ++j) {
+            const int i = lane + 64 * j;
+            token[j] = -1, teacher[j] = -__builtin_inff();
+            if (i < a.list.listed) {
+                const int64_t one = token_at(a.list.tokens, a.list.list_type, row * a.list.listed + i), local = one < 0 ? -1 : one - a.first;
+                teacher[j] = a.list.teacher[row * a.list.listed + i];
+                if (local >= 0 && local < vocab && local >= from && local < to) token[j] = (int32_t)local;
+            }
+        }
+    }
+    load(v0);   // (on their way while the bitmap is made)
+    for (int i = t; i < (a.width * VEC + 31) / 32; i += THREADS) bits[i] = 0;
+    if (t == 0) repeats = 0;
+    __syncthreads();
+    typename T::raw at_place[PLACES], of_target = T::down(-__builtin_inff());
+    if (wave == 0) {
+        bool again = false;
+#pragma unroll
+        for (int j = 0; j < PLACES; ++j) {
+            const uint32_t bit = 1u << ((token[j] - from) & 31);
+            if (token[j] >= 0 && teacher[j] != -__builtin_inff()) again |= (atomicOr(&bits[(token[j] - from) >> 5], bit) & bit) != 0;
+        }
+#pragma unroll
+        for (int j = 0; j < PLACES; ++j) {
+            at_place[j] = T::down(-__builtin_inff());
+            if (token[j] < 0) continue;
+            at_place[j] = x[token[j]];
+            again |= teacher[j] == -__builtin_inff() && (bits[(token[j] - from) >> 5] >> ((token[j] - from) & 31) & 1);
+        }
+        if (again) repeats = 1;
+        if (lane == 0 && a.list.targets) {
+            const int64_t target = token_at(a.list.targets, a.list.target_type, row), local = target < 0 ? -1 : target - a.first;
+            if (local >= 0 && local < vocab && local >= from && local < to) of_target = x[local];
+        }
+    }
+    __syncthreads();
+    const float c = a.c;
+    const uint8_t *const bytes = reinterpret_cast<const uint8_t *>(bits);
+    Sums own{-__builtin_inff(), 0.0f};
+    for (int base = v0; base < v1; base += THREADS * AHEAD) {
         float most = own.m;
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
@@ -305,6 +339,7 @@ __global__ __launch_bounds__(THREADS) void distill_scan_kernel(Scan a, const typ
 #pragma unroll
             for (int i = 0; i < VEC; ++i) sum += exp2_fast((p[u][i] - level) * c);
         own.s += sum;
+        if (base + THREADS * AHEAD < v1) load(base + THREADS * AHEAD);
     }
     own = wave_join(own, c);
     if (lane == 0) of_wave[wave] = own;
@@ -316,16 +351,19 @@ __global__ __launch_bounds__(THREADS) void distill_scan_kernel(Scan a, const typ
     Sums all{m, 0.0f};
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) all.s += rescaled(of_wave[w], m, c).s;
+    float x_k[PLACES];
+#pragma unroll
+    for (int j = 0; j < PLACES; ++j) x_k[j] = T::up(at_place[j]);
     if (!a.part.sums) {
-        finish_row<PLACES>(a.out, a.list, row, lane, all, token, teacher, at_place, of_target, seen, probability);
+        finish_row<PLACES>(a.out, a.list, row, lane, all, token, teacher, x_k, T::up(of_target), repeats != 0, seen, probability);
         return;
     }
     const int64_t at = (int64_t)slice * a.n + row;
-    if (lane == 0) a.part.sums[at] = make_float4(all.m, all.s, of_target, 0.0f);
+    if (lane == 0) a.part.sums[at] = make_float4(all.m, all.s, T::up(of_target), 0.0f);
 #pragma unroll
     for (int j = 0; j < PLACES; ++j) {
         const int i = lane + 64 * j;
-        if (i < a.list.listed) a.part.logits[at * a.list.listed + i] = at_place[j];
+        if (i < a.list.listed) a.part.logits[at * a.list.listed + i] = x_k[j];
     }
 }
 
@@ -375,7 +413,7 @@ template <int PLACES> __global__ __launch_bounds__(64) void distill_join_kernel(
     const bool no_number = __ballot(of_target != of_target) != 0;
     of_target = no_number ? __builtin_nanf("") : wave_max(of_target);
     if (!a.part.sums) {
-        finish_row<PLACES>(a.out, a.list, row, lane, all, token, teacher, x, of_target, seen, probability);
+        finish_row<PLACES>(a.out, a.list, row, lane, all, token, teacher, x, of_target, true, seen, probability);
         return;
     }
     if (lane == 0) a.part.sums[row] = make_float4(all.m, all.s, of_target, 0.0f);
@@ -387,6 +425,7 @@ template <int PLACES> __global__ __launch_bounds__(64) void distill_join_kernel(
 struct Grad {
     int64_t vocab, stride, out_stride, first, whole;
     int32_t slices, width;
+    int32_t past;            // written past the caches
     float scale;
     List list;
     const float *stats, *grad_loss, *grad_lse, *grad_logp;
@@ -395,8 +434,8 @@ struct Grad {
 template <typename T>
 __global__ __launch_bounds__(THREADS) void distill_grad_kernel(Grad a, const typename T::raw *logits, typename T::raw *out)
 {
-    constexpr int VEC = T::VEC, ENTRIES = (GDP_MAX_LISTED + 1 + THREADS - 1) / THREADS;
-    __shared__ int32_t target_is_listed;
+    constexpr int VEC = T::VEC, ENTRIES = (GDP_MAX_LISTED + THREADS - 1) / THREADS;
+    __shared__ int32_t has_target[THREADS / 64];   // whether a wave's places hold the target
     const int t = threadIdx.x;
     const int64_t row = blockIdx.x / a.slices;
     const int slice = (int)(blockIdx.x % a.slices);
@@ -408,10 +447,31 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(Grad a, const typ
     const int from = v0 * VEC - off, to = v1 * VEC - off;
     const int listed = a.list.listed;
     const float *const stats = a.stats + row * (HEAD + listed);
-    const float m = stats[0], log_s = stats[1], m_out = stats[2], log_out = stats[3];
-    const bool dead = log_s < -__FLT_MAX__, none = log_out < -__FLT_MAX__;   // no logit above -inf; none that is not listed
+    const auto column_of = [&](int64_t one) -> int32_t {   // of this slice, or -1
+        const int64_t local = one < 0 ? -1 : one - a.first;
+        return local >= 0 && local < vocab && local >= from && local < to ? (int32_t)local : -1;
+    };
+    Pack<T, VEC> p[AHEAD];
+    const auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int v = base + u * THREADS + t, j = v * VEC - off;
+            if (v < v1 && j >= 0 && j + VEC <= vocab) p[u].load(x + j);
+        }
+    };
+    int64_t one[ENTRIES];
+    float pull[ENTRIES];
+#pragma unroll
+    for (int k = 0; k < ENTRIES; ++k) {
+        const int e = t + k * THREADS;
+        one[k] = -1;
+        if (e < listed) one[k] = token_at(a.list.tokens, a.list.list_type, row * listed + e), pull[k] = stats[HEAD + e];
+    }
     int64_t target = a.list.targets && a.grad_logp ? token_at(a.list.targets, a.list.target_type, row) : -1;
     if (target >= a.whole) target = -1;
+    load(v0);   // (on their way while the places are looked at)
+    const float m = stats[0], log_s = stats[1], m_out = stats[2], log_out = stats[3];
+    const bool dead = log_s < -__FLT_MAX__, none = log_out < -__FLT_MAX__;   // no logit above -inf; none that is not listed
     const float g = target >= 0 && !dead ? a.grad_logp[row] : 0.0f;
     const float of_p = dead ? 0.0f : (a.grad_lse ? a.grad_lse[row] : 0.0f) - g, of_loss = a.grad_loss ? a.grad_loss[row] : 0.0f;
     const auto p_of = [&](float f) { return dead ? 0.0f : exp2_fast(fmaf(f - m, a.scale, -log_s) * LOG2E); };
@@ -422,43 +482,24 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(Grad a, const typ
     const auto grad_of = [&](float f) { return factor * exp2_fast(fmaf(f - level, a.scale, -away) * LOG2E); };
     // The listed places and the target, from their logits, before anything is written (out may be the logits).  A token in several
     // places has the same gradient at each.
-    if (t == 0) target_is_listed = 0;
-    __syncthreads();
     int32_t column[ENTRIES];
     float value[ENTRIES];
+    bool mine = false;
 #pragma unroll
     for (int k = 0; k < ENTRIES; ++k) {
-        const int e = t + k * THREADS;
-        column[k] = -1;
-        if (e < listed) {
-            const int64_t one = token_at(a.list.tokens, a.list.list_type, row * listed + e), local = one < 0 ? -1 : one - a.first;
-            if (local >= 0 && local < vocab && local >= from && local < to) {
-                column[k] = (int32_t)local;
-                value[k] = of_loss != 0.0f ? of_loss * stats[HEAD + e] : 0.0f;
-                if (of_p != 0.0f) value[k] += of_p * p_of(T::up(x[local]));
-                if (one == target) value[k] += g, target_is_listed = 1;
-                value[k] *= a.scale;
-            }
-        }
+        column[k] = column_of(one[k]);
+        if (column[k] < 0) continue;
+        value[k] = of_loss != 0.0f ? of_loss * pull[k] : 0.0f;
+        if (of_p != 0.0f) value[k] += of_p * p_of(T::up(x[column[k]]));
+        if (one[k] == target) value[k] += g, mine = true;
+        value[k] *= a.scale;
     }
-    __syncthreads();
-    float again = 0.0f;
-    int32_t at_target = -1;
-    if (t == 0 && target >= 0 && !target_is_listed) {
-        const int64_t local = target - a.first;
-        if (local >= 0 && local < vocab && local >= from && local < to) {
-            at_target = (int32_t)local;
-            again = grad_of(T::up(x[local])) + a.scale * g;
-        }
-    }
+    const bool any = __ballot(mine) != 0;
+    if ((t & 63) == 0) has_target[t >> 6] = any;
+    const int32_t at_target = t == 0 ? column_of(target) : -1;
+    const float again = at_target >= 0 ? grad_of(T::up(x[at_target])) + a.scale * g : 0.0f;
     __syncthreads();
     for (int base = v0; base < v1; base += THREADS * AHEAD) {
-        Pack<T, VEC> p[AHEAD];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int v = base + u * THREADS + t, j = v * VEC - off;
-            if (v < v1 && j >= 0 && j + VEC <= vocab) p[u].load(x + j);
-        }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int v = base + u * THREADS + t, j = v * VEC - off;
@@ -468,18 +509,27 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(Grad a, const typ
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) f[i] = grad_of(p[u][i]);
                 p[u].set(f);
-                p[u].store(y + j);
+                if (a.past)
+                    p[u].store_past(y + j);
+                else
+                    p[u].store(y + j);
             } else {
                 for (int i = 0; i < VEC; ++i)
                     if (j + i >= 0 && j + i < vocab) y[j + i] = T::down(grad_of(T::up(x[j + i])));
             }
         }
+        if (base + THREADS * AHEAD < v1) load(base + THREADS * AHEAD);
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < ENTRIES; ++k)
         if (column[k] >= 0) y[column[k]] = T::down(value[k]);
-    if (at_target >= 0) y[at_target] = T::down(again);
+    if (at_target >= 0) {
+        bool is_listed = false;
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) is_listed |= has_target[w] != 0;
+        if (!is_listed) y[at_target] = T::down(again);
+    }
 }
 
 // ---- host ----
@@ -504,6 +554,7 @@ Part part_at(void *p, int64_t parts, int64_t n)
     return {static_cast<float4 *>(p), reinterpret_cast<float *>(static_cast<char *>(p) + sums_bytes(parts, n))};
 }
 
+constexpr int64_t READ_PAST = 256 << 20, WRITE_PAST = 128 << 20;
 constexpr int64_t MOST_ROWS = (int64_t)1 << 21, MOST_GROUPS = (int64_t)1 << 23;   // a grid has less than 2^32 threads
 int check(int64_t n, int64_t vocab, int64_t first, int type, int listed)
 {
@@ -547,13 +598,17 @@ int check_out(const Out &o, const List &l)
 int scan(Scan s, const void *logits, int type, const Split &split, const char *who, void *stream)
 {
     s.slices = split.slices, s.width = split.width;
+    const bool past = s.n * s.vocab * size_of(type) >= READ_PAST;
     return with_type(type, [&](auto T) {
         using TT = decltype(T);
         const auto *x = static_cast<const typename TT::raw *>(logits);
         const dim3 grid((unsigned)(s.n * split.slices));
         const size_t lds = round_up(ceil_div((size_t)split.width * TT::VEC, (size_t)32) * 4, 16);
-        return s.list.listed <= 64 ? launch(who, distill_scan_kernel<TT, 1>, grid, THREADS, lds, stream, s, x)
-                                   : launch(who, distill_scan_kernel<TT, 4>, grid, THREADS, lds, stream, s, x);
+        const auto with = [&](auto PAST) {
+            return s.list.listed <= 64 ? launch(who, distill_scan_kernel<TT, 1, PAST.value>, grid, THREADS, lds, stream, s, x)
+                                       : launch(who, distill_scan_kernel<TT, 4, PAST.value>, grid, THREADS, lds, stream, s, x);
+        };
+        return past ? with(std::true_type{}) : with(std::false_type{});
     });
 }
 int join(const Join &j, const char *who, void *stream)
@@ -659,11 +714,12 @@ extern "C" int gdp_distill_backward(const gdp_distill_grad *d, void *stream)
     if (d->out == d->logits && d->n > 1 && d->out_stride != d->logits_stride) return gdp_fail(GDP_E_BADARG, "gdp_distill: a gradient in the place of the logits needs their stride");
     const int vec = 16 / size_of(d->logits_type);
     const int64_t vectors = ceil_div(d->vocab, (int64_t)vec) + 1;
-    int64_t slices = 1;   // two rounds of reads for each workgroup, more where the grid would be too large
-    while (vectors / slices > 2 * THREADS * AHEAD && d->n * slices < (1 << 22)) slices *= 2;
-    const int64_t width = ceil_div(vectors, slices);
-    slices = ceil_div(vectors, width);
-    const Grad g{d->vocab, d->logits_stride, d->out_stride, d->first, d->whole_vocab, (int32_t)slices, (int32_t)width, d->scale, list, d->stats,
+    // A workgroup has its columns in registers; more than once where the grid would be too large.
+    int64_t width = THREADS * AHEAD;
+    while (d->n * ceil_div(vectors, width) > MOST_GROUPS) width *= 2;
+    const int64_t slices = ceil_div(vectors, width);
+    const Grad g{d->vocab, d->logits_stride, d->out_stride, d->first, d->whole_vocab, (int32_t)slices, (int32_t)width,
+                 d->n * d->vocab * size_of(d->logits_type) >= WRITE_PAST, d->scale, list, d->stats,
                  d->grad_loss, d->grad_lse, d->grad_logp};
     return with_type(d->logits_type, [&](auto T) {
         using TT = decltype(T);
