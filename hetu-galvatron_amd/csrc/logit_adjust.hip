@@ -74,7 +74,7 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
     constexpr int ENTRY = TABLE == HALVES ? 16 : 32;            // bits of a table's entry
     constexpr uint32_t OF_PROMPT = 1u << (ENTRY - 1), HAS_BIAS = 1u << (ENTRY - 2), COUNT = HAS_BIAS - 1;
     extern __shared__ __align__(16) uint32_t table[];           // then the slice's biases; BITS: in the history, then above 0
-    __shared__ int32_t n_biases;
+    __shared__ int32_t again;                                   // a token has several biases
     const int t = threadIdx.x;
     const int64_t row = blockIdx.x / a.slices;
     const int slice = (int)(blockIdx.x % a.slices);
@@ -90,10 +90,10 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
     const int vocab = (int)a.vocab, from = slice * COLUMNS - off;   // the slice's first column
     const gdp_adjust_history &h = a.history;
     Bias *const biases = reinterpret_cast<Bias *>(table + TABLE_WORDS);
-    constexpr int BIAS_WAVE = THREADS - 64;
     const int64_t first = a.first + from;     // token of the slice's first column
-    uint64_t bias_token = 0;
-    float bias_value = 0.0f;
+    constexpr int BIASES = TABLE == HALVES || TABLE == WORDS ? GDP_MAX_BIASES / THREADS : 0;   // of each thread
+    float bias_value[BIASES + 1], of_bias[BIASES + 1];   // of a column, and its logit
+    int bias_column[BIASES + 1];                         // of the slice, or -1
     int length = 0, prompt = 0;               // in words of 32 bits
     const bool wide = h.token_type == GDP_I64;
     const uint32_t *history = nullptr;
@@ -110,9 +110,15 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
                 if (i + Tokens::WORDS <= length) token[u].load(history + i);
             }
         }
-        if (!BACK && t - BIAS_WAVE >= 0 && t - BIAS_WAVE < a.biases) {
-            bias_token = (uint64_t)token_at(a.bias_tokens, a.bias_token_type, row * a.bias_stride + t - BIAS_WAVE);
-            bias_value = a.bias[row * a.bias_stride + t - BIAS_WAVE];
+#pragma unroll
+        for (int b = 0; b < BIASES; ++b) {
+            const int i = b * THREADS + t;
+            bias_column[b] = -1;
+            if (i < a.biases) {
+                const uint64_t local = (uint64_t)token_at(a.bias_tokens, a.bias_token_type, row * a.bias_stride + i) - (uint64_t)first;
+                bias_value[b] = a.bias[row * a.bias_stride + i];
+                if (local < COLUMNS && from + (int)local >= 0 && from + (int)local < vocab) bias_column[b] = (int)local;
+            }
         }
     }
     // VEC bits of the mask for each whole vector, from the byte or the two that hold them
@@ -131,7 +137,7 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
     if constexpr (TABLE != NONE) {
 #pragma unroll
         for (int i = t; i < TABLE_WORDS / 4; i += THREADS) reinterpret_cast<uint4 *>(table)[i] = make_uint4(0, 0, 0, 0);
-        if (t == 0) n_biases = 0;
+        if (t == 0) again = 0;
     }
     Pack<R, VEC> p[VECTORS];
 #pragma unroll
@@ -158,15 +164,17 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
         // N tokens' columns; those of other slices, or of none, are above all.  The first `of_prompt` are of the prompt.
         const auto count = [&](auto N, const uint32_t *column, int of_prompt) {
             if constexpr (TABLE == BITS) {
-                bool positive[N.value];
+                bool positive[N.value], fresh[N.value];
 #pragma unroll
                 for (int k = 0; k < N.value; ++k) {
                     const int j = from + (int)column[k];
-                    positive[k] = column[k] < COLUMNS && j >= 0 && j < vocab && T::up(x[j]) > 0.0f;
+                    // (once is enough for a token that is there often)
+                    fresh[k] = column[k] < COLUMNS && j >= 0 && j < vocab && !(table[column[k] >> 5] >> (column[k] & 31) & 1);
+                    positive[k] = fresh[k] && T::up(x[j]) > 0.0f;
                 }
 #pragma unroll
                 for (int k = 0; k < N.value; ++k)
-                    if (column[k] < COLUMNS) {
+                    if (fresh[k]) {
                         atomicOr(&table[column[k] >> 5], 1u << (column[k] & 31));
                         if (positive[k]) atomicOr(&table[TABLE_WORDS / 2 + (column[k] >> 5)], 1u << (column[k] & 31));
                     }
@@ -211,27 +219,40 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
                 if (next + Tokens::WORDS <= length) token[u].load(history + next);
             }
         }
-        if (!BACK && a.biases && t >= BIAS_WAVE) {   // one wave, in order
-            const int lane = t - BIAS_WAVE;
-            int found = 0;
-            for (int i = lane; i - lane < a.biases; i += 64) {
-                if (i >= 64 && i < a.biases) {
-                    bias_token = (uint64_t)token_at(a.bias_tokens, a.bias_token_type, row * a.bias_stride + i);
-                    bias_value = a.bias[row * a.bias_stride + i];
-                }
-                const uint64_t local = bias_token - (uint64_t)first;
-                const bool here = i < a.biases && local < COLUMNS;
-                const uint64_t all = __ballot(here);
-                if (here) {
-                    biases[found + __popcll(all & ((1ull << lane) - 1))] = {(int32_t)local, bias_value};
-                    atomicOr(&table[TABLE == HALVES ? local >> 1 : local], TABLE == HALVES ? HAS_BIAS << (local & 1) * 16 : HAS_BIAS);
-                }
-                found += __popcll(all);
+#pragma unroll
+        for (int b = 0; b < BIASES; ++b)
+            if (b * THREADS + t < a.biases) {
+                const int column = bias_column[b];
+                biases[b * THREADS + t] = {column, bias_value[b]};
+                if (column < 0) continue;
+                of_bias[b] = T::up(x[from + column]);   // (before anything is written)
+                const int shift = TABLE == HALVES ? (column & 1) * 16 : 0;
+                if (atomicOr(&table[TABLE == HALVES ? column >> 1 : column], HAS_BIAS << shift) >> shift & HAS_BIAS) again = 1;
             }
-            if (lane == 0) n_biases = found;
-        }
         __syncthreads();
     }
+    // pen(f) less frequency and presence
+    const auto penalised = [&](float f, uint32_t entry) -> float {
+        const uint32_t n = entry & COUNT;
+        f *= entry & (OF_PROMPT | COUNT) ? f > 0.0f ? inverse : repetition : 1.0f;
+        return fmaf(-frequency, (float)n, f) - (n ? presence : 0.0f);
+    };
+    // The results of columns with biases, which are written behind the others
+#pragma unroll
+    for (int b = 0; b < BIASES; ++b)
+        if (bias_column[b] >= 0) {
+            const int column = bias_column[b];
+            if (again) {   // all that its token has, in their order, at each of them
+                bias_value[b] = 0.0f;
+                for (int i = 0; i < a.biases; ++i) bias_value[b] += biases[i].column == column ? biases[i].value : 0.0f;
+            }
+            const uint32_t entry = TABLE == HALVES ? table[column >> 1] >> (column & 1) * 16 & 0xffff : table[column];
+            of_bias[b] = (penalised(of_bias[b], entry) + bias_value[b]) * scale;
+            const uint32_t bit = bit_of(from + column);
+            if (allowed && !(allowed[bit >> 3] >> (bit & 7) & 1)) bias_column[b] = -1;
+        }
+    if constexpr (BIASES > 0)
+        if (a.biases && static_cast<const void *>(out) == logits) __syncthreads();   // (their logits are overwritten below)
     constexpr uint32_t RULED_OUT = BACK ? 0u : 0xff800000u;   // 0, -inf
 #pragma unroll
     for (int u = 0; u < VECTORS; ++u) {
@@ -239,7 +260,6 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
         if (j >= vocab) continue;
         // the vector's entries
         uint32_t c[TABLE == BITS ? 2 : VEC * ENTRY / 32], any = 0;
-        bool biased = false;
         if constexpr (TABLE == BITS) {
             const uint8_t *const bytes = reinterpret_cast<const uint8_t *>(table);
             const int at = VEC == 8 ? v : v >> 1, shift = VEC == 8 ? 0 : 4 * (v & 1);
@@ -250,23 +270,13 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
             entries.load(table + v * (VEC * ENTRY / 32));
 #pragma unroll
             for (int i = 0; i < VEC * ENTRY / 32; ++i) any |= c[i] = entries.w[i];
-            biased = any & (TABLE == HALVES ? HAS_BIAS << 16 | HAS_BIAS : HAS_BIAS);
         }
         const auto of_column = [&](float f, int i) -> float {
             if constexpr (TABLE == BITS) {
                 f *= scale;
                 return c[0] >> i & 1 ? f * (c[1] >> i & 1 ? inverse : repetition) : f;
             }
-            if constexpr (TABLE == HALVES || TABLE == WORDS) {
-                const uint32_t e = TABLE == HALVES ? c[i / 2] >> (i % 2) * 16 & 0xffff : c[i], n = e & COUNT;
-                f *= e & (OF_PROMPT | COUNT) ? f > 0.0f ? inverse : repetition : 1.0f;
-                f = fmaf(-frequency, (float)n, f) - (n ? presence : 0.0f);
-                if (biased && e & HAS_BIAS) {
-                    float sum = 0.0f;
-                    for (int b = 0; b < n_biases; ++b) sum += biases[b].column == v * VEC + i ? biases[b].value : 0.0f;
-                    f += sum;
-                }
-            }
+            if constexpr (TABLE == HALVES || TABLE == WORDS) f = penalised(f, TABLE == HALVES ? c[i / 2] >> (i % 2) * 16 & 0xffff : c[i]);
             return f * scale;
         };
         if (j >= 0 && j + VEC <= vocab) {
@@ -303,6 +313,12 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
                 y[j + i] = W::down(keep ? of_column(R::up(from_row[j + i]), i) : __builtin_bit_cast(float, RULED_OUT));
             }
         }
+    }
+    if (BIASES && a.biases) {
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < BIASES; ++b)
+            if (bias_column[b] >= 0) y[from + bias_column[b]] = W::down(of_bias[b]);
     }
 }
 

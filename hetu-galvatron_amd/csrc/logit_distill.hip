@@ -76,7 +76,7 @@ struct Out {
     int32_t rest;
     int64_t whole;       // tokens outside [0, whole) are none
 };
-struct Part {   // of slices or shards: [parts][n][4], [parts][n][listed]
+struct Part {   // of slices or shards: [parts][n][4]; of shards [parts][n][listed], of slices one for all, of which each writes its own tokens'
     float4 *sums;
     float *logits;
 };
@@ -119,24 +119,28 @@ __device__ void finish_row(const Out &o, const List &l, int64_t row, int lane, S
         }
         __builtin_amdgcn_wave_barrier();
         __threadfence_block();
+        int first[PLACES], times[PLACES];
+        double sum[PLACES];
+#pragma unroll
+        for (int j = 0; j < PLACES; ++j) first[j] = lane + 64 * j, times[j] = 0, sum[j] = 0.0;
+        for (int k = 0; k < l.listed; ++k) {
+            const int one = seen[k];
+#pragma unroll
+            for (int j = 0; j < PLACES; ++j)
+                if (one >= 0 && one == token[j]) {
+                    sum[j] += probability[k];
+                    first[j] = times[j]++ ? first[j] : k;
+                }
+        }
 #pragma unroll
         for (int j = 0; j < PLACES; ++j) {
-            const int i = lane + 64 * j;
-            int first = i, times = 0;
-            double sum = 0.0;
-            if (token[j] >= 0)
-                for (int k = 0; k < l.listed; ++k)
-                    if (seen[k] == token[j]) {
-                        sum += probability[k];
-                        first = times++ ? first : k;
-                    }
-            is_listed[j] = times > 0;
-            counts[j] = times > 0 && first == i;
+            is_listed[j] = times[j] > 0;
+            counts[j] = times[j] > 0 && first[j] == lane + 64 * j;
             // (the same bits at all places of a token, an unused one among them)
-            if (times > 1)
-                q[j] = sum, lq[j] = log(sum);
-            else if (times == 1 && first != i)
-                q[j] = sum, lq[j] = (double)l.teacher[row * l.listed + first] - level;
+            if (times[j] > 1)
+                q[j] = sum[j], lq[j] = log(sum[j]);
+            else if (times[j] == 1 && !counts[j])
+                q[j] = sum[j], lq[j] = (double)l.teacher[row * l.listed + first[j]] - level;
         }
     }
     // probabilities of the student, relative to its largest logit: of places, of the rest
@@ -236,10 +240,10 @@ struct Scan {
 };
 
 // PAST: read past the caches.
-template <typename T, int PLACES, bool PAST>
-__global__ __launch_bounds__(THREADS) void distill_scan_kernel(Scan a, const typename T::raw *__restrict__ logits)
+template <typename T, int PLACES, bool PAST, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void distill_scan_kernel(Scan a, const typename T::raw *__restrict__ logits)
 {
-    constexpr int VEC = T::VEC, WAVES = THREADS / 64;
+    constexpr int VEC = T::VEC, THREADS = 64 * WAVES;
     extern __shared__ __align__(16) uint32_t bits[];   // a bit for each column of the slice's vectors
     __shared__ Sums of_wave[WAVES];
     __shared__ int32_t seen[64 * PLACES], repeats;
@@ -359,17 +363,18 @@ __global__ __launch_bounds__(THREADS) void distill_scan_kernel(Scan a, const typ
         return;
     }
     const int64_t at = (int64_t)slice * a.n + row;
-    if (lane == 0) a.part.sums[at] = make_float4(all.m, all.s, T::up(of_target), 0.0f);
+    if (lane == 0) a.part.sums[at] = make_float4(all.m, all.s, T::up(of_target), repeats ? 1.0f : 0.0f);
 #pragma unroll
     for (int j = 0; j < PLACES; ++j) {
         const int i = lane + 64 * j;
-        if (i < a.list.listed) a.part.logits[at * a.list.listed + i] = x_k[j];
+        if (i < a.list.listed && (a.slices == 1 || token[j] >= 0)) a.part.logits[row * a.list.listed + i] = x_k[j];
     }
 }
 
 struct Join {
     int64_t n;
-    int32_t parts;
+    int64_t first, columns;  // the tokens that the lists are of
+    int32_t parts, lists;    // lists: 1 of slices
     float c;
     List list;
     Part in;
@@ -389,12 +394,13 @@ template <int PLACES> __global__ __launch_bounds__(64) void distill_join_kernel(
     const int64_t row = blockIdx.x;
     const int listed = a.list.listed;
     Sums own{-__builtin_inff(), 0.0f};
-    float of_target = -__builtin_inff();
+    float of_target = -__builtin_inff(), again = 0.0f;
     if (lane < a.parts) {
         const float4 s = a.in.sums[(int64_t)lane * a.n + row];
         own = {s.x, s.y};
-        of_target = s.z;
+        of_target = s.z, again = s.w;
     }
+    const bool repeats = __ballot(again != 0.0f) != 0;   // (a token's places are all seen by the part that holds it)
     int32_t token[PLACES];
     float teacher[PLACES], x[PLACES];
 #pragma unroll
@@ -403,20 +409,21 @@ template <int PLACES> __global__ __launch_bounds__(64) void distill_join_kernel(
         token[j] = -1, teacher[j] = x[j] = -__builtin_inff();
         if (i < listed) {
             const int64_t one = token_at(a.list.tokens, a.list.list_type, row * listed + i);
-            if (one >= 0 && one < a.out.whole) token[j] = (int32_t)one;
+            if (one >= a.first && one < a.first + a.columns) token[j] = (int32_t)one;
             teacher[j] = a.list.teacher[row * listed + i];
-#pragma unroll 4
-            for (int p = 0; p < a.parts; ++p) x[j] = most_or_nan(a.in.logits[((int64_t)p * a.n + row) * listed + i], x[j]);
+            if (token[j] >= 0)
+#pragma unroll 8
+                for (int p = 0; p < a.lists; ++p) x[j] = most_or_nan(a.in.logits[((int64_t)p * a.n + row) * listed + i], x[j]);
         }
     }
     const Sums all = wave_join(own, a.c);
     const bool no_number = __ballot(of_target != of_target) != 0;
     of_target = no_number ? __builtin_nanf("") : wave_max(of_target);
     if (!a.part.sums) {
-        finish_row<PLACES>(a.out, a.list, row, lane, all, token, teacher, x, of_target, true, seen, probability);
+        finish_row<PLACES>(a.out, a.list, row, lane, all, token, teacher, x, of_target, repeats, seen, probability);
         return;
     }
-    if (lane == 0) a.part.sums[row] = make_float4(all.m, all.s, of_target, 0.0f);
+    if (lane == 0) a.part.sums[row] = make_float4(all.m, all.s, of_target, repeats ? 1.0f : 0.0f);
 #pragma unroll
     for (int j = 0; j < PLACES; ++j)
         if (lane + 64 * j < listed) a.part.logits[row * listed + lane + 64 * j] = x[j];
@@ -548,12 +555,14 @@ Split split_of(int64_t n, int64_t vocab, int type)
     return {(int)ceil_div(vectors, width), (int)width};
 }
 size_t sums_bytes(int64_t parts, int64_t n) { return round_up((size_t)parts * n * 16, 256); }
-size_t part_bytes(int64_t parts, int64_t n, int listed) { return sums_bytes(parts, n) + round_up((size_t)parts * n * listed * 4, 256); }
+size_t part_bytes(int64_t parts, int64_t n, int listed) { return sums_bytes(parts, n) + round_up((size_t)n * listed * 4, 256); }
 Part part_at(void *p, int64_t parts, int64_t n)
 {
     return {static_cast<float4 *>(p), reinterpret_cast<float *>(static_cast<char *>(p) + sums_bytes(parts, n))};
 }
 
+// Rows of up to so many vectors (16 KB), and at least so many of them: a wave for each row instead of four.
+constexpr int SHORT = 1024, SHORT_ROWS = 2048;
 constexpr int64_t READ_PAST = 256 << 20, WRITE_PAST = 128 << 20;
 constexpr int64_t MOST_ROWS = (int64_t)1 << 21, MOST_GROUPS = (int64_t)1 << 23;   // a grid has less than 2^32 threads
 int check(int64_t n, int64_t vocab, int64_t first, int type, int listed)
@@ -604,11 +613,15 @@ int scan(Scan s, const void *logits, int type, const Split &split, const char *w
         const auto *x = static_cast<const typename TT::raw *>(logits);
         const dim3 grid((unsigned)(s.n * split.slices));
         const size_t lds = round_up(ceil_div((size_t)split.width * TT::VEC, (size_t)32) * 4, 16);
-        const auto with = [&](auto PAST) {
-            return s.list.listed <= 64 ? launch(who, distill_scan_kernel<TT, 1, PAST.value>, grid, THREADS, lds, stream, s, x)
-                                       : launch(who, distill_scan_kernel<TT, 4, PAST.value>, grid, THREADS, lds, stream, s, x);
+        const auto with = [&](auto PAST, auto WAVES) {
+            constexpr int waves = WAVES.value;
+            return s.list.listed <= 64 ? launch(who, distill_scan_kernel<TT, 1, PAST.value, waves>, grid, 64 * waves, lds, stream, s, x)
+                                       : launch(who, distill_scan_kernel<TT, 4, PAST.value, waves>, grid, 64 * waves, lds, stream, s, x);
         };
-        return past ? with(std::true_type{}) : with(std::false_type{});
+        const std::integral_constant<int, 1> one;
+        const std::integral_constant<int, 4> four;
+        if (split.slices == 1 && s.n >= SHORT_ROWS && split.width <= SHORT) return with(std::false_type{}, one);
+        return past ? with(std::true_type{}, four) : with(std::false_type{}, four);
     });
 }
 int join(const Join &j, const char *who, void *stream)
@@ -624,7 +637,7 @@ int rows(Scan s, const void *logits, int type, void *workspace, size_t bytes, co
     if (split.slices == 1) return scan(s, logits, type, split, who, stream);
     if (!workspace || !aligned(workspace, 256) || bytes < part_bytes(split.slices, s.n, s.list.listed))
         return gdp_fail(GDP_E_BADARG, "gdp_distill: the workspace is smaller than gdp_distill_workspace says, or not aligned to 256 bytes");
-    Join j{s.n, split.slices, s.c, s.list, part_at(workspace, split.slices, s.n), s.out, s.part};
+    Join j{s.n, s.first, s.vocab, split.slices, 1, s.c, s.list, part_at(workspace, split.slices, s.n), s.out, s.part};
     s.part = j.in;
     if (const int rc = scan(s, logits, type, split, who, stream)) return rc;
     return join(j, who, stream);
@@ -694,7 +707,7 @@ extern "C" int gdp_distill_join(const gdp_distill_joint *d, void *stream)
     if (!d->sums || !aligned(d->sums, 16) || !d->listed_logits || !aligned(d->listed_logits, 4))
         return gdp_fail(GDP_E_BADARG, "gdp_distill: null pointer, or sums not aligned to 16 bytes");
     const Part in{reinterpret_cast<float4 *>(const_cast<float *>(d->sums)), const_cast<float *>(d->listed_logits)};
-    return join({d->n, d->parts, d->scale * LOG2E, list, in, out, {}}, "gdp_distill_join", stream);
+    return join({d->n, 0, d->vocab, d->parts, d->parts, d->scale * LOG2E, list, in, out, {}}, "gdp_distill_join", stream);
 }
 
 extern "C" int gdp_distill_backward(const gdp_distill_grad *d, void *stream)

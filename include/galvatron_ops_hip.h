@@ -232,7 +232,7 @@ int gdp_distill_forward(const gdp_distill *d, void *stream);
 
 /* The same for a vocabulary in shards: `parts` of each, joined after the ranks have exchanged them (16 + 4 * listed
  * bytes a row).  Of a part: sums [n][4] float32 (largest unlisted logit; sum of exp2 over the unlisted; the target's logit or -inf;
- * 0), and the listed tokens' logits, -inf for those of other shards. */
+ * 1 where a token of the shard is at several places, else 0), and the listed tokens' logits, -inf for those of other shards. */
 typedef struct gdp_distill_part {
     int64_t n, vocab, first;
     const void *logits;
