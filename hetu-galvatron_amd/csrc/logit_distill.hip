@@ -83,7 +83,7 @@ struct Part {   // of slices or shards: [parts][n][4]; of shards [parts][n][list
 
 // The finish of a row, by one wave: PLACES places for each lane.  `all` of the unlisted; token (-1: none here), teacher and logit x of the
 // places; x_target of the row's target; whether tokens may be there at several places.  LDS: `seen` and `probability` of 64 PLACES each.
-// Some 8 exponentials and logarithms of float64, each of which takes a wave a tenth of a microsecond or two.
+// Some 8 exponentials and logarithms of float64: 3 us a wave, hidden behind other rows' reads where there are many.
 template <int PLACES>
 __device__ void finish_row(const Out &o, const List &l, int64_t row, int lane, Sums all, const int32_t (&token)[PLACES], const float (&teacher)[PLACES],
                            const float (&x)[PLACES], float x_target, bool repeats, int32_t *seen, double *probability)
@@ -239,7 +239,11 @@ struct Scan {
     Part part;
 };
 
-// PAST: read past the caches.
+// Bound by memory where rows are long and many: 8192 x 128256 bf16 with 20 listed tokens 320 us, 2.1 GB at 6.6 TB/s; 2048 x 50257 float16 with 64 and beta
+// 0.5 48 us, 4.3 TB/s: two rounds of workgroups, and a finish of 3 us behind each row.  With more than 64 listed tokens the finish holds 100
+// registers and lasts longer: 8192 x 128256 with 256 448 us, 358 with 20 in the same run.  Rows of 2 KB are mostly finish: 32089 x 1180 61 us, 36 of them without it.
+// Few rows wait for memory four times (lists, bitmap, logits, the join): 16 x 128256 10 us.
+// PLACES: of each lane of the wave that finishes.  PAST: read past the caches.
 template <typename T, int PLACES, bool PAST, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void distill_scan_kernel(Scan a, const typename T::raw *__restrict__ logits)
 {
@@ -385,7 +389,8 @@ struct Join {
 // The larger; NaN where one of them is.
 __device__ __forceinline__ float most_or_nan(float a, float b) { return a > b || a != a ? a : b; }
 
-// A wave for each row.
+// A wave for each row: lists, sums and logits are read side by side, then the finish.  8192 rows of 8 shards with 20 listed tokens 14 us, 16 rows of
+// slices 4 us.
 template <int PLACES> __global__ __launch_bounds__(64) void distill_join_kernel(Join a)
 {
     __shared__ int32_t seen[64 * PLACES];
@@ -438,11 +443,14 @@ struct Grad {
     const float *stats, *grad_loss, *grad_lse, *grad_logp;
 };
 
-template <typename T>
-__global__ __launch_bounds__(THREADS) void distill_grad_kernel(Grad a, const typename T::raw *logits, typename T::raw *out)
+// Elementwise with one exponential, bound by memory: 8192 x 128256 bf16 713 us, 4.2 GB at 5.9 TB/s; a shard's 4096 x 19008 with 128 listed places 54 us,
+// 5.8 TB/s; 517 x 32003 float16 15 us.  A workgroup has its columns in registers while it looks at the places, 512 vectors of two for
+// each thread: with two rounds of them 8192 x 128256 832 us, with one 786 (both written in the caches).
+template <typename T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void distill_grad_kernel(Grad a, const typename T::raw *logits, typename T::raw *out)
 {
-    constexpr int VEC = T::VEC, ENTRIES = (GDP_MAX_LISTED + THREADS - 1) / THREADS;
-    __shared__ int32_t has_target[THREADS / 64];   // whether a wave's places hold the target
+    constexpr int VEC = T::VEC, THREADS = 64 * WAVES, ENTRIES = (GDP_MAX_LISTED + THREADS - 1) / THREADS;
+    __shared__ int32_t has_target[WAVES];   // whether a wave's places hold the target
     const int t = threadIdx.x;
     const int64_t row = blockIdx.x / a.slices;
     const int slice = (int)(blockIdx.x % a.slices);
@@ -534,7 +542,7 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(Grad a, const typ
     if (at_target >= 0) {
         bool is_listed = false;
 #pragma unroll
-        for (int w = 0; w < THREADS / 64; ++w) is_listed |= has_target[w] != 0;
+        for (int w = 0; w < WAVES; ++w) is_listed |= has_target[w] != 0;
         if (!is_listed) y[at_target] = T::down(again);
     }
 }
@@ -565,8 +573,12 @@ Part part_at(void *p, int64_t parts, int64_t n)
     return {static_cast<float4 *>(p), reinterpret_cast<float *>(static_cast<char *>(p) + sums_bytes(parts, n))};
 }
 
-// Rows of up to so many vectors (16 KB), and at least so many of them: a wave for each row instead of four.
-constexpr int SHORT = 1024, SHORT_ROWS = 2048;
+// Rows of up to so many vectors (16 KB; gradients 4 KB), and at least so many of them: a wave for each row instead of four.  32089 x 1180 bf16 61 us, 99 with
+// four waves, the gradient 49 and 65; 10350 x 1638 float32 31 and 35, its gradient (410 vectors) 42 and 31.
+constexpr int SHORT = 1024, SHORT_GRAD = 256, SHORT_ROWS = 2048;
+// The last of the caches has 256 MB.  Logits that do not fit it are read past the caches, 8192 x 128256 bf16 399 us and 358; what does is read again by the
+// gradient: 2048 x 50257 bf16 forward and backward 99 us, 109 with reads past the caches.  Gradients of half as much are written past them:
+// 8192 x 128256 786 and 741.
 constexpr int64_t READ_PAST = 256 << 20, WRITE_PAST = 128 << 20;
 constexpr int64_t MOST_ROWS = (int64_t)1 << 21, MOST_GROUPS = (int64_t)1 << 23;   // a grid has less than 2^32 threads
 int check(int64_t n, int64_t vocab, int64_t first, int type, int listed)
@@ -734,7 +746,8 @@ extern "C" int gdp_distill_backward(const gdp_distill_grad *d, void *stream)
     const int vec = 16 / size_of(d->logits_type);
     const int64_t vectors = ceil_div(d->vocab, (int64_t)vec) + 1;
     // A workgroup has its columns in registers; more than once where the grid would be too large.
-    int64_t width = THREADS * AHEAD;
+    const bool by_waves = d->n >= SHORT_ROWS && vectors <= SHORT_GRAD;
+    int64_t width = by_waves ? SHORT_GRAD : THREADS * AHEAD;
     while (d->n * ceil_div(vectors, width) > MOST_GROUPS) width *= 2;
     const int64_t slices = ceil_div(vectors, width);
     const Grad g{d->vocab, d->logits_stride, d->out_stride, d->first, d->whole_vocab, (int32_t)slices, (int32_t)width,
@@ -742,7 +755,10 @@ extern "C" int gdp_distill_backward(const gdp_distill_grad *d, void *stream)
                  d->grad_loss, d->grad_lse, d->grad_logp};
     return with_type(d->logits_type, [&](auto T) {
         using TT = decltype(T);
-        return launch("gdp_distill_backward", distill_grad_kernel<TT>, dim3((unsigned)(d->n * slices)), THREADS, 0, stream, g,
-                      static_cast<const typename TT::raw *>(d->logits), static_cast<typename TT::raw *>(d->out));
+        const auto *x = static_cast<const typename TT::raw *>(d->logits);
+        auto *y = static_cast<typename TT::raw *>(d->out);
+        const dim3 grid((unsigned)(d->n * slices));
+        return by_waves ? launch("gdp_distill_backward", distill_grad_kernel<TT, 1>, grid, 64, 0, stream, g, x, y)
+                        : launch("gdp_distill_backward", distill_grad_kernel<TT, THREADS / 64>, grid, THREADS, 0, stream, g, x, y);
     });
 }

@@ -472,6 +472,9 @@ def test_many_biases_and_long_histories():
     tokens[0, 500:520] = tokens[0, 3]
     check_adjusted(x, bias_tokens=tokens.cuda(), bias=normal(g, 2, 1024))
     check_adjusted(x, bias_tokens=tokens[:, :0].cuda(), bias=torch.zeros(2, 0, device="cuda"), scale=2.0)
+    # entries of 32 bits and all the biases that a row may have: the most LDS that a call takes
+    wide, long = normal(g, 2, 40000, dtype=BF16), history_of(g, 2, 17000, 40000)
+    check_adjusted(wide, history=long, repetition=1.1, frequency=0.01, bias_tokens=torch.randint(0, 40000, (2, 1024), generator=g).cuda(), bias=normal(g, 2, 1024))
     check_adjusted(x, history=history_of(g, 2, 70001, 9000), repetition=1.1, frequency=0.01, prompts=torch.tensor([70000, 35000]).cuda())
 
 

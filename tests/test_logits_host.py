@@ -165,14 +165,15 @@ def test_tangents_are_refused():
 
 @pytest.mark.skipif(shutil.which("nm") is None, reason="no nm")
 def test_every_kernel_has_calls_that_reach_it():
-    """Scans: few or many listed places; a wave a row, or four or eight that read in or past the caches.  Adjusted logits: results of the logits' type or float32;
+    """Scans: few or many listed places; a wave a row, or four or eight that read in or past the caches; gradients by
+    a wave or four.  Adjusted logits: results of the logits' type or float32;
     no table, entries of 16 or 32 bits (long histories: four vectors a thread), two bits for the gradient; one vector a thread, or four, read
     in or past the caches."""
     names = subprocess.run(["nm", "-C", _lib.LIB_PATH], capture_output=True, text=True, check=True).stdout
     clean = re.sub(r"\(anonymous namespace\)::|ops::", "", names)
     got = {(k, *re.sub(r"\(\w+\)", "", a).split(", ")) for k, a in re.findall(r" ((?:distill|adjust)_\w*kernel)<([^>]*)>", clean)}
     types = ("F32", "F16", "BF16")
-    want = {("distill_join_kernel", p) for p in "14"} | {("distill_grad_kernel", t) for t in types}
+    want = {("distill_join_kernel", p) for p in "14"} | {("distill_grad_kernel", t, w) for t in types for w in "14"}
     want |= {("distill_scan_kernel", t, p, *form) for t in types for p in "14" for form in (("false", "1"), ("false", "4"), ("true", "4"), ("false", "8"), ("true", "8"))}
     sizes = (("1", "false"), ("4", "false"), ("4", "true"))
     for t in types:
