@@ -328,9 +328,9 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
 }
 
 // ---- host ----
-// The last of the caches has 256 MB.  Logits that do not fit it are read past the caches, results of half as much written past them: 1024 x 128256
-// bf16 with histories, biases and masks 132 us with neither, 126 with results and 121 with both past the caches, the gradient of 2048 rows 258, 249 and
-// 241.  What fits is left to who reads it next.
+// The last of the caches has 256 MB.  What does not fit it is read past the caches, results of half as much are written past them: the gradient of
+// 2048 x 128256 bf16 258 us with neither, 249 with the result and 241 with both past the caches; forward 1024 x 128256 132 us, 126 with the result
+// past them.  What fits is left to who reads it next.
 constexpr int64_t READ_PAST = 256 << 20, WRITE_PAST = 128 << 20;
 // Entries of 16 bits for histories whose counts they hold leave a core twice the columns: with entries of 32 bits and half the columns to a workgroup
 // 1024 x 128256 with histories of 1024 147 us, not 133.  One read of the history in flight: four are 154 us there, for 64 registers are
