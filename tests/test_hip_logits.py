@@ -80,6 +80,45 @@ def test_distillation_sizes(case, dtype):
         check_distillation(x, tokens, teacher, 1.0, 0.0, True, targets)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("case", [(2100, 517, 20), (2050, 1000, 100), (3001, 9, 9), (2048, 4090, 256), (2049, 8185, 3)], ids=str)
+def test_distillation_of_many_short_rows(case, dtype):
+    """A wave for each row: the same bits as rows by themselves have in the gradient, and results within the bounds; lists with unused and
+    repeated places among them."""
+    n, V, K = case
+    g = gen(n + K)
+    x = normal(g, n, V, dtype=dtype, size=2.0)
+    tokens, teacher = lists(g, 64, V, K)
+    tokens, teacher = tokens.repeat(n // 64 + 1, 1)[:n].contiguous(), teacher.repeat(n // 64 + 1, 1)[:n].contiguous()
+    if K > 2:
+        tokens[1, 1], tokens[2, 0], teacher[3, 2] = tokens[1, 0], -1, -INF
+    targets = torch.randint(-1, V + 1, (n,), generator=g).cuda()
+    targets[:5] = tokens[:5, 0]
+    r = ops.distillation(x, tokens, teacher, beta=0.25, targets=targets, stats=True)
+    some = torch.cat([torch.arange(6), torch.arange(n - 2, n)]).cuda()
+    check_distillation(x[some], tokens[some], teacher[some], 1.0, 0.25, True, targets[some], ops.Distillation(*(t[some] for t in r)))
+    d, d_logp = torch.rand(n, generator=g).cuda(), torch.rand(n, generator=g).cuda()
+    whole = ops.distillation_grad(x, tokens, r.stats, d, targets=targets, grad_logp=d_logp)
+    part = ops.distillation_grad(x[some], tokens[some], r.stats[some], d[some], targets=targets[some], grad_logp=d_logp[some])
+    assert torch.equal(whole[some], part)
+    place = x.clone()
+    assert torch.equal(ops.distillation_grad(place, tokens, r.stats, d, targets=targets, grad_logp=d_logp, into=place), whole)
+
+
+def test_logits_that_no_cache_holds():
+    """Few rows, but more than 256 MB; results as of rows by themselves."""
+    g = gen(15)
+    for n, V, dtype in ((600, 262400, BF16), (300, 262400, F32)):
+        x = torch.randn(n, V, device="cuda", dtype=dtype)
+        for K in (20, 70):
+            tokens, teacher = lists(g, 8, V, K)
+            tokens, teacher = tokens.repeat(n // 8, 1)[:n].contiguous(), teacher.repeat(n // 8, 1)[:n].contiguous()
+            tokens, teacher = torch.cat([tokens, tokens])[:n].contiguous(), torch.cat([teacher, teacher])[:n].contiguous()
+            r = ops.distillation(x, tokens, teacher, stats=True)
+            some = torch.tensor([0, n // 2, n - 1]).cuda()
+            check_distillation(x[some], tokens[some], teacher[some], 1.0, 0.0, True, None, ops.Distillation(*(t if t is None else t[some] for t in r)))
+
+
 @pytest.mark.parametrize("scale", [1.0, 0.5, 3.25])
 @pytest.mark.parametrize("rest", [True, False], ids=["rest", "renormed"])
 @pytest.mark.parametrize("beta", [0.0, 0.125, 0.5, 1.0])
@@ -476,6 +515,27 @@ def test_many_biases_and_long_histories():
     wide, long = normal(g, 2, 40000, dtype=BF16), history_of(g, 2, 17000, 40000)
     check_adjusted(wide, history=long, repetition=1.1, frequency=0.01, bias_tokens=torch.randint(0, 40000, (2, 1024), generator=g).cuda(), bias=normal(g, 2, 1024))
     check_adjusted(x, history=history_of(g, 2, 70001, 9000), repetition=1.1, frequency=0.01, prompts=torch.tensor([70000, 35000]).cuda())
+
+
+@pytest.mark.parametrize("places", [0, 40, 17000])
+def test_adjusted_logits_that_no_cache_holds(places):
+    """More than 256 MB: the same bits as rows by themselves have."""
+    g = gen(26)
+    n, V = 1100, 128250
+    x = torch.randn(n, V, device="cuda").to(BF16)
+    given = dict(allowed=C.words_of(torch.rand(V, generator=g) < 0.5).cuda(), scale=(0.5 + torch.rand(n, generator=g)).cuda())
+    if places:
+        given.update(history=torch.randint(0, V, (n, places), generator=g).cuda(), repetition=(0.5 + torch.rand(n, generator=g)).cuda())
+    more = dict(given, bias_tokens=torch.randint(0, V, (n, 9), generator=g).cuda(), bias=normal(g, n, 9)) if places else given
+    some = torch.tensor([0, 1, n // 2, n - 1]).cuda()
+    of = lambda d: {k: v if v.dim() == 1 and k == "allowed" else v[some] for k, v in d.items()}   # noqa: E731
+    y = ops.adjust_logits(x, **more)
+    part = ops.adjust_logits(x[some], **of(more))
+    assert torch.equal(y[some], part)
+    ref, bound = C.adjusted(x[some[:1]], **{k: v if k == "allowed" else v[:1] for k, v in of(more).items()})
+    C.close(part[:1], ref, bound + C.rounded(ref, BF16))
+    d = ops.adjust_logits_grad(x, x, **given)
+    assert torch.equal(d[some], ops.adjust_logits_grad(x[some], x[some], **of(given)))
 
 
 def test_adjusted_through_autograd():
