@@ -240,11 +240,10 @@ struct Scan {
 };
 
 // Bound by memory where rows are long and many: 8192 x 128256 bf16 with 20 listed tokens 320 us, 2.1 GB at 6.6 TB/s; 2048 x 50257 float16 with 64 and beta
-// 0.5 48 us, 4.3 TB/s: two rounds of workgroups, and a finish of 3 us behind each row.  With more than 64 listed tokens the finish holds 100
-// registers and lasts longer: 8192 x 128256 with 256 448 us, 358 with 20 in the same run.  Rows of 2 KB are mostly finish: 32089 x 1180 61 us, 36 of them without it.
+// 0.5 48 us, 4.3 TB/s: two rounds of workgroups, and a finish of 3 us behind each row.  Rows of 2 KB are mostly finish: 32089 x 1180 61 us, 36 of them without it.
 // Few rows wait for memory four times (lists, bitmap, logits, the join): 16 x 128256 10 us.
-// PLACES: of each lane of the wave that finishes.  PAST: read past the caches.
-template <typename T, int PLACES, bool PAST, int WAVES>
+// PLACES: of each lane of the wave that finishes, 1 or 4; the finish of four holds 100 registers.  FINISH: whole rows are finished here.  PAST: read past the caches.
+template <typename T, int PLACES, bool FINISH, bool PAST, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void distill_scan_kernel(Scan a, const typename T::raw *__restrict__ logits)
 {
     constexpr int VEC = T::VEC, THREADS = 64 * WAVES;
@@ -362,10 +361,11 @@ __global__ __launch_bounds__(64 * WAVES) void distill_scan_kernel(Scan a, const 
     float x_k[PLACES];
 #pragma unroll
     for (int j = 0; j < PLACES; ++j) x_k[j] = T::up(at_place[j]);
-    if (!a.part.sums) {
-        finish_row<PLACES>(a.out, a.list, row, lane, all, token, teacher, x_k, T::up(of_target), repeats != 0, seen, probability);
-        return;
-    }
+    if constexpr (FINISH)
+        if (!a.part.sums) {
+            finish_row<PLACES>(a.out, a.list, row, lane, all, token, teacher, x_k, T::up(of_target), repeats != 0, seen, probability);
+            return;
+        }
     const int64_t at = (int64_t)slice * a.n + row;
     if (lane == 0) a.part.sums[at] = make_float4(all.m, all.s, T::up(of_target), repeats ? 1.0f : 0.0f);
 #pragma unroll
@@ -566,6 +566,15 @@ Split split_of(int64_t n, int64_t vocab, int type)
     const int64_t width = ceil_div(vectors, slices);
     return {(int)ceil_div(vectors, width), (int)width};
 }
+// The last of the caches has 256 MB.  Logits that do not fit it are read past the caches, 8192 x 128256 bf16 399 us and 358; what does is read again by the
+// gradient: 2048 x 50257 bf16 forward and backward 99 us, 109 with reads past the caches.  Gradients of half as much are written past them:
+// 8192 x 128256 786 and 741.
+constexpr int64_t READ_PAST = 256 << 20, WRITE_PAST = 128 << 20;
+// Whether rows are finished by a kernel of their own: those in slices, and, of lists with more than a place for each lane, whose finish holds
+// registers that the scan could read with, those that take longer than a launch.  8192 x 128256 bf16 with 100 listed tokens 362 us, 399 where
+// the scan finishes them, 4096 x 19008 with 128 57 and 63, 700 x 32000 23 and 23; but 2050 x 1000 with 100 14 and 10.
+bool by_join(const Split &s, int64_t n, int64_t vocab, int listed) { return s.slices > 1 || (listed > 64 && n * vocab >= 1 << 25); }
+static_assert(READ_PAST / 4 >= 1 << 25, "rows that are read past the caches are joined");
 size_t sums_bytes(int64_t parts, int64_t n) { return round_up((size_t)parts * n * 16, 256); }
 size_t part_bytes(int64_t parts, int64_t n, int listed) { return sums_bytes(parts, n) + round_up((size_t)n * listed * 4, 256); }
 Part part_at(void *p, int64_t parts, int64_t n)
@@ -576,10 +585,6 @@ Part part_at(void *p, int64_t parts, int64_t n)
 // Rows of up to so many vectors (16 KB; gradients 4 KB), and at least so many of them: a wave for each row instead of four.  32089 x 1180 bf16 61 us, 99 with
 // four waves, the gradient 49 and 65; 10350 x 1638 float32 31 and 35, its gradient (410 vectors) 42 and 31.
 constexpr int SHORT = 1024, SHORT_GRAD = 256, SHORT_ROWS = 2048;
-// The last of the caches has 256 MB.  Logits that do not fit it are read past the caches, 8192 x 128256 bf16 399 us and 358; what does is read again by the
-// gradient: 2048 x 50257 bf16 forward and backward 99 us, 109 with reads past the caches.  Gradients of half as much are written past them:
-// 8192 x 128256 786 and 741.
-constexpr int64_t READ_PAST = 256 << 20, WRITE_PAST = 128 << 20;
 constexpr int64_t MOST_ROWS = (int64_t)1 << 21, MOST_GROUPS = (int64_t)1 << 23;   // a grid has less than 2^32 threads
 int check(int64_t n, int64_t vocab, int64_t first, int type, int listed)
 {
@@ -631,8 +636,10 @@ int scan(Scan s, const void *logits, int type, const Split &split, const char *w
         const size_t lds = round_up(ceil_div((size_t)split.width * TT::VEC, (size_t)32) * 4, 16);
         const auto with = [&](auto PAST, auto WAVES) {
             constexpr int waves = WAVES.value;
-            return s.list.listed <= 64 ? launch(who, distill_scan_kernel<TT, 1, PAST.value, waves>, grid, 64 * waves, lds, stream, s, x)
-                                       : launch(who, distill_scan_kernel<TT, 4, PAST.value, waves>, grid, 64 * waves, lds, stream, s, x);
+            if (s.list.listed <= 64) return launch(who, distill_scan_kernel<TT, 1, true, PAST.value, waves>, grid, 64 * waves, lds, stream, s, x);
+            if constexpr (!PAST.value)   // (rows that are read past the caches are joined)
+                if (!s.part.sums) return launch(who, distill_scan_kernel<TT, 4, true, false, waves>, grid, 64 * waves, lds, stream, s, x);
+            return launch(who, distill_scan_kernel<TT, 4, false, PAST.value, waves>, grid, 64 * waves, lds, stream, s, x);
         };
         const std::integral_constant<int, 1> one;
         const std::integral_constant<int, 4> four;
@@ -647,12 +654,12 @@ int join(const Join &j, const char *who, void *stream)
     const dim3 grid((unsigned)j.n);
     return j.list.listed <= 64 ? launch(who, distill_join_kernel<1>, grid, 64, 0, stream, j) : launch(who, distill_join_kernel<4>, grid, 64, 0, stream, j);
 }
-// Slices of a row, joined where there are several.
+// Rows, or their slices, and what joins them.
 int rows(Scan s, const void *logits, int type, void *workspace, size_t bytes, const char *who, void *stream)
 {
     const Split split = split_of(s.n, s.vocab, type);
     if (s.n * split.slices > MOST_GROUPS) return gdp_fail(GDP_E_BADARG, "gdp_distill: too many rows of so many columns");
-    if (split.slices == 1) return scan(s, logits, type, split, who, stream);
+    if (split.slices == 1 && (s.part.sums || !by_join(split, s.n, s.vocab, s.list.listed))) return scan(s, logits, type, split, who, stream);
     if (!workspace || !aligned(workspace, 256) || bytes < part_bytes(split.slices, s.n, s.list.listed))
         return gdp_fail(GDP_E_BADARG, "gdp_distill: the workspace is smaller than gdp_distill_workspace says, or not aligned to 256 bytes");
     Join j{s.n, s.first, s.vocab, split.slices, 1, s.c, s.list, part_at(workspace, split.slices, s.n), s.out, s.part};
@@ -669,7 +676,7 @@ extern "C" int gdp_distill_workspace(int64_t n, int64_t vocab, int32_t logits_ty
     if (!bytes) return gdp_fail(GDP_E_BADARG, "gdp_distill: null argument");
     if (const int rc = check(n, vocab, 0, logits_type, listed)) return rc;
     const Split s = split_of(n, vocab, logits_type);
-    *bytes = s.slices > 1 ? part_bytes(s.slices, n, listed) : 0;
+    *bytes = by_join(s, n, vocab, listed) ? part_bytes(s.slices, n, listed) : 0;
     return GDP_OK;
 }
 

@@ -60,7 +60,7 @@ def check_distillation(x, tokens, teacher, scale, beta, rest, targets=None, got=
 SIZES = [  # rows, vocabulary, listed
     (1, 1, 1), (1, 2, 1), (3, 5, 2), (4, 5, 5), (7, 33, 4), (5, 64, 64), (64, 1000, 20), (5, 4097, 63), (3, 8190, 65), (3, 50257, 128),
     (2, 128256, 256), (1, 300003, 20), (1100, 517, 20), (1030, 5003, 7),
-    (1024, 262400, 20)]
+    (1024, 262400, 20), (1300, 26000, 100)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)

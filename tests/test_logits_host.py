@@ -129,7 +129,8 @@ def test_workspaces():
     for bad in ((-1, 5, 0, 1), (1, 0, 0, 1), (1, 5, 3, 1), (1, 5, 0, 0), (1, 5, 0, 257)):
         assert of(*bad) == _lib.GDP_E_BADARG
     assert lib.gdp_distill_workspace(1, 5, 0, 1, None) == _lib.GDP_E_BADARG
-    assert of(4096, 50000, 2, 20) == 0                                      # a workgroup for each row
+    assert of(4096, 50000, 2, 20) == of(2050, 1000, 2, 100) == 0            # a workgroup, or a wave, for each row
+    assert of(4096, 50000, 2, 100) == 4096 * (16 + 4 * 100)                 # long lists, finished apart
     assert 2 * 16 + 4 * 20 <= of(1, 128000, 2, 20) <= 64 * 16 + 4 * 20 + 512  # sums of each slice, the listed logits once
     assert of(1 << 21, 1 << 22, 2, 256) >= (1 << 21) * (16 * 16 + 4 * 256)  # 2^18 columns of a slice at most
 
@@ -165,7 +166,7 @@ def test_tangents_are_refused():
 
 @pytest.mark.skipif(shutil.which("nm") is None, reason="no nm")
 def test_every_kernel_has_calls_that_reach_it():
-    """Scans: few or many listed places; a wave a row, or four or eight that read in or past the caches; gradients by
+    """Scans: few or many listed places, many with the finish behind them where that is short or by the join; a wave a row, or four or eight that read in or past the caches; gradients by
     a wave or four.  Adjusted logits: results of the logits' type or float32;
     no table, entries of 16 or 32 bits (long histories: four vectors a thread), two bits for the gradient; one vector a thread, or four, read
     in or past the caches."""
@@ -174,7 +175,9 @@ def test_every_kernel_has_calls_that_reach_it():
     got = {(k, *re.sub(r"\(\w+\)", "", a).split(", ")) for k, a in re.findall(r" ((?:distill|adjust)_\w*kernel)<([^>]*)>", clean)}
     types = ("F32", "F16", "BF16")
     want = {("distill_join_kernel", p) for p in "14"} | {("distill_grad_kernel", t, w) for t in types for w in "14"}
-    want |= {("distill_scan_kernel", t, p, *form) for t in types for p in "14" for form in (("false", "1"), ("false", "4"), ("true", "4"), ("false", "8"), ("true", "8"))}
+    forms = (("false", "1"), ("false", "4"), ("true", "4"), ("false", "8"), ("true", "8"))
+    want |= {("distill_scan_kernel", t, p, "true", *form) for t in types for p in "14" for form in forms if p == "1" or form[0] == "false"}
+    want |= {("distill_scan_kernel", t, "4", "false", *form) for t in types for form in forms}
     sizes = (("1", "false"), ("4", "false"), ("4", "true"))
     for t in types:
         for o in {t, "F32"}:
