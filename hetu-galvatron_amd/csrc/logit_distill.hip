@@ -4,15 +4,15 @@
 // byte or half a byte for each read of 16 bytes) and left out of the sum of exponentials, so that what a teacher's rest is held against is
 // the sum of the unlisted alone: 1 - sum(p) would have no digits left where a student is sure.  A listed token's own logit is read by
 // itself.  With m and s of the unlisted and the list's logits everything else is a row's few numbers, which one wave takes in float64: 1 - sum(q) of
-// float32 log probabilities keeps their digits only there, and 64 exponentials and logarithms are nothing next to a row.
+// float32 log probabilities keeps their digits only there.  That is 3 us of a wave, behind long rows hidden, of short ones the larger part.
 //
 // For any function of the probabilities p_b of the listed tokens and the rest, dL/dz_j = p_j (h_b - H), h_b = dL/dp_b of the alternative
 // that j belongs to and H = sum of p_b h_b.  Of the unlisted this is one number for the row, C = p_rest (h_rest - H), times each one's share
 // w_j = exp(scale (x_j - m_rest)) / s_rest of the unlisted: w_j and C stay in range where p_rest itself is far below float32.  So the
 // gradient is elementwise with one exponential, and the listed places are written again.
 //
-// A row is one workgroup, or, where there are few rows, several of a slice each, whose sums a second kernel joins; the same kernel joins
-// the shards of a vocabulary.
+// A row is one workgroup, or a wave of its own where rows are short and many, or, where there are few rows, several workgroups of a slice
+// each, whose sums a second kernel joins; the same kernel joins the shards of a vocabulary.
 #include "ops_common.h"
 
 #include <type_traits>
