@@ -106,7 +106,7 @@ __device__ void finish_row(const Out &o, const List &l, int64_t row, int lane, S
 #pragma unroll
     for (int j = 0; j < PLACES; ++j) {
         counts[j] = is_listed[j] = token[j] >= 0 && teacher[j] != -__builtin_inff();
-        lq[j] = counts[j] ? (double)teacher[j] - level : -INF;
+        lq[j] = !counts[j] ? -INF : teacher[j] == __builtin_inff() ? __builtin_nan("") : (double)teacher[j] - level;
         q[j] = exp(lq[j]);
         if (counts[j]) m = fmaxf(m, x[j]);
     }
@@ -167,7 +167,8 @@ __device__ void finish_row(const Out &o, const List &l, int64_t row, int lane, S
     const double logs = log(lane == 0 ? s : lane == 1 ? (double)all.s : lane == 2 ? norm : r);
     const double log_s = of_lane(logs, 0), log_out = of_lane(logs, 1), log_norm = of_lane(logs, 2), lr = of_lane(logs, 3);
     const bool nothing = s == 0.0;
-    const double l_out = all.s == 0.0f ? -INF : d_out + log_out - log_s, of_s = 1.0 / s, p_out = s_out * of_s, of_norm = 1.0 / norm;
+    // (a teacher that is no number makes the student's probabilities none, and so the loss and all that goes by it)
+    const double l_out = all.s == 0.0f ? -INF : d_out + log_out - log_s, of_s = mass != mass ? mass : 1.0 / s, p_out = s_out * of_s, of_norm = 1.0 / norm;
     mass *= of_norm;
 #pragma unroll
     for (int j = 0; j < PLACES; ++j) q[j] *= of_norm, lq[j] -= log_norm, lp[j] -= log_s, p[j] *= of_s;
