@@ -137,9 +137,19 @@ __device__ void finish_row(const Out &o, const List &l, int64_t row, int lane, S
             is_listed[j] = times[j] > 0;
             counts[j] = times[j] > 0 && first[j] == lane + 64 * j;
             // (the same bits at all places of a token, an unused one among them)
-            if (times[j] > 1)
+            if (times[j] > 1) {
                 q[j] = sum[j], lq[j] = log(sum[j]);
-            else if (times[j] == 1 && !counts[j])
+                if (sum[j] < __DBL_MIN__) {   // (what float64 has few digits for, or none: relative to the token's largest)
+                    const float *const of_row = l.teacher + row * l.listed;
+                    float most = -__builtin_inff();
+                    for (int k = 0; k < l.listed; ++k)
+                        if (seen[k] == token[j]) most = fmaxf(most, of_row[k]);
+                    double relative = 0.0;
+                    for (int k = 0; k < l.listed; ++k)
+                        if (seen[k] == token[j]) relative += exp((double)of_row[k] - most);
+                    lq[j] = (double)most - level + log(relative);
+                }
+            } else if (times[j] == 1 && !counts[j])
                 q[j] = sum[j], lq[j] = (double)l.teacher[row * l.listed + first[j]] - level;
         }
     }

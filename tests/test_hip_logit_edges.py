@@ -44,3 +44,37 @@ def test_a_teacher_that_is_no_number(beta, rest, score):
         assert torch.isnan(grad[4].gather(0, tokens[4])[torch.isfinite(x[4].gather(0, tokens[4]))]).all()
         parts = [ops.distillation_parts(x[:, a:a + 100], tokens, teacher, first=a) for a in (0, 100, 200)]
         assert torch.isnan(ops.join_distillation(parts, tokens, teacher, 300, beta=beta, rest=rest).loss).tolist() == [True] * 5 + [False] * 2
+
+
+def listed_by_logsumexp(tokens, teacher, vocab):
+    """Of each row {token: log of the sum of q} over its used places, whatever float64 has of q itself."""
+    rows = []
+    for ts, ls in zip(tokens.long().cpu().tolist(), C.f64(teacher).tolist()):
+        got = {}
+        for t, v in zip(ts, ls):
+            if 0 <= t < vocab and v != -INF:
+                got.setdefault(t, []).append(v)
+        rows.append({t: max(v) + math.log(sum(math.exp(a - max(v)) for a in v)) for t, v in got.items()})
+    return rows
+
+
+@pytest.mark.parametrize("beta", [0.0, 0.5, 1.0])
+def test_unlikely_tokens_in_several_places(beta, monkeypatch):
+    """Probabilities that float64 does not hold, or holds with few digits: their sum's logarithm is a number all the same."""
+    monkeypatch.setattr(C, "listed_of", listed_by_logsumexp)
+    g = gen(41)
+    for K in (6, 90):
+        x = normal(g, 5, 400, size=2.0)
+        tokens, teacher = lists(g, 5, 400, K)
+        tokens[0, 1] = tokens[0, 2] = tokens[0, 0]
+        teacher[0, :3] = torch.tensor([-800.0, -801.0, -900.0])
+        tokens[1, 1] = tokens[1, 0]
+        teacher[1, :2] = -1e9                                   # as a grammar's mask leaves them
+        tokens[2, 4] = tokens[2, 3]
+        teacher[2, 3], teacher[2, 4] = -744.5, -744.0           # a few units of the least number
+        tokens[3, 1] = tokens[3, 0]
+        teacher[3, 1] = -3e38                                   # next to a likely one
+        tokens[4, 2] = tokens[4, 1] = tokens[4, 0]
+        teacher[4, 0], teacher[4, 1], teacher[4, 2] = -800.0, -INF, -800.0
+        r = check_distillation(x, tokens, teacher, 1.0, beta, True, tokens[:, 0])
+        assert torch.isfinite(r.loss).all() and torch.isfinite(r.stats).all()
