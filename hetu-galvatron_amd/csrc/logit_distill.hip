@@ -297,7 +297,7 @@ __global__ __launch_bounds__(64 * WAVES) void distill_scan_kernel(Scan a, const 
             const int i = lane + 64 * j;
             token[j] = -1, teacher[j] = -__builtin_inff();
             if (i < a.list.listed) {
-                const int64_t one = token_at(a.list.tokens, a.list.list_type, row * a.list.listed + i), local = one < 0 ? -1 : one - a.first;
+                const int64_t one = token_at(a.list.tokens, a.list.list_type, row * a.list.listed + i), local = one < 0 || one >= a.out.whole ? -1 : one - a.first;
                 teacher[j] = a.list.teacher[row * a.list.listed + i];
                 if (local >= 0 && local < vocab && local >= from && local < to) token[j] = (int32_t)local;
             }
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(64 * WAVES) void distill_scan_kernel(Scan a, const 
 
 struct Join {
     int64_t n;
-    int64_t first, columns;  // the tokens that the lists are of
+    int64_t first, columns;  // the tokens that the lists are of (none where columns is not above 0)
     int32_t parts, lists;    // lists: 1 of slices
     float c;
     List list;
@@ -492,6 +492,7 @@ __global__ __launch_bounds__(64 * WAVES) void distill_grad_kernel(Grad a, const 
         const int e = t + k * THREADS;
         one[k] = -1;
         if (e < listed) one[k] = token_at(a.list.tokens, a.list.list_type, row * listed + e), pull[k] = stats[HEAD + e];
+        if (one[k] >= a.whole) one[k] = -1;
     }
     int64_t target = a.list.targets && a.grad_logp ? token_at(a.list.targets, a.list.target_type, row) : -1;
     if (target >= a.whole) target = -1;
@@ -673,7 +674,8 @@ int rows(Scan s, const void *logits, int type, void *workspace, size_t bytes, co
     if (split.slices == 1 && (s.part.sums || !by_join(split, s.n, s.vocab, s.list.listed))) return scan(s, logits, type, split, who, stream);
     if (!workspace || !aligned(workspace, 256) || bytes < part_bytes(split.slices, s.n, s.list.listed))
         return gdp_fail(GDP_E_BADARG, "gdp_distill: the workspace is smaller than gdp_distill_workspace says, or not aligned to 256 bytes");
-    Join j{s.n, s.first, s.vocab, split.slices, 1, s.c, s.list, part_at(workspace, split.slices, s.n), s.out, s.part};
+    const int64_t columns = s.out.whole - s.first < s.vocab ? s.out.whole - s.first : s.vocab;
+    Join j{s.n, s.first, columns, split.slices, 1, s.c, s.list, part_at(workspace, split.slices, s.n), s.out, s.part};
     s.part = j.in;
     if (const int rc = scan(s, logits, type, split, who, stream)) return rc;
     return join(j, who, stream);
@@ -713,6 +715,7 @@ extern "C" int gdp_distill_parts(const gdp_distill_part *d, void *stream)
     gdp_clear_error();
     if (!d) return gdp_fail(GDP_E_BADARG, "gdp_distill: null argument");
     if (const int rc = check(d->n, d->vocab, d->first, d->logits_type, d->listed)) return rc;
+    if (d->whole_vocab < 0) return gdp_fail(GDP_E_BADARG, "gdp_distill: whole_vocab is negative");
     if (const int rc = check_scale(d->scale)) return rc;
     if (d->n == 0) return GDP_OK;
     const List list{d->tokens, d->targets, d->teacher, d->listed, d->list_type, d->target_type};
@@ -721,7 +724,7 @@ extern "C" int gdp_distill_parts(const gdp_distill_part *d, void *stream)
         return gdp_fail(GDP_E_BADARG, "gdp_distill: null pointer, or sums not aligned to 16 bytes");
     if (const int rc = check_logits(d->logits, d->n, d->vocab, d->logits_stride, d->logits_type, false)) return rc;
     Out out{};
-    out.whole = INT32_MAX;
+    out.whole = d->whole_vocab ? d->whole_vocab : INT32_MAX;
     return rows({d->n, d->vocab, d->logits_stride, d->first, 0, 0, d->scale * LOG2E, list, out, {reinterpret_cast<float4 *>(d->sums), d->listed_logits}}, d->logits,
                 d->logits_type, d->workspace, d->workspace_bytes, "gdp_distill_parts", stream);
 }

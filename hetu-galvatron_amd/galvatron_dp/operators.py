@@ -132,7 +132,7 @@ class gdp_distill(ctypes.Structure):
 class gdp_distill_part(ctypes.Structure):
     _fields_ = [("n", _i64), ("vocab", _i64), ("first", _i64), ("logits", _p), ("logits_stride", _i64), ("logits_type", _i32),
                 ("list_type", _i32), ("target_type", _i32), ("listed", _i32), ("tokens", _p), ("teacher", _p), ("targets", _p),
-                ("scale", _f32), ("reserved", _i32), ("sums", _p), ("listed_logits", _p), ("workspace", _p),
+                ("scale", _f32), ("whole_vocab", _i32), ("sums", _p), ("listed_logits", _p), ("workspace", _p),
                 ("workspace_bytes", _size)]
 
 
@@ -1010,9 +1010,13 @@ def _place(t, columns):
     return rows.data_ptr(), rows.stride(0)
 
 
-def distillation_parts(logits, tokens, teacher, *, first: int, scale: float = 1.0, targets=None) -> DistillationParts:
+def distillation_parts(logits, tokens, teacher, *, first: int, vocab: Optional[int] = None, scale: float = 1.0,
+                       targets=None) -> DistillationParts:
     """``distillation`` of a shard of the vocabulary, ``logits`` [n, columns] of the tokens from ``first`` on, up to what the other
-    shards have to say: 16 + 4 * listed bytes for each row, to be gathered from all shards and joined."""
+    shards have to say: 16 + 4 * listed bytes for each row, to be gathered from all shards and joined.
+
+    ``vocab``: of all shards, as ``join_distillation`` and ``distillation_grad`` get it; needed where shards have columns behind it, as a head
+    that is padded does.  These count as unlisted tokens (rule them out with -inf where they are to have no part)."""
     if forward_ad._current_level >= 0:
         _no_tangents(logits, teacher)
     if torch.is_grad_enabled():
@@ -1021,6 +1025,8 @@ def distillation_parts(logits, tokens, teacher, *, first: int, scale: float = 1.
     if logits.dim() != 2:
         raise ValueError(f"logits must be [n, columns], not {list(logits.shape)}")
     device, (n, columns) = logits.device, logits.shape
+    if vocab is not None and not 0 < vocab < 2 ** 31:
+        raise ValueError(f"vocab must be 1 to 2^31 - 1, not {vocab}")
     flat, list_type, teacher, targets, target_type, listed = _list_of(tokens, teacher, targets, logits.shape[:1], device)
     rows, stride = _rows(logits, columns, "logits") if n and columns else (logits, columns)
     parts = DistillationParts(torch.empty(n, 4, dtype=torch.float32, device=device),
@@ -1028,7 +1034,7 @@ def distillation_parts(logits, tokens, teacher, *, first: int, scale: float = 1.
     work, size = _workspace("gdp_distill_workspace", n, columns, logits_type, listed, device=device)
     _queue(_ops().gdp_distill_parts,
            gdp_distill_part(n, columns, first, rows.data_ptr(), stride, logits_type, list_type, target_type, listed,
-                            flat.data_ptr(), teacher.data_ptr(), _ptr(targets), scale, 0, parts.sums.data_ptr(),
+                            flat.data_ptr(), teacher.data_ptr(), _ptr(targets), scale, vocab or 0, parts.sums.data_ptr(),
                             parts.listed_logits.data_ptr(), _ptr(work), size), device)
     return parts
 

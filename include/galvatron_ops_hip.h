@@ -232,7 +232,9 @@ int gdp_distill_forward(const gdp_distill *d, void *stream);
 
 /* The same for a vocabulary in shards: `parts` of each, joined after the ranks have exchanged them (16 + 4 * listed
  * bytes a row).  Of a part: sums [n][4] float32 (largest unlisted logit; sum of exp2 over the unlisted; the target's logit or -inf;
- * 1 where a token of the shard is at several places, else 0), and the listed tokens' logits, -inf for those of other shards. */
+ * 1 where a token of the shard is at several places, else 0), and the listed tokens' logits, -inf for those of other shards.
+ * Shards may have columns behind the vocabulary, which a head is padded with: they are unlisted ones, and ruled out by -inf where they
+ * are to have no part.  The parts, their join and the gradient are given the same vocabulary then. */
 typedef struct gdp_distill_part {
     int64_t n, vocab, first;
     const void *logits;
@@ -245,7 +247,7 @@ typedef struct gdp_distill_part {
     const float *teacher;
     const void *targets;
     float scale;
-    int32_t reserved;
+    int32_t whole_vocab;    /* of all shards, or 0 where none has columns behind it: tokens outside [0, whole_vocab) are none */
     float *sums, *listed_logits; /* [n][4], [n][listed]                   */
     void *workspace;
     size_t workspace_bytes; /* gdp_distill_workspace of the shard's sizes */

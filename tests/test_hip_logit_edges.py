@@ -78,3 +78,32 @@ def test_unlikely_tokens_in_several_places(beta, monkeypatch):
         teacher[4, 0], teacher[4, 1], teacher[4, 2] = -800.0, -INF, -800.0
         r = check_distillation(x, tokens, teacher, 1.0, beta, True, tokens[:, 0])
         assert torch.isfinite(r.loss).all() and torch.isfinite(r.stats).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("case", [(6, 1000, 1040, 20, 2), (2, 128000, 128256, 100, 1), (1500, 250, 260, 5, 4), (5, 90, 120, 9, 4)], ids=str)
+def test_shards_with_columns_behind_the_vocabulary(case, dtype):
+    """Tokens from ``vocab`` on are none, for the parts, their join and the gradient alike; their columns are unlisted ones."""
+    n, V, padded, K, shards = case
+    g = gen(42)
+    x = normal(g, n, padded, dtype=dtype, size=2.0)
+    tokens, teacher = lists(g, n, padded, K)
+    for i, t in ((0, V), (1, padded - 1)):      # (each once)
+        tokens[i] = torch.where(tokens[i] == t, tokens[i, 0], tokens[i])
+        tokens[i, 0] = t
+    targets = torch.randint(-1, padded, (n,), generator=g).cuda()
+    targets[0], targets[1] = tokens[0, 0], V - 1
+    used, wanted = torch.where(tokens < V, tokens, -1), torch.where(targets < V, targets, -100)
+    edges = [padded * i // shards for i in range(shards + 1)]
+    of = [x[:, a:b] for a, b in zip(edges, edges[1:])]
+    parts = [ops.distillation_parts(s, tokens, teacher, first=a, vocab=V, targets=targets) for s, a in zip(of, edges)]
+    r = ops.join_distillation(parts, tokens, teacher, V, beta=0.25, targets=targets, stats=True)
+    few = slice(0, 6)
+    check_distillation(x[few], used[few], teacher[few], 1.0, 0.25, True, wanted[few], ops.Distillation(*(t[few] for t in r)))
+    d_loss, d_logp = torch.rand(n, generator=g).cuda(), torch.rand(n, generator=g).cuda()
+    whole = ops.distillation_grad(x, used, r.stats, d_loss, targets=wanted, grad_logp=d_logp)
+    pieces = [ops.distillation_grad(s, tokens, r.stats, d_loss, targets=targets, grad_logp=d_logp, first=a, vocab=V) for s, a in zip(of, edges)]
+    assert torch.equal(whole, torch.cat(pieces, 1))
+    for bad in (-1, 0, 2 ** 31, 2 ** 32):
+        with pytest.raises(ValueError, match="vocab"):
+            ops.distillation_parts(x, tokens, teacher, first=0, vocab=bad)
