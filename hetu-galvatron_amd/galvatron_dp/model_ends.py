@@ -127,7 +127,7 @@ class ModelEnds:
                 loss, d_logp = loss - (1.0 - teacher.weight) * r.logp, each * (loss_scale * (teacher.weight - 1.0))
             loss = torch.where(held, loss, 0.0)     # (a place without a target has no part in it, whatever its divergence)
             d_logits = ops.distillation_grad(logits, teacher.tokens, r.stats, each * (loss_scale * teacher.weight), targets=targets,
-                                             grad_logp=d_logp, into=logits)
+                                             grad_logp=d_logp, into=logits.detach())
         rows, normed = (t.reshape(-1, t.shape[-1]) for t in (d_logits, joined.normed))
         d_normed, d_head = rows @ self.head, rows.t() @ normed
         g = ops.residual_norm_grad(joined.stream, block, joined.stats, d_normed.view_as(joined.normed), pre=self.norm)

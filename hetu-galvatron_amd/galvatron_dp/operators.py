@@ -253,6 +253,13 @@ def _written(t):
     torch.autograd.graph.increment_version(t)
 
 
+def _no_history(into):
+    """Refuses to write over a tensor that wants a gradient, whose history would be that of its former values.  (Asked where gradients are
+    taken.)"""
+    if into.requires_grad:
+        raise ValueError("into wants a gradient, which what is written there does not have: detach it")
+
+
 def _constant(t, what):
     """Refuses an input that wants a gradient which there is none of.  (Asked where gradients are taken.)"""
     if isinstance(t, torch.Tensor) and t.requires_grad:
@@ -964,9 +971,11 @@ def distillation_grad(logits, tokens, stats, grad_loss=None, *, scale: float = 1
 
     ``tokens`` and ``targets`` as they were given to the forward pass, ``stats`` as it left them.  Of a vocabulary in shards, ``logits`` are
     those of the shard that begins with token ``first``, of ``vocab`` tokens in all, and ``stats`` those of ``join_distillation``.
-    ``into``: written there; it may be ``logits`` itself."""
+    ``into``: written there; it may be ``logits`` itself, and wants no gradient (detach it)."""
     if forward_ad._current_level >= 0:
         _no_tangents(logits, stats, grad_loss, grad_lse, grad_logp, into)
+    if into is not None and torch.is_grad_enabled():
+        _no_history(into)
     logits_type = _type(logits, "logits")
     if logits.dim() < 1:
         raise ValueError("logits must be [..., vocab]")
@@ -1265,7 +1274,7 @@ def adjust_logits(logits, history=None, *, lengths=None, prompts=None, repetitio
 
     ``logits`` of a shard of the vocabulary begin with token ``first``; everything else is of all of it.  ``into``: written there; it may be
     ``logits`` itself, of which 16 bytes without a change are neither read nor written where there is no scale.  Differentiable with respect to
-    ``logits`` (not ``into`` a tensor); nothing else gets a gradient."""
+    ``logits`` (not ``into`` a tensor, which wants no gradient either: detach it); nothing else gets a gradient."""
     if forward_ad._current_level >= 0:
         _no_tangents(*(t for t in (logits, repetition, frequency, presence, bias, scale, into) if isinstance(t, torch.Tensor)))
     by_autograd = False
@@ -1274,6 +1283,8 @@ def adjust_logits(logits, history=None, *, lengths=None, prompts=None, repetitio
             if t is not None:
                 _constant(t, what)
         by_autograd = logits.requires_grad
+        if into is not None and not by_autograd:
+            _no_history(into)
     if by_autograd:
         if into is not None:
             raise ValueError("into: logits that want a gradient are not written over, nor adjusted into a tensor")
@@ -1290,9 +1301,12 @@ def adjust_logits_grad(logits, grad, history=None, *, lengths=None, repetition=N
                        into: Optional[torch.Tensor] = None):
     """Gradient with respect to ``logits`` [..., vocab], in their type, from that of ``adjust_logits``' result, in its type.  The rest as
     it was given to the forward pass, of which frequencies, presences, prompts and biases have no part in the gradient.  Where the
-    mask rules a token out it is 0, whatever ``grad`` is there.  ``into``: written there; it may be ``grad`` itself."""
+    mask rules a token out it is 0, whatever ``grad`` is there.  ``into``: written there; it may be ``grad`` itself, and wants no
+    gradient (detach it)."""
     if forward_ad._current_level >= 0:
         _no_tangents(*(t for t in (logits, grad, repetition, scale, into) if isinstance(t, torch.Tensor)))
+    if into is not None and torch.is_grad_enabled():
+        _no_history(into)
     _type(logits, "logits")
     _type(grad, "grad")
     if logits.dim() < 1 or grad.shape != logits.shape:

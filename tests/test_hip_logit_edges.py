@@ -15,6 +15,31 @@ F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 INF = math.inf
 
 
+def test_results_in_the_place_of_what_autograd_does_not_follow():
+    """A detached view of a tensor that wants a gradient may be written, and the graph that holds its values says so; a student's gradients
+    are the same where its block wants one."""
+    g = gen(45)
+    leaf = normal(g, 3, 60).requires_grad_(True)
+    y = leaf * 5
+    kept = (y * y).sum()
+    want = ops.adjust_logits(y.detach(), scale=2.0)
+    assert torch.equal(ops.adjust_logits(y.detach(), scale=2.0, into=y.detach()), want) and torch.equal(y, want)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        kept.backward()
+    with torch.no_grad():
+        ops.adjust_logits(leaf, scale=2.0, into=leaf)
+    assert torch.equal(leaf * 5, want)
+    ends = model_ends.ModelEnds(96, 1000, dtype=BF16, seed=7)
+    tokens, targets = torch.randint(0, 1000, (6,), generator=g).cuda(), torch.randint(0, 1000, (6,), generator=g).cuda()
+    block = normal(g, 6, 96, dtype=BF16)
+    listed, q = lists(g, 6, 1000, 8)
+    for weight in (1.0, 0.5):
+        teacher = model_ends.Teacher(listed, q, weight=weight)
+        a = ends.loss_and_grads(tokens, targets, block, teacher=teacher)
+        b = ends.loss_and_grads(tokens, targets, block.clone().requires_grad_(True), teacher=teacher)
+        assert all(torch.equal(s, t) for s, t in zip(a, b) if s is not None)
+
+
 @pytest.mark.parametrize("score", [INF, math.nan], ids=["inf", "nan"])
 @pytest.mark.parametrize("beta,rest", [(0.0, True), (0.5, True), (1.0, True), (0.0, False), (0.5, False)])
 def test_a_teacher_that_is_no_number(beta, rest, score):
