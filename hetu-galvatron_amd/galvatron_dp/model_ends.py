@@ -80,12 +80,15 @@ class ModelEnds:
                 adjust: Optional[Mapping] = None):
         """From tokens to log probabilities of the targets, with ``block`` [..., hidden] in the place of what the layers add to the
         stream; of a shard, the ``LogprobParts`` to be exchanged.  With a ``teacher`` ``ops.Distillation`` from it, or its parts.
-        ``adjust``: what ``ops.adjust_logits`` is given besides the logits (histories, penalties, biases, a mask), for a step that chooses."""
+        ``adjust``: what ``ops.adjust_logits`` is given besides the logits (histories, penalties, biases, a mask, a
+        type), for a step that chooses."""
         if teacher is not None and (entropy or top):
             raise ValueError("a teacher's distillation has no entropies and no alternatives")
         _, logits = self.logits(self.embed(tokens), block)
         if adjust is not None:
-            logits = ops.adjust_logits(logits, first=self.first, into=logits, **adjust)
+            # In the logits' place, where they are not differentiated and nothing asks for another type.
+            place = not logits.requires_grad and adjust.get("dtype") in (None, logits.dtype)
+            logits = ops.adjust_logits(logits, first=self.first, into=logits if place else None, **adjust)
         if teacher is not None:
             if self.shards > 1:
                 flat = lambda t: t.reshape(-1, t.shape[-1])   # noqa: E731

@@ -132,3 +132,26 @@ def test_shards_with_columns_behind_the_vocabulary(case, dtype):
     for bad in (-1, 0, 2 ** 31, 2 ** 32):
         with pytest.raises(ValueError, match="vocab"):
             ops.distillation_parts(x, tokens, teacher, first=0, vocab=bad)
+
+
+@pytest.mark.parametrize("dtype", [None, F32], ids=["same", "float32"])
+def test_a_step_that_is_differentiated_or_in_float32(dtype):
+    """``ModelEnds.forward`` with adjusted logits: towards the block as without them, and in the type that is asked for."""
+    ends = model_ends.ModelEnds(96, 1000, dtype=BF16, seed=7)
+    g = gen(44)
+    tokens, targets = torch.randint(0, 1000, (6,), generator=g).cuda(), torch.randint(0, 1000, (6,), generator=g).cuda()
+    block = normal(g, 6, 96, dtype=BF16)
+    adjust = dict(history=history_of(g, 6, 40, 1000), repetition=1.2, frequency=0.5, scale=0.8, **({"dtype": dtype} if dtype else {}))
+    plain = block.clone().requires_grad_(True)
+    want = ops.token_logprobs(ops.adjust_logits(ends.logits(ends.embed(tokens), plain)[1], **adjust), targets)
+    want.logp.sum().backward()
+    leaf = block.clone().requires_grad_(True)
+    r = ends.forward(tokens, targets, leaf, adjust=adjust)
+    r.logp.sum().backward()
+    assert torch.equal(r.logp, want.logp) and torch.equal(leaf.grad, plain.grad) and bool((leaf.grad != 0).any())
+    with torch.no_grad():
+        assert torch.equal(ends.forward(tokens, targets, leaf, adjust=adjust).logp, want.logp)
+        listed, q = lists(g, 6, 1000, 8)
+        r = ends.forward(tokens, targets, block, teacher=model_ends.Teacher(listed, q), adjust=adjust)
+        same = ops.distillation(ops.adjust_logits(ends.logits(ends.embed(tokens), block)[1], **adjust), listed, q, targets=targets)
+        assert torch.equal(r.loss, same.loss) and torch.equal(r.logp, same.logp)
