@@ -870,8 +870,12 @@ class DistillationParts(NamedTuple):
 _STATS = 5      # numbers of a row's stats in front of those of its places
 
 
-def _list_of(tokens, teacher, targets, shape, device):
-    """Checked lists and targets: tokens, their type, log probabilities, targets, their type."""
+def _list_of(tokens, teacher, targets, shape, device, taught=True):
+    """Checked lists and targets: tokens, their type, log probabilities (not where nothing is ``taught``), targets, their type."""
+    if tokens is None:
+        raise ValueError("tokens are needed: token_logprobs gives them where top is asked for")
+    if taught and teacher is None:
+        raise ValueError("teacher is needed: the log probabilities of the tokens")
     list_type = _type(tokens, "tokens", _TOKEN_TYPES)
     listed = tokens.shape[-1] if tokens.dim() else 0
     if tokens.dim() != len(shape) + 1 or tokens.shape[:-1] != shape or not 1 <= listed <= MAX_LISTED:
@@ -982,7 +986,9 @@ def distillation_grad(logits, tokens, stats, grad_loss=None, *, scale: float = 1
     device, columns, shape = logits.device, logits.shape[-1], logits.shape[:-1]
     if vocab is None:
         vocab = first + columns
-    flat, list_type, _, targets, target_type, listed = _list_of(tokens, None, targets, shape, device)
+    flat, list_type, _, targets, target_type, listed = _list_of(tokens, None, targets, shape, device, taught=False)
+    if stats is None:
+        raise ValueError("stats are needed: distillation returns them where they are asked for")
     if stats.dtype != torch.float32:
         raise ValueError(f"stats must be as distillation gives them: float32, not {stats.dtype}")
     stats = _floats(stats, shape + (_STATS + listed,), "stats", device)

@@ -155,3 +155,19 @@ def test_a_step_that_is_differentiated_or_in_float32(dtype):
         r = ends.forward(tokens, targets, block, teacher=model_ends.Teacher(listed, q), adjust=adjust)
         same = ops.distillation(ops.adjust_logits(ends.logits(ends.embed(tokens), block)[1], **adjust), listed, q, targets=targets)
         assert torch.equal(r.loss, same.loss) and torch.equal(r.logp, same.logp)
+
+
+def test_missing_tensors_are_named():
+    """What a call that did not ask for them leaves as None."""
+    g = gen(43)
+    x = normal(g, 3, 50)
+    tokens, teacher = lists(g, 3, 50, 4)
+    r, one = ops.distillation(x, tokens, teacher), torch.ones(3, device="cuda")
+    assert r.stats is None
+    parts = ops.distillation_parts(x, tokens, teacher, first=0)
+    for what, call in (("stats", lambda: ops.distillation_grad(x, tokens, r.stats, one)), ("tokens", lambda: ops.distillation(x, None, teacher)),
+                       ("teacher", lambda: ops.distillation(x, tokens, None)), ("tokens", lambda: ops.distillation_parts(x, None, teacher, first=0)),
+                       ("teacher", lambda: ops.distillation_parts(x, tokens, None, first=0)), ("tokens", lambda: ops.join_distillation([parts], None, teacher, 50)),
+                       ("teacher", lambda: ops.join_distillation([parts], tokens, None, 50))):
+        with pytest.raises(ValueError, match=what):
+            call()
