@@ -171,3 +171,41 @@ def test_missing_tensors_are_named():
                        ("teacher", lambda: ops.join_distillation([parts], tokens, None, 50))):
         with pytest.raises(ValueError, match=what):
             call()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("columns", [1, 7, 2049, 50257], ids=str)
+def test_gradients_of_adjusted_logits_in_place(columns, dtype):
+    """Without a scale what does not change is neither read nor written: the same bits as in a new tensor, rows at any alignment."""
+    g = gen(46)
+    n = 5
+    x = normal(g, n, columns, dtype=dtype)
+    history = history_of(g, n, 70, columns)
+    ok = torch.rand(n, columns, generator=g) < 0.5
+    ok[1], ok[2], ok[3, columns // 3:] = True, False, True
+    mask, rep = C.words_of(ok).cuda(), (0.5 + torch.rand(n, generator=g)).cuda()
+    for given in (dict(history=history, repetition=1.3), dict(history=history, repetition=rep, allowed=mask), dict(allowed=mask), dict(history=history[:, :0], allowed=mask),
+                  dict(history=history, repetition=rep, lengths=torch.tensor([0, 1, 70, 35, 0]).cuda(), allowed=mask[1]), dict()):
+        grad = normal(g, n, columns + 9, dtype=dtype)
+        for at in (0, 1, 3):
+            want = ops.adjust_logits_grad(x, grad[:, at:at + columns], **given)
+            ref, bound = C.adjusted_grad(x, grad[:, at:at + columns], **given)
+            C.close(want, ref, bound + C.rounded(ref, dtype), "gradient")
+            place = grad.clone()
+            got = ops.adjust_logits_grad(x, place[:, at:at + columns], into=place[:, at:at + columns], **given)
+            assert torch.equal(got, want) and torch.equal(place[:, :at], grad[:, :at]) and torch.equal(place[:, at + columns:], grad[:, at + columns:])
+
+
+def test_large_adjusted_logits_in_place():
+    """More than 256 MB in the place of what is read, in both directions: the same bits as in a new tensor."""
+    g = gen(47)
+    n, V = 1100, 128250
+    x = torch.randn(n, V, device="cuda").to(BF16)
+    given = dict(history=torch.randint(0, V, (n, 40), generator=g).cuda(), repetition=1.2, allowed=C.words_of(torch.rand(V, generator=g) < 0.5).cuda())
+    more = dict(frequency=0.5, bias_tokens=torch.randint(0, V, (n, 9), generator=g).cuda(), bias=normal(g, n, 9))
+    for each in (dict(given, **more), dict(allowed=given["allowed"])):
+        want, place = ops.adjust_logits(x, **each), x.clone()
+        assert torch.equal(ops.adjust_logits(place, into=place, **each), want)
+    for each in (given, dict(allowed=given["allowed"])):
+        want, place = ops.adjust_logits_grad(x, x, **each), x.clone()
+        assert torch.equal(ops.adjust_logits_grad(x, place, into=place, **each), want)
