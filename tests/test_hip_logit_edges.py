@@ -209,3 +209,35 @@ def test_large_adjusted_logits_in_place():
     for each in (given, dict(allowed=given["allowed"])):
         want, place = ops.adjust_logits_grad(x, x, **each), x.clone()
         assert torch.equal(ops.adjust_logits_grad(x, place, into=place, **each), want)
+
+
+@pytest.mark.parametrize("listed", [20, 70])
+@pytest.mark.parametrize("case", [(600, 262400, BF16), (300, 262400, F32), (4100, 16500, F16)], ids=["bfloat16", "float32", "many rows"])
+def test_distillation_gradients_that_are_written_past_the_caches(case, listed):
+    """More than 128 MB: the same bits as rows by themselves have, in a new tensor and in the logits' place, with targets that are listed and
+    targets that are not."""
+    n, V, dtype = case
+    g = gen(48)
+    x = torch.randn(n, V, device="cuda").to(dtype)
+    assert x.numel() * x.element_size() >= 128 << 20
+    tokens, teacher = lists(g, 9, V, listed)
+    tokens, teacher = tokens.repeat(n // 9 + 1, 1)[:n].contiguous(), teacher.repeat(n // 9 + 1, 1)[:n].contiguous()
+    targets = torch.randint(0, V, (n,), generator=g).cuda()
+    targets[::3] = tokens[::3, 1]
+    r = ops.distillation(x, tokens, teacher, targets=targets, stats=True)
+    d, d_logp = torch.rand(n, generator=g).cuda(), torch.rand(n, generator=g).cuda()
+    whole = ops.distillation_grad(x, tokens, r.stats, d, targets=targets, grad_logp=d_logp)
+    some = torch.cat([torch.arange(8), torch.arange(n // 2, n // 2 + 4), torch.arange(n - 4, n)]).cuda()
+    part = ops.distillation_grad(x[some], tokens[some], r.stats[some], d[some], targets=targets[some], grad_logp=d_logp[some])
+    assert torch.equal(whole[some], part)
+    one = slice(0, 2)
+    want, bound = C.distillation_grad(x[one], tokens[one], r.stats[one], d[one], 1.0, targets[one], None, d_logp[one])
+    C.close(part[one], want, bound + C.rounded(want, dtype), "gradient by stats")
+    # the listed places and the targets, of all rows
+    at = torch.cat([tokens, targets[:, None]], 1)
+    for a in range(0, n, 97):
+        rows = slice(a, a + 97)
+        same = ops.distillation_grad(x[rows], tokens[rows], r.stats[rows], d[rows], targets=targets[rows], grad_logp=d_logp[rows])
+        assert torch.equal(whole[rows].gather(1, at[rows]), same.gather(1, at[rows]))
+    place = x.clone()
+    assert torch.equal(ops.distillation_grad(place, tokens, r.stats, d, targets=targets, grad_logp=d_logp, into=place), whole)
