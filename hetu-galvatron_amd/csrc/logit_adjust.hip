@@ -329,14 +329,18 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(Adjust a, const typenam
 
 // ---- host ----
 // The last of the caches has 256 MB.  What does not fit it is read past the caches, results of half as much are written past them: the gradient of
-// 2048 x 128256 bf16 258 us with neither, 249 with the result and 241 with both past the caches; forward 1024 x 128256 132 us, 126 with the result
+// 2048 x 128256 bf16 252 us with neither, 243 with the result and 226 with both past the caches; forward 1024 x 128256 115 us, 107 with the result
 // past them.  What fits is left to who reads it next.
 constexpr int64_t READ_PAST = 256 << 20, WRITE_PAST = 128 << 20;
 // Entries of 16 bits for histories whose counts they hold leave a core twice the columns: with entries of 32 bits and half the columns to a workgroup
-// 1024 x 128256 with histories of 1024 147 us, not 133.  One read of the history in flight: four are 154 us there, for 64 registers are
-// exceeded, and 23 us and 20 at 128 x 50257 with histories of 16384.
+// 1024 x 128256 with histories of 1024 147 us, not 133 (by graphs replayed after a wait, up to a tenth longer than on a busy
+// device, as the rest was measured).  One read of the history in flight: with four, for which 64 registers are exceeded, 120 us there, not 107,
+// and at 128 x 50257 float32 with all of 16384 places used 33 us, not 28.
 // Four vectors a thread where that leaves no core without a workgroup, else one: 16 x 128256 bf16 with histories of 2048 12.2 us with four and 8.0
 // with one, 77 x 32003 float32 (gradient) 10.6 and 11.8.
+// Entries of 32 bits are built for four alone, few rows or many, and chosen by the places that a history has, not by those that count.  That leaves cores idle:
+// one row of 128256 bf16 with a history of 16383 places 9.2 us, of 16384 11.1, of 32768 16.3; 16 rows 11.3, 11.9 and 22; where 1000 of the places count
+// one row takes 5 us with 16383 of them and 7 with 32768.
 constexpr int64_t CORES = 256;
 // Slices of a row; one more vector where it begins within 16 bytes.
 constexpr int64_t slices_of(int64_t vocab, int vec, int columns) { return ((vocab + vec - 1) / vec * vec + vec + columns - 1) / columns; }

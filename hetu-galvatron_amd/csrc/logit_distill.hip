@@ -251,8 +251,8 @@ struct Scan {
 };
 
 // Bound by memory where rows are long and many: 8192 x 128256 bf16 with 20 listed tokens 320 us, 2.1 GB at 6.6 TB/s; 2048 x 50257 float16 with 64 and beta
-// 0.5 48 us, 4.3 TB/s: two rounds of workgroups, and a finish of 3 us behind each row.  Rows of 2 KB are mostly finish: 32089 x 1180 61 us, 36 of them without it.
-// Few rows wait for memory four times (lists, bitmap, logits, the join): 16 x 128256 10 us.
+// 0.5 48 us, 4.3 TB/s: two rounds of workgroups, and a finish of 3 us behind each row.  Rows of 2 KB are mostly finish: 32089 x 1180 57 us, some 25 less without it.
+// Few rows wait for memory four times (lists, bitmap, logits, the join): 16 x 128256 9 us.
 // PLACES: of each lane of the wave that finishes, 1 or 4; the finish of four holds 100 registers.  FINISH: whole rows are finished here.  PAST: read past the caches.
 template <typename T, int PLACES, bool FINISH, bool PAST, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void distill_scan_kernel(Scan a, const typename T::raw *__restrict__ logits)
@@ -400,7 +400,7 @@ struct Join {
 // The larger; NaN where one of them is.
 __device__ __forceinline__ float most_or_nan(float a, float b) { return a > b || a != a ? a : b; }
 
-// A wave for each row: lists, sums and logits are read side by side, then the finish.  8192 rows of 8 shards with 20 listed tokens 14 us, 16 rows of
+// A wave for each row: lists, sums and logits are read side by side, then the finish.  8192 rows of 8 shards with 20 listed tokens 12 us, 16 rows of
 // slices 4 us.
 template <int PLACES> __global__ __launch_bounds__(64) void distill_join_kernel(Join a)
 {
@@ -454,9 +454,9 @@ struct Grad {
     const float *stats, *grad_loss, *grad_lse, *grad_logp;
 };
 
-// Elementwise with one exponential, bound by memory: 8192 x 128256 bf16 713 us, 4.2 GB at 5.9 TB/s; a shard's 4096 x 19008 with 128 listed places 54 us,
+// Elementwise with one exponential, bound by memory: 8192 x 128256 bf16 716 us, 4.2 GB at 5.9 TB/s; a shard's 4096 x 19008 with 128 listed places 54 us,
 // 5.8 TB/s; 517 x 32003 float16 15 us.  A workgroup has its columns in registers while it looks at the places, 512 vectors of two for
-// each thread: with two rounds of them 8192 x 128256 832 us, with one 786 (both written in the caches).
+// each thread: with two rounds of them 8192 x 128256 796 us, with one 757 (both written in the caches).
 template <typename T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void distill_grad_kernel(Grad a, const typename T::raw *logits, typename T::raw *out)
 {
@@ -560,6 +560,9 @@ __global__ __launch_bounds__(64 * WAVES) void distill_grad_kernel(Grad a, const 
 }
 
 // ---- host ----
+// Figures that stand side by side were measured in one way, behind each other.  Some are of graphs that were replayed after a wait, which takes up to a tenth
+// longer than on a busy device: they are for holding against each other.
+//
 // How a row is shared out: slices of 512 vectors (8 KB) at least, a workgroup for each core, and no more columns in a slice than LDS has bits
 // for.  A slice is read by eight waves where there are few, else by four.  Bf16, 20 listed tokens, with 1024 workgroups of four waves and
 // with 256 of eight: 333 x 32003 (float32) 16.3 and 13.9 us, 512 x 128256 33.1 and 29.9, 700 x 32000 18.5 and 16.2, 16 x 128256 9.8 and 9.7; eight
@@ -578,9 +581,9 @@ Split split_of(int64_t n, int64_t vocab, int type)
     const int64_t width = ceil_div(vectors, slices);
     return {(int)ceil_div(vectors, width), (int)width};
 }
-// The last of the caches has 256 MB.  Logits that do not fit it are read past the caches, 8192 x 128256 bf16 399 us and 358; what does is read again by the
+// The last of the caches has 256 MB.  Logits that do not fit it are read past the caches, 8192 x 128256 bf16 363 us and 320; what does is read again by the
 // gradient: 2048 x 50257 bf16 forward and backward 99 us, 109 with reads past the caches.  Gradients of half as much are written past them:
-// 8192 x 128256 786 and 741.
+// 8192 x 128256 757 and 728 (here each result in memory of its own).
 constexpr int64_t READ_PAST = 256 << 20, WRITE_PAST = 128 << 20;
 // Whether rows are finished by a kernel of their own: those in slices, and, of lists with more than a place for each lane, whose finish holds
 // registers that the scan could read with, those that take longer than a launch.  8192 x 128256 bf16 with 100 listed tokens 362 us, 399 where

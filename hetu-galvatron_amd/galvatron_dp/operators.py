@@ -1279,8 +1279,9 @@ def adjust_logits(logits, history=None, *, lengths=None, prompts=None, repetitio
     scales have to be above 0, which is looked at for numbers only.
 
     ``logits`` of a shard of the vocabulary begin with token ``first``; everything else is of all of it.  ``into``: written there; it may be
-    ``logits`` itself, of which 16 bytes without a change are neither read nor written where there is no scale.  Differentiable with respect to
-    ``logits`` (not ``into`` a tensor, which wants no gradient either: detach it); nothing else gets a gradient."""
+    ``logits`` itself (and does not overlap them otherwise), of which 16 bytes without a change are neither read nor written where there
+    is no scale.  Differentiable with respect to ``logits`` (not ``into`` a tensor, which wants no gradient either: detach it); nothing else
+    gets a gradient."""
     if forward_ad._current_level >= 0:
         _no_tangents(*(t for t in (logits, repetition, frequency, presence, bias, scale, into) if isinstance(t, torch.Tensor)))
     by_autograd = False

@@ -300,7 +300,8 @@ int gdp_distill_backward(const gdp_distill_grad *d, void *stream);
  * the mask does not allow token j, whatever x_j is.  pen(x) is x / repetition above 0 and x * repetition else for the tokens of the row's history,
  * and x for others; count_j is how often token j is in it from place `prompt` on; bias_j the sum of the biases that the row has for it.
  * Any of the four may be missing.  The places of a history from `length` on do not count (a length above `places` is taken as `places`), nor do
- * tokens of other shards or outside the vocabulary.  Each term is rounded to float32, the result once more to its type.
+ * tokens of other shards or outside the vocabulary.  Each term is rounded to float32 (x / repetition is x times the float32 of 1 / repetition, two
+ * roundings), the result once more to its type.  Biases come behind the penalties, so that one adds the same whatever the history has.
  * Repetitions and scales have to be above 0; what the device holds of them is not looked at. */
 #define GDP_MAX_BIASES 1024
 typedef struct gdp_adjust_history {
@@ -329,7 +330,7 @@ typedef struct gdp_adjust {
     const float *scales;    /* [n] or NULL: `scale`                       */
     float scale;
     int32_t reserved;
-    void *out;              /* [n][vocab]; may be logits itself with their type: 16 bytes in which nothing changes are not written then */
+    void *out;              /* [n][vocab]; may be logits itself with their type, and does not overlap them otherwise: 16 bytes in which nothing changes are not written then */
     int64_t out_stride;
 } gdp_adjust;
 int gdp_adjust_forward(const gdp_adjust *a, void *stream);
@@ -337,7 +338,7 @@ int gdp_adjust_forward(const gdp_adjust *a, void *stream);
 /* Its gradient with respect to the logits:  grad_j * scale, divided by or times the repetition as pen(x_j) is, and 0 where the mask
  * does not allow token j, whatever grad_j is.  Frequencies, presences, prompts and biases have no part in it. */
 typedef struct gdp_adjust_grad {
-    gdp_adjust given;       /* its out is the gradient of the logits, of their type; out_type is that of grad; out may be grad itself with that type */
+    gdp_adjust given;       /* its out is the gradient of the logits, of their type; out_type is that of grad; out may be grad itself with that type, and overlaps neither it nor the logits otherwise */
     const void *grad;       /* [n][vocab]                                 */
     int64_t grad_stride;
 } gdp_adjust_grad;
